@@ -289,6 +289,49 @@ int pbg_sub_bucket(pbg_context *ctx, const int64_t *lhs_in, const int64_t *rhs_i
                    int32_t num_lhs_sub_parts, int32_t num_rhs_sub_parts, int32_t dynamic_relations,
                    int64_t *sub_bucket_counts);
 
+/* ---- Token operators: rows of a table by id, log probabilities over rows of scores and over all rows of a table, with
+ * their gradients.  They have no counterpart in the reference, which gathers with F.embedding and scores with bmm.  No
+ * context: every call is queued on `stream` (a cudaStream_t, NULL = default stream) of the current device and returns
+ * at once; nothing is allocated and nothing synchronises, so calls may be captured into a graph.  What a call needs beside its
+ * outputs is `workspace`, device memory of the size its *_workspace function gives (256-byte aligned, contents
+ * irrelevant); two calls in flight need two of them.  All pointers are device memory; row strides are in elements, the elements of
+ * a row lie next to each other.  Types are pbg_dtype; sums, statistics and softmax sums are fp32, results are rounded once.
+ * errors: device int32 word or NULL; bit 1 is set by an id or target outside of its range, bit 2 where a bounded
+ * wait ran out.  Sizes: dim 1 to 65536, ids and rows below 2^31.
+ * A target equal to ignore_index marks a row of padding: it is not read, its outputs are 0 (top_ids -1), its gradients 0. ---- */
+typedef enum { PBG_F32 = 0, PBG_BF16 = 1, PBG_F16 = 2 } pbg_dtype;
+
+/* out[i] = scale * table[ids[i]]; out [n, dim], rows one behind the other.  An id outside [0, num_rows) gives a row of NaN. */
+int pbg_embedding_lookup(const void *table, int64_t row_stride, int64_t num_rows, int32_t dim, int32_t dtype,
+                         const int64_t *ids, int64_t n, float scale, void *out, int32_t *errors, void *stream);
+
+/* Gradient of the table: out[v] = scale * sum of grad[i] over the i with ids[i] == v, in the order of i (sorted by id:
+ * the same bits every time); rows without an id get 0.  accumulate = 1: the sums are added to out, whose other rows
+ * are left alone.  An id outside [0, num_rows) is skipped.  out [num_rows, dim], of grad's type. */
+int64_t pbg_embedding_lookup_grad_workspace(int64_t n, int64_t num_rows, int32_t dim);
+int pbg_embedding_lookup_grad(const void *grad, int64_t grad_stride, const int64_t *ids, int64_t n, int64_t num_rows,
+                              int32_t dim, int32_t dtype, float scale, void *out, int64_t out_stride, int32_t accumulate,
+                              void *workspace, int64_t workspace_bytes, int32_t *errors, void *stream);
+
+/* Per row of logits [n, vocab], with z = scale * logits, p = softmax(z), t = the row's target:
+ *   logprob = log p_t;  entropy = -sum p log p;  lse = log sum exp z   (float32 [n])
+ *   rank    = 1 + #(x_v > x_t) + #(x_v == x_t, v < t)                  (int64 [n])
+ *   top_ids, top_logprobs [n, top]: the `top` (0 to 32) largest, descending, equal ones in the order of their ids; NaN
+ *                                   counts as -inf in this order.  NULL with top == 0.
+ * A row of -inf alone has lse -inf, logprob -inf and entropy 0; NaN or +inf in a row makes its statistics NaN.  A target outside
+ * [0, vocab) gives logprob NaN and rank 0.  The row is read once. */
+int pbg_token_logprobs(const void *logits, int64_t row_stride, int64_t n, int64_t vocab, int32_t dtype,
+                       const int64_t *targets, int64_t ignore_index, float scale, int32_t top, float *logprob,
+                       float *entropy, float *lse, int64_t *rank, float *top_logprobs, int64_t *top_ids, int32_t *errors, void *stream);
+
+/* d(sum of grad_logprob * logprob + grad_entropy * entropy) / d(logits), from the lse and entropy of the forward call:
+ *   out_v = scale * (grad_logprob * ([v == t] - p_v) - grad_entropy * p_v * (log p_v + entropy))
+ * Either gradient may be NULL (zero); entropy is read where grad_entropy is given.  out may be logits itself (with its row stride). */
+int pbg_token_logprobs_grad(const void *logits, int64_t row_stride, int64_t n, int64_t vocab, int32_t dtype,
+                            const int64_t *targets, int64_t ignore_index, float scale, const float *lse, const float *entropy,
+                            const float *grad_logprob, const float *grad_entropy, void *out, int64_t out_stride,
+                            int32_t *errors, void *stream);
+
 /* Kernel launches issued by this context since creation (for launch accounting). */
 int64_t pbg_launch_count(const pbg_context *ctx);
 

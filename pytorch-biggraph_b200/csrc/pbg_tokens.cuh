@@ -1,0 +1,71 @@
+// Shared by the token operators (lookup, log probabilities over scores, log probabilities over a table): element types, 16-byte
+// vectors of them, and the exponential they all use.
+//
+// These entry points take no context: the caller hands over the stream and the workspace, nothing here allocates or
+// synchronises, and a bad id is skipped and reported through the caller's error word.
+#pragma once
+#include <cuda_fp16.h>
+#include <limits>
+
+#include "pbg_common.cuh"
+
+#define TOK_LOG2E 1.4426950408889634f
+#define TOK_LN2 0.6931471805599453f
+#define TOK_ERR_ID 1                       // bits of the caller's error word
+#define TOK_ERR_TIMEOUT 2
+
+// ex2 takes z to 2^z within 2 ulp, results below 2^-126 to 0.
+__device__ __forceinline__ float tok_ex2(float z) { float e; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z)); return e; }
+__device__ __forceinline__ float tok_lg2(float s) { return log2f(s); }
+// the larger, NaN if either is one
+__device__ __forceinline__ float tok_max_nan(float a, float b) { float m; asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b)); return m; }
+
+// Element types: storage type, elements of a 16-byte vector, conversions.  Results are rounded to nearest, once.
+template <class T> struct Tok;
+template <> struct Tok<float> {
+  static constexpr int VEC = 4;
+  static __device__ __forceinline__ float up(float x) { return x; }
+  static __device__ __forceinline__ float down(float x) { return x; }
+};
+template <> struct Tok<__nv_bfloat16> {
+  static constexpr int VEC = 8;
+  static __device__ __forceinline__ float up(__nv_bfloat16 x) { return __bfloat162float(x); }
+  static __device__ __forceinline__ __nv_bfloat16 down(float x) { return __float2bfloat16_rn(x); }
+};
+template <> struct Tok<__half> {
+  static constexpr int VEC = 8;
+  static __device__ __forceinline__ float up(__half x) { return __half2float(x); }
+  static __device__ __forceinline__ __half down(float x) { return __float2half_rn(x); }
+};
+
+template <class T>
+__device__ __forceinline__ void tok_unpack(const uint4 &v, float (&x)[Tok<T>::VEC]) {
+  const T *p = reinterpret_cast<const T *>(&v);
+#pragma unroll
+  for (int i = 0; i < Tok<T>::VEC; ++i) x[i] = Tok<T>::up(p[i]);
+}
+template <class T>
+__device__ __forceinline__ uint4 tok_pack(const float (&x)[Tok<T>::VEC]) {
+  uint4 v;
+  T *p = reinterpret_cast<T *>(&v);
+#pragma unroll
+  for (int i = 0; i < Tok<T>::VEC; ++i) p[i] = Tok<T>::down(x[i]);
+  return v;
+}
+
+inline size_t tok_size(int dtype) { return dtype == PBG_F32 ? 4 : 2; }
+inline bool tok_type(int dtype) { return dtype == PBG_F32 || dtype == PBG_BF16 || dtype == PBG_F16; }
+inline bool tok_scale(float s) { return s > 0.f && s <= std::numeric_limits<float>::max(); }     // (false for NaN)
+inline bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+// CALL<element type>(...) by the run-time type
+#define TOK_DISPATCH(DTYPE, CALL, ...)                                 \
+  do {                                                                 \
+    if ((DTYPE) == PBG_F32) CALL<float>(__VA_ARGS__);                  \
+    else if ((DTYPE) == PBG_BF16) CALL<__nv_bfloat16>(__VA_ARGS__);    \
+    else CALL<__half>(__VA_ARGS__);                                    \
+  } while (0)
+
+// The first failed launch of a call, as its status.
+inline int tok_status() { return pbg_take_launch_error() == cudaSuccess ? PBG_OK : PBG_ERR_CUDA; }
+inline int64_t tok_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }

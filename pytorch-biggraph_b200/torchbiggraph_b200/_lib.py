@@ -12,6 +12,7 @@ LIB_PATH = os.path.join(_HERE, "libpbg_b200.so")
 OPERATOR_CODES = {"none": 0, "diagonal": 1, "translation": 2, "complex_diagonal": 3, "linear": 4, "affine": 5}
 COMPARATOR_CODES = {"dot": 0, "cos": 1, "l2": 2, "squared_l2": 3}
 LOSS_CODES = {"logistic": 0, "ranking": 1, "softmax": 2}
+DTYPE_CODES = {"float32": 0, "bfloat16": 1, "float16": 2}                        # pbg_dtype
 PRECISION_CODES = {"fp32": 0, "tf32x3": 1, "tf32": 2, "bf16x6": 3, "bf16x3": 4}
 
 PBG_OK, PBG_ERR_BAD_ARGUMENT, PBG_ERR_UNSUPPORTED, PBG_ERR_INDEX_RANGE = 0, 1, 2, 3
@@ -80,6 +81,13 @@ SYMBOLS = [
     ("pbg_sub_bucket", C.c_int, [_P, _P, _P, _P, C.c_int64, C.c_int32, C.POINTER(C.c_int64), C.POINTER(_P),
                                  C.POINTER(C.c_int64), C.POINTER(_P), _P, _P, _P, C.c_int32, C.c_int32, C.c_int32,
                                  C.POINTER(C.c_int64)]),
+    ("pbg_embedding_lookup", C.c_int, [_P, C.c_int64, C.c_int64, C.c_int32, C.c_int32, _P, C.c_int64, C.c_float, _P, _P, _P]),
+    ("pbg_embedding_lookup_grad_workspace", C.c_int64, [C.c_int64, C.c_int64, C.c_int32]),
+    ("pbg_embedding_lookup_grad", C.c_int, [_P, C.c_int64, _P, C.c_int64, C.c_int64, C.c_int32, C.c_int32, C.c_float, _P, C.c_int64,
+                                            C.c_int32, _P, C.c_int64, _P, _P]),
+    ("pbg_token_logprobs", C.c_int, [_P, C.c_int64, C.c_int64, C.c_int64, C.c_int32, _P, C.c_int64, C.c_float, C.c_int32] + [_P] * 8),
+    ("pbg_token_logprobs_grad", C.c_int, [_P, C.c_int64, C.c_int64, C.c_int64, C.c_int32, _P, C.c_int64, C.c_float, _P, _P, _P, _P, _P,
+                                          C.c_int64, _P, _P]),
     ("pbg_launch_count", C.c_int64, [_P]),
     ("pbg_set_edge_weights", C.c_int, [_P, C.c_void_p]),
     ("pbg_set_profiling", C.c_int, [_P, C.c_int]),

@@ -1,0 +1,247 @@
+"""Token operators on CUDA tensors: rows of a table by id, log probabilities over rows of scores, and their gradients.
+
+They stand on either side of what this package trains: a table of embeddings, and answers that are rows of a table.  The
+reference has no counterpart (it gathers with F.embedding and takes its losses over sampled negatives).  As everywhere
+here the arithmetic runs in libpbg_b200.so and gradients are functions of their own: nothing is recorded for autograd, and a tensor
+that requires a gradient is refused while gradients are being recorded -- detach it, or call under torch.no_grad().
+
+All calls are queued on PyTorch's current stream of the tensors' device and return at once; workspaces come from PyTorch's allocator.
+No call synchronises, so all of them can be captured into a CUDA graph.  Ids and targets are int64.  One outside of its range
+cannot raise: its row of the result is NaN (its part of a gradient is left out), and bit 1 is set in `errors`, an
+int32 tensor of one element, where one is given (`check_errors` reads it and raises).
+
+Types: float32, bfloat16, float16; sums and statistics are float32 and results rounded once."""
+import math
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _lib
+
+IGNORE_INDEX = -100
+MAX_TOP = 32
+
+
+class TokenLogprobs(NamedTuple):
+    """Per row: log probability of the target, entropy, log of the sum of exponentials (float32), rank of the target (1 = best; 0
+    for padding); with top > 0 the best log probabilities [n, top] and their ids."""
+    logprob: torch.Tensor
+    entropy: torch.Tensor
+    lse: torch.Tensor
+    rank: torch.Tensor
+    top_logprobs: Optional[torch.Tensor]
+    top_ids: Optional[torch.Tensor]
+
+
+def _matrix(name, t, dtype=None, device=None):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor")
+    if t.device.type != "cuda":
+        raise RuntimeError(f"{name} is on {t.device}: the token operators work on CUDA tensors only (no CPU fallback)")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    code = _lib.DTYPE_CODES.get(str(t.dtype)[6:])
+    if code is None or (dtype is not None and t.dtype != dtype):
+        raise TypeError(f"{name} has type {t.dtype}" + (f", not {dtype}" if dtype is not None else "; float32, bfloat16 and float16 are supported"))
+    if t.dim() != 2:
+        raise ValueError(f"{name} must have two dimensions")
+    if t.shape[1] < 1:
+        raise ValueError(f"{name} has rows without elements")
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError(f"the elements of a row of {name} must lie next to each other")
+    _no_grad(name, t)
+    return code
+
+
+def _no_grad(name, t):
+    if t.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{name} requires a gradient, which the token operators do not record: detach it or call under torch.no_grad()")
+
+
+def _vector(name, t, dtype, n, device):
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype:
+        raise TypeError(f"{name} must be a tensor of {dtype}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    if t.dim() != 1 or t.shape[0] != n:
+        raise ValueError(f"{name} must have one dimension of {n} elements")
+    _no_grad(name, t)
+    return t.contiguous()
+
+
+def _scale(scale, positive):
+    scale = float(scale)
+    if not math.isfinite(scale) or (positive and not 0.0 < scale < 3.4e38):
+        raise ValueError(f"scale must be {'positive and ' if positive else ''}finite")
+    return scale
+
+
+def _error_word(errors, device):
+    if errors is None:
+        return None
+    if not isinstance(errors, torch.Tensor) or errors.dtype != torch.int32 or errors.numel() != 1:
+        raise TypeError("errors must be an int32 tensor of one element")
+    if errors.device != device:
+        raise ValueError(f"errors is on {errors.device}, not on {device}")
+    return errors.data_ptr()
+
+
+def _row_stride(t):
+    """Elements from row to row (a single row's stride says nothing)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _workspace(size, device):
+    return torch.empty(size, dtype=torch.uint8, device=device)
+
+
+def _overlap(a, b):
+    """Whether the address ranges of two strided matrices meet."""
+    def span(t):
+        first = t.data_ptr()
+        return first, first + (sum((s - 1) * abs(k) for s, k in zip(t.shape, t.stride())) + 1) * t.element_size()
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
+def _call(name, device, *args):
+    """The entry point `name` on the current stream of `device`."""
+    with torch.cuda.device(device):
+        _lib.check(getattr(_lib.lib(), name)(*args, torch.cuda.current_stream(device).cuda_stream))
+
+
+def check_errors(errors: torch.Tensor) -> None:
+    """Raises what the calls that were given `errors` have found so far, and clears it.  Waits for them."""
+    found = int(errors.item())
+    if found:
+        errors.zero_()
+    if found & 2:
+        raise _lib.PbgError(_lib.PBG_ERR_TIMEOUT, "a bounded device-side wait ran out")
+    if found & 1:
+        raise IndexError("an id or target lies outside of its range")
+
+
+def embedding_lookup(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, errors: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """scale * table[ids]: a tensor of the table's type and of shape ids.shape + (dim,).  The table's rows may lie apart (a
+    view of some columns); ids of any shape.  An id outside of the table gives a row of NaN."""
+    code = _matrix("table", table)
+    if not isinstance(ids, torch.Tensor) or ids.dtype != torch.long:
+        raise TypeError("ids must be an int64 tensor")
+    if ids.device != table.device:
+        raise ValueError(f"ids is on {ids.device}, not on {table.device}")
+    rows, dim = table.shape
+    if rows == 0 and ids.numel() > 0:
+        raise ValueError("table has no rows")
+    flat = ids.reshape(-1).contiguous()
+    out = torch.empty((flat.shape[0], dim), dtype=table.dtype, device=table.device)
+    _call("pbg_embedding_lookup", table.device, table.data_ptr(), _row_stride(table), rows, dim, code, flat.data_ptr(), flat.shape[0],
+          _scale(scale, False), out.data_ptr(), _error_word(errors, table.device))
+    return out.view(*ids.shape, dim)
+
+
+def embedding_lookup_grad(grad: torch.Tensor, ids: torch.Tensor, num_rows: int, *, scale: float = 1.0, out: Optional[torch.Tensor] = None,
+                          accumulate: bool = False, errors: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Gradient of embedding_lookup with respect to the table: [num_rows, dim] of grad's type, out[v] = scale * (sum of the
+    rows of `grad` whose id is v).  grad: ids.shape + (dim,), or one row per id.  The rows of an id are added in their
+    order, in float32: the same input gives the same bits.  With `out` the result goes there; accumulate=True adds the sums to what `out` holds
+    and leaves its other rows alone (a table that also serves as the output layer).  An id outside of the table is skipped."""
+    if isinstance(grad, torch.Tensor) and grad.dim() != 2 and isinstance(ids, torch.Tensor) and tuple(grad.shape[:-1]) == tuple(ids.shape):
+        grad = grad.reshape(-1, grad.shape[-1])
+    code = _matrix("grad", grad)
+    if not isinstance(ids, torch.Tensor) or ids.dtype != torch.long:
+        raise TypeError("ids must be an int64 tensor")
+    n, dim = grad.shape
+    flat = _vector("ids", ids.reshape(-1), torch.long, n, grad.device)
+    num_rows = int(num_rows)
+    if num_rows < 1:
+        raise ValueError("num_rows must be positive")
+    if accumulate and out is None:
+        raise ValueError("accumulate=True adds to `out`, which is missing")
+    if out is None:
+        out = torch.empty((num_rows, dim), dtype=grad.dtype, device=grad.device)
+    else:
+        _matrix("out", out, grad.dtype, grad.device)
+        if tuple(out.shape) != (num_rows, dim):
+            raise ValueError(f"out has shape {tuple(out.shape)}, not {(num_rows, dim)}")
+        if num_rows > 1 and out.stride(0) < dim:
+            raise ValueError("the rows of out overlap")
+        if _overlap(out, grad):
+            raise ValueError("out and grad share memory")
+    L = _lib.lib()
+    size = L.pbg_embedding_lookup_grad_workspace(n, num_rows, dim)
+    ws = _workspace(size, grad.device)
+    _call("pbg_embedding_lookup_grad", grad.device, grad.data_ptr(), _row_stride(grad), flat.data_ptr(), n, num_rows, dim, code,
+          _scale(scale, False), out.data_ptr(), _row_stride(out), int(bool(accumulate)), ws.data_ptr(), size, _error_word(errors, grad.device))
+    return out
+
+
+def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, scale: float = 1.0, top: int = 0, ignore_index: int = IGNORE_INDEX,
+                   errors: Optional[torch.Tensor] = None) -> TokenLogprobs:
+    """Log probabilities of `targets` [n] under softmax(scale * logits) of rows [n, vocab], with each row's entropy, log of the sum,
+    the target's rank (scores in front of it: larger ones, and equal ones with a smaller id; 1 = best) and, with top > 0
+    (at most 32), the best alternatives in order.  scale is the inverse temperature.  Rows may lie apart (a padded vocabulary).
+
+    A row whose target is ignore_index is padding: it is not read, its results are 0 (top_ids -1).  A row of -inf alone has log
+    probabilities -inf and entropy 0; NaN or +inf in a row makes its log probabilities NaN; in the order of `top` NaN counts as -inf."""
+    code = _matrix("logits", logits)
+    n, vocab = logits.shape
+    targets = _vector("targets", targets, torch.long, n, logits.device)
+    top = int(top)
+    if not 0 <= top <= min(MAX_TOP, vocab):
+        raise ValueError(f"top must lie between 0 and {min(MAX_TOP, vocab)}")
+    f32 = lambda *shape: torch.empty(shape, dtype=torch.float32, device=logits.device)  # noqa: E731
+    i64 = lambda *shape: torch.empty(shape, dtype=torch.long, device=logits.device)  # noqa: E731
+    r = TokenLogprobs(f32(n), f32(n), f32(n), i64(n), f32(n, top) if top else None, i64(n, top) if top else None)
+    _call("pbg_token_logprobs", logits.device, logits.data_ptr(), _row_stride(logits), n, vocab, code, targets.data_ptr(), int(ignore_index),
+          _scale(scale, True), top, r.logprob.data_ptr(), r.entropy.data_ptr(), r.lse.data_ptr(), r.rank.data_ptr(),
+          r.top_logprobs.data_ptr() if top else None, r.top_ids.data_ptr() if top else None, _error_word(errors, logits.device))
+    return r
+
+
+def _row_grads(n, device, lse, entropy, grad_logprob, grad_entropy):
+    """The statistics and gradients of a forward call's rows, checked."""
+    if grad_logprob is None and grad_entropy is None:
+        raise ValueError("neither grad_logprob nor grad_entropy is given")
+    lse = _vector("lse", lse, torch.float32, n, device)
+    if grad_entropy is not None:
+        if entropy is None:
+            raise ValueError("the gradient of the entropy needs the entropy")
+        grad_entropy = _vector("grad_entropy", grad_entropy, torch.float32, n, device)
+        entropy = _vector("entropy", entropy, torch.float32, n, device)
+    if grad_logprob is not None:
+        grad_logprob = _vector("grad_logprob", grad_logprob, torch.float32, n, device)
+    return lse, entropy, grad_logprob, grad_entropy
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def token_logprobs_grad(logits: torch.Tensor, targets: torch.Tensor, lse: torch.Tensor, entropy: Optional[torch.Tensor],
+                        grad_logprob: Optional[torch.Tensor], grad_entropy: Optional[torch.Tensor] = None, *, scale: float = 1.0,
+                        ignore_index: int = IGNORE_INDEX, out: Optional[torch.Tensor] = None, errors: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Gradient with respect to the logits of sum(grad_logprob * logprob + grad_entropy * entropy), from the lse and the entropy that
+    token_logprobs returned (the entropy only where grad_entropy is given).  `out` may be `logits` itself: the gradient then takes the scores'
+    place.  Rows of padding, rows whose target is out of range and rows of -inf alone get zeros."""
+    code = _matrix("logits", logits)
+    n, vocab = logits.shape
+    targets = _vector("targets", targets, torch.long, n, logits.device)
+    lse, entropy, grad_logprob, grad_entropy = _row_grads(n, logits.device, lse, entropy, grad_logprob, grad_entropy)
+    if out is None:
+        # rows as far apart as those of the scores, so that both lie alike against 16 bytes
+        stride = max(_row_stride(logits), vocab)
+        out = torch.empty_strided((n, vocab), (stride if stride < vocab + 4096 else vocab, 1), dtype=logits.dtype, device=logits.device)
+    else:
+        _matrix("out", out, logits.dtype, logits.device)
+        if out.shape != logits.shape:
+            raise ValueError(f"out has shape {tuple(out.shape)}, not {tuple(logits.shape)}")
+        if n > 1 and out.stride(0) < vocab:
+            raise ValueError("the rows of out overlap")
+        if _overlap(out, logits) and (out.data_ptr() != logits.data_ptr() or _row_stride(out) != _row_stride(logits)):
+            raise ValueError("out shares memory with logits without being them")
+    _call("pbg_token_logprobs_grad", logits.device, logits.data_ptr(), _row_stride(logits), n, vocab, code, targets.data_ptr(), int(ignore_index),
+          _scale(scale, True), lse.data_ptr(), _ptr(entropy), _ptr(grad_logprob), _ptr(grad_entropy), out.data_ptr(), _row_stride(out),
+          _error_word(errors, logits.device))
+    return out

@@ -1,0 +1,353 @@
+"""The token operators against their definitions in 64 bits: rows by id and their gradient, log probabilities over rows of scores
+and their gradient.
+
+Tolerances: a result is rounded to its type once, by at most half a step, finfo.eps / 2 of its value.  What comes before is fp32:
+  - a sum of c terms is off by at most (c - 1) 2^-24 of the sum of the terms' sizes;
+  - log probabilities, entropy and lse: an exponential 2^y, |y| <= 150 where it counts, with y off by 3 roundings and ex2 by 2 ulp, is
+    relatively off by at most 150 * 3 * 2^-24 + 2^-22 < 3e-5, which only scores 100 below the largest reach; those within 20 of it,
+    which make up the sums, stay below 6e-6.  S and T carry that and the sums' own roundings, thread by thread and joined
+    (below 600 terms each and a tree of 11: 4e-5 at the worst of all signs, a hundredth of that in the mean); 2e-5 is used, relative to
+    1 + |lse| (the larger of what is subtracted) resp. 1 + |entropy| + log S."""
+import math
+
+import pytest
+import torch
+
+import torchbiggraph_b200 as T
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+DEV = "cuda"
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def f32(scale):
+    """A scale as the entry points take it, in single precision: 1.3 is another number there."""
+    return float(torch.tensor(scale, dtype=torch.float32))
+
+
+def half_step(t):
+    return torch.finfo(t).eps / 2
+
+
+def close(got, want, rel, scale, floor=0.0):
+    """|got - want| <= rel * scale + floor everywhere, NaN and infinities in the same places."""
+    got, want = got.double(), want.double()
+    assert torch.equal(got.isnan(), want.isnan())
+    inf = want.isinf()
+    assert torch.equal(got[inf], want[inf])
+    ok = want.isfinite()
+    err = ((got - want).abs() - (rel * (scale if torch.is_tensor(scale) else torch.full_like(want, scale)) + floor))[ok]
+    assert err.numel() == 0 or err.max().item() <= 0, err.max().item()
+
+
+# ------------------------------------------------------------------------------------------------ lookup
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,rows,dim", [(1, 1, 1), (3, 7, 2), (5, 100, 37), (64, 50, 100), (33, 1000, 400), (700, 300, 1026), (9, 10, 4096), (2, 3, 65_536),
+                                        (3000, 5000, 256)])
+def test_lookup(dtype, n, rows, dim):
+    g = gen(n + dim)
+    table = torch.randn(rows, dim, device=DEV, generator=g).to(dtype)
+    ids = torch.randint(0, rows, (n,), device=DEV, generator=g)
+    close(T.embedding_lookup(table, ids, scale=1.7), table.double()[ids] * 1.7, half_step(dtype) + 2 ** -23, (table.double()[ids] * 1.7).abs(),
+          floor=torch.finfo(dtype).smallest_normal)
+    assert torch.equal(T.embedding_lookup(table, ids), table[ids])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("stride,first", [(40, 0), (41, 0), (40, 1), (48, 3)])
+def test_lookup_of_a_strided_table(dtype, stride, first):
+    g = gen(stride)
+    table = torch.randn(50, stride, device=DEV, generator=g).to(dtype)[:, first:first + 36]
+    ids = torch.randint(0, 50, (4, 5), device=DEV, generator=g)
+    got = T.embedding_lookup(table, ids)
+    assert got.shape == (4, 5, 36) and torch.equal(got, table[ids])
+    assert torch.equal(T.embedding_lookup(table, ids.t()), table[ids.t()])
+    assert T.embedding_lookup(table, ids[:0]).shape == (0, 5, 36)
+
+
+def test_lookup_reports_ids_outside_of_the_table():
+    table = torch.randn(10, 8, device=DEV)
+    errors = torch.zeros(1, dtype=torch.int32, device=DEV)
+    got = T.embedding_lookup(table, torch.tensor([3, -1, 10, 2 ** 40, 0], device=DEV), errors=errors)
+    assert torch.equal(got[[0, 4]], table[[3, 0]]) and got[1:4].isnan().all()
+    with pytest.raises(IndexError):
+        T.check_errors(errors)
+    T.check_errors(errors)
+    assert T.embedding_lookup(table, torch.tensor([11], device=DEV)).isnan().all()          # (without an error word as well)
+
+
+def _grad_want(grad, ids, rows, scale):
+    out = torch.zeros(rows, grad.shape[1], dtype=torch.float64, device=DEV)
+    ok = (ids >= 0) & (ids < rows)
+    out.index_add_(0, ids[ok], grad.double()[ok])
+    size = torch.zeros_like(out).index_add_(0, ids[ok], grad.double()[ok].abs())
+    return out * scale, size * abs(scale)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,rows,dim,kind", [(1, 1, 1, "any"), (1, 500, 33, "any"), (16, 4, 8, "any"), (17, 4, 8, "one"), (33, 3, 100, "few"), (1000, 7, 400, "few"),
+                                             (4096, 3000, 130, "any"), (5000, 2000, 1, "one"), (2500, 100_003, 24, "few"), (20_001, 4000, 64, "any"),
+                                             (300_000, 1000, 4, "any"), (263_000, 70_000, 8, "one")])
+def test_lookup_grad(dtype, n, rows, dim, kind):
+    g = gen(n + dim)
+    ids = torch.randint(0, rows, (n,), device=DEV, generator=g)
+    if kind == "one":
+        ids.fill_(rows - 1)
+    elif kind == "few":
+        ids = torch.where(torch.rand(n, device=DEV, generator=g) < 0.8, ids % 3 % rows, ids)
+    grad = torch.randn(n, dim, device=DEV, generator=g).to(dtype)
+    want, size = _grad_want(grad, ids, rows, 0.5)
+    most = int(torch.bincount(ids).max())
+    rel = (most + 4) * 2 ** -24
+    got = T.embedding_lookup_grad(grad, ids, rows, scale=0.5)
+    close(got, want, 1.0, half_step(dtype) * want.abs() + rel * size, floor=torch.finfo(dtype).smallest_normal)
+    assert torch.equal(got, T.embedding_lookup_grad(grad, ids, rows, scale=0.5))             # the same bits again
+    # added to what is there: rows without an id keep their bits
+    base = torch.randn(rows, dim, device=DEV, generator=g).to(dtype)
+    got = T.embedding_lookup_grad(grad, ids, rows, scale=0.5, out=base.clone(), accumulate=True)
+    close(got, base.double() + want, 1.0, half_step(dtype) * (base.double() + want).abs() + rel * size + 2 ** -24 * base.double().abs(), floor=torch.finfo(dtype).smallest_normal)
+    empty = torch.ones(rows, dtype=torch.bool, device=DEV)
+    empty[ids] = False
+    assert torch.equal(got[empty], base[empty])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_lookup_grad_strides_and_bad_ids(dtype):
+    g = gen(5)
+    wide = torch.randn(40, 61, device=DEV, generator=g).to(dtype)
+    for first, dim in ((0, 56), (1, 48), (3, 33)):
+        grad = wide[:, first:first + dim]
+        ids = torch.randint(0, 9, (40,), device=DEV, generator=g)
+        ids[[3, 17, 39]] = torch.tensor([-5, 9, 2 ** 50], device=DEV)
+        room = torch.full((9, 70), 7.0, device=DEV, dtype=dtype)
+        errors = torch.zeros(1, dtype=torch.int32, device=DEV)
+        out = T.embedding_lookup_grad(grad, ids, 9, out=room[:, 2:2 + dim], errors=errors)
+        want, size = _grad_want(grad, ids, 9, 1.0)
+        close(out, want, 1.0, half_step(dtype) * want.abs() + 44 * 2 ** -24 * size)
+        assert (room[:, :2] == 7).all() and (room[:, 2 + dim:] == 7).all() and errors.item() == 1
+    assert (T.embedding_lookup_grad(wide[:0], torch.empty(0, dtype=torch.long, device=DEV), 4) == 0).all()
+    one = T.embedding_lookup_grad(wide.view(8, 5, 61), torch.zeros(8, 5, dtype=torch.long, device=DEV), 1)
+    assert one.shape == (1, 61)
+
+
+def test_lookup_gradient_is_the_slope_of_the_lookup():
+    """<W + d, .> differences: the lookup is linear in the table, so one step of any size gives the slope."""
+    g = gen(1)
+    ids = torch.randint(0, 30, (100,), device=DEV, generator=g)
+    out_grad = torch.randn(100, 20, device=DEV, generator=g)
+    W, d = torch.randn(30, 20, device=DEV, generator=g), torch.randn(30, 20, device=DEV, generator=g)
+    dW = T.embedding_lookup_grad(out_grad, ids, 30, scale=3.0).double()
+    slope = ((T.embedding_lookup(W + d, ids, scale=3.0).double() - T.embedding_lookup(W, ids, scale=3.0).double()) * out_grad.double()).sum()
+    assert abs((dW * d.double()).sum() - slope).item() < 2000 * 20 * 2 ** -22
+
+
+# --------------------------------------------------------------------------------------------- log probabilities
+def _scores(n, vocab, dtype, seed, kind="plain", pad=0):
+    g = gen(seed)
+    x = torch.randn(n, vocab + pad, device=DEV, generator=g) * 3
+    if kind == "ties":
+        x = x.round()
+    if kind == "sharp":
+        x[torch.arange(n), torch.randint(0, vocab, (n,), device=DEV, generator=g)] += 30
+    if kind == "masked":
+        x[torch.rand(n, vocab + pad, device=DEV, generator=g) < 0.7] = -math.inf
+        x[0] = -math.inf
+        if n > 1:
+            x[1] = torch.finfo(dtype).min
+        if n > 2:
+            x[2] = torch.finfo(dtype).min
+            x[2, vocab // 2] = 1.0
+        if n > 3:
+            x[3, :-1] = -math.inf
+    return x.to(dtype)[:, :vocab]
+
+
+def _want(x, targets, scale, top):
+    z = x.double() * f32(scale)
+    m = z.amax(1)
+    # (against the maximum first: next to a row of the type's lowest value, log 2 is lost in 64 bits too)
+    d = z - torch.where(m == -math.inf, 0.0, m)[:, None]
+    log_sum = torch.logsumexp(d, 1)
+    lse, logp = m + torch.where(m == -math.inf, 0.0, log_sum), d - log_sum[:, None]
+    logp[lse == -math.inf] = -math.inf
+    ent = torch.special.entr(logp.exp()).sum(1)
+    real = targets >= 0
+    t = targets.clamp(min=0)[:, None]
+    mine = x.gather(1, t)
+    ids = torch.arange(x.shape[1], device=DEV)
+    rank = 1 + ((x > mine) | ((x == mine) & (ids < t))).sum(1)
+    order = torch.sort(torch.where(x.isnan(), -math.inf, x.float()), dim=1, descending=True, stable=True).indices[:, :top]
+    z0 = lambda v, pad=0: torch.where(real if v.dim() == 1 else real[:, None], v, pad)  # noqa: E731
+    return z0(logp.gather(1, t)[:, 0]), z0(ent), z0(lse), z0(rank), z0(logp.gather(1, order)), z0(order, -1)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kind", ["plain", "ties", "sharp", "masked"])
+@pytest.mark.parametrize("n,vocab,pad,top", [(1, 1, 0, 1), (4, 2, 0, 2), (5, 31, 0, 31), (7, 33, 6, 32), (6, 1000, 0, 0), (9, 1025, 0, 5), (3, 14_951, 57, 20), (300, 2048, 0, 8),
+                                             (2, 131_072, 0, 20), (1, 70_001, 3, 32), (700, 517, 0, 1)])
+def test_logprobs(dtype, kind, n, vocab, pad, top):
+    x = _scores(n, vocab, dtype, n + vocab, kind, pad)
+    targets = torch.randint(0, vocab, (n,), device=DEV, generator=gen(vocab))
+    if n > 5:
+        targets[5] = -100
+    r = T.token_logprobs(x, targets, scale=0.8, top=top)
+    logprob, ent, lse, rank, best, ids = _want(x, targets, 0.8, top)
+    size = 1 + torch.where(lse.isfinite(), lse.abs(), 1.0)
+    close(r.lse, lse, 2e-5, size)
+    close(r.logprob, logprob, 2e-5, size + torch.where(logprob.isfinite(), logprob.abs(), 0.0))
+    close(r.entropy, ent, 2e-5, 1 + ent + math.log(vocab))
+    assert torch.equal(r.rank, rank)
+    if top:
+        assert torch.equal(r.top_ids, ids)
+        close(r.top_logprobs, best, 2e-5, size[:, None] + torch.where(best.isfinite(), best.abs(), 0.0))
+    else:
+        assert r.top_ids is None and r.top_logprobs is None
+
+
+def test_logprobs_of_rows_of_equal_scores_keep_the_order_of_ids():
+    for vocab in (64, 5000, 131_073):
+        for value in (0.0, -3.0, -math.inf):
+            x = torch.full((3, vocab), value, device=DEV, dtype=torch.bfloat16)
+            x[1, ::2] = -x[1, ::2] if value == 0.0 else x[1, ::2]              # -0 and 0 are equal
+            r = T.token_logprobs(x, torch.tensor([0, vocab - 1, vocab // 2], device=DEV), top=32)
+            assert torch.equal(r.top_ids, torch.arange(32, device=DEV).expand(3, 32))
+            assert r.rank.tolist() == [1, vocab, vocab // 2 + 1]
+
+
+def test_logprobs_with_nan_infinity_and_bad_targets():
+    x = torch.randn(6, 3000, device=DEV, generator=gen(2))
+    x[0, 5], x[1, 7], x[2, 2999] = math.nan, math.inf, math.nan
+    targets = torch.tensor([1, 2, 3, 3000, -7, -100], device=DEV)
+    errors = torch.zeros(1, dtype=torch.int32, device=DEV)
+    r = T.token_logprobs(x, targets, top=4, errors=errors)
+    assert r.logprob[:5].isnan().all() and r.lse[:3].isnan().all() and r.entropy[:3].isnan().all()
+    assert r.lse[3:5].isfinite().all() and r.rank[3:].tolist() == [0, 0, 0] and errors.item() == 1
+    order = torch.sort(torch.where(x.isnan(), -math.inf, x), dim=1, descending=True, stable=True).indices[:, :4]
+    assert torch.equal(r.top_ids[:5], order[:5]) and (r.top_ids[5] == -1).all() and r.logprob[5] == 0
+
+
+def _want_grad(x, targets, scale, lse, ent, g, h):
+    keep = (targets >= 0) & (targets < x.shape[1])
+    lse, ent = lse.double(), ent.double()
+    scale = f32(scale)
+    logp = x.double() * scale - lse[:, None]
+    p = logp.exp()
+    w = -p
+    w[torch.arange(len(x)), targets.clamp(0, x.shape[1] - 1)] += 1.0
+    size = p.clone()
+    size[torch.arange(len(x)), targets.clamp(0, x.shape[1] - 1)] += 1.0
+    plogp = torch.special.entr(p)
+    out = g.double()[:, None] * w + h.double()[:, None] * (plogp - p * ent[:, None])
+    size = g.double().abs()[:, None] * size + h.double().abs()[:, None] * (plogp.abs() + p * ent.abs()[:, None])
+    dead = ~keep | (lse == -math.inf)
+    out[dead] = 0.0
+    size[dead] = 0.0
+    return out * scale, size * scale
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kind", ["plain", "masked", "sharp"])
+@pytest.mark.parametrize("n,vocab,pad,out", [(1, 1, 0, None), (5, 31, 0, None), (6, 1000, 24, None), (9, 1025, 0, "other"), (8, 14_951, 57, None), (7, 14_951, 0, "self"),
+                                             (3, 70_001, 3, "other"), (200, 4096, 0, "self")])
+def test_logprobs_grad(dtype, kind, n, vocab, pad, out):
+    x = _scores(n, vocab, dtype, n + vocab, kind, pad)
+    targets = torch.randint(0, vocab, (n,), device=DEV, generator=gen(vocab))
+    if n > 5:
+        targets[5] = -100
+    if n > 7:
+        targets[7] = vocab
+    errors = torch.zeros(1, dtype=torch.int32, device=DEV)
+    f = T.token_logprobs(x, targets, scale=1.3)
+    g, h = torch.randn(n, device=DEV, generator=gen(3)), torch.randn(n, device=DEV, generator=gen(4))
+    want, size = _want_grad(x, targets, 1.3, f.lse, f.entropy, g, h)
+    # p is off by at most |log p| * 4 * 2^-24 + 2^-21 relatively: below 2e-5 where log p > -60, and nothing elsewhere
+    tol = half_step(dtype) * want.abs() + 2e-5 * size
+    floor = torch.finfo(dtype).smallest_normal
+    room = {None: None, "self": x.clone(), "other": torch.empty(n, vocab + 5, dtype=dtype, device=DEV)[:, 1:1 + vocab]}[out]
+    src = room if out == "self" else x
+    got = T.token_logprobs_grad(src, targets, f.lse, f.entropy, g, h, scale=1.3, out=room, errors=errors)
+    close(got, want, 1.0, tol, floor)
+    assert errors.item() == (1 if n > 7 else 0)
+    if out is None:
+        want, size = _want_grad(x, targets, 1.3, f.lse, f.entropy, g, torch.zeros_like(h))
+        close(T.token_logprobs_grad(x, targets, f.lse, None, g, scale=1.3), want, 1.0, half_step(dtype) * want.abs() + 2e-5 * size, floor)
+        want, size = _want_grad(x, targets, 1.3, f.lse, f.entropy, torch.zeros_like(g), h)
+        close(T.token_logprobs_grad(x, targets, f.lse, f.entropy, None, h, scale=1.3), want, 1.0, half_step(dtype) * want.abs() + 2e-5 * size, floor)
+
+
+def test_logprobs_gradient_is_the_slope():
+    """Central differences of the 64-bit definition with step e: off by e^2 / 6 of a third derivative below 2, and by what fp32 makes
+    of the gradient itself."""
+    x = torch.randn(4, 50, device=DEV, generator=gen(1))
+    targets = torch.tensor([3, 0, 49, 20], device=DEV)
+    g, h = torch.randn(4, device=DEV, generator=gen(3)), torch.randn(4, device=DEV, generator=gen(4))
+    f = T.token_logprobs(x, targets)
+    got = T.token_logprobs_grad(x, targets, f.lse, f.entropy, g, h).double()
+
+    def value(v):
+        logp = torch.log_softmax(v, 1)
+        return (g.double() * logp.gather(1, targets[:, None])[:, 0] + h.double() * torch.special.entr(logp.exp()).sum(1)).sum()
+    for seed in range(5):
+        d = torch.randn(4, 50, device=DEV, generator=gen(10 + seed)).double()
+        e = 1e-4
+        slope = (value(x.double() + e * d) - value(x.double() - e * d)) / (2 * e)
+        assert abs((got * d).sum() - slope).item() < 200 * 2e-5
+
+
+# ------------------------------------------------------------------------------------- streams, graphs, large offsets
+def test_on_a_side_stream_and_in_a_graph():
+    g = gen(9)
+    table = torch.randn(1000, 64, device=DEV, generator=g)
+    ids = torch.randint(0, 1000, (300,), device=DEV, generator=g)
+    targets = torch.randint(0, 1000, (300,), device=DEV, generator=g)
+
+    def chain():
+        rows = T.embedding_lookup(table, ids, scale=2.0)
+        logits = rows @ table.t()
+        f = T.token_logprobs(logits, targets, top=3)
+        dx = T.token_logprobs_grad(logits, targets, f.lse, f.entropy, torch.ones_like(f.lse), f.entropy)
+        return f.logprob, f.top_ids, T.embedding_lookup_grad(dx @ table, ids, 1000, scale=2.0)
+    want = [t.clone() for t in chain()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = chain()
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graphs, outs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(chain())
+        graphs.append(graph)
+    targets.add_(1).remainder_(1000)
+    want = [t.clone() for t in chain()]
+    for graph in graphs + graphs:
+        graph.replay()
+    torch.cuda.synchronize()
+    for out in outs:
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_offsets_beyond_32_bits():
+    rows, dim = 2_200_000, 1024                      # 2.25e9 elements
+    table = torch.empty(rows, dim, dtype=torch.bfloat16, device=DEV)
+    table[-3:] = torch.randn(3, dim, device=DEV, generator=gen(1)).to(torch.bfloat16)
+    ids = torch.tensor([rows - 1, rows - 3, rows - 1], device=DEV)
+    assert torch.equal(T.embedding_lookup(table, ids), table[ids])
+    grad = torch.randn(3, dim, device=DEV, generator=gen(2)).to(torch.bfloat16)
+    out = T.embedding_lookup_grad(grad, ids, rows, out=table)
+    assert torch.equal(out[-3], grad[1]) and (out[:-3:100_000] == 0).all() and (out[-2] == 0).all()
+    close(out[-1], grad[0].double() + grad[2].double(), 2 ** -8, (grad[0].double() + grad[2].double()).abs(), 2 ** -20)
+    logits = table.view(-1)[: 2200 * 1_024_000].view(2200, 1_024_000)
+    logits[-1].normal_()
+    targets = torch.full((2200,), -100, device=DEV)
+    targets[-1] = 77
+    r = T.token_logprobs(logits, targets, top=2)
+    assert r.top_ids[-1, 0] == logits[-1].float().argmax()
+    d = T.token_logprobs_grad(logits, targets, r.lse, None, torch.ones(2200, device=DEV), out=logits)
+    assert abs(d[-1].float().sum().item()) < 1024 * 1000 * 2 ** -9 * 1e-3 and (d[-2] == 0).all()

@@ -1,0 +1,112 @@
+"""What the token operators refuse, on the CPU: tensors on another device than a GPU, wrong types and shapes in the Python
+functions, and bad arguments at the C entry points, which return before they touch the device."""
+import pytest
+import torch
+
+import torchbiggraph_b200 as T
+from torchbiggraph_b200 import _lib
+
+BAD, LARGE = _lib.PBG_ERR_BAD_ARGUMENT, _lib.PBG_ERR_TOO_LARGE
+P = 4096            # an address that is never read
+
+
+def test_python_refuses_cpu_tensors():
+    x, ids = torch.zeros(3, 4), torch.zeros(3, dtype=torch.long)
+    for call in (lambda: T.embedding_lookup(x, ids), lambda: T.embedding_lookup_grad(x, ids, 5), lambda: T.token_logprobs(x, ids),
+                 lambda: T.token_logprobs_grad(x, ids, x[:, 0], None, x[:, 0])):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            call()
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(table=None), BAD), (dict(ids=None), BAD), (dict(out=None), BAD), (dict(dim=0), BAD), (dict(dim=65_537), LARGE), (dict(rows=-1), BAD), (dict(rows=0), BAD),
+    (dict(rows=2 ** 31), LARGE), (dict(n=-1), BAD), (dict(n=2 ** 31), LARGE), (dict(dtype=3), BAD), (dict(dtype=-1), BAD), (dict(stride=-4), BAD), (dict(scale=float("nan")), BAD)])
+def test_lookup_arguments(change, status):
+    a = dict(table=P, stride=8, rows=10, dim=8, dtype=0, ids=P, n=4, scale=1.0, out=P)
+    a.update(change)
+    assert _lib.lib().pbg_embedding_lookup(*a.values(), None, None) == status
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(grad=None), BAD), (dict(ids=None), BAD), (dict(out=None), BAD), (dict(ws=None), BAD), (dict(ws=P + 16), BAD), (dict(size=10), BAD), (dict(dim=0), BAD),
+    (dict(dim=65_537, out_stride=65_537), LARGE), (dict(rows=0), BAD), (dict(n=-1), BAD), (dict(n=2 ** 30 + 1), LARGE), (dict(dtype=5), BAD), (dict(out_stride=7), BAD), (dict(stride=-1), BAD)])
+def test_lookup_grad_arguments(change, status):
+    L = _lib.lib()
+    a = dict(grad=P, stride=8, ids=P, n=40, rows=10, dim=8, dtype=1, scale=1.0, out=P, out_stride=8, accumulate=0, ws=P, size=L.pbg_embedding_lookup_grad_workspace(40, 10, 8))
+    a.update(change)
+    assert L.pbg_embedding_lookup_grad(*a.values(), None, None) == status
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(logits=None), BAD), (dict(targets=None), BAD), (dict(lse=None), BAD), (dict(rank=None), BAD), (dict(vocab=0), BAD), (dict(vocab=2 ** 31), LARGE), (dict(n=-1), BAD),
+    (dict(n=2 ** 31), LARGE), (dict(dtype=3), BAD), (dict(scale=0.0), BAD), (dict(scale=-1.0), BAD), (dict(scale=float("inf")), BAD), (dict(scale=float("nan")), BAD),
+    (dict(top=-1), BAD), (dict(top=101), BAD), (dict(top=33), LARGE), (dict(top=2, top_ids=None), BAD), (dict(stride=-1), BAD)])
+def test_logprobs_arguments(change, status):
+    a = dict(logits=P, stride=100, n=4, vocab=100, dtype=0, targets=P, ignore=-100, scale=1.0, top=0, logprob=P, entropy=P, lse=P, rank=P, top_logprobs=P, top_ids=P)
+    a.update(change)
+    assert _lib.lib().pbg_token_logprobs(*a.values(), None, None) == status
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(logits=None), BAD), (dict(targets=None), BAD), (dict(lse=None), BAD), (dict(entropy=None), BAD), (dict(out=None), BAD), (dict(vocab=0), BAD), (dict(n=-1), BAD),
+    (dict(out_stride=99), BAD), (dict(dtype=9), BAD), (dict(scale=0.0), BAD), (dict(vocab=2 ** 31, out_stride=2 ** 31), LARGE), (dict(n=2 ** 31), LARGE)])
+def test_logprobs_grad_arguments(change, status):
+    a = dict(logits=P, stride=100, n=4, vocab=100, dtype=0, targets=P, ignore=-100, scale=1.0, lse=P, entropy=P, g=P, h=P, out=P, out_stride=100)
+    a.update(change)
+    assert _lib.lib().pbg_token_logprobs_grad(*a.values(), None, None) == status
+
+
+def test_nothing_to_do_is_no_error():
+    L = _lib.lib()
+    assert L.pbg_embedding_lookup(None, 8, 0, 8, 0, None, 0, 1.0, None, None, None) == 0
+    assert L.pbg_token_logprobs(None, 8, 0, 8, 0, None, -100, 1.0, 0, *[None] * 8) == 0
+    assert L.pbg_token_logprobs_grad(None, 8, 0, 8, 0, None, -100, 1.0, None, None, None, None, None, 8, None, None) == 0
+    assert L.pbg_embedding_lookup_grad_workspace(0, 10, 8) == 0
+
+
+@pytest.mark.gpu
+def test_python_refuses_what_does_not_fit():
+    x, ids, f = torch.zeros(6, 8, device="cuda"), torch.zeros(6, dtype=torch.long, device="cuda"), torch.zeros(6, device="cuda")
+    with pytest.raises(TypeError):
+        T.embedding_lookup(x.double(), ids)
+    with pytest.raises(TypeError):
+        T.embedding_lookup(x, ids.int())
+    with pytest.raises(ValueError):
+        T.embedding_lookup(x, ids.cpu())
+    with pytest.raises(ValueError):
+        T.embedding_lookup(x[:0], ids)
+    with pytest.raises(ValueError):
+        T.embedding_lookup(x.t(), ids)
+    with pytest.raises(ValueError):
+        T.embedding_lookup(x, ids, scale=float("nan"))
+    with pytest.raises(RuntimeError, match="gradient"):
+        T.embedding_lookup(x.clone().requires_grad_(), ids)
+    with torch.no_grad():
+        T.embedding_lookup(x.clone().requires_grad_(), ids)
+    with pytest.raises(ValueError):
+        T.embedding_lookup_grad(x, ids[:5], 4)
+    with pytest.raises(ValueError):
+        T.embedding_lookup_grad(x, ids, 0)
+    with pytest.raises(ValueError):
+        T.embedding_lookup_grad(x, ids, 4, accumulate=True)
+    with pytest.raises(ValueError, match="share"):
+        T.embedding_lookup_grad(x, ids, 6, out=x)
+    with pytest.raises(TypeError):
+        T.embedding_lookup_grad(x, ids, 4, out=torch.zeros(4, 8, device="cuda", dtype=torch.half))
+    with pytest.raises(ValueError):
+        T.embedding_lookup_grad(x, ids, 4, out=torch.zeros(1, 8, device="cuda").expand(4, 8))
+    for kw in (dict(top=9), dict(top=-1), dict(scale=0.0), dict(scale=-2.0)):
+        with pytest.raises(ValueError):
+            T.token_logprobs(x, ids, **kw)
+    with pytest.raises(TypeError):
+        T.token_logprobs(x, ids, errors=f[:1])
+    with pytest.raises(ValueError):
+        T.token_logprobs_grad(x, ids, f, None, None)
+    with pytest.raises(ValueError):
+        T.token_logprobs_grad(x, ids, f, None, f, f)
+    with pytest.raises(TypeError):
+        T.token_logprobs_grad(x, ids, f.double(), None, f)
+    with pytest.raises(ValueError, match="shares"):
+        T.token_logprobs_grad(x[:4], ids[:4], f[:4], None, f[:4], out=x[2:])
+    assert T.token_logprobs(x[:0], ids[:0], top=3).top_ids.shape == (0, 3)
+    assert T.token_logprobs_grad(x[:0], ids[:0], f[:0], None, f[:0]).shape == (0, 8)

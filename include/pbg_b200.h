@@ -332,6 +332,26 @@ int pbg_token_logprobs_grad(const void *logits, int64_t row_stride, int64_t n, i
                             const float *grad_logprob, const float *grad_entropy, void *out, int64_t out_stride,
                             int32_t *errors, void *stream);
 
+/* The same statistics with z = scale * queries . table^T, which is never stored: queries [n, dim], table [rows, dim], targets rows of the
+ * table.  16-bit operands are multiplied as they are; fp32 ones as two fp16 planes each (22 bits), at fp32's accuracy
+ * for elements down to 2^-17 of the largest, and an absolute one of 2^-39 of it below.  workspace: of
+ * pbg_table_logprobs_workspace(n, rows, dim, dtype, 0) bytes. */
+int64_t pbg_table_logprobs_workspace(int64_t n, int64_t rows, int32_t dim, int32_t dtype, int32_t grad);
+int pbg_table_logprobs(const void *queries, int64_t q_stride, int64_t n, const void *table, int64_t t_stride, int64_t rows,
+                       int32_t dim, int32_t dtype, const int64_t *targets, int64_t ignore_index, float scale,
+                       float *logprob, float *entropy, float *lse, void *workspace, int64_t workspace_bytes,
+                       int32_t *errors, void *stream);
+
+/* Gradients of sum(grad_logprob * logprob + grad_entropy * entropy) with respect to the queries [n, dim] and the table [rows, dim],
+ * rows one behind the other, of their type; either may be NULL (not wanted).  lse, entropy: of the forward call.  The scores are
+ * computed again; their gradient is rounded to the operands' type (fp32: two fp16 planes) for the two products.
+ * workspace: of pbg_table_logprobs_workspace(n, rows, dim, dtype, 1) bytes, at most about 2 GiB beside copies of the operands. */
+int pbg_table_logprobs_grad(const void *queries, int64_t q_stride, int64_t n, const void *table, int64_t t_stride, int64_t rows,
+                            int32_t dim, int32_t dtype, const int64_t *targets, int64_t ignore_index, float scale,
+                            const float *lse, const float *entropy, const float *grad_logprob, const float *grad_entropy,
+                            void *grad_queries, void *grad_table, void *workspace, int64_t workspace_bytes,
+                            int32_t *errors, void *stream);
+
 /* Kernel launches issued by this context since creation (for launch accounting). */
 int64_t pbg_launch_count(const pbg_context *ctx);
 

@@ -7,7 +7,8 @@ from .model import MultiRelationEmbedder, Scores, make_model
 from .plugin import PluginRegistry
 from .registries import COMPARATORS, DYNAMIC_OPERATORS, LOSS_FUNCTIONS, OPERATORS
 from .row_adagrad import AsyncAdagrad, RowAdagrad, make_optimizer
-from .tokens import TokenLogprobs, check_errors, embedding_lookup, embedding_lookup_grad, token_logprobs, token_logprobs_grad
+from .tokens import (TableLogprobs, TokenLogprobs, check_errors, embedding_lookup, embedding_lookup_grad, table_logprobs, table_logprobs_grad, token_logprobs,
+                     token_logprobs_grad)
 from .trainer import AbstractBatchProcessor, B200RankingEvaluator, B200Trainer, process_in_batches
 from .types import EdgeList, EntityList, Side, Stats
 
@@ -16,5 +17,5 @@ __all__ = [
     "PluginRegistry", "COMPARATORS", "DYNAMIC_OPERATORS", "LOSS_FUNCTIONS", "OPERATORS", "AsyncAdagrad",
     "RowAdagrad", "make_optimizer", "AbstractBatchProcessor", "B200RankingEvaluator", "B200Trainer", "process_in_batches",
     "EdgeList", "EntityList", "Side", "Stats", "TokenLogprobs", "check_errors", "embedding_lookup", "embedding_lookup_grad",
-    "token_logprobs", "token_logprobs_grad",
+    "token_logprobs", "token_logprobs_grad", "TableLogprobs", "table_logprobs", "table_logprobs_grad",
 ]

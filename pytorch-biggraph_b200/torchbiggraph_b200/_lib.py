@@ -88,6 +88,11 @@ SYMBOLS = [
     ("pbg_token_logprobs", C.c_int, [_P, C.c_int64, C.c_int64, C.c_int64, C.c_int32, _P, C.c_int64, C.c_float, C.c_int32] + [_P] * 8),
     ("pbg_token_logprobs_grad", C.c_int, [_P, C.c_int64, C.c_int64, C.c_int64, C.c_int32, _P, C.c_int64, C.c_float, _P, _P, _P, _P, _P,
                                           C.c_int64, _P, _P]),
+    ("pbg_table_logprobs_workspace", C.c_int64, [C.c_int64, C.c_int64, C.c_int32, C.c_int32, C.c_int32]),
+    ("pbg_table_logprobs", C.c_int, [_P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64, C.c_int32, C.c_int32, _P, C.c_int64, C.c_float,
+                                     _P, _P, _P, _P, C.c_int64, _P, _P]),
+    ("pbg_table_logprobs_grad", C.c_int, [_P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64, C.c_int32, C.c_int32, _P, C.c_int64, C.c_float,
+                                          _P, _P, _P, _P, _P, _P, _P, C.c_int64, _P, _P]),
     ("pbg_launch_count", C.c_int64, [_P]),
     ("pbg_set_edge_weights", C.c_int, [_P, C.c_void_p]),
     ("pbg_set_profiling", C.c_int, [_P, C.c_int]),

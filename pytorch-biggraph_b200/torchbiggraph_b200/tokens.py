@@ -245,3 +245,59 @@ def token_logprobs_grad(logits: torch.Tensor, targets: torch.Tensor, lse: torch.
           _scale(scale, True), lse.data_ptr(), _ptr(entropy), _ptr(grad_logprob), _ptr(grad_entropy), out.data_ptr(), _row_stride(out),
           _error_word(errors, logits.device))
     return out
+
+
+class TableLogprobs(NamedTuple):
+    """Per query: log probability of its target, entropy, log of the sum of exponentials (float32)."""
+    logprob: torch.Tensor
+    entropy: torch.Tensor
+    lse: torch.Tensor
+
+
+def _queries_and_table(queries, table, targets):
+    code = _matrix("queries", queries)
+    _matrix("table", table, queries.dtype, queries.device)
+    if queries.shape[1] != table.shape[1]:
+        raise ValueError(f"queries have {queries.shape[1]} elements, the table's rows {table.shape[1]}")
+    if table.shape[0] == 0:
+        raise ValueError("table has no rows")
+    n, dim = queries.shape
+    return code, n, table.shape[0], dim, _vector("targets", targets, torch.long, n, queries.device)
+
+
+def table_logprobs(queries: torch.Tensor, table: torch.Tensor, targets: torch.Tensor, *, scale: float = 1.0, ignore_index: int = IGNORE_INDEX,
+                   errors: Optional[torch.Tensor] = None) -> TableLogprobs:
+    """Log probabilities of rows `targets` [n] of the table under softmax(scale * queries . table^T), with the entropies and logs of the
+    sums; the n x rows scores are never stored.  What token_logprobs(queries @ table.T, targets) gives, at the accuracy of
+    float32 sums over the operands as they are (float32 operands are multiplied at 22 bits and more).  Queries
+    whose target is ignore_index are padding: 0."""
+    code, n, rows, dim, targets = _queries_and_table(queries, table, targets)
+    device = queries.device
+    r = TableLogprobs(*(torch.empty(n, dtype=torch.float32, device=device) for _ in range(3)))
+    scale, word = _scale(scale, True), _error_word(errors, device)
+    with torch.cuda.device(device):
+        size = _lib.lib().pbg_table_logprobs_workspace(n, rows, dim, code, 0)
+        ws = _workspace(size, device)
+        _call("pbg_table_logprobs", device, queries.data_ptr(), _row_stride(queries), n, table.data_ptr(), _row_stride(table), rows, dim, code, targets.data_ptr(),
+              int(ignore_index), scale, r.logprob.data_ptr(), r.entropy.data_ptr(), r.lse.data_ptr(), ws.data_ptr(), size, word)
+    return r
+
+
+def table_logprobs_grad(queries: torch.Tensor, table: torch.Tensor, targets: torch.Tensor, lse: torch.Tensor, entropy: Optional[torch.Tensor],
+                        grad_logprob: Optional[torch.Tensor], grad_entropy: Optional[torch.Tensor] = None, *, scale: float = 1.0,
+                        ignore_index: int = IGNORE_INDEX, errors: Optional[torch.Tensor] = None):
+    """Gradients (of the queries, of the table) of sum(grad_logprob * logprob + grad_entropy * entropy), from the lse and the entropy that
+    table_logprobs returned (the entropy only where grad_entropy is given).  Queries that are padding, and those whose
+    target is out of range, get zeros and add nothing to the table's gradient, whatever they hold."""
+    code, n, rows, dim, targets = _queries_and_table(queries, table, targets)
+    device = queries.device
+    lse, entropy, grad_logprob, grad_entropy = _row_grads(n, device, lse, entropy, grad_logprob, grad_entropy)
+    dq = torch.empty((n, dim), dtype=queries.dtype, device=device)
+    dt = torch.empty((rows, dim), dtype=table.dtype, device=device)
+    scale, word = _scale(scale, True), _error_word(errors, device)
+    with torch.cuda.device(device):
+        size = _lib.lib().pbg_table_logprobs_workspace(n, rows, dim, code, 1)
+        ws = _workspace(size, device)
+        _call("pbg_table_logprobs_grad", device, queries.data_ptr(), _row_stride(queries), n, table.data_ptr(), _row_stride(table), rows, dim, code, targets.data_ptr(),
+              int(ignore_index), scale, lse.data_ptr(), _ptr(entropy), _ptr(grad_logprob), _ptr(grad_entropy), dq.data_ptr(), dt.data_ptr(), ws.data_ptr(), size, word)
+    return dq, dt

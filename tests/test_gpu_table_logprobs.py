@@ -1,0 +1,235 @@
+"""Log probabilities over all rows of a table and their gradients, against the definition in 64 bits.
+
+Tolerances.  u = 2^-24.
+  - A score is a dot product of dim exact products (16-bit operands) added up in fp32, at worst truncated: off by dim * 2 u of the sum of
+    the products' sizes; float32 operands are two fp16 planes, which drop 2^-22 of a product and round each operand by 2^-22: 3 * 2^-22
+    more.  E = (dim * 2^-23 + 3 * 2^-22) * max |q||w| summed bounds a score's error, and with it that of lse and log p (all scores off by E at
+    most; softmax moves by no more than its scores), beside 2e-5 of 1 + |lse| for the sums as in the tests of scores in memory; the
+    entropy moves by at most 2 E times its own slope, |log p| + H <= 40 where p counts.
+  - dz is off by p (E + 2e-5) relatively and rounded by half a step of the operands' type (float32: two planes, 2^-22); the products
+    with the table and the queries carry that as a sum of sizes, and 2^-23 per term of fp32 adding."""
+import math
+
+import pytest
+import torch
+
+import torchbiggraph_b200 as T
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+DEV = "cuda"
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def f32(scale):
+    return float(torch.tensor(scale, dtype=torch.float32))
+
+
+def half_step(t):
+    return torch.finfo(t).eps / 2
+
+
+def inputs(n, rows, dim, dtype, seed, spread=1.0):
+    g = gen(seed)
+    table = (torch.randn(rows, dim, device=DEV, generator=g) / math.sqrt(dim)).to(dtype)
+    targets = torch.randint(0, rows, (n,), device=DEV, generator=g)
+    queries = (spread * (torch.randn(n, dim, device=DEV, generator=g) + 2 * table[targets].float())).to(dtype)
+    return queries, table, targets
+
+
+def scores(q, t, scale):
+    """64-bit scores, and the bound E per row on the error of one."""
+    z = q.double() @ t.double().T * f32(scale)
+    size = (q.double().abs() @ t.double().abs().T).amax(1) * scale
+    dim = q.shape[1]
+    return z, size * (dim * 2 ** -23 + (3 * 2 ** -22 if q.dtype == torch.float32 else 0))
+
+
+def want_forward(z, targets):
+    lse = torch.logsumexp(z, 1)
+    logp = z - lse[:, None]
+    return logp.gather(1, targets[:, None])[:, 0], torch.special.entr(logp.exp()).sum(1), lse
+
+
+def check_forward(q, t, targets, scale, ignore=()):
+    r = T.table_logprobs(q, t, targets, scale=scale)
+    keep = torch.ones(len(q), dtype=torch.bool, device=DEV)
+    keep[list(ignore)] = False
+    z, E = scores(q[keep], t, scale)
+    logprob, ent, lse = want_forward(z, targets[keep])
+    tol = E + 2e-5 * (1 + lse.abs())
+    assert ((r.lse[keep].double() - lse).abs() <= tol).all()
+    assert ((r.logprob[keep].double() - logprob).abs() <= 2 * tol + 2e-5 * logprob.abs()).all()
+    assert ((r.entropy[keep].double() - ent).abs() <= 80 * E + 2e-5 * (1 + ent + math.log(len(t)))).all()
+    for x in r:
+        assert (x[~keep] == 0).all() and x.dtype == torch.float32
+    return r
+
+
+SHAPES = [(1, 1, 1), (1, 300, 8), (3, 64, 64), (5, 65, 33), (127, 255, 40), (129, 257, 72), (7, 20_011, 400), (200, 1000, 1), (64, 3000, 520), (300, 5000, 100), (1000, 14_951, 400)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,rows,dim", SHAPES)
+def test_forward(dtype, n, rows, dim):
+    q, t, targets = inputs(n, rows, dim, dtype, n + rows)
+    ignore = [4] if n > 4 else []
+    targets[ignore] = -100
+    check_forward(q, t, targets, 0.9, ignore)
+
+
+def check_grad(q, t, targets, scale, g, h, r, got, dead=()):
+    dq, dt = got
+    keep = torch.ones(len(q), dtype=torch.bool, device=DEV)
+    keep[list(dead)] = False
+    qk, tk = q[keep], targets[keep]
+    z, E = scores(qk, t, scale)
+    logp = z - r.lse[keep].double()[:, None]
+    p = logp.exp()
+    hot = torch.zeros_like(p)
+    hot[torch.arange(len(p), device=DEV), tk] = 1.0
+    gk = g[keep].double()[:, None] if g is not None else torch.zeros(len(p), 1, device=DEV, dtype=torch.float64)
+    hk = h[keep].double()[:, None] if h is not None else torch.zeros_like(gk)
+    H = r.entropy[keep].double()[:, None]
+    w = scale * (gk * (hot - p) + hk * (torch.special.entr(p) - p * H))
+    size = scale * (gk.abs() * (hot + p) + hk.abs() * (torch.special.entr(p).abs() + p * H))
+    err = size * (E[:, None] * 2 + 2e-5) + scale * hk.abs() * p * E[:, None] + w.abs() * (2 ** -22 if q.dtype == torch.float32 else half_step(q.dtype))
+    if q.dtype != torch.bfloat16:
+        # a power of two brings the bound of dz to 2^14; half a step of the smallest half-precision numbers is 2^-25 of 1
+        bound = scale * ((g[keep].abs().max().item() if g is not None else 0) + 23 * (h[keep].abs().max().item() if h is not None else 0))
+        err = err + bound * 2 ** -38
+    A, Q = t.double(), qk.double()
+    planes = 3 * 2 ** -22 if q.dtype == torch.float32 else 0
+    floor = torch.finfo(q.dtype).smallest_normal
+    want = w @ A
+    tol = err @ A.abs() + (w.abs() @ A.abs()) * (len(t) * 2 ** -23 + planes) + want.abs() * half_step(q.dtype) + floor
+    assert ((dq[keep].double() - want).abs() <= tol).all(), ((dq[keep].double() - want).abs() - tol).max()
+    want = w.T @ Q
+    tol = err.T @ Q.abs() + (w.abs().T @ Q.abs()) * (len(qk) * 2 ** -23 + planes) + want.abs() * half_step(q.dtype) + floor
+    assert ((dt.double() - want).abs() <= tol).all(), ((dt.double() - want).abs() - tol).max()
+    assert (dq[~keep] == 0).all() and dq.dtype == q.dtype and dt.dtype == t.dtype
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,rows,dim", SHAPES)
+def test_gradients(dtype, n, rows, dim):
+    q, t, targets = inputs(n, rows, dim, dtype, n + rows)
+    dead = [x for x in (4, 6) if x < n]
+    if n > 4:
+        targets[4] = -100
+        q[4] = math.nan                                     # what stands in padding does not matter
+    if n > 6:
+        targets[6] = rows
+        q[6] = math.inf
+    errors = torch.zeros(1, dtype=torch.int32, device=DEV)
+    r = T.table_logprobs(q, t, targets, scale=1.1)
+    g, h = torch.randn(n, device=DEV, generator=gen(1)) / n, torch.randn(n, device=DEV, generator=gen(2)) / n
+    g[dead] = math.nan
+    check_grad(q, t, targets, 1.1, g, h, r, T.table_logprobs_grad(q, t, targets, r.lse, r.entropy, g, h, scale=1.1, errors=errors), dead)
+    assert errors.item() == (1 if n > 6 else 0)
+    check_grad(q, t, targets, 1.1, g, None, r, T.table_logprobs_grad(q, t, targets, r.lse, None, g, scale=1.1), dead)
+    check_grad(q, t, targets, 1.1, None, h, r, T.table_logprobs_grad(q, t, targets, r.lse, r.entropy, None, h, scale=1.1), dead)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width,first", [(80, 0), (80, 8), (77, 0), (80, 1)])
+def test_strides(dtype, width, first):
+    q, t, targets = inputs(50, 700, width, dtype, width)
+    q, t = q[:, first:first + 64], t[:, first:first + 64]
+    r = check_forward(q, t, targets, 1.0)
+    g = torch.ones(50, device=DEV)
+    check_grad(q, t, targets, 1.0, g, None, r, T.table_logprobs_grad(q, t, targets, r.lse, None, g))
+    same = q[:1].expand(50, 64)
+    r2 = check_forward(same, t, targets, 1.0)
+    check_grad(same, t, targets, 1.0, g, None, r2, T.table_logprobs_grad(same, t, targets, r2.lse, None, g))
+
+
+def test_float32_operands_of_any_size():
+    """Both planes are scaled by the largest element: tables of tiny and of large numbers come out as accurately."""
+    q, t, targets = inputs(40, 900, 96, torch.float32, 5)
+    for a, b in ((1e-12, 1e12), (1e15, 1e-15), (3e-20, 1e19), (1.0, 1e-30)):
+        r = check_forward(q * a, t * b, targets, 1.0)
+        g = torch.ones(40, device=DEV)
+        check_grad(q * a, t * b, targets, 1.0, g, None, r, T.table_logprobs_grad(q * a, t * b, targets, r.lse, None, g))
+    zero = T.table_logprobs(q * 0, t, targets)
+    assert (zero.entropy - math.log(900)).abs().max() < 1e-5
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_small_gradients_do_not_vanish(dtype):
+    """Most of dz = 2e-5 p lies below the smallest half-precision number, the scaled dz does not."""
+    q, t, targets = inputs(100, 500, 64, dtype, 3)
+    r = T.table_logprobs(q, t, targets)
+    g = torch.full((100,), 2e-5, device=DEV)
+    check_grad(q, t, targets, 1.0, g, None, r, T.table_logprobs_grad(q, t, targets, r.lse, None, g))
+
+
+def test_gradients_are_the_slope():
+    """Central differences of the 64-bit definition."""
+    q, t, targets = inputs(6, 40, 12, torch.float32, 9)
+    r = T.table_logprobs(q, t, targets, scale=1.5)
+    g, h = torch.randn(6, device=DEV, generator=gen(1)), torch.randn(6, device=DEV, generator=gen(2))
+    dq, dt = T.table_logprobs_grad(q, t, targets, r.lse, r.entropy, g, h, scale=1.5)
+
+    def value(a, b):
+        logp = torch.log_softmax(a @ b.T * 1.5, 1)
+        return (g.double() * logp.gather(1, targets[:, None])[:, 0] + h.double() * torch.special.entr(logp.exp()).sum(1)).sum()
+    e = 1e-4
+    for seed in range(4):
+        a, b = torch.randn(6, 12, device=DEV, generator=gen(20 + seed)).double(), torch.randn(40, 12, device=DEV, generator=gen(30 + seed)).double()
+        Q, W = q.double(), t.double()
+        slope = (value(Q + e * a, W + e * b) - value(Q - e * a, W - e * b)) / (2 * e)
+        assert abs((dq.double() * a).sum() + (dt.double() * b).sum() - slope).item() < 1e-3
+
+
+def test_same_bits_and_graphs():
+    q, t, targets = inputs(500, 3000, 200, torch.bfloat16, 4)
+    g = torch.randn(500, device=DEV, generator=gen(1))
+
+    def step():
+        r = T.table_logprobs(q, t, targets)
+        return (*r, *T.table_logprobs_grad(q, t, targets, r.lse, r.entropy, g, r.lse))
+    want = step()
+    assert all(torch.equal(a, b) for a, b in zip(want, step()))
+    graphs, outs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(step())
+        graphs.append(graph)
+    targets.copy_(targets.roll(1))
+    q.mul_(0.5)
+    want = step()
+    for graph in graphs + graphs:
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for out in outs for a, b in zip(out, want))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step()
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_refusals_and_nothing_to_do():
+    q, t, targets = inputs(4, 10, 8, torch.float32, 4)
+    f = torch.zeros(4, device=DEV)
+    for bad in (lambda: T.table_logprobs(q, t[:, :7], targets), lambda: T.table_logprobs(q, t[:0], targets), lambda: T.table_logprobs(q, t, targets[:3]),
+                lambda: T.table_logprobs(q, t, targets, scale=0.0), lambda: T.table_logprobs(q, t.t().contiguous().t(), targets),
+                lambda: T.table_logprobs_grad(q, t, targets, f, None, None), lambda: T.table_logprobs_grad(q, t, targets, f, None, None, f)):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(TypeError):
+        T.table_logprobs(q, t.half(), targets)
+    r = T.table_logprobs(q[:0], t, targets[:0])
+    assert r.lse.shape == (0,)
+    dq, dt = T.table_logprobs_grad(q[:0], t, targets[:0], f[:0], None, f[:0])
+    assert dq.shape == (0, 8) and (dt == 0).all()
+    errors = torch.zeros(1, dtype=torch.int32, device=DEV)
+    targets[2] = 10
+    r = T.table_logprobs(q, t, targets, errors=errors)
+    assert r.logprob[2].isnan() and r.lse.isfinite().all() and errors.item() == 1

@@ -110,3 +110,25 @@ def test_python_refuses_what_does_not_fit():
         T.token_logprobs_grad(x[:4], ids[:4], f[:4], None, f[:4], out=x[2:])
     assert T.token_logprobs(x[:0], ids[:0], top=3).top_ids.shape == (0, 3)
     assert T.token_logprobs_grad(x[:0], ids[:0], f[:0], None, f[:0]).shape == (0, 8)
+
+
+TABLE = dict(queries=P, q_stride=8, n=4, table=P, t_stride=8, rows=100, dim=8, dtype=1, targets=P, ignore=-100, scale=1.0)
+TABLE_CHANGES = [(dict(queries=None), BAD), (dict(table=None), BAD), (dict(targets=None), BAD), (dict(n=-1), BAD), (dict(rows=0), BAD), (dict(dim=0), BAD), (dict(dim=65_537), LARGE),
+                 (dict(n=2 ** 30 + 1), LARGE), (dict(rows=2 ** 31), LARGE), (dict(dtype=7), BAD), (dict(scale=0.0), BAD), (dict(q_stride=-1), BAD), (dict(t_stride=-1), BAD)]
+
+
+@pytest.mark.parametrize("change,status", TABLE_CHANGES + [(dict(ws=None), BAD), (dict(ws=P + 8), BAD), (dict(size=255), BAD), (dict(lse=None), BAD)])
+def test_table_arguments(change, status):
+    L = _lib.lib()
+    a = dict(TABLE, logprob=P, entropy=P, lse=P, ws=P, size=L.pbg_table_logprobs_workspace(4, 100, 8, 1, 0))
+    a.update(change)
+    assert L.pbg_table_logprobs(*a.values(), None, None) == status
+
+
+@pytest.mark.parametrize("change,status", TABLE_CHANGES + [(dict(ws=None), BAD), (dict(ws=P + 8), BAD), (dict(size=255), BAD), (dict(lse=None), BAD), (dict(entropy=None), BAD),
+                                                           (dict(dq=None, dt=None), BAD)])
+def test_table_grad_arguments(change, status):
+    L = _lib.lib()
+    a = dict(TABLE, lse=P, entropy=P, g=P, h=P, dq=P, dt=P, ws=P, size=L.pbg_table_logprobs_workspace(4, 100, 8, 1, 1))
+    a.update(change)
+    assert L.pbg_table_logprobs_grad(*a.values(), None, None) == status

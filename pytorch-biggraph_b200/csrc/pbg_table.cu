@@ -10,131 +10,192 @@
 //                planes of everything down to 2^-17 of it are whole), and the three products b1 b0 + b0 b1 + b0 b0: the
 //                dropped b1 b1 is 2^-22 of a product, the size of fp32 rounding.  Half the work of three bf16 planes.
 //
-// One persistent kernel per product, one CTA per SM, tiles of 128 x BN (BN <= 256):
-//   warp 0     TMA: stages of 48 KB (64 k-values of one plane, or 32 of two) in a ring of four
+// One persistent kernel per product, one CTA per SM, tiles of 128 x BN (BN <= 256) or, by a pair of CTAs, 256 x BN:
+//   warp 0     TMA into a ring of stages (64 k-values of one plane, or 32 of two)
 //   warp 1     issues tcgen05.mma into one of two accumulators of 256 columns
 //   warps 2-9  read the other accumulator and, two warps to every 32 rows: reduce it to (maximum, S, T) per row; or turn it into dz and
 //              write that; or write the product
+// A pair (cta_group::2): each CTA holds 128 rows of A and half of B's columns, the first one issues for both, and an operand byte
+// in shared memory feeds twice as many products.  Alone, a tile of 128 x 256 writes and reads 192 bytes of shared memory per cycle of
+// its products where the SM moves 128; a pair 128.
+//
 // Every wait is bounded: one that runs out sets bit 2 of the error word, and the CTA stops, frees its tensor memory and returns.
 #include "pbg_tc.cuh"
 #include "pbg_tokens.cuh"
+#include <type_traits>
 
-enum { TAB_BF16 = 0, TAB_F16 = 1, TAB_F32 = 2 };            // operands: bf16, fp16, two fp16 planes
 enum { EPI_STATS = 0, EPI_DZ = 1, EPI_OUT = 2 };
 
-#define TAB_STAGES 4
-#define TAB_STAGE_BYTES 49152
+#define TAB_RING_BYTES 196608                               // stages; as many as fit
+#define TAB_STAGES_MAX 6
 #define TAB_EPI_WARPS 8
 #define TAB_THREADS (64 + 32 * TAB_EPI_WARPS)
-#define TAB_SMEM (1024 + TAB_STAGES * TAB_STAGE_BYTES + TAB_EPI_WARPS * 4096)
+#define TAB_SMEM (1024 + TAB_RING_BYTES + TAB_EPI_WARPS * 4096)
 #define TAB_DZ_BYTES (2ll << 30)                            // most memory for dz: beyond it the table goes in pieces
 #define TAB_PARTS_BYTES (512ll << 20)                       // and for the tiles' partial sums: beyond it the queries do
+// The tensor cores cut off what they add up instead of rounding it, a bias of half a step per addition.  Contractions of
+// fp32 operands are therefore cut into parts of this many blocks of 32 k-values (24 additions), which are added in registers.
+#define TAB_F32_PART 4
 
-template <int KIND> struct TabType;
-template <> struct TabType<TAB_BF16> { using out = __nv_bfloat16; using elem = __nv_bfloat16; static constexpr int NPL = 1; static constexpr uint32_t FMT = 1; };
-template <> struct TabType<TAB_F16> { using out = __half; using elem = __half; static constexpr int NPL = 1; static constexpr uint32_t FMT = 0; };
-template <> struct TabType<TAB_F32> { using out = float; using elem = __half; static constexpr int NPL = 2; static constexpr uint32_t FMT = 0; };
+// Operands: their elements, the planes of A and B, the type of results
+template <class E, class O, int PA, int PB> struct TabMath { using elem = E; using out = O; static constexpr int NPA = PA, NPB = PB; };
+using TabBf16 = TabMath<__nv_bfloat16, __nv_bfloat16, 1, 1>;
+using TabF16 = TabMath<__half, __half, 1, 1>;
+using TabF32 = TabMath<__half, float, 2, 2>;
+using TabBf16Fine = TabMath<__nv_bfloat16, __nv_bfloat16, 2, 1>;          // dz in two planes
+using TabF16Fine = TabMath<__half, __half, 2, 1>;
 
-// Powers of two that the operands were multiplied by, and their inverses; filled by tab_exponents_kernel.
-struct TabScales { float q, w, dz, iq, iw, idz; unsigned max_q, max_w, max_g, unused; };
+// Powers of two that the operands were multiplied by, and their inverses
+struct TabScales { float q, w, dz, iq, iw, idz; };
 
 struct TabMaps { CUtensorMap a, b; };
 struct TabArgs {
   long long M, N;                     // rows and columns of the product
   long long kblocks;                  // blocks of KB k-values
   int BN, splits, m_first;            // tile columns; parts of the contraction; the tiles of one column go to neighbouring CTAs
+  int stages, part;                   // stages of the ring; k-blocks added up in tensor memory at a time
   float scale;
-  const TabScales *sc;
+  const TabScales *sc;                // null: all 1
   int *err;
   float4 *parts; int nparts;          // EPI_STATS: [M][nparts] (reference in base 2, S, T)
   const long long *targets; long long ignore_index, vocab, v0;         // EPI_DZ; v0: the table's row of column 0
   const float *lse, *entropy, *g, *h;
-  void *dz; long long ldz, dz_plane;
+  void *dz; long long ldz, dz_plane; int dz_planes;
   void *out; long long ldo;           // EPI_OUT: the result, or
   float *partial; int add;            //          [splits][M][N] fp32, stored or added
-  float unscale_q, unscale_w, unscale_dz;                              // which inverses the product takes (1 or 0)
+  int by_q, by_w, by_dz;              // which powers the product carries
 };
 
-template <int EPI, int KIND, bool A_MN, bool B_MN>
+__device__ __forceinline__ uint32_t cta_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+// the address of the pair's first CTA that corresponds to an address of this one
+__device__ __forceinline__ uint32_t in_first_cta(uint32_t a) { uint32_t r; asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(a)); return r; }
+__device__ __forceinline__ void pair_sync() {
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+template <int CG>
+__device__ __forceinline__ void tab_load(uint32_t dst, const CUtensorMap *map, int c0, int c1, uint32_t bar) {
+  if (CG == 1) tma_load_3d(dst, map, c0, c1, 0, bar);
+  else asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                    :: "r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(0), "r"(bar) : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void tab_mma(uint32_t acc, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+  if (CG == 1) mma_f16(acc, a, b, idesc, add);
+  else asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" :: "r"(acc), "l"(a), "l"(b), "r"(idesc), "r"(add ? 1u : 0u) : "memory");
+}
+// arrives on the barrier (the pair's two) when the products issued so far are done
+template <int CG>
+__device__ __forceinline__ void tab_commit(uint32_t bar) {
+  if (CG == 1) mma_commit(bar);
+  else asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" :: "r"(bar), "h"((unsigned short)3) : "memory");
+}
+// a wait for arrivals of both CTAs of a pair
+__device__ __forceinline__ bool pair_wait(uint32_t bar, uint32_t parity, int *err) {
+  for (int it = 0; it < TC_WAIT_LIMIT; ++it) {
+    uint32_t ok;
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    if (ok) return true;
+  }
+  atomicOr(err, TOK_ERR_TIMEOUT);
+  return false;
+}
+
+template <int EPI, class MATH, bool A_MN, bool B_MN, int CG>
 __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_constant__ TabMaps maps, TabArgs g) {
-  using Elem = typename TabType<KIND>::elem;
-  using Out = typename TabType<KIND>::out;
-  constexpr int NPL = TabType<KIND>::NPL, KB = NPL == 1 ? 64 : 32;
+  using Elem = typename MATH::elem;
+  using Out = typename MATH::out;
+  constexpr int NPA = MATH::NPA, NPB = MATH::NPB, KB = NPA == 1 ? 64 : 32;
+  constexpr bool PARTS = NPB == 2;                                        // fp32: the contraction is added up in registers
+  constexpr uint32_t FMT = std::is_same<Elem, __nv_bfloat16>::value ? 1u : 0u;
   constexpr uint32_t ROW_BYTES = KB * 2, ATOM_BYTES = KB * 128;          // a K-major row; 64 columns of an MN-major operand's plane
-  constexpr uint32_t A_BYTES = NPL * 128 * ROW_BYTES;
+  constexpr uint32_t A_BYTES = NPA * 128 * ROW_BYTES;
   extern __shared__ unsigned char smem_raw[];
   unsigned char *smem = (unsigned char *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  unsigned char *ostage = smem + TAB_STAGES * TAB_STAGE_BYTES;
-  __shared__ __align__(8) unsigned long long bars[2 * TAB_STAGES + 4];
+  unsigned char *ostage = smem + TAB_RING_BYTES;
+  __shared__ __align__(8) unsigned long long bars[2 * TAB_STAGES_MAX + 4];
   __shared__ uint32_t tmem_base_s;
   __shared__ volatile int failed;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = CG == 2 ? cta_rank() : 0u;
   const uint32_t bar0 = smem_u32(&bars[0]);
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
-  auto empty_bar = [&](int s) { return bar0 + 8u * (TAB_STAGES + s); };
-  auto accf_bar = [&](int a) { return bar0 + 8u * (2 * TAB_STAGES + a); };
-  auto acce_bar = [&](int a) { return bar0 + 8u * (2 * TAB_STAGES + 2 + a); };
+  auto empty_bar = [&](int s) { return bar0 + 8u * (TAB_STAGES_MAX + s); };
+  auto accf_bar = [&](int a) { return bar0 + 8u * (2 * TAB_STAGES_MAX + a); };
+  auto acce_bar = [&](int a) { return bar0 + 8u * (2 * TAB_STAGES_MAX + 2 + a); };
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2 * TAB_STAGES + 2; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar0 + 8u * i));
-    for (int a = 0; a < 2; ++a) asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(acce_bar(a)), "r"(32 * TAB_EPI_WARPS));
+    for (int i = 0; i < 2 * TAB_STAGES_MAX + 2; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar0 + 8u * i));
+    for (int a = 0; a < 2; ++a) asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(acce_bar(a)), "r"(32 * TAB_EPI_WARPS * CG));
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     failed = 0;
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" :: "r"(smem_u32(&tmem_base_s)) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if (CG == 1) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" :: "r"(smem_u32(&tmem_base_s)) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" :: "r"(smem_u32(&tmem_base_s)) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  if (CG == 2) pair_sync();                                              // the other CTA's barriers are set up too
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = tmem_base_s;
+  pdl_begin();
 
-  const long long tiles_m = (g.M + 127) / 128, tiles_n = (g.N + g.BN - 1) / g.BN, per_split = tiles_m * tiles_n, ntiles = per_split * g.splits;
+  const long long tiles_m = (g.M + 128 * CG - 1) / (128 * CG), tiles_n = (g.N + g.BN - 1) / g.BN, per_split = tiles_m * tiles_n, ntiles = per_split * g.splits;
+  const long long first = blockIdx.x / CG, step = gridDim.x / CG;
+  // m0: this CTA's rows; n0: the tile's columns
   auto tile = [&](long long t, long long &m0, long long &n0, int &split, long long &kb0, long long &kb1) {
     split = (int)(t / per_split);
     t -= split * per_split;
     const long long m = g.m_first ? t % tiles_m : t / tiles_n, n = g.m_first ? t / tiles_m : t % tiles_n;
-    m0 = m * 128;
+    m0 = m * 128 * CG + 128 * rank;
     n0 = n * g.BN;
     kb0 = g.kblocks * split / g.splits;
     kb1 = g.kblocks * (split + 1) / g.splits;
   };
-  const int b_atoms = g.BN / 64;
-  const uint32_t b_plane = B_MN ? ATOM_BYTES : (uint32_t)g.BN * ROW_BYTES;
-  const uint32_t stage_tx = A_BYTES + NPL * (uint32_t)g.BN * ROW_BYTES;
+  const int b_cols = g.BN / CG;                                          // columns of B in this CTA
+  const uint32_t b_plane = B_MN ? ATOM_BYTES : (uint32_t)b_cols * ROW_BYTES;
+  const uint32_t stage_bytes = A_BYTES + NPB * (uint32_t)b_cols * ROW_BYTES;
 
   if (warp == 0) {
     // ---------------- TMA: one box per K-major operand, one per 64 columns of an MN-major one, each from its own lane
     StageRing at;
     bool stop = false;
     constexpr int A_BOXES = A_MN ? 2 : 1;
-    const int boxes = A_BOXES + (B_MN ? b_atoms : 1);
-    for (long long t = blockIdx.x; t < ntiles && !stop; t += gridDim.x) {
+    const int boxes = A_BOXES + (B_MN ? b_cols / 64 : 1);
+    for (long long t = first; t < ntiles && !stop; t += step) {
       long long m0, n0, kb0, kb1;
       int split;
       tile(t, m0, n0, split, kb0, kb1);
-      for (long long kb = kb0; kb < kb1; ++kb, at.next(TAB_STAGES)) {
+      n0 += rank * b_cols;
+      for (long long kb = kb0; kb < kb1; ++kb, at.next(g.stages)) {
         bool ok = failed == 0;
         if (ok && lane == 0) ok = mbar_wait(empty_bar(at.s), at.parity ^ 1u, g.err);
         if (!__all_sync(0xffffffffu, ok)) { failed = 1; stop = true; break; }
-        const uint32_t fb = full_bar(at.s), a = smem_u32(smem) + (uint32_t)at.s * TAB_STAGE_BYTES, b = a + A_BYTES;
-        if (lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(fb), "r"(stage_tx) : "memory");
+        const uint32_t a = smem_u32(smem) + (uint32_t)at.s * stage_bytes, b = a + A_BYTES;
+        // a pair's loads are all counted by the first CTA, which issues the products
+        const uint32_t fb = CG == 1 ? full_bar(at.s) : in_first_cta(full_bar(at.s));
+        if (lane == 0 && rank == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(full_bar(at.s)), "r"(CG * stage_bytes) : "memory");
         __syncwarp();
         const int k = (int)(kb * KB);
         if (lane < A_BOXES) {
-          if (A_MN) tma_load_3d(a + lane * NPL * ATOM_BYTES, &maps.a, (int)m0 + 64 * lane, k, 0, fb);
-          else tma_load_3d(a, &maps.a, k, (int)m0, 0, fb);
+          if (A_MN) tab_load<CG>(a + lane * NPA * ATOM_BYTES, &maps.a, (int)m0 + 64 * lane, k, fb);
+          else tab_load<CG>(a, &maps.a, k, (int)m0, fb);
         } else if (lane < boxes) {
           const int j = lane - A_BOXES;
-          if (B_MN) tma_load_3d(b + j * NPL * ATOM_BYTES, &maps.b, (int)n0 + 64 * j, k, 0, fb);
-          else tma_load_3d(b, &maps.b, k, (int)n0, 0, fb);
+          if (B_MN) tab_load<CG>(b + j * NPB * ATOM_BYTES, &maps.b, (int)n0 + 64 * j, k, fb);
+          else tab_load<CG>(b, &maps.b, k, (int)n0, fb);
         }
       }
     }
   } else if (warp == 1) {
     // ---------------- products.  D fp32; both operands of one type; planes (a, b): b1 b0, b0 b1, b0 b0
-    const uint32_t idesc = (1u << 4) | (TabType<KIND>::FMT << 7) | (TabType<KIND>::FMT << 10) | ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16) |
-                           ((uint32_t)(g.BN >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+    const uint32_t idesc = (1u << 4) | (FMT << 7) | (FMT << 10) | ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16) |
+                           ((uint32_t)(g.BN >> 3) << 17) | ((uint32_t)(128 * CG >> 4) << 24);
     // K-major: 128-byte rows in the 128-byte swizzle (layout 2) or 64-byte rows in the 64-byte one (layout 4), 32 bytes per 16 k-values;
     // MN-major: 64 columns x KB rows in the 128-byte swizzle, 2048 bytes per 16 k-values
     constexpr uint32_t K_SBO = KB == 64 ? 1024 : 512, K_LAYOUT = KB == 64 ? 2 : 4;
@@ -142,45 +203,53 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
     const bool leader = elect_one();
     StageRing at;
     int j = 0;
-    for (long long t = blockIdx.x; t < ntiles; t += gridDim.x, ++j) {
+    bool ok = rank == 0;
+    for (long long t = first; t < ntiles && ok; t += step) {
       long long m0, n0, kb0, kb1;
       int split;
       tile(t, m0, n0, split, kb0, kb1);
-      const int ab = j & 1;
-      if (!__all_sync(0xffffffffu, failed == 0 && mbar_wait(acce_bar(ab), (uint32_t)((j >> 1) & 1) ^ 1u, g.err))) { failed = 1; break; }
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint32_t acc = tmem + (uint32_t)ab * 256u;
-      bool ok = true;
-      for (long long kb = kb0; kb < kb1; ++kb, at.next(TAB_STAGES)) {
-        if (!__all_sync(0xffffffffu, mbar_wait(full_bar(at.s), at.parity, g.err))) { failed = 1; ok = false; break; }
+      for (long long p0 = kb0; p0 < kb1 && ok; p0 += g.part, ++j) {
+        const int ab = j & 1;
+        const long long p1 = kb1 - p0 < g.part ? kb1 : p0 + g.part;
+        ok = failed == 0 && (CG == 1 ? mbar_wait(acce_bar(ab), (uint32_t)((j >> 1) & 1) ^ 1u, g.err) : pair_wait(acce_bar(ab), (uint32_t)((j >> 1) & 1) ^ 1u, g.err));
+        if (!__all_sync(0xffffffffu, ok)) { failed = 1; ok = false; break; }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t a = smem_u32(smem) + (uint32_t)at.s * TAB_STAGE_BYTES, b = a + A_BYTES;
-        const uint64_t da = A_MN ? smem_desc(a, NPL * ATOM_BYTES, 1024, 2) : smem_desc(a, 0, K_SBO, K_LAYOUT);
-        const uint64_t db = B_MN ? smem_desc(b, NPL * ATOM_BYTES, 1024, 2) : smem_desc(b, 0, K_SBO, K_LAYOUT);
+        const uint32_t acc = tmem + (uint32_t)ab * 256u;
+        for (long long kb = p0; kb < p1; ++kb, at.next(g.stages)) {
+          ok = CG == 1 ? mbar_wait(full_bar(at.s), at.parity, g.err) : pair_wait(full_bar(at.s), at.parity, g.err);
+          if (!__all_sync(0xffffffffu, ok)) { failed = 1; ok = false; break; }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t a = smem_u32(smem) + (uint32_t)at.s * stage_bytes, b = a + A_BYTES;
+          const uint64_t da = A_MN ? smem_desc(a, NPA * ATOM_BYTES, 1024, 2) : smem_desc(a, 0, K_SBO, K_LAYOUT);
+          const uint64_t db = B_MN ? smem_desc(b, NPB * ATOM_BYTES, 1024, 2) : smem_desc(b, 0, K_SBO, K_LAYOUT);
 #pragma unroll
-        for (int k = 0; k < KB / 16; ++k) {
-          if (NPL == 2 && leader) {
-            mma_f16(acc, desc_at(da, a_plane + k * a_step), desc_at(db, k * b_step), idesc, kb > kb0 || k > 0);
-            mma_f16(acc, desc_at(da, k * a_step), desc_at(db, b_plane + k * b_step), idesc, true);
+          for (int k = 0; k < KB / 16; ++k) {
+            const bool more = kb > p0 || k > 0;
+            if (NPA == 2 && leader) tab_mma<CG>(acc, desc_at(da, a_plane + k * a_step), desc_at(db, k * b_step), idesc, more);
+            if (NPB == 2 && leader) tab_mma<CG>(acc, desc_at(da, k * a_step), desc_at(db, b_plane + k * b_step), idesc, true);
+            if (leader) tab_mma<CG>(acc, desc_at(da, k * a_step), desc_at(db, k * b_step), idesc, NPA == 2 || more);
           }
-          if (leader) mma_f16(acc, desc_at(da, k * a_step), desc_at(db, k * b_step), idesc, NPL == 2 || kb > kb0 || k > 0);
+          if (leader) tab_commit<CG>(empty_bar(at.s));
         }
-        if (leader) mma_commit(empty_bar(at.s));
+        if (ok && leader) tab_commit<CG>(accf_bar(ab));
       }
-      if (!ok) break;
-      if (leader) mma_commit(accf_bar(ab));
     }
   } else {
     // ---------------- epilogue
     const int q = warp & 3, half = (warp - 2) >> 2, hc = g.BN / 2;       // 32 rows of the tile; half of its columns
     unsigned char *buf = ostage + (size_t)(warp - 2) * 4096;
-    const float unscale = (g.unscale_q != 0.f ? g.sc->iq : 1.f) * (g.unscale_w != 0.f ? g.sc->iw : 1.f) * (g.unscale_dz != 0.f ? g.sc->idz : 1.f);
+    const uint32_t drained = CG == 1 ? 0u : in_first_cta(acce_bar(0));
+    float unscale = 1.f, up = g.scale;
+    if (g.sc) {
+      unscale = (g.by_q ? g.sc->iq : 1.f) * (g.by_w ? g.sc->iw : 1.f) * (g.by_dz ? g.sc->idz : 1.f);
+      up *= g.sc->dz;
+    }
     int j = 0;
-    for (long long t = blockIdx.x; t < ntiles; t += gridDim.x, ++j) {
+    bool ok = true;
+    for (long long t = first; t < ntiles && ok; t += step) {
       long long m0, n0, kb0, kb1;
       int split;
       tile(t, m0, n0, split, kb0, kb1);
-      const int ab = j & 1;
       const long long m = m0 + q * 32 + lane;
       // what a row of dz takes, read while the products run
       float lse = 0.f, H = 0.f, gg = 0.f, hh = 0.f;
@@ -189,7 +258,6 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
       if (EPI == EPI_DZ && m < g.M) {
         const long long target = g.targets[m];
         if (target >= 0 && target < g.vocab && target != g.ignore_index) {
-          const float up = g.scale * g.sc->dz;
           lse = g.lse[m];
           if (g.g) gg = g.g[m] * up;
           if (g.h) { hh = g.h[m] * up; H = g.entropy[m]; }
@@ -197,27 +265,79 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
           live = true;
         } else if (target != g.ignore_index && n0 == 0 && half == 0 && g.v0 == 0) atomicOr(g.err, TOK_ERR_ID);
       }
-      bool ok = failed == 0;
-      if (ok && lane == 0) ok = mbar_wait(accf_bar(ab), (uint32_t)(j >> 1) & 1, g.err);
-      if (!__all_sync(0xffffffffu, ok)) { failed = 1; break; }
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint32_t acc = tmem + (uint32_t)ab * 256u + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * hc);
       const long long c0 = n0 + half * hc;                               // first column of this warp
       const int cols = c0 >= g.N ? 0 : g.N - c0 < hc ? (int)(g.N - c0) : hc;
+      const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * hc);
+      // The tile's values.  PARTS: all of them, added up in registers as the accumulators fill; else read by 32 columns below.
+      float sum[PARTS ? 128 : 1];
+      auto wait_full = [&]() {
+        bool w = failed == 0;
+        if (w && lane == 0) w = CG == 1 ? mbar_wait(accf_bar(j & 1), (uint32_t)(j >> 1) & 1, g.err) : pair_wait(accf_bar(j & 1), (uint32_t)(j >> 1) & 1, g.err);
+        if (!__all_sync(0xffffffffu, w)) { failed = 1; return false; }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        return true;
+      };
+      auto give_back = [&]() {
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        if (CG == 1) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(acce_bar(j & 1)) : "memory");
+        else asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" :: "r"(drained + 8u * (j & 1)) : "memory");
+        ++j;
+      };
+      if (PARTS) {
+#pragma unroll
+        for (int i = 0; i < 128; ++i) sum[PARTS ? i : 0] = 0.f;
+        for (long long p0 = kb0; p0 < kb1; p0 += g.part) {
+          ok = wait_full();
+          if (!ok) break;
+#pragma unroll
+          for (int x = 0; x < 128; x += 32) {
+            if (x >= hc) continue;
+            uint32_t v[32];
+            tmem_ld32(lanes + (uint32_t)(j & 1) * 256u + x, v);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) sum[PARTS ? x + i : 0] += __uint_as_float(v[i]);
+          }
+          give_back();
+        }
+        if (!ok) break;
+      } else if (kb0 < kb1) {
+        ok = wait_full();
+        if (!ok) break;
+      }
+      // 32 columns of the tile (a split without k-values holds zeros)
+      auto values = [&](int x, float (&v)[32]) {
+        if (PARTS) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = sum[PARTS ? x + i : 0];
+        } else if (kb0 < kb1) {
+          uint32_t r[32];
+          tmem_ld32(lanes + (uint32_t)(j & 1) * 256u + x, r);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = 0.f;
+        }
+      };
 
-      if (EPI == EPI_STATS) {
-        const float c = g.scale * unscale * TOK_LOG2E;
-        float mx = -INFINITY, r = 0.f, S = 0.f, T = 0.f;
-        for (int x = 0; x < cols; x += 32) {
-          uint32_t v[32];
-          tmem_ld32(acc + x, v);
+      float mx = -INFINITY, r = 0.f, S = 0.f, T = 0.f;                   // EPI_STATS
+      // the padding of dz's last columns is written too, as zeros: the contraction over the table's rows reads whole blocks
+      const int span = EPI == EPI_DZ ? (c0 >= g.ldz ? 0 : g.ldz - c0 < hc ? (int)(g.ldz - c0) : hc) : cols;
+      const int rows = g.M - (m0 + q * 32) < 32 ? (int)(g.M - (m0 + q * 32)) : 32;
+#pragma unroll PARTS ? 4 : 1
+      for (int x = 0; x < 128; x += 32) {
+        if (x >= span) break;
+        float v[32];
+        values(x, v);
+        if (EPI == EPI_STATS) {
+          const float c = g.scale * unscale * TOK_LOG2E;
           if (cols - x < 32) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) if (i >= cols - x) v[i] = __float_as_uint(-INFINITY);     // (columns that do not exist)
+            for (int i = 0; i < 32; ++i) if (i >= cols - x) v[i] = -INFINITY;                        // (columns that do not exist)
           }
-          float cm = __uint_as_float(v[0]);
+          float cm = v[0];
 #pragma unroll
-          for (int i = 1; i < 32; ++i) cm = fmaxf(cm, __uint_as_float(v[i]));
+          for (int i = 1; i < 32; ++i) cm = fmaxf(cm, v[i]);
           if (cm > mx) {
             mx = cm;
             const float d = fminf(fmaxf(r - cm * c, -1e30f), 0.f), f = tok_ex2(d);
@@ -227,79 +347,59 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
           }
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
-            const float y = tok_max_nan(fmaf(__uint_as_float(v[i]), c, -r), -1000.f), e = tok_ex2(y);
+            const float y = tok_max_nan(fmaf(v[i], c, -r), -1000.f), e = tok_ex2(y);
             S += e;
             T = fmaf(y, e, T);
           }
-        }
-        if (m < g.M) g.parts[m * g.nparts + n0 / g.BN * 2 + half] = make_float4(S == 0.f ? -1e30f : r, S, T, 0.f);
-      } else if (EPI == EPI_DZ) {
-        const float zs = g.scale * unscale;
-        // the padding of the last columns is written too, as zeros: the contraction over the table's rows reads whole blocks
-        const int span = c0 >= g.ldz ? 0 : g.ldz - c0 < hc ? (int)(g.ldz - c0) : hc;
-        for (int x = 0; x < span; x += 64) {
-          uint32_t pk[NPL][32];
+        } else if (EPI == EPI_DZ) {
+          const float zs = g.scale * unscale;
+          const long long col = c0 + x;
 #pragma unroll
-          for (int part = 0; part < 2; ++part) {
-            uint32_t v[32];
-            tmem_ld32(acc + x + part * 32, v);
-            const long long col = c0 + x + part * 32;
-            float d[32];
+          for (int i = 0; i < 32; ++i) {
+            const float logp = fmaf(v[i], zs, -lse), p = tok_ex2(logp * TOK_LOG2E);
+            v[i] = live && (p > 0.f || p != p) ? -p * fmaf(hh, logp + H, gg) : 0.f;
+          }
+          if (__any_sync(0xffffffffu, hot >= col && hot < col + 32)) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const float logp = fmaf(__uint_as_float(v[i]), zs, -lse), p = tok_ex2(logp * TOK_LOG2E);
-              d[i] = live && (p > 0.f || p != p) ? -p * fmaf(hh, logp + H, gg) : 0.f;
-            }
-            if (__any_sync(0xffffffffu, hot >= col && hot < col + 32)) {
+            for (int i = 0; i < 32; ++i) if (hot == col + i) v[i] += gg;
+          }
+          if (col + 32 > g.N) {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) if (hot == col + i) d[i] += gg;
-            }
-            if (col + 32 > g.N) {
+            for (int i = 0; i < 32; ++i) if (col + i >= g.N) v[i] = 0.f;
+          }
+          // a plane of 32 x 32 values at a time through shared memory: a row's 64 bytes leave together
+          for (int pl = 0; pl < g.dz_planes; ++pl) {
+            __syncwarp();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) if (col + i >= g.N) d[i] = 0.f;
-            }
+            for (int u = 0; u < 4; ++u) {
+              uint32_t w[4];
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              Elem e[2] = {Tok<Elem>::down(d[i]), Tok<Elem>::down(d[i + 1])};
-              pk[0][part * 16 + i / 2] = *reinterpret_cast<uint32_t *>(e);
-              if (NPL == 2) {
-                Elem f[2] = {Tok<Elem>::down(d[i] - Tok<Elem>::up(e[0])), Tok<Elem>::down(d[i + 1] - Tok<Elem>::up(e[1]))};
-                pk[NPL - 1][part * 16 + i / 2] = *reinterpret_cast<uint32_t *>(f);
+              for (int i = 0; i < 4; ++i) {
+                Elem e[2] = {Tok<Elem>::down(v[8 * u + 2 * i]), Tok<Elem>::down(v[8 * u + 2 * i + 1])};
+                v[8 * u + 2 * i] -= Tok<Elem>::up(e[0]);                 // what the next plane holds
+                v[8 * u + 2 * i + 1] -= Tok<Elem>::up(e[1]);
+                w[i] = *reinterpret_cast<uint32_t *>(e);
               }
+              *reinterpret_cast<uint4 *>(buf + lane * 64 + ((u ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
             }
-          }
-          // through shared memory: a row's 64 values leave as one line
-#pragma unroll
-          for (int pl = 0; pl < NPL; ++pl) {
             __syncwarp();
-#pragma unroll
-            for (int u = 0; u < 8; ++u)
-              *reinterpret_cast<uint4 *>(buf + lane * 128 + ((u ^ (lane & 7)) << 4)) = make_uint4(pk[pl][4 * u], pk[pl][4 * u + 1], pk[pl][4 * u + 2], pk[pl][4 * u + 3]);
-            __syncwarp();
-            Elem *to = (Elem *)g.dz + pl * g.dz_plane + (m0 + q * 32) * g.ldz + c0 + x;
-            const int rows = g.M - (m0 + q * 32) < 32 ? (int)(g.M - (m0 + q * 32)) : 32;
+            Elem *to = (Elem *)g.dz + pl * g.dz_plane + (m0 + q * 32) * g.ldz + col;
 #pragma unroll 8
-            for (int r = 0; r < rows; ++r)
-              reinterpret_cast<uint32_t *>(to + r * g.ldz)[lane] = *reinterpret_cast<uint32_t *>(buf + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + ((lane & 3) << 2));
+            for (int r0 = lane >> 4; r0 < rows; r0 += 2)
+              reinterpret_cast<uint32_t *>(to + r0 * g.ldz)[lane & 15] = *reinterpret_cast<uint32_t *>(buf + r0 * 64 + ((((lane & 15) >> 2) ^ ((r0 >> 1) & 3)) << 4) + ((lane & 3) << 2));
           }
-        }
-      } else {
-        const int rows = g.M - (m0 + q * 32) < 32 ? (int)(g.M - (m0 + q * 32)) : 32;
-        for (int x = 0; x < cols; x += 32) {
-          uint32_t v[32];
-          tmem_ld32(acc + x, v);
+        } else {
           __syncwarp();
 #pragma unroll
           for (int u = 0; u < 8; ++u)
-            *reinterpret_cast<uint4 *>(buf + lane * 128 + ((u ^ (lane & 7)) << 4)) = make_uint4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
+            *reinterpret_cast<float4 *>(buf + lane * 128 + ((u ^ (lane & 7)) << 4)) = make_float4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
           __syncwarp();
           const long long col = c0 + x + lane;
           if (x + lane < cols) {
 #pragma unroll 8
-            for (int r = 0; r < rows; ++r) {
-              float val = *reinterpret_cast<float *>(buf + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + ((lane & 3) << 2)) * unscale;
-              if (kb0 == kb1) val = 0.f;                                 // (a part without k-values: nothing was multiplied)
-              const long long row = m0 + q * 32 + r;
+            for (int r0 = 0; r0 < rows; ++r0) {
+              const float val = *reinterpret_cast<float *>(buf + r0 * 128 + (((lane >> 2) ^ (r0 & 7)) << 4) + ((lane & 3) << 2)) * unscale;
+              const long long row = m0 + q * 32 + r0;
               if (g.partial) {
                 float *to = g.partial + ((long long)split * g.M + row) * g.N + col;
                 *to = g.add ? *to + val : val;
@@ -308,16 +408,18 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
           }
         }
       }
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(acce_bar(ab)) : "memory");
+      if (EPI == EPI_STATS && m < g.M) g.parts[m * g.nparts + n0 / g.BN * 2 + half] = make_float4(S == 0.f ? -1e30f : r, S, T, 0.f);
+      if (!PARTS && kb0 < kb1) give_back();
     }
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  if (CG == 2) pair_sync();                                              // the other CTA's products read this one's shared memory
   if (warp == 1) {
     // after a wait that ran out copies and products may still be in flight: a bounded grace before the tensor memory goes back
     if (failed) for (int i = 0; i < 200000; ++i) __nanosleep(20);
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" :: "r"(tmem) : "memory");
+    if (CG == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" :: "r"(tmem) : "memory");
+    else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" :: "r"(tmem) : "memory");
   }
 }
 
@@ -327,6 +429,7 @@ __global__ void __launch_bounds__(128) tab_stats_kernel(const T *__restrict__ qu
                                                         int dim, const long long *__restrict__ targets, long long ignore_index, float scale,
                                                         const float4 *__restrict__ parts, int nparts, float *logprob, float *entropy, float *lse, int *errors) {
   __shared__ float4 sums[4];
+  pdl_begin();
   const long long n = blockIdx.x, target = targets[n];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   if (target == ignore_index) {
@@ -373,30 +476,50 @@ struct TabRows {
     return t != ignore_index && (any || (t >= 0 && t < vocab));
   }
 };
-// Largest finite |x| of a matrix, as its bits.
-__global__ void __launch_bounds__(256) tab_absmax_kernel(const float *__restrict__ x, long long stride, long long rows, int dim, TabRows counts, unsigned *out) {
+// A matrix on its way to becoming an operand: `blocks` CTAs of a preparing kernel work on it.
+struct TabSource { const void *x; long long stride, rows; TabRows counts; int blocks; void *to; long long ld, plane; };
+struct TabPrep {
+  TabSource q, w;                                          // blocks 0: not prepared
+  const float *g, *h; long long n; int gblocks;            // gblocks 0: dz is not scaled
+  float scale; int dim, planes, wide;                      // wide: rows of float4 on 16-byte boundaries
+  unsigned *block_max; TabScales *sc;
+};
+
+// Largest finite |x| that each CTA has seen: of the queries, of the table, of the bound of dz / scale:
+// |g| + |h| (p |log p| + p H), p |log p| <= 1 / e, H <= log rows < 22.
+__global__ void __launch_bounds__(256) tab_max_kernel(TabPrep a) {
+  __shared__ unsigned tops[8];
+  pdl_begin();
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  int b = blockIdx.x;
   unsigned top = 0u;
-  for (long long r = blockIdx.x; r < rows; r += gridDim.x)
-    if (counts(r)) for (int i = threadIdx.x; i < dim; i += 256) {
-      const unsigned b = __float_as_uint(x[r * stride + i]) & 0x7fffffffu;
-      if (b < 0x7f800000u && b > top) top = b;
+  auto see = [&](float v) {
+    const unsigned bits = __float_as_uint(v) & 0x7fffffffu;
+    if (bits < 0x7f800000u && bits > top) top = bits;
+  };
+  if (b < a.q.blocks + a.w.blocks) {
+    const TabSource &s = b < a.q.blocks ? a.q : a.w;
+    if (b >= a.q.blocks) b -= a.q.blocks;
+    for (long long r = (long long)b * 8 + w; r < s.rows; r += s.blocks * 8) {
+      if (!s.counts(r)) continue;
+      const float *x = (const float *)s.x + r * s.stride;
+      if (a.wide) {
+#pragma unroll 4
+        for (int i = lane; i < a.dim / 4; i += 32) { const float4 v = ((const float4 *)x)[i]; see(v.x); see(v.y); see(v.z); see(v.w); }
+      } else for (int i = lane; i < a.dim; i += 32) see(x[i]);
     }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if ((threadIdx.x & 31) == 0 && top) atomicMax(out, top);
-}
-// Bound of |dz| / scale: |g| + |h| (p |log p| + p H), p |log p| <= 1 / e, H <= log vocab < 22.
-__global__ void __launch_bounds__(256) tab_gradmax_kernel(const float *__restrict__ g, const float *__restrict__ h, long long n, TabRows counts, unsigned *out) {
-  unsigned top = 0u;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-    if (!counts(i)) continue;
-    const float v = (g ? fabsf(g[i]) : 0.f) + (h ? 23.f * fabsf(h[i]) : 0.f);
-    const unsigned b = __float_as_uint(v);
-    if (b < 0x7f800000u && b > top) top = b;
+  } else {
+    b -= a.q.blocks + a.w.blocks;
+    for (long long i = (long long)b * 256 + threadIdx.x; i < a.n; i += a.gblocks * 256)
+      if (a.q.counts(i)) see((a.g ? fabsf(a.g[i]) : 0.f) + (a.h ? 23.f * fabsf(a.h[i]) : 0.f));
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if ((threadIdx.x & 31) == 0 && top) atomicMax(out, top);
+  top = __reduce_max_sync(0xffffffffu, top);
+  if (lane == 0) tops[w] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 8; ++i) top = max(top, tops[i]);
+    a.block_max[blockIdx.x] = top;
+  }
 }
 // 2^k that brings a number below 2^top, -100 <= k <= 100
 __device__ __forceinline__ float tab_power(unsigned bits, int top, float &inverse) {
@@ -405,33 +528,72 @@ __device__ __forceinline__ float tab_power(unsigned bits, int top, float &invers
   inverse = __uint_as_float((unsigned)(127 - k) << 23);
   return __uint_as_float((unsigned)(127 + k) << 23);
 }
-__global__ void tab_exponents_kernel(TabScales *sc, float scale, int planes, int dz) {
-  sc->q = sc->w = sc->dz = sc->iq = sc->iw = sc->idz = 1.f;
-  if (planes) { sc->q = tab_power(sc->max_q, 14, sc->iq); sc->w = tab_power(sc->max_w, 14, sc->iw); }
-  if (dz) sc->dz = tab_power(__float_as_uint(fminf(__uint_as_float(sc->max_g) * scale, 1e38f)), 14, sc->idz);
-}
-// fp32 to two fp16 planes; 16-bit elements as they are.  Rows that do not count become zeros: whatever stands in padding, a
-// product with its zero gradient is zero.
+// fp32 to two fp16 planes; 16-bit elements as they are (rows that TMA cannot read where they lie, and the gradient's queries).
+// Rows that do not count become zeros: whatever stands in padding, a product with its zero gradient is zero.
 template <class T>
-__global__ void __launch_bounds__(256) tab_pack_kernel(const T *__restrict__ x, long long stride, long long rows, int dim, TabRows counts, void *to, long long ld, long long plane,
-                                                       const float *power) {
-  const float up = sizeof(T) == 4 ? *power : 1.f;
-  for (long long r = blockIdx.x; r < rows; r += gridDim.x) {
-    const bool keep = counts(r);
-    for (int i = threadIdx.x; i < dim; i += 256) {
-      const T e = keep ? x[r * stride + i] : Tok<T>::down(0.f);
-      if (sizeof(T) == 4) {
-        const float v = Tok<T>::up(e) * up;
-        const __half b0 = __float2half_rn(v), b1 = __float2half_rn(v - __half2float(b0));
-        ((__half *)to)[r * ld + i] = b0;
-        ((__half *)to)[plane + r * ld + i] = __hisinf(b0) || __hisnan(b0) ? __float2half_rn(0.f) : b1;
-      } else ((T *)to)[r * ld + i] = e;
+__global__ void __launch_bounds__(256) tab_pack_kernel(TabPrep a) {
+  __shared__ unsigned tops[3];
+  pdl_begin();
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  float up_q = 1.f, up_w = 1.f;
+  if (a.sc) {
+    const int nq = a.planes ? a.q.blocks : 0, nw = a.planes ? a.w.blocks : 0;
+    if (w < 3) {                                                          // a warp each: queries, table, gradients
+      const int lo = w == 0 ? 0 : w == 1 ? nq : nq + nw, hi = w == 0 ? nq : w == 1 ? nq + nw : nq + nw + a.gblocks;
+      unsigned top = 0u;
+      for (int i = lo + lane; i < hi; i += 32) top = max(top, a.block_max[i]);
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (lane == 0) tops[w] = top;
+    }
+    __syncthreads();
+    TabScales s = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
+    if (a.planes) { s.q = tab_power(tops[0], 14, s.iq); s.w = tab_power(tops[1], 14, s.iw); }
+    if (a.gblocks) s.dz = tab_power(__float_as_uint(fminf(__uint_as_float(tops[2]) * a.scale, 1e38f)), 14, s.idz);
+    up_q = s.q;
+    up_w = s.w;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.sc = s;
+  }
+  const bool of_q = (int)blockIdx.x < a.q.blocks;
+  const TabSource &s = of_q ? a.q : a.w;
+  const int b = of_q ? blockIdx.x : blockIdx.x - a.q.blocks;
+  const float up = of_q ? up_q : up_w;
+  for (long long r = (long long)b * 8 + w; r < s.rows; r += s.blocks * 8) {
+    const bool keep = s.counts(r);
+    const T *x = (const T *)s.x + r * s.stride;
+    if (sizeof(T) == 4) {
+      auto split = [&](float v, __half &b0, __half &b1) {
+        b0 = __float2half_rn(v * up);
+        b1 = __hisinf(b0) || __hisnan(b0) ? __float2half_rn(0.f) : __float2half_rn(v * up - __half2float(b0));
+      };
+      __half *p0 = (__half *)s.to + r * s.ld, *p1 = p0 + s.plane;
+      if (a.wide) {
+#pragma unroll 4
+        for (int i = lane; i < a.dim / 4; i += 32) {
+          const float4 v = keep ? ((const float4 *)x)[i] : make_float4(0.f, 0.f, 0.f, 0.f);
+          __align__(8) __half h0[4], h1[4];
+          split(v.x, h0[0], h1[0]); split(v.y, h0[1], h1[1]); split(v.z, h0[2], h1[2]); split(v.w, h0[3], h1[3]);
+          ((uint2 *)p0)[i] = *(uint2 *)h0;
+          ((uint2 *)p1)[i] = *(uint2 *)h1;
+        }
+      } else for (int i = lane; i < a.dim; i += 32) {
+        __half h0, h1;
+        split(keep ? (float)Tok<T>::up(x[i]) : 0.f, h0, h1);
+        p0[i] = h0;
+        p1[i] = h1;
+      }
+    } else {
+      T *to = (T *)s.to + r * s.ld;
+      if (a.wide) {
+#pragma unroll 4
+        for (int i = lane; i < a.dim / 8; i += 32) ((uint4 *)to)[i] = keep ? ((const uint4 *)x)[i] : make_uint4(0u, 0u, 0u, 0u);
+      } else for (int i = lane; i < a.dim; i += 32) to[i] = keep ? x[i] : Tok<T>::down(0.f);
     }
   }
 }
 // The parts of a split contraction, added in their order.
 template <class T>
 __global__ void __launch_bounds__(256) tab_join_kernel(const float *__restrict__ partial, int splits, long long count, T *__restrict__ out) {
+  pdl_begin();
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < count; i += (long long)gridDim.x * 256) {
     float s = partial[i];
     for (int k = 1; k < splits; ++k) s += partial[k * count + i];
@@ -440,78 +602,96 @@ __global__ void __launch_bounds__(256) tab_join_kernel(const float *__restrict__
 }
 
 // ---- host --------------------------------------------------------------------------------------------------
-struct TabOperand { const void *base; long long rows, inner, ld, plane; };   // [planes][rows][ld], 16-bit elements
+struct TabOperand { const void *base; long long rows, inner, ld, plane; int planes; };   // [planes][rows][ld], 16-bit elements
 
-static bool tab_encode(CUtensorMap *tm, int kind, const TabOperand &o, int box_inner, int box_rows) {
-  const int npl = kind == TAB_F32 ? 2 : 1;
-  const cuuint64_t dims[3] = {(cuuint64_t)o.inner, (cuuint64_t)o.rows, (cuuint64_t)npl};
-  const cuuint64_t strides[2] = {(cuuint64_t)o.ld * 2, (cuuint64_t)(npl > 1 ? o.plane : o.ld * 8) * 2};
-  const cuuint32_t box[3] = {(cuuint32_t)box_inner, (cuuint32_t)box_rows, (cuuint32_t)npl};
-  return encode_map(tm, kind == TAB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, o.base, 3, dims, strides, box,
+static bool tab_encode(CUtensorMap *tm, bool bf16, const TabOperand &o, int box_inner, int box_rows) {
+  const cuuint64_t dims[3] = {(cuuint64_t)o.inner, (cuuint64_t)o.rows, (cuuint64_t)o.planes};
+  const cuuint64_t strides[2] = {(cuuint64_t)o.ld * 2, (cuuint64_t)(o.planes > 1 ? o.plane : o.ld * 8) * 2};
+  const cuuint32_t box[3] = {(cuuint32_t)box_inner, (cuuint32_t)box_rows, (cuuint32_t)o.planes};
+  return encode_map(tm, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, o.base, 3, dims, strides, box,
                     box_inner == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <int EPI, int KIND, bool A_MN, bool B_MN>
-static bool tab_launch(const TabOperand &a, const TabOperand &b, const TabArgs &g, cudaStream_t st) {
-  constexpr int KB = KIND == TAB_F32 ? 32 : 64;
+template <int EPI, class MATH, bool A_MN, bool B_MN, int CG>
+static bool tab_launch_as(const TabOperand &a, const TabOperand &b, TabArgs &g, cudaStream_t st) {
+  constexpr int KB = MATH::NPA == 1 ? 64 : 32;
+  constexpr bool bf16 = std::is_same<typename MATH::elem, __nv_bfloat16>::value;
   if (pbg_launch_failed()) return true;
   TabMaps maps;
-  if (!tab_encode(&maps.a, KIND, a, A_MN ? 64 : KB, A_MN ? KB : 128) || !tab_encode(&maps.b, KIND, b, B_MN ? 64 : KB, B_MN ? KB : g.BN)) return false;
-  void (*kernel)(TabMaps, TabArgs) = tab_kernel<EPI, KIND, A_MN, B_MN>;
+  if (!tab_encode(&maps.a, bf16, a, A_MN ? 64 : KB, A_MN ? KB : 128) || !tab_encode(&maps.b, bf16, b, B_MN ? 64 : KB, B_MN ? KB : g.BN / CG)) return false;
+  const int stage = MATH::NPA * 128 * KB * 2 + MATH::NPB * (g.BN / CG) * KB * 2;
+  g.stages = TAB_RING_BYTES / stage < TAB_STAGES_MAX ? TAB_RING_BYTES / stage : TAB_STAGES_MAX;
+  void (*kernel)(TabMaps, TabArgs) = tab_kernel<EPI, MATH, A_MN, B_MN, CG>;
   pbg_opt_in_smem((const void *)kernel, TAB_SMEM);
-  const long long tiles = (g.M + 127) / 128 * ((g.N + g.BN - 1) / g.BN) * g.splits, sms = pbg_sm_count();
-  pbg_launch_in_order(kernel, dim3((unsigned)(tiles < sms ? tiles : sms)), TAB_THREADS, TAB_SMEM, st, maps, g);
+  const long long tiles = (g.M + 128 * CG - 1) / (128 * CG) * ((g.N + g.BN - 1) / g.BN) * g.splits, most = pbg_sm_count() / CG;
+  const unsigned groups = (unsigned)(tiles < most ? tiles : most);
+  if (CG == 1) pbg_launch(kernel, dim3(groups), TAB_THREADS, TAB_SMEM, st, maps, g);
+  else pbg_launch_clusters(kernel, (int)groups, CG, TAB_THREADS, TAB_SMEM, st, maps, g);
   return true;
 }
 
-// Tile columns: the fewest columns for the SM with the most of them, with what a tile costs beside them.
-static int tab_columns(long long tiles_m, long long N, int step) {
-  const long long sms = pbg_sm_count();
+// Tile columns, a multiple of `step`: the fewest columns for the SM with the most of them, with what a tile costs beside them.
+static int tab_columns(long long tiles_m, long long N, int step, int cg) {
+  const long long groups = pbg_sm_count() / cg > 0 ? pbg_sm_count() / cg : 1;
   int best = 256;
   long long cost = -1;
   for (int bn = 256; bn >= step; bn -= step) {
-    const long long tiles = tiles_m * ((N + bn - 1) / bn), c = (tiles + sms - 1) / sms * (bn + 16);
+    const long long tiles = tiles_m * ((N + bn - 1) / bn), c = (tiles + groups - 1) / groups * (bn + 16);
     if (cost < 0 || c < cost) { cost = c; best = bn; }
   }
   return best;
 }
+// Pairs of CTAs where there are two row tiles for them and columns for whole halves.
+static bool tab_pairs(long long M, long long N) { return M > 128 && N > 64; }
 
-static int tab_kind(int dtype) { return dtype == PBG_F32 ? TAB_F32 : dtype == PBG_BF16 ? TAB_BF16 : TAB_F16; }
+template <int EPI, class MATH, bool A_MN, bool B_MN>
+static bool tab_launch(const TabOperand &a, const TabOperand &b, TabArgs &g, bool pairs, cudaStream_t st) {
+  g.part = MATH::NPB == 2 ? TAB_F32_PART : 0x7fffffff;
+  return pairs ? tab_launch_as<EPI, MATH, A_MN, B_MN, 2>(a, b, g, st) : tab_launch_as<EPI, MATH, A_MN, B_MN, 1>(a, b, g, st);
+}
+
 // TMA reads rows where they lie if they start on 16-byte boundaries
 static bool tab_packed(const void *p, long long stride, int dim, int dtype) { return dtype == PBG_F32 || !aligned16(p) || stride % 8 != 0 || stride < dim; }
 
 // What the workspace holds.  Its size is asked for without addresses, so it has room for packed operands wherever they may be needed.
+#define TAB_MAX_BLOCKS 1024                                  // of a preparing kernel
 struct TabPlace {
-  int64_t scales, q, w, parts, dz, partial, bytes;
+  int64_t scales, block_max, q, w, parts, dz, partial, bytes;
   long long ld, columns, ldz;         // packed rows' length; table rows per piece of dz, and its rows' length
   long long piece;                    // queries per pass of the forward
-  int npl, bn, nparts, splits;
+  int npl, bn, nparts, splits, dz_planes;
+  bool pairs;
 };
 static TabPlace tab_place(long long n, long long rows, int dim, int dtype, bool grad) {
   TabPlace p;
   p.npl = dtype == PBG_F32 ? 2 : 1;
   p.ld = tok_up(dim, 8);
   p.scales = 0;
-  p.q = 256;
+  p.block_max = 256;
+  p.q = p.block_max + TAB_MAX_BLOCKS * 4;
   p.w = p.q + tok_up(n * p.ld * 2 * p.npl, 256);
   int64_t at = p.w + tok_up(rows * p.ld * 2 * p.npl, 256);
   p.parts = p.dz = p.partial = at;
   p.columns = p.ldz = 0;
   p.piece = n;
-  p.bn = p.nparts = p.splits = 0;
+  p.bn = p.nparts = p.splits = p.dz_planes = 0;
+  p.pairs = tab_pairs(n, rows);
   if (!grad) {
-    p.bn = tab_columns((n + 127) / 128, rows, 64);
+    p.bn = tab_columns((n + (p.pairs ? 255 : 127)) / (p.pairs ? 256 : 128), rows, p.pairs ? 128 : 64, p.pairs ? 2 : 1);
     p.nparts = (int)((rows + p.bn - 1) / p.bn * 2);
-    long long most = TAB_PARTS_BYTES / (16ll * p.nparts) / 128 * 128;
-    if (most < 128) most = 128;
+    long long most = TAB_PARTS_BYTES / (16ll * p.nparts) / 256 * 256;
+    if (most < 256) most = 256;
     if (p.piece > most) p.piece = most;
     at += p.piece * p.nparts * 16;
   } else {
-    long long most = TAB_DZ_BYTES / (2 * p.npl * n) / 256 * 256;
+    // dz of 16-bit operands in two planes where the queries leave most of a tile's rows idle: few targets do not average the
+    // rounding of dz out, and the products with more planes cost nothing that the reading of the table does not cover
+    p.dz_planes = dtype == PBG_F32 || n <= 128 ? 2 : 1;
+    long long most = TAB_DZ_BYTES / (2 * p.dz_planes * n) / 256 * 256;
     if (most < 256) most = 256;
     p.columns = rows < most ? rows : most;
     p.ldz = tok_up(p.columns, 64);
-    at += tok_up(n * p.ldz * 2 * p.npl, 256);
+    at += tok_up(n * p.ldz * 2 * p.dz_planes, 256);
     p.partial = at;
     const long long tiles = (n + 127) / 128 * ((dim + 255) / 256), blocks = (p.columns + 63) / 64;
     long long s = pbg_sm_count() / tiles;
@@ -530,98 +710,113 @@ struct TabCall {
   TabOperand q, w;
 };
 
-static unsigned tab_grid(long long rows) { return (unsigned)(rows < 4096 ? rows : 4096); }
-template <class T>
-static void tab_pack(const TabCall &c, const void *x, long long stride, long long rows, bool always, const TabRows &counts, unsigned char *to, const TabPlace &p, const float *power,
-                     TabOperand &o) {
-  o = TabOperand{x, rows, c.dim, stride, 0};
-  if (!always && !tab_packed(x, stride, c.dim, c.dtype)) return;
-  o = TabOperand{to, rows, c.dim, p.ld, rows * p.ld};
-  pbg_launch_in_order(tab_pack_kernel<T>, dim3(tab_grid(rows)), 256, 0, c.st, (const T *)x, (long long)stride, rows, c.dim, counts, (void *)to, p.ld, o.plane, power);
-}
+static int tab_blocks(long long rows, int most) { const long long b = (rows + 7) / 8; return (int)(b < most ? b : most); }
 // Scales and operands.  For the gradient the queries are always copied: the rows that do not count have to be zeros.
 template <class T>
 static void tab_prepare(TabCall &c, const TabPlace &p, bool grad, const float *g, const float *h) {
-  c.sc = (TabScales *)(c.ws + p.scales);
-  c.err = c.errors ? c.errors : (int *)(c.ws + p.scales + 128);
-  if (cudaMemsetAsync(c.ws, 0, 256, c.st) != cudaSuccess) pbg_note_launch();
-  const TabRows counts{c.targets, c.ignore_index, c.rows, grad ? 0 : 1}, all{nullptr, 0, 0, 1};
   const bool planes = c.dtype == PBG_F32, dz = grad && c.dtype != PBG_BF16;
-  if (planes) {
-    pbg_launch_in_order(tab_absmax_kernel, dim3(tab_grid(c.n)), 256, 0, c.st, (const float *)c.queries, (long long)c.q_stride, (long long)c.n, c.dim, counts, &c.sc->max_q);
-    pbg_launch_in_order(tab_absmax_kernel, dim3(tab_grid(c.rows)), 256, 0, c.st, (const float *)c.table, (long long)c.t_stride, (long long)c.rows, c.dim, all, &c.sc->max_w);
+  c.sc = planes || dz ? (TabScales *)(c.ws + p.scales) : nullptr;
+  c.err = c.errors ? c.errors : (int *)(c.ws + p.scales + 128);          // (nobody reads the latter)
+  c.q = TabOperand{c.queries, c.n, c.dim, c.q_stride, 0, 1};
+  c.w = TabOperand{c.table, c.rows, c.dim, c.t_stride, 0, 1};
+  const bool pack_q = grad || tab_packed(c.queries, c.q_stride, c.dim, c.dtype), pack_w = tab_packed(c.table, c.t_stride, c.dim, c.dtype);
+  if (!pack_q && !pack_w) return;
+  constexpr int V = sizeof(T) == 4 ? 4 : 8;
+  TabPrep a = {};
+  a.q.counts = TabRows{c.targets, c.ignore_index, c.rows, grad ? 0 : 1};
+  a.w.counts = TabRows{nullptr, 0, 0, 1};
+  a.g = g; a.h = h; a.n = c.n; a.scale = c.scale; a.dim = c.dim; a.planes = planes; a.sc = c.sc;
+  a.gblocks = dz ? tab_blocks((c.n + 31) / 32, 64) : 0;
+  a.block_max = (unsigned *)(c.ws + p.block_max);
+  a.wide = c.dim % V == 0;
+  auto source = [&](TabSource &s, TabOperand &o, const void *x, long long stride, long long rows, int64_t at, int most) {
+    s.x = x; s.stride = stride; s.rows = rows; s.to = c.ws + at; s.ld = p.ld; s.plane = rows * p.ld;
+    s.blocks = tab_blocks(rows, most);
+    if (!aligned16(x) || stride % V != 0) a.wide = 0;
+    o = TabOperand{s.to, rows, c.dim, p.ld, s.plane, p.npl};
+  };
+  if (pack_q) source(a.q, c.q, c.queries, c.q_stride, c.n, p.q, 296);
+  if (pack_w) source(a.w, c.w, c.table, c.t_stride, c.rows, p.w, 592);
+  if (planes || dz) {
+    TabPrep m = a;
+    if (!planes) m.q.blocks = m.w.blocks = 0;
+    pbg_launch(tab_max_kernel, dim3(m.q.blocks + m.w.blocks + m.gblocks), 256, 0, c.st, m);
   }
-  if (dz) pbg_launch_in_order(tab_gradmax_kernel, dim3(tab_grid((c.n + 255) / 256)), 256, 0, c.st, g, h, (long long)c.n, counts, &c.sc->max_g);
-  pbg_launch_in_order(tab_exponents_kernel, dim3(1), 1, 0, c.st, c.sc, c.scale, (int)planes, (int)dz);
-  tab_pack<T>(c, c.queries, c.q_stride, c.n, grad, counts, c.ws + p.q, p, &c.sc->q, c.q);
-  tab_pack<T>(c, c.table, c.t_stride, c.rows, false, all, c.ws + p.w, p, &c.sc->w, c.w);
+  pbg_launch(tab_pack_kernel<T>, dim3(a.q.blocks + a.w.blocks), 256, 0, c.st, a);
 }
 
 struct TabForward { TabCall c; TabPlace p; float *logprob, *entropy, *lse; bool ok; };
-template <class T, int KIND>
+template <class T, class MATH>
 static void tab_forward(TabForward &f) {
   TabCall &c = f.c;
   tab_prepare<T>(c, f.p, false, nullptr, nullptr);
+  constexpr int KB = MATH::NPA == 1 ? 64 : 32;
   for (long long n0 = 0; n0 < c.n && f.ok; n0 += f.p.piece) {
     const long long n = c.n - n0 < f.p.piece ? c.n - n0 : f.p.piece;
     TabOperand q = c.q;
     q.base = (const char *)q.base + n0 * q.ld * 2;
     q.rows = n;
     TabArgs g = {};
-    g.M = n; g.N = c.rows; g.kblocks = (c.dim + (KIND == TAB_F32 ? 31 : 63)) / (KIND == TAB_F32 ? 32 : 64);
-    g.BN = f.p.bn;
-    g.splits = 1; g.m_first = 1; g.scale = c.scale; g.sc = c.sc; g.err = c.err;
-    g.unscale_q = g.unscale_w = 1.f;
+    g.M = n; g.N = c.rows; g.kblocks = (c.dim + KB - 1) / KB;
+    g.BN = f.p.bn; g.splits = 1; g.m_first = 1; g.scale = c.scale; g.sc = c.sc; g.err = c.err;
+    g.by_q = g.by_w = 1;
     g.parts = (float4 *)(c.ws + f.p.parts); g.nparts = f.p.nparts;
-    f.ok = tab_launch<EPI_STATS, KIND, false, false>(q, c.w, g, c.st);
-    pbg_launch_in_order(tab_stats_kernel<T>, dim3((unsigned)n), 128, 0, c.st, (const T *)c.queries + n0 * c.q_stride, (long long)c.q_stride, (const T *)c.table, (long long)c.t_stride,
-                        (long long)c.rows, c.dim, c.targets + n0, (long long)c.ignore_index, c.scale, (const float4 *)g.parts, g.nparts, f.logprob + n0, f.entropy + n0, f.lse + n0, c.errors);
+    f.ok = tab_launch<EPI_STATS, MATH, false, false>(q, c.w, g, f.p.pairs, c.st);
+    pbg_launch(tab_stats_kernel<T>, dim3((unsigned)n), 128, 0, c.st, (const T *)c.queries + n0 * c.q_stride, (long long)c.q_stride, (const T *)c.table, (long long)c.t_stride,
+               (long long)c.rows, c.dim, c.targets + n0, (long long)c.ignore_index, c.scale, (const float4 *)g.parts, g.nparts, f.logprob + n0, f.entropy + n0, f.lse + n0, c.errors);
   }
 }
 
 struct TabBackward { TabCall c; TabPlace p; const float *lse, *entropy, *g, *h; void *dq, *dt; bool ok; };
-template <class T, int KIND>
+// MATH: of the scores; DZMATH: of the products with dz
+template <class T, class MATH, class DZMATH>
 static void tab_backward(TabBackward &f) {
   TabCall &c = f.c;
-  constexpr int KB = KIND == TAB_F32 ? 32 : 64;
+  constexpr int KB = MATH::NPA == 1 ? 64 : 32, KB2 = DZMATH::NPA == 1 ? 64 : 32;
   tab_prepare<T>(c, f.p, true, f.g, f.h);
-  const long long tiles_m = (c.n + 127) / 128;
   const bool partial = f.p.splits > 1 || f.p.columns < c.rows;
+  auto plan = [&](TabArgs &a, bool &pairs, long long M, long long N, int splits, int step) {
+    pairs = tab_pairs(M, N);
+    a.M = M; a.N = N; a.splits = splits; a.sc = c.sc; a.err = c.err;
+    a.BN = tab_columns((M + (pairs ? 255 : 127)) / (pairs ? 256 : 128) * splits, N, pairs ? 128 : step, pairs ? 2 : 1);
+  };
   for (long long v0 = 0; v0 < c.rows && f.ok; v0 += f.p.columns) {
     const long long cols = c.rows - v0 < f.p.columns ? c.rows - v0 : f.p.columns;
     TabOperand w = c.w;
     w.base = (const char *)w.base + v0 * w.ld * 2;
     w.rows = cols;
     TabArgs g = {};
-    g.M = c.n; g.N = cols; g.kblocks = (c.dim + KB - 1) / KB; g.BN = tab_columns(tiles_m, cols, 128);
-    g.splits = 1; g.m_first = 1; g.scale = c.scale; g.sc = c.sc; g.err = c.err;
-    g.unscale_q = g.unscale_w = 1.f;
+    bool pairs;
+    plan(g, pairs, c.n, cols, 1, 64);
+    g.kblocks = (c.dim + KB - 1) / KB;
+    g.m_first = 1; g.scale = c.scale;
+    g.by_q = g.by_w = 1;
     g.targets = c.targets; g.ignore_index = c.ignore_index; g.vocab = c.rows; g.v0 = v0;
     g.lse = f.lse; g.entropy = f.entropy; g.g = f.g; g.h = f.h;
-    g.dz = c.ws + f.p.dz; g.ldz = f.p.ldz; g.dz_plane = c.n * f.p.ldz;
-    f.ok = tab_launch<EPI_DZ, KIND, false, false>(c.q, w, g, c.st);
-    const TabOperand dz{g.dz, c.n, cols, f.p.ldz, g.dz_plane};
+    g.dz = c.ws + f.p.dz; g.ldz = f.p.ldz; g.dz_plane = c.n * f.p.ldz; g.dz_planes = f.p.dz_planes;
+    f.ok = tab_launch<EPI_DZ, MATH, false, false>(c.q, w, g, pairs, c.st);
+    const TabOperand dz{g.dz, c.n, cols, f.p.ldz, g.dz_plane, f.p.dz_planes};
     if (f.dq && f.ok) {
       TabArgs d = {};
-      d.M = c.n; d.N = c.dim; d.kblocks = (cols + KB - 1) / KB; d.BN = tab_columns(tiles_m * f.p.splits, c.dim, 64);
-      d.splits = f.p.splits; d.scale = 1.f; d.sc = c.sc; d.err = c.err;
-      d.unscale_dz = d.unscale_w = 1.f;
+      plan(d, pairs, c.n, c.dim, f.p.splits, 64);
+      d.kblocks = (cols + KB2 - 1) / KB2;
+      d.by_dz = d.by_w = 1;
       d.out = f.dq; d.ldo = c.dim;
       if (partial) { d.partial = (float *)(c.ws + f.p.partial); d.add = v0 > 0; }
-      f.ok = tab_launch<EPI_OUT, KIND, false, true>(dz, w, d, c.st);
+      f.ok = tab_launch<EPI_OUT, DZMATH, false, true>(dz, w, d, pairs, c.st);
     }
     if (f.dt && f.ok) {
       TabArgs d = {};
-      d.M = cols; d.N = c.dim; d.kblocks = (c.n + KB - 1) / KB; d.BN = tab_columns((cols + 127) / 128, c.dim, 64);
-      d.splits = 1; d.scale = 1.f; d.sc = c.sc; d.err = c.err;
-      d.unscale_dz = d.unscale_q = 1.f;
+      plan(d, pairs, cols, c.dim, 1, 64);
+      d.kblocks = (c.n + KB2 - 1) / KB2;
+      d.by_dz = d.by_q = 1;
       d.out = (T *)f.dt + v0 * c.dim; d.ldo = c.dim;
-      f.ok = tab_launch<EPI_OUT, KIND, true, true>(dz, c.q, d, c.st);
+      f.ok = tab_launch<EPI_OUT, DZMATH, true, true>(dz, c.q, d, pairs, c.st);
     }
   }
   if (f.dq && partial && f.ok) {
     const long long count = c.n * c.dim, blocks = (count + 255) / 256;
-    pbg_launch_in_order(tab_join_kernel<T>, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), 256, 0, c.st, (const float *)(c.ws + f.p.partial), f.p.splits, count, (T *)f.dq);
+    pbg_launch(tab_join_kernel<T>, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), 256, 0, c.st, (const float *)(c.ws + f.p.partial), f.p.splits, count, (T *)f.dq);
   }
 }
 
@@ -651,9 +846,9 @@ extern "C" int pbg_table_logprobs(const void *queries, int64_t q_stride, int64_t
   if (!get_encode()) return PBG_ERR_CUDA;
   pbg_launch_error() = cudaSuccess;
   f.p = tab_place(n, rows, dim, dtype, false);
-  if (dtype == PBG_F32) tab_forward<float, TAB_F32>(f);
-  else if (dtype == PBG_BF16) tab_forward<__nv_bfloat16, TAB_BF16>(f);
-  else tab_forward<__half, TAB_F16>(f);
+  if (dtype == PBG_F32) tab_forward<float, TabF32>(f);
+  else if (dtype == PBG_BF16) tab_forward<__nv_bfloat16, TabBf16>(f);
+  else tab_forward<__half, TabF16>(f);
   const int status = tok_status();
   return f.ok ? status : PBG_ERR_CUDA;
 }
@@ -673,9 +868,14 @@ extern "C" int pbg_table_logprobs_grad(const void *queries, int64_t q_stride, in
   if (!lse || (grad_entropy && !entropy) || (!grad_queries && !grad_table)) return PBG_ERR_BAD_ARGUMENT;
   if (!get_encode()) return PBG_ERR_CUDA;
   f.p = tab_place(n, rows, dim, dtype, true);
-  if (dtype == PBG_F32) tab_backward<float, TAB_F32>(f);
-  else if (dtype == PBG_BF16) tab_backward<__nv_bfloat16, TAB_BF16>(f);
-  else tab_backward<__half, TAB_F16>(f);
+  if (dtype == PBG_F32) tab_backward<float, TabF32, TabF32>(f);
+  else if (dtype == PBG_BF16) {
+    if (f.p.dz_planes == 2) tab_backward<__nv_bfloat16, TabBf16, TabBf16Fine>(f);
+    else tab_backward<__nv_bfloat16, TabBf16, TabBf16>(f);
+  } else {
+    if (f.p.dz_planes == 2) tab_backward<__half, TabF16, TabF16Fine>(f);
+    else tab_backward<__half, TabF16, TabF16>(f);
+  }
   const int status = tok_status();
   return f.ok ? status : PBG_ERR_CUDA;
 }

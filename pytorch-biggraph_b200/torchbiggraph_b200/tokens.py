@@ -33,40 +33,60 @@ class TokenLogprobs(NamedTuple):
     top_ids: Optional[torch.Tensor]
 
 
+# A call is tens of microseconds of host work or it is not: the checks below ask each tensor for as little as they can.
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}                    # pbg_dtype
+_entry_points = {}
+
+
 def _matrix(name, t, dtype=None, device=None):
+    """The pbg_dtype of a matrix whose rows can be read."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor")
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise RuntimeError(f"{name} is on {t.device}: the token operators work on CUDA tensors only (no CPU fallback)")
     if device is not None and t.device != device:
         raise ValueError(f"{name} is on {t.device}, not on {device}")
-    code = _lib.DTYPE_CODES.get(str(t.dtype)[6:])
-    if code is None or (dtype is not None and t.dtype != dtype):
+    code = _DTYPES.get(t.dtype)
+    if code is None or (dtype is not None and t.dtype is not dtype):
         raise TypeError(f"{name} has type {t.dtype}" + (f", not {dtype}" if dtype is not None else "; float32, bfloat16 and float16 are supported"))
     if t.dim() != 2:
         raise ValueError(f"{name} must have two dimensions")
-    if t.shape[1] < 1:
+    width = t.shape[1]
+    if width < 1:
         raise ValueError(f"{name} has rows without elements")
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    if width > 1 and t.stride(1) != 1:
         raise ValueError(f"the elements of a row of {name} must lie next to each other")
-    _no_grad(name, t)
+    if t.requires_grad:
+        _no_grad(name)
     return code
 
 
-def _no_grad(name, t):
-    if t.requires_grad and torch.is_grad_enabled():
+def _no_grad(name):
+    if torch.is_grad_enabled():
         raise RuntimeError(f"{name} requires a gradient, which the token operators do not record: detach it or call under torch.no_grad()")
 
 
 def _vector(name, t, dtype, n, device):
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype:
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype:
         raise TypeError(f"{name} must be a tensor of {dtype}")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, not on {device}")
     if t.dim() != 1 or t.shape[0] != n:
         raise ValueError(f"{name} must have one dimension of {n} elements")
-    _no_grad(name, t)
-    return t.contiguous()
+    if t.requires_grad:
+        _no_grad(name)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _ids(ids, device):
+    if not isinstance(ids, torch.Tensor) or ids.dtype is not torch.long:
+        raise TypeError("ids must be an int64 tensor")
+    if ids.device != device:
+        raise ValueError(f"ids is on {ids.device}, not on {device}")
+    if ids.dim() != 1:
+        ids = ids.reshape(-1)
+    return ids if ids.is_contiguous() else ids.contiguous()
 
 
 def _scale(scale, positive):
@@ -91,10 +111,6 @@ def _row_stride(t):
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _workspace(size, device):
-    return torch.empty(size, dtype=torch.uint8, device=device)
-
-
 def _overlap(a, b):
     """Whether the address ranges of two strided matrices meet."""
     def span(t):
@@ -108,8 +124,30 @@ def _overlap(a, b):
 
 def _call(name, device, *args):
     """The entry point `name` on the current stream of `device`."""
-    with torch.cuda.device(device):
-        _lib.check(getattr(_lib.lib(), name)(*args, torch.cuda.current_stream(device).cuda_stream))
+    fn = _entry_points.get(name)
+    if fn is None:
+        fn = _entry_points[name] = getattr(_lib.lib(), name)
+    index = device.index
+    if torch.cuda.current_device() == index:
+        status = fn(*args, _current_stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, _current_stream(index))
+    if status:
+        _lib.check(status)
+
+
+def _workspace(name, device, *sizes):
+    """Device memory of the size that the function `name` gives, and that size.  (Under the tensors' device: it may depend on it.)"""
+    fn = _entry_points.get(name)
+    if fn is None:
+        fn = _entry_points[name] = getattr(_lib.lib(), name)
+    if torch.cuda.current_device() == device.index:
+        size = fn(*sizes)
+    else:
+        with torch.cuda.device(device.index):
+            size = fn(*sizes)
+    return torch.empty(size, dtype=torch.uint8, device=device), size
 
 
 def check_errors(errors: torch.Tensor) -> None:
@@ -126,19 +164,15 @@ def check_errors(errors: torch.Tensor) -> None:
 def embedding_lookup(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, errors: Optional[torch.Tensor] = None) -> torch.Tensor:
     """scale * table[ids]: a tensor of the table's type and of shape ids.shape + (dim,).  The table's rows may lie apart (a
     view of some columns); ids of any shape.  An id outside of the table gives a row of NaN."""
-    code = _matrix("table", table)
-    if not isinstance(ids, torch.Tensor) or ids.dtype != torch.long:
-        raise TypeError("ids must be an int64 tensor")
-    if ids.device != table.device:
-        raise ValueError(f"ids is on {ids.device}, not on {table.device}")
-    rows, dim = table.shape
-    if rows == 0 and ids.numel() > 0:
+    code, device = _matrix("table", table), table.device
+    flat = _ids(ids, device)
+    (rows, dim), n = table.shape, flat.shape[0]
+    if rows == 0 and n > 0:
         raise ValueError("table has no rows")
-    flat = ids.reshape(-1).contiguous()
-    out = torch.empty((flat.shape[0], dim), dtype=table.dtype, device=table.device)
-    _call("pbg_embedding_lookup", table.device, table.data_ptr(), _row_stride(table), rows, dim, code, flat.data_ptr(), flat.shape[0],
-          _scale(scale, False), out.data_ptr(), _error_word(errors, table.device))
-    return out.view(*ids.shape, dim)
+    out = torch.empty((n, dim), dtype=table.dtype, device=device)
+    _call("pbg_embedding_lookup", device, table.data_ptr(), _row_stride(table), rows, dim, code, flat.data_ptr(), n, _scale(scale, False),
+          out.data_ptr(), _error_word(errors, device))
+    return out if ids.dim() == 1 else out.view(*ids.shape, dim)
 
 
 def embedding_lookup_grad(grad: torch.Tensor, ids: torch.Tensor, num_rows: int, *, scale: float = 1.0, out: Optional[torch.Tensor] = None,
@@ -149,31 +183,29 @@ def embedding_lookup_grad(grad: torch.Tensor, ids: torch.Tensor, num_rows: int, 
     and leaves its other rows alone (a table that also serves as the output layer).  An id outside of the table is skipped."""
     if isinstance(grad, torch.Tensor) and grad.dim() != 2 and isinstance(ids, torch.Tensor) and tuple(grad.shape[:-1]) == tuple(ids.shape):
         grad = grad.reshape(-1, grad.shape[-1])
-    code = _matrix("grad", grad)
-    if not isinstance(ids, torch.Tensor) or ids.dtype != torch.long:
-        raise TypeError("ids must be an int64 tensor")
+    code, device = _matrix("grad", grad), grad.device
+    flat = _ids(ids, device)
     n, dim = grad.shape
-    flat = _vector("ids", ids.reshape(-1), torch.long, n, grad.device)
+    if flat.shape[0] != n:
+        raise ValueError(f"{flat.shape[0]} ids for {n} rows of grad")
     num_rows = int(num_rows)
     if num_rows < 1:
         raise ValueError("num_rows must be positive")
     if accumulate and out is None:
         raise ValueError("accumulate=True adds to `out`, which is missing")
     if out is None:
-        out = torch.empty((num_rows, dim), dtype=grad.dtype, device=grad.device)
+        out = torch.empty((num_rows, dim), dtype=grad.dtype, device=device)
     else:
-        _matrix("out", out, grad.dtype, grad.device)
+        _matrix("out", out, grad.dtype, device)
         if tuple(out.shape) != (num_rows, dim):
             raise ValueError(f"out has shape {tuple(out.shape)}, not {(num_rows, dim)}")
         if num_rows > 1 and out.stride(0) < dim:
             raise ValueError("the rows of out overlap")
         if _overlap(out, grad):
             raise ValueError("out and grad share memory")
-    L = _lib.lib()
-    size = L.pbg_embedding_lookup_grad_workspace(n, num_rows, dim)
-    ws = _workspace(size, grad.device)
-    _call("pbg_embedding_lookup_grad", grad.device, grad.data_ptr(), _row_stride(grad), flat.data_ptr(), n, num_rows, dim, code,
-          _scale(scale, False), out.data_ptr(), _row_stride(out), int(bool(accumulate)), ws.data_ptr(), size, _error_word(errors, grad.device))
+    ws, size = _workspace("pbg_embedding_lookup_grad_workspace", device, n, num_rows, dim)
+    _call("pbg_embedding_lookup_grad", device, grad.data_ptr(), _row_stride(grad), flat.data_ptr(), n, num_rows, dim, code, _scale(scale, False),
+          out.data_ptr(), _row_stride(out), int(bool(accumulate)), ws.data_ptr(), size, _error_word(errors, device))
     return out
 
 
@@ -185,19 +217,20 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, scale: float 
 
     A row whose target is ignore_index is padding: it is not read, its results are 0 (top_ids -1).  A row of -inf alone has log
     probabilities -inf and entropy 0; NaN or +inf in a row makes its log probabilities NaN; in the order of `top` NaN counts as -inf."""
-    code = _matrix("logits", logits)
+    code, device = _matrix("logits", logits), logits.device
     n, vocab = logits.shape
-    targets = _vector("targets", targets, torch.long, n, logits.device)
+    targets = _vector("targets", targets, torch.long, n, device)
     top = int(top)
     if not 0 <= top <= min(MAX_TOP, vocab):
         raise ValueError(f"top must lie between 0 and {min(MAX_TOP, vocab)}")
-    f32 = lambda *shape: torch.empty(shape, dtype=torch.float32, device=logits.device)  # noqa: E731
-    i64 = lambda *shape: torch.empty(shape, dtype=torch.long, device=logits.device)  # noqa: E731
-    r = TokenLogprobs(f32(n), f32(n), f32(n), i64(n), f32(n, top) if top else None, i64(n, top) if top else None)
-    _call("pbg_token_logprobs", logits.device, logits.data_ptr(), _row_stride(logits), n, vocab, code, targets.data_ptr(), int(ignore_index),
-          _scale(scale, True), top, r.logprob.data_ptr(), r.entropy.data_ptr(), r.lse.data_ptr(), r.rank.data_ptr(),
-          r.top_logprobs.data_ptr() if top else None, r.top_ids.data_ptr() if top else None, _error_word(errors, logits.device))
-    return r
+    logprob, entropy, lse = torch.empty((3, n), dtype=torch.float32, device=device).unbind(0)
+    rank = torch.empty(n, dtype=torch.long, device=device)
+    best = torch.empty((n, top), dtype=torch.float32, device=device) if top else None
+    best_ids = torch.empty((n, top), dtype=torch.long, device=device) if top else None
+    _call("pbg_token_logprobs", device, logits.data_ptr(), _row_stride(logits), n, vocab, code, targets.data_ptr(), int(ignore_index),
+          _scale(scale, True), top, logprob.data_ptr(), entropy.data_ptr(), lse.data_ptr(), rank.data_ptr(), _ptr(best), _ptr(best_ids),
+          _error_word(errors, device))
+    return TokenLogprobs(logprob, entropy, lse, rank, best, best_ids)
 
 
 def _row_grads(n, device, lse, entropy, grad_logprob, grad_entropy):
@@ -225,25 +258,25 @@ def token_logprobs_grad(logits: torch.Tensor, targets: torch.Tensor, lse: torch.
     """Gradient with respect to the logits of sum(grad_logprob * logprob + grad_entropy * entropy), from the lse and the entropy that
     token_logprobs returned (the entropy only where grad_entropy is given).  `out` may be `logits` itself: the gradient then takes the scores'
     place.  Rows of padding, rows whose target is out of range and rows of -inf alone get zeros."""
-    code = _matrix("logits", logits)
+    code, device = _matrix("logits", logits), logits.device
     n, vocab = logits.shape
-    targets = _vector("targets", targets, torch.long, n, logits.device)
-    lse, entropy, grad_logprob, grad_entropy = _row_grads(n, logits.device, lse, entropy, grad_logprob, grad_entropy)
+    targets = _vector("targets", targets, torch.long, n, device)
+    lse, entropy, grad_logprob, grad_entropy = _row_grads(n, device, lse, entropy, grad_logprob, grad_entropy)
     if out is None:
         # rows as far apart as those of the scores, so that both lie alike against 16 bytes
         stride = max(_row_stride(logits), vocab)
-        out = torch.empty_strided((n, vocab), (stride if stride < vocab + 4096 else vocab, 1), dtype=logits.dtype, device=logits.device)
+        out = torch.empty_strided((n, vocab), (stride if stride < vocab + 4096 else vocab, 1), dtype=logits.dtype, device=device)
     else:
-        _matrix("out", out, logits.dtype, logits.device)
+        _matrix("out", out, logits.dtype, device)
         if out.shape != logits.shape:
             raise ValueError(f"out has shape {tuple(out.shape)}, not {tuple(logits.shape)}")
         if n > 1 and out.stride(0) < vocab:
             raise ValueError("the rows of out overlap")
         if _overlap(out, logits) and (out.data_ptr() != logits.data_ptr() or _row_stride(out) != _row_stride(logits)):
             raise ValueError("out shares memory with logits without being them")
-    _call("pbg_token_logprobs_grad", logits.device, logits.data_ptr(), _row_stride(logits), n, vocab, code, targets.data_ptr(), int(ignore_index),
+    _call("pbg_token_logprobs_grad", device, logits.data_ptr(), _row_stride(logits), n, vocab, code, targets.data_ptr(), int(ignore_index),
           _scale(scale, True), lse.data_ptr(), _ptr(entropy), _ptr(grad_logprob), _ptr(grad_entropy), out.data_ptr(), _row_stride(out),
-          _error_word(errors, logits.device))
+          _error_word(errors, device))
     return out
 
 
@@ -273,13 +306,10 @@ def table_logprobs(queries: torch.Tensor, table: torch.Tensor, targets: torch.Te
     whose target is ignore_index are padding: 0."""
     code, n, rows, dim, targets = _queries_and_table(queries, table, targets)
     device = queries.device
-    r = TableLogprobs(*(torch.empty(n, dtype=torch.float32, device=device) for _ in range(3)))
-    scale, word = _scale(scale, True), _error_word(errors, device)
-    with torch.cuda.device(device):
-        size = _lib.lib().pbg_table_logprobs_workspace(n, rows, dim, code, 0)
-        ws = _workspace(size, device)
-        _call("pbg_table_logprobs", device, queries.data_ptr(), _row_stride(queries), n, table.data_ptr(), _row_stride(table), rows, dim, code, targets.data_ptr(),
-              int(ignore_index), scale, r.logprob.data_ptr(), r.entropy.data_ptr(), r.lse.data_ptr(), ws.data_ptr(), size, word)
+    r = TableLogprobs(*torch.empty((3, n), dtype=torch.float32, device=device).unbind(0))
+    ws, size = _workspace("pbg_table_logprobs_workspace", device, n, rows, dim, code, 0)
+    _call("pbg_table_logprobs", device, queries.data_ptr(), _row_stride(queries), n, table.data_ptr(), _row_stride(table), rows, dim, code, targets.data_ptr(),
+          int(ignore_index), _scale(scale, True), r.logprob.data_ptr(), r.entropy.data_ptr(), r.lse.data_ptr(), ws.data_ptr(), size, _error_word(errors, device))
     return r
 
 
@@ -294,10 +324,8 @@ def table_logprobs_grad(queries: torch.Tensor, table: torch.Tensor, targets: tor
     lse, entropy, grad_logprob, grad_entropy = _row_grads(n, device, lse, entropy, grad_logprob, grad_entropy)
     dq = torch.empty((n, dim), dtype=queries.dtype, device=device)
     dt = torch.empty((rows, dim), dtype=table.dtype, device=device)
-    scale, word = _scale(scale, True), _error_word(errors, device)
-    with torch.cuda.device(device):
-        size = _lib.lib().pbg_table_logprobs_workspace(n, rows, dim, code, 1)
-        ws = _workspace(size, device)
-        _call("pbg_table_logprobs_grad", device, queries.data_ptr(), _row_stride(queries), n, table.data_ptr(), _row_stride(table), rows, dim, code, targets.data_ptr(),
-              int(ignore_index), scale, lse.data_ptr(), _ptr(entropy), _ptr(grad_logprob), _ptr(grad_entropy), dq.data_ptr(), dt.data_ptr(), ws.data_ptr(), size, word)
+    ws, size = _workspace("pbg_table_logprobs_workspace", device, n, rows, dim, code, 1)
+    _call("pbg_table_logprobs_grad", device, queries.data_ptr(), _row_stride(queries), n, table.data_ptr(), _row_stride(table), rows, dim, code, targets.data_ptr(),
+          int(ignore_index), _scale(scale, True), lse.data_ptr(), _ptr(entropy), _ptr(grad_logprob), _ptr(grad_entropy), dq.data_ptr(), dt.data_ptr(),
+          ws.data_ptr(), size, _error_word(errors, device))
     return dq, dt

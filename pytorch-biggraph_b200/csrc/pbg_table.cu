@@ -51,7 +51,7 @@ struct TabScales { float q, w, dz, iq, iw, idz; };
 struct TabMaps { CUtensorMap a, b; };
 struct TabArgs {
   long long M, N;                     // rows and columns of the product
-  long long kblocks;                  // blocks of KB k-values
+  int kblocks;                        // blocks of KB k-values
   int BN, splits, m_first;            // tile columns; parts of the contraction; the tiles of one column go to neighbouring CTAs
   int stages, part;                   // stages of the ring; k-blocks added up in tensor memory at a time
   float scale;
@@ -64,6 +64,7 @@ struct TabArgs {
   void *out; long long ldo;           // EPI_OUT: the result, or
   float *partial; int add;            //          [splits][M][N] fp32, stored or added
   int by_q, by_w, by_dz;              // which powers the product carries
+  int b_whole;                        // MN-major B: its rows are whole blocks of 64 columns, read as one box
 };
 
 __device__ __forceinline__ uint32_t cta_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
@@ -78,6 +79,13 @@ __device__ __forceinline__ void tab_load(uint32_t dst, const CUtensorMap *map, i
   if (CG == 1) tma_load_3d(dst, map, c0, c1, 0, bar);
   else asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
                     :: "r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(0), "r"(bar) : "memory");
+}
+// blocks of 64 columns: (0, k row, 0, block)
+template <int CG>
+__device__ __forceinline__ void tab_load_blocks(uint32_t dst, const CUtensorMap *map, int k, int block, uint32_t bar) {
+  if (CG == 1) tma_load_4d(dst, map, 0, k, 0, block, bar);
+  else asm volatile("cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                    :: "r"(dst), "l"(map), "r"(0), "r"(k), "r"(0), "r"(block), "r"(bar) : "memory");
 }
 template <int CG>
 __device__ __forceinline__ void tab_mma(uint32_t acc, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
@@ -148,47 +156,45 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
   const long long tiles_m = (g.M + 128 * CG - 1) / (128 * CG), tiles_n = (g.N + g.BN - 1) / g.BN, per_split = tiles_m * tiles_n, ntiles = per_split * g.splits;
   const long long first = blockIdx.x / CG, step = gridDim.x / CG;
   // m0: this CTA's rows; n0: the tile's columns
-  auto tile = [&](long long t, long long &m0, long long &n0, int &split, long long &kb0, long long &kb1) {
+  auto tile = [&](long long t, long long &m0, long long &n0, int &split, int &kb0, int &kb1) {
     split = (int)(t / per_split);
     t -= split * per_split;
     const long long m = g.m_first ? t % tiles_m : t / tiles_n, n = g.m_first ? t / tiles_m : t % tiles_n;
     m0 = m * 128 * CG + 128 * rank;
     n0 = n * g.BN;
-    kb0 = g.kblocks * split / g.splits;
-    kb1 = g.kblocks * (split + 1) / g.splits;
+    kb0 = (int)((long long)g.kblocks * split / g.splits);
+    kb1 = (int)((long long)g.kblocks * (split + 1) / g.splits);
   };
   const int b_cols = g.BN / CG;                                          // columns of B in this CTA
   const uint32_t b_plane = B_MN ? ATOM_BYTES : (uint32_t)b_cols * ROW_BYTES;
   const uint32_t stage_bytes = A_BYTES + NPB * (uint32_t)b_cols * ROW_BYTES;
 
   if (warp == 0) {
-    // ---------------- TMA: one box per K-major operand, one per 64 columns of an MN-major one, each from its own lane
-    StageRing at;
-    bool stop = false;
-    constexpr int A_BOXES = A_MN ? 2 : 1;
-    const int boxes = A_BOXES + (B_MN ? b_cols / 64 : 1);
-    for (long long t = first; t < ntiles && !stop; t += step) {
-      long long m0, n0, kb0, kb1;
-      int split;
-      tile(t, m0, n0, split, kb0, kb1);
-      n0 += rank * b_cols;
-      for (long long kb = kb0; kb < kb1; ++kb, at.next(g.stages)) {
-        bool ok = failed == 0;
-        if (ok && lane == 0) ok = mbar_wait(empty_bar(at.s), at.parity ^ 1u, g.err);
-        if (!__all_sync(0xffffffffu, ok)) { failed = 1; stop = true; break; }
-        const uint32_t a = smem_u32(smem) + (uint32_t)at.s * stage_bytes, b = a + A_BYTES;
-        // a pair's loads are all counted by the first CTA, which issues the products
-        const uint32_t fb = CG == 1 ? full_bar(at.s) : in_first_cta(full_bar(at.s));
-        if (lane == 0 && rank == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(full_bar(at.s)), "r"(CG * stage_bytes) : "memory");
-        __syncwarp();
-        const int k = (int)(kb * KB);
-        if (lane < A_BOXES) {
-          if (A_MN) tab_load<CG>(a + lane * NPA * ATOM_BYTES, &maps.a, (int)m0 + 64 * lane, k, fb);
+    // ---------------- TMA: one box per operand, or one per 64 columns of an MN-major one.  One thread does it all: a stage takes
+    // it 294 cycles with two boxes.  One lane that waits, a vote, and a box from each of two lanes took 560, which is more than the
+    // stage's products (512).
+    if (lane == 0) {
+      StageRing at;
+      bool ok = true;
+      for (long long t = first; t < ntiles && ok; t += step) {
+        long long m0, n0;
+        int split, kb0, kb1;
+        tile(t, m0, n0, split, kb0, kb1);
+        n0 += rank * b_cols;
+        ok = failed == 0;
+        for (int kb = kb0; kb < kb1 && ok; ++kb, at.next(g.stages)) {
+          ok = mbar_wait(empty_bar(at.s), at.parity ^ 1u, g.err);
+          if (!ok) { failed = 1; break; }
+          const uint32_t a = smem_u32(smem) + (uint32_t)at.s * stage_bytes, b = a + A_BYTES;
+          // a pair's loads are all counted by the first CTA, which issues the products
+          const uint32_t fb = CG == 1 ? full_bar(at.s) : in_first_cta(full_bar(at.s));
+          if (rank == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(full_bar(at.s)), "r"(CG * stage_bytes) : "memory");
+          const int k = kb * KB;
+          if (A_MN) tab_load_blocks<CG>(a, &maps.a, k, (int)(m0 / 64), fb);
           else tab_load<CG>(a, &maps.a, k, (int)m0, fb);
-        } else if (lane < boxes) {
-          const int j = lane - A_BOXES;
-          if (B_MN) tab_load<CG>(b + j * NPB * ATOM_BYTES, &maps.b, (int)n0 + 64 * j, k, fb);
-          else tab_load<CG>(b, &maps.b, k, (int)n0, fb);
+          if (!B_MN) tab_load<CG>(b, &maps.b, k, (int)n0, fb);
+          else if (g.b_whole) tab_load_blocks<CG>(b, &maps.b, k, (int)(n0 / 64), fb);
+          else for (int j = 0; j < b_cols / 64; ++j) tab_load<CG>(b + j * NPB * ATOM_BYTES, &maps.b, (int)n0 + 64 * j, k, fb);
         }
       }
     }
@@ -205,31 +211,34 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
     int j = 0;
     bool ok = rank == 0;
     for (long long t = first; t < ntiles && ok; t += step) {
-      long long m0, n0, kb0, kb1;
-      int split;
+      long long m0, n0;
+      int split, kb0, kb1;
       tile(t, m0, n0, split, kb0, kb1);
-      for (long long p0 = kb0; p0 < kb1 && ok; p0 += g.part, ++j) {
+      for (int p0 = kb0, p1; p0 < kb1 && ok; p0 = p1, ++j) {
         const int ab = j & 1;
-        const long long p1 = kb1 - p0 < g.part ? kb1 : p0 + g.part;
+        p1 = kb1 - p0 < g.part ? kb1 : p0 + g.part;
         ok = failed == 0 && (CG == 1 ? mbar_wait(acce_bar(ab), (uint32_t)((j >> 1) & 1) ^ 1u, g.err) : pair_wait(acce_bar(ab), (uint32_t)((j >> 1) & 1) ^ 1u, g.err));
         if (!__all_sync(0xffffffffu, ok)) { failed = 1; ok = false; break; }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t acc = tmem + (uint32_t)ab * 256u;
-        for (long long kb = p0; kb < p1; ++kb, at.next(g.stages)) {
-          ok = CG == 1 ? mbar_wait(full_bar(at.s), at.parity, g.err) : pair_wait(full_bar(at.s), at.parity, g.err);
+        for (int kb = p0; kb < p1; ++kb, at.next(g.stages)) {
+          ok = mbar_wait(full_bar(at.s), at.parity, g.err);
           if (!__all_sync(0xffffffffu, ok)) { failed = 1; ok = false; break; }
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           const uint32_t a = smem_u32(smem) + (uint32_t)at.s * stage_bytes, b = a + A_BYTES;
           const uint64_t da = A_MN ? smem_desc(a, NPA * ATOM_BYTES, 1024, 2) : smem_desc(a, 0, K_SBO, K_LAYOUT);
           const uint64_t db = B_MN ? smem_desc(b, NPB * ATOM_BYTES, 1024, 2) : smem_desc(b, 0, K_SBO, K_LAYOUT);
+          // (one branch for all of a stage: each of its own costs the issuing warp more than a product takes)
+          if (leader) {
 #pragma unroll
-          for (int k = 0; k < KB / 16; ++k) {
-            const bool more = kb > p0 || k > 0;
-            if (NPA == 2 && leader) tab_mma<CG>(acc, desc_at(da, a_plane + k * a_step), desc_at(db, k * b_step), idesc, more);
-            if (NPB == 2 && leader) tab_mma<CG>(acc, desc_at(da, k * a_step), desc_at(db, b_plane + k * b_step), idesc, true);
-            if (leader) tab_mma<CG>(acc, desc_at(da, k * a_step), desc_at(db, k * b_step), idesc, NPA == 2 || more);
+            for (int k = 0; k < KB / 16; ++k) {
+              const bool more = k > 0 || kb > p0;
+              if (NPA == 2) tab_mma<CG>(acc, desc_at(da, a_plane + k * a_step), desc_at(db, k * b_step), idesc, more);
+              if (NPB == 2) tab_mma<CG>(acc, desc_at(da, k * a_step), desc_at(db, b_plane + k * b_step), idesc, true);
+              tab_mma<CG>(acc, desc_at(da, k * a_step), desc_at(db, k * b_step), idesc, NPA == 2 || more);
+            }
+            tab_commit<CG>(empty_bar(at.s));
           }
-          if (leader) tab_commit<CG>(empty_bar(at.s));
+          __syncwarp();
         }
         if (ok && leader) tab_commit<CG>(accf_bar(ab));
       }
@@ -247,8 +256,8 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
     int j = 0;
     bool ok = true;
     for (long long t = first; t < ntiles && ok; t += step) {
-      long long m0, n0, kb0, kb1;
-      int split;
+      long long m0, n0;
+      int split, kb0, kb1;
       tile(t, m0, n0, split, kb0, kb1);
       const long long m = m0 + q * 32 + lane;
       // what a row of dz takes, read while the products run
@@ -272,7 +281,7 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
       float sum[PARTS ? 128 : 1];
       auto wait_full = [&]() {
         bool w = failed == 0;
-        if (w && lane == 0) w = CG == 1 ? mbar_wait(accf_bar(j & 1), (uint32_t)(j >> 1) & 1, g.err) : pair_wait(accf_bar(j & 1), (uint32_t)(j >> 1) & 1, g.err);
+        if (w && lane == 0) w = mbar_wait(accf_bar(j & 1), (uint32_t)(j >> 1) & 1, g.err);
         if (!__all_sync(0xffffffffu, w)) { failed = 1; return false; }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         return true;
@@ -286,7 +295,7 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
       if (PARTS) {
 #pragma unroll
         for (int i = 0; i < 128; ++i) sum[PARTS ? i : 0] = 0.f;
-        for (long long p0 = kb0; p0 < kb1; p0 += g.part) {
+        for (int p0 = kb0; p0 < kb1; p0 = kb1 - p0 < g.part ? kb1 : p0 + g.part) {
           ok = wait_full();
           if (!ok) break;
 #pragma unroll
@@ -612,13 +621,25 @@ static bool tab_encode(CUtensorMap *tm, bool bf16, const TabOperand &o, int box_
                     box_inner == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// The same for an MN-major operand whose rows (with the room behind them) are whole blocks of 64 columns: the blocks are a dimension
+// of their own, so that `blocks` of them are one box.  A box costs its issue; what lies beyond `inner` belongs to columns that are clipped.
+static bool tab_encode_blocks(CUtensorMap *tm, bool bf16, const TabOperand &o, int box_rows, int blocks) {
+  const cuuint64_t dims[4] = {64, (cuuint64_t)o.rows, (cuuint64_t)o.planes, (cuuint64_t)((o.inner + 63) / 64)};
+  const cuuint64_t strides[3] = {(cuuint64_t)o.ld * 2, (cuuint64_t)(o.planes > 1 ? o.plane : o.ld * 8) * 2, 128};
+  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, (cuuint32_t)o.planes, (cuuint32_t)blocks};
+  return encode_map(tm, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, o.base, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+static bool tab_whole(const TabOperand &o) { return o.inner % 64 == 0 || o.ld >= tok_up(o.inner, 64); }
+
 template <int EPI, class MATH, bool A_MN, bool B_MN, int CG>
 static bool tab_launch_as(const TabOperand &a, const TabOperand &b, TabArgs &g, cudaStream_t st) {
   constexpr int KB = MATH::NPA == 1 ? 64 : 32;
   constexpr bool bf16 = std::is_same<typename MATH::elem, __nv_bfloat16>::value;
   if (pbg_launch_failed()) return true;
   TabMaps maps;
-  if (!tab_encode(&maps.a, bf16, a, A_MN ? 64 : KB, A_MN ? KB : 128) || !tab_encode(&maps.b, bf16, b, B_MN ? 64 : KB, B_MN ? KB : g.BN / CG)) return false;
+  g.b_whole = B_MN && tab_whole(b);
+  if (!(A_MN ? tab_encode_blocks(&maps.a, bf16, a, KB, 2) : tab_encode(&maps.a, bf16, a, KB, 128))) return false;
+  if (!(g.b_whole ? tab_encode_blocks(&maps.b, bf16, b, KB, g.BN / CG / 64) : tab_encode(&maps.b, bf16, b, B_MN ? 64 : KB, B_MN ? KB : g.BN / CG))) return false;
   const int stage = MATH::NPA * 128 * KB * 2 + MATH::NPB * (g.BN / CG) * KB * 2;
   g.stages = TAB_RING_BYTES / stage < TAB_STAGES_MAX ? TAB_RING_BYTES / stage : TAB_STAGES_MAX;
   void (*kernel)(TabMaps, TabArgs) = tab_kernel<EPI, MATH, A_MN, B_MN, CG>;
@@ -665,7 +686,7 @@ struct TabPlace {
 static TabPlace tab_place(long long n, long long rows, int dim, int dtype, bool grad) {
   TabPlace p;
   p.npl = dtype == PBG_F32 ? 2 : 1;
-  p.ld = tok_up(dim, 8);
+  p.ld = tok_up(dim, 64);
   p.scales = 0;
   p.block_max = 256;
   p.q = p.block_max + TAB_MAX_BLOCKS * 4;
@@ -757,7 +778,7 @@ static void tab_forward(TabForward &f) {
     q.base = (const char *)q.base + n0 * q.ld * 2;
     q.rows = n;
     TabArgs g = {};
-    g.M = n; g.N = c.rows; g.kblocks = (c.dim + KB - 1) / KB;
+    g.M = n; g.N = c.rows; g.kblocks = (int)((c.dim + KB - 1) / KB);
     g.BN = f.p.bn; g.splits = 1; g.m_first = 1; g.scale = c.scale; g.sc = c.sc; g.err = c.err;
     g.by_q = g.by_w = 1;
     g.parts = (float4 *)(c.ws + f.p.parts); g.nparts = f.p.nparts;
@@ -788,7 +809,7 @@ static void tab_backward(TabBackward &f) {
     TabArgs g = {};
     bool pairs;
     plan(g, pairs, c.n, cols, 1, 64);
-    g.kblocks = (c.dim + KB - 1) / KB;
+    g.kblocks = (int)((c.dim + KB - 1) / KB);
     g.m_first = 1; g.scale = c.scale;
     g.by_q = g.by_w = 1;
     g.targets = c.targets; g.ignore_index = c.ignore_index; g.vocab = c.rows; g.v0 = v0;
@@ -799,7 +820,7 @@ static void tab_backward(TabBackward &f) {
     if (f.dq && f.ok) {
       TabArgs d = {};
       plan(d, pairs, c.n, c.dim, f.p.splits, 64);
-      d.kblocks = (cols + KB2 - 1) / KB2;
+      d.kblocks = (int)((cols + KB2 - 1) / KB2);
       d.by_dz = d.by_w = 1;
       d.out = f.dq; d.ldo = c.dim;
       if (partial) { d.partial = (float *)(c.ws + f.p.partial); d.add = v0 > 0; }
@@ -808,7 +829,7 @@ static void tab_backward(TabBackward &f) {
     if (f.dt && f.ok) {
       TabArgs d = {};
       plan(d, pairs, cols, c.dim, 1, 64);
-      d.kblocks = (c.n + KB2 - 1) / KB2;
+      d.kblocks = (int)((c.n + KB2 - 1) / KB2);
       d.by_dz = d.by_q = 1;
       d.out = (T *)f.dt + v0 * c.dim; d.ldo = c.dim;
       f.ok = tab_launch<EPI_OUT, DZMATH, true, true>(dz, c.q, d, pairs, c.st);

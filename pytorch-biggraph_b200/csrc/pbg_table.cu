@@ -98,17 +98,6 @@ __device__ __forceinline__ void tab_commit(uint32_t bar) {
   if (CG == 1) mma_commit(bar);
   else asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" :: "r"(bar), "h"((unsigned short)3) : "memory");
 }
-// a wait for arrivals of both CTAs of a pair
-__device__ __forceinline__ bool pair_wait(uint32_t bar, uint32_t parity, int *err) {
-  for (int it = 0; it < TC_WAIT_LIMIT; ++it) {
-    uint32_t ok;
-    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-    if (ok) return true;
-  }
-  atomicOr(err, TOK_ERR_TIMEOUT);
-  return false;
-}
-
 template <int EPI, class MATH, bool A_MN, bool B_MN, int CG>
 __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_constant__ TabMaps maps, TabArgs g) {
   using Elem = typename MATH::elem;
@@ -133,7 +122,7 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
   auto acce_bar = [&](int a) { return bar0 + 8u * (2 * TAB_STAGES_MAX + 2 + a); };
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2 * TAB_STAGES_MAX + 2; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar0 + 8u * i));
-    for (int a = 0; a < 2; ++a) asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(acce_bar(a)), "r"(32 * TAB_EPI_WARPS * CG));
+    for (int a = 0; a < 2; ++a) asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(acce_bar(a)), "r"(TAB_EPI_WARPS * CG));
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     failed = 0;
   }
@@ -217,7 +206,7 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
       for (int p0 = kb0, p1; p0 < kb1 && ok; p0 = p1, ++j) {
         const int ab = j & 1;
         p1 = kb1 - p0 < g.part ? kb1 : p0 + g.part;
-        ok = failed == 0 && (CG == 1 ? mbar_wait(acce_bar(ab), (uint32_t)((j >> 1) & 1) ^ 1u, g.err) : pair_wait(acce_bar(ab), (uint32_t)((j >> 1) & 1) ^ 1u, g.err));
+        ok = failed == 0 && mbar_wait(acce_bar(ab), (uint32_t)((j >> 1) & 1) ^ 1u, g.err);
         if (!__all_sync(0xffffffffu, ok)) { failed = 1; ok = false; break; }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t acc = tmem + (uint32_t)ab * 256u;
@@ -253,6 +242,7 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
       unscale = (g.by_q ? g.sc->iq : 1.f) * (g.by_w ? g.sc->iw : 1.f) * (g.by_dz ? g.sc->idz : 1.f);
       up *= g.sc->dz;
     }
+    const float to2 = g.scale * unscale * TOK_LOG2E;                      // from an accumulator to a score in base 2
     int j = 0;
     bool ok = true;
     for (long long t = first; t < ntiles && ok; t += step) {
@@ -260,18 +250,16 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
       int split, kb0, kb1;
       tile(t, m0, n0, split, kb0, kb1);
       const long long m = m0 + q * 32 + lane;
-      // what a row of dz takes, read while the products run
-      float lse = 0.f, H = 0.f, gg = 0.f, hh = 0.f;
+      // what a row of dz takes, read while the products run: dz = -p (gg + hh log2 p) (+ g0 at the target)
+      float lse = 0.f, g0 = 0.f, gg = 0.f, hh = 0.f;
       long long hot = -1;
-      bool live = false;                                                 // neither padding nor without a target
       if (EPI == EPI_DZ && m < g.M) {
         const long long target = g.targets[m];
         if (target >= 0 && target < g.vocab && target != g.ignore_index) {
-          lse = g.lse[m];
-          if (g.g) gg = g.g[m] * up;
-          if (g.h) { hh = g.h[m] * up; H = g.entropy[m]; }
+          lse = g.lse[m] * TOK_LOG2E;
+          if (g.g) g0 = gg = g.g[m] * up;
+          if (g.h) { const float h = g.h[m] * up; hh = h * TOK_LN2; gg = fmaf(h, g.entropy[m], gg); }
           hot = target - g.v0;
-          live = true;
         } else if (target != g.ignore_index && n0 == 0 && half == 0 && g.v0 == 0) atomicOr(g.err, TOK_ERR_ID);
       }
       const long long c0 = n0 + half * hc;                               // first column of this warp
@@ -286,10 +274,14 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         return true;
       };
+      // (one arrival per warp, and no release beyond the tensor memory's: a release to the cluster waits for every store made so far)
       auto give_back = [&]() {
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        if (CG == 1) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(acce_bar(j & 1)) : "memory");
-        else asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" :: "r"(drained + 8u * (j & 1)) : "memory");
+        __syncwarp();
+        if (lane == 0) {
+          if (CG == 1) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(acce_bar(j & 1)) : "memory");
+          else asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" :: "r"(drained + 8u * (j & 1)) : "memory");
+        }
         ++j;
       };
       if (PARTS) {
@@ -339,38 +331,43 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
         float v[32];
         values(x, v);
         if (EPI == EPI_STATS) {
-          const float c = g.scale * unscale * TOK_LOG2E;
-          if (cols - x < 32) {
+          float cm = -INFINITY;
+          const bool whole = cols - x >= 32;                               // (else columns that do not exist are left out)
 #pragma unroll
-            for (int i = 0; i < 32; ++i) if (i >= cols - x) v[i] = -INFINITY;                        // (columns that do not exist)
-          }
-          float cm = v[0];
-#pragma unroll
-          for (int i = 1; i < 32; ++i) cm = fmaxf(cm, v[i]);
+          for (int i = 0; i < 32; ++i) if (whole || i < cols - x) cm = fmaxf(cm, v[i]);
           if (cm > mx) {
             mx = cm;
-            const float d = fminf(fmaxf(r - cm * c, -1e30f), 0.f), f = tok_ex2(d);
+            const float d = fminf(fmaxf(r - cm * to2, -1e30f), 0.f), f = tok_ex2(d);
             T = (T + d * S) * f;
             S *= f;
-            r = cm * c;
+            r = cm * to2;
           }
+          if (whole) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float y = tok_max_nan(fmaf(v[i], c, -r), -1000.f), e = tok_ex2(y);
-            S += e;
-            T = fmaf(y, e, T);
+            for (int i = 0; i < 32; ++i) {
+              const float y = fmaf(v[i], to2, -r), e = tok_ex2(y);
+              S += e;
+              T = fmaf(y, e, T);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) if (i < cols - x) {
+              const float y = fmaf(v[i], to2, -r), e = tok_ex2(y);
+              S += e;
+              T = fmaf(y, e, T);
+            }
           }
         } else if (EPI == EPI_DZ) {
-          const float zs = g.scale * unscale;
           const long long col = c0 + x;
+          // a row that does not count is a query of zeros: its score is 0, and with lse = gg = hh = 0 so is its dz
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
-            const float logp = fmaf(v[i], zs, -lse), p = tok_ex2(logp * TOK_LOG2E);
-            v[i] = live && (p > 0.f || p != p) ? -p * fmaf(hh, logp + H, gg) : 0.f;
+            const float y = fmaf(v[i], to2, -lse), p = tok_ex2(y);       // log p and p, in base 2
+            v[i] = -p * fmaf(hh, y, gg);
           }
           if (__any_sync(0xffffffffu, hot >= col && hot < col + 32)) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) if (hot == col + i) v[i] += gg;
+            for (int i = 0; i < 32; ++i) if (hot == col + i) v[i] += g0;
           }
           if (col + 32 > g.N) {
 #pragma unroll
@@ -662,6 +659,22 @@ static int tab_columns(long long tiles_m, long long N, int step, int cg) {
   }
   return best;
 }
+// Parts of dQ's contraction over K table rows: the rounds of tiles that the SMs make, shortened by the parts, against writing and
+// reading the parts' sums (in ns: 4096 products a cycle and SM at 1.7 GHz, 5 TB/s, 3 us for the launch that joins them).
+static bool tab_pairs(long long M, long long N);
+static int tab_splits(long long n, long long dim, long long K, int products) {
+  const bool pairs = tab_pairs(n, dim);
+  const long long groups = pbg_sm_count() / (pairs ? 2 : 1) > 0 ? pbg_sm_count() / (pairs ? 2 : 1) : 1;
+  const long long tiles = (n + (pairs ? 255 : 127)) / (pairs ? 256 : 128) * ((dim + 255) / 256);
+  int best = 1;
+  double cost = 0.;
+  for (int s = 1; s <= 64 && (s == 1 || s * 512ll <= K); ++s) {
+    const double rounds = (double)((tiles * s + groups - 1) / groups) / s;
+    const double c = rounds * ((double)K / 16 * products * 128 / 1.7) + (s > 1 ? 3000. + s * 8. * n * dim / 5000. : 0.);
+    if (s == 1 || c < cost) { cost = c; best = s; }
+  }
+  return best;
+}
 // Pairs of CTAs where there are two row tiles for them and columns for whole halves.
 static bool tab_pairs(long long M, long long N) { return M > 128 && N > 64; }
 
@@ -714,10 +727,7 @@ static TabPlace tab_place(long long n, long long rows, int dim, int dtype, bool 
     p.ldz = tok_up(p.columns, 64);
     at += tok_up(n * p.ldz * 2 * p.dz_planes, 256);
     p.partial = at;
-    const long long tiles = (n + 127) / 128 * ((dim + 255) / 256), blocks = (p.columns + 63) / 64;
-    long long s = pbg_sm_count() / tiles;
-    if (s > blocks / 8) s = blocks / 8;
-    p.splits = (int)(s < 1 ? 1 : s);
+    p.splits = tab_splits(n, dim, p.columns, dtype == PBG_F32 ? 3 : p.dz_planes);
     if (p.splits > 1 || p.columns < rows) at += tok_up((int64_t)p.splits * n * dim * 4, 256);
   }
   p.bytes = at;

@@ -34,8 +34,8 @@ enum { EPI_STATS = 0, EPI_DZ = 1, EPI_OUT = 2 };
 #define TAB_DZ_BYTES (2ll << 30)                            // most memory for dz: beyond it the table goes in pieces
 #define TAB_PARTS_BYTES (512ll << 20)                       // and for the tiles' partial sums: beyond it the queries do
 // The tensor cores cut off what they add up instead of rounding it, a bias of half a step per addition.  Contractions of
-// fp32 operands are therefore cut into parts of this many blocks of 32 k-values (24 additions), which are added in registers.
-#define TAB_F32_PART 4
+// fp32 operands are therefore cut into parts of this many blocks of 32 k-values (48 additions), which are added in registers.
+#define TAB_F32_PART 8
 
 // Operands: their elements, the planes of A and B, the type of results
 template <class E, class O, int PA, int PB> struct TabMath { using elem = E; using out = O; static constexpr int NPA = PA, NPB = PB; };
@@ -48,7 +48,7 @@ using TabF16Fine = TabMath<__half, __half, 2, 1>;
 // Powers of two that the operands were multiplied by, and their inverses
 struct TabScales { float q, w, dz, iq, iw, idz; };
 
-struct TabMaps { CUtensorMap a, b; };
+struct TabMaps { CUtensorMap a, b, c; };                              // operands; dz, to be written
 struct TabArgs {
   long long M, N;                     // rows and columns of the product
   int kblocks;                        // blocks of KB k-values
@@ -60,7 +60,7 @@ struct TabArgs {
   float4 *parts; int nparts;          // EPI_STATS: [M][nparts] (reference in base 2, S, T)
   const long long *targets; long long ignore_index, vocab, v0;         // EPI_DZ; v0: the table's row of column 0
   const float *lse, *entropy, *g, *h;
-  void *dz; long long ldz, dz_plane; int dz_planes;
+  long long ldz; int dz_planes;
   void *out; long long ldo;           // EPI_OUT: the result, or
   float *partial; int add;            //          [splits][M][N] fp32, stored or added
   int by_q, by_w, by_dz;              // which powers the product carries
@@ -243,6 +243,7 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
       up *= g.sc->dz;
     }
     const float to2 = g.scale * unscale * TOK_LOG2E;                      // from an accumulator to a score in base 2
+    const int planes = NPB == 2 ? 2 : g.dz_planes;
     int j = 0;
     bool ok = true;
     for (long long t = first; t < ntiles && ok; t += step) {
@@ -373,26 +374,32 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
 #pragma unroll
             for (int i = 0; i < 32; ++i) if (col + i >= g.N) v[i] = 0.f;
           }
-          // a plane of 32 x 32 values at a time through shared memory: a row's 64 bytes leave together
-          for (int pl = 0; pl < g.dz_planes; ++pl) {
-            __syncwarp();
+          // planes of 32 x 32 values through shared memory (64-byte swizzle); each leaves as one bulk store, clipped at the last row
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          __syncwarp();
+#pragma unroll
+          for (int pl = 0; pl < 2; ++pl) {
+            if (pl >= planes) break;
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
               uint32_t w[4];
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                Elem e[2] = {Tok<Elem>::down(v[8 * u + 2 * i]), Tok<Elem>::down(v[8 * u + 2 * i + 1])};
-                v[8 * u + 2 * i] -= Tok<Elem>::up(e[0]);                 // what the next plane holds
-                v[8 * u + 2 * i + 1] -= Tok<Elem>::up(e[1]);
-                w[i] = *reinterpret_cast<uint32_t *>(e);
+                float &a = v[8 * u + 2 * i], &b = v[8 * u + 2 * i + 1];
+                const typename TokPair<Elem>::type e = TokPair<Elem>::down(a, b);
+                if (pl == 0) { const float2 f = TokPair<Elem>::up(e); a -= f.x; b -= f.y; }          // what the second plane holds
+                w[i] = *reinterpret_cast<const uint32_t *>(&e);
               }
-              *reinterpret_cast<uint4 *>(buf + lane * 64 + ((u ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+              *reinterpret_cast<uint4 *>(buf + pl * 2048 + lane * 64 + ((u ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
             }
-            __syncwarp();
-            Elem *to = (Elem *)g.dz + pl * g.dz_plane + (m0 + q * 32) * g.ldz + col;
-#pragma unroll 8
-            for (int r0 = lane >> 4; r0 < rows; r0 += 2)
-              reinterpret_cast<uint32_t *>(to + r0 * g.ldz)[lane & 15] = *reinterpret_cast<uint32_t *>(buf + r0 * 64 + ((((lane & 15) >> 2) ^ ((r0 >> 1) & 3)) << 4) + ((lane & 3) << 2));
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0 && rows > 0) {
+            for (int pl = 0; pl < planes; ++pl)
+              asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];"
+                           :: "l"(&maps.c), "r"((int)col), "r"((int)(m0 + q * 32)), "r"(pl), "r"(smem_u32(buf + pl * 2048)) : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
           }
         } else {
           __syncwarp();
@@ -417,6 +424,7 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
       if (EPI == EPI_STATS && m < g.M) g.parts[m * g.nparts + n0 / g.BN * 2 + half] = make_float4(S == 0.f ? -1e30f : r, S, T, 0.f);
       if (!PARTS && kb0 < kb1) give_back();
     }
+    if (EPI == EPI_DZ && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");         // the stores are performed
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
@@ -610,10 +618,10 @@ __global__ void __launch_bounds__(256) tab_join_kernel(const float *__restrict__
 // ---- host --------------------------------------------------------------------------------------------------
 struct TabOperand { const void *base; long long rows, inner, ld, plane; int planes; };   // [planes][rows][ld], 16-bit elements
 
-static bool tab_encode(CUtensorMap *tm, bool bf16, const TabOperand &o, int box_inner, int box_rows) {
+static bool tab_encode(CUtensorMap *tm, bool bf16, const TabOperand &o, int box_inner, int box_rows, int box_planes) {
   const cuuint64_t dims[3] = {(cuuint64_t)o.inner, (cuuint64_t)o.rows, (cuuint64_t)o.planes};
   const cuuint64_t strides[2] = {(cuuint64_t)o.ld * 2, (cuuint64_t)(o.planes > 1 ? o.plane : o.ld * 8) * 2};
-  const cuuint32_t box[3] = {(cuuint32_t)box_inner, (cuuint32_t)box_rows, (cuuint32_t)o.planes};
+  const cuuint32_t box[3] = {(cuuint32_t)box_inner, (cuuint32_t)box_rows, (cuuint32_t)box_planes};
   return encode_map(tm, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, o.base, 3, dims, strides, box,
                     box_inner == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
 }
@@ -629,14 +637,15 @@ static bool tab_encode_blocks(CUtensorMap *tm, bool bf16, const TabOperand &o, i
 static bool tab_whole(const TabOperand &o) { return o.inner % 64 == 0 || o.ld >= tok_up(o.inner, 64); }
 
 template <int EPI, class MATH, bool A_MN, bool B_MN, int CG>
-static bool tab_launch_as(const TabOperand &a, const TabOperand &b, TabArgs &g, cudaStream_t st) {
+static bool tab_launch_as(const TabOperand &a, const TabOperand &b, const TabOperand *c, TabArgs &g, cudaStream_t st) {
   constexpr int KB = MATH::NPA == 1 ? 64 : 32;
   constexpr bool bf16 = std::is_same<typename MATH::elem, __nv_bfloat16>::value;
   if (pbg_launch_failed()) return true;
   TabMaps maps;
   g.b_whole = B_MN && tab_whole(b);
-  if (!(A_MN ? tab_encode_blocks(&maps.a, bf16, a, KB, 2) : tab_encode(&maps.a, bf16, a, KB, 128))) return false;
-  if (!(g.b_whole ? tab_encode_blocks(&maps.b, bf16, b, KB, g.BN / CG / 64) : tab_encode(&maps.b, bf16, b, B_MN ? 64 : KB, B_MN ? KB : g.BN / CG))) return false;
+  if (!(A_MN ? tab_encode_blocks(&maps.a, bf16, a, KB, 2) : tab_encode(&maps.a, bf16, a, KB, 128, a.planes))) return false;
+  if (EPI == EPI_DZ && !tab_encode(&maps.c, bf16, *c, 32, 32, 1)) return false;
+  if (!(g.b_whole ? tab_encode_blocks(&maps.b, bf16, b, KB, g.BN / CG / 64) : tab_encode(&maps.b, bf16, b, B_MN ? 64 : KB, B_MN ? KB : g.BN / CG, b.planes))) return false;
   const int stage = MATH::NPA * 128 * KB * 2 + MATH::NPB * (g.BN / CG) * KB * 2;
   g.stages = TAB_RING_BYTES / stage < TAB_STAGES_MAX ? TAB_RING_BYTES / stage : TAB_STAGES_MAX;
   void (*kernel)(TabMaps, TabArgs) = tab_kernel<EPI, MATH, A_MN, B_MN, CG>;
@@ -679,9 +688,9 @@ static int tab_splits(long long n, long long dim, long long K, int products) {
 static bool tab_pairs(long long M, long long N) { return M > 128 && N > 64; }
 
 template <int EPI, class MATH, bool A_MN, bool B_MN>
-static bool tab_launch(const TabOperand &a, const TabOperand &b, TabArgs &g, bool pairs, cudaStream_t st) {
+static bool tab_launch(const TabOperand &a, const TabOperand &b, TabArgs &g, bool pairs, cudaStream_t st, const TabOperand *c = nullptr) {
   g.part = MATH::NPB == 2 ? TAB_F32_PART : 0x7fffffff;
-  return pairs ? tab_launch_as<EPI, MATH, A_MN, B_MN, 2>(a, b, g, st) : tab_launch_as<EPI, MATH, A_MN, B_MN, 1>(a, b, g, st);
+  return pairs ? tab_launch_as<EPI, MATH, A_MN, B_MN, 2>(a, b, c, g, st) : tab_launch_as<EPI, MATH, A_MN, B_MN, 1>(a, b, c, g, st);
 }
 
 // TMA reads rows where they lie if they start on 16-byte boundaries
@@ -824,9 +833,11 @@ static void tab_backward(TabBackward &f) {
     g.by_q = g.by_w = 1;
     g.targets = c.targets; g.ignore_index = c.ignore_index; g.vocab = c.rows; g.v0 = v0;
     g.lse = f.lse; g.entropy = f.entropy; g.g = f.g; g.h = f.h;
-    g.dz = c.ws + f.p.dz; g.ldz = f.p.ldz; g.dz_plane = c.n * f.p.ldz; g.dz_planes = f.p.dz_planes;
-    f.ok = tab_launch<EPI_DZ, MATH, false, false>(c.q, w, g, pairs, c.st);
-    const TabOperand dz{g.dz, c.n, cols, f.p.ldz, g.dz_plane, f.p.dz_planes};
+    g.ldz = f.p.ldz; g.dz_planes = f.p.dz_planes;
+    const TabOperand dz{c.ws + f.p.dz, c.n, cols, f.p.ldz, c.n * f.p.ldz, f.p.dz_planes};
+    TabOperand written = dz;
+    written.inner = f.p.ldz;
+    f.ok = tab_launch<EPI_DZ, MATH, false, false>(c.q, w, g, pairs, c.st, &written);
     if (f.dq && f.ok) {
       TabArgs d = {};
       plan(d, pairs, c.n, c.dim, f.p.splits, 64);

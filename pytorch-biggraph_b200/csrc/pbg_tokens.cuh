@@ -38,6 +38,19 @@ template <> struct Tok<__half> {
   static __device__ __forceinline__ __half down(float x) { return __float2half_rn(x); }
 };
 
+// two 16-bit elements at a time
+template <class T> struct TokPair;
+template <> struct TokPair<__nv_bfloat16> {
+  using type = __nv_bfloat162;
+  static __device__ __forceinline__ type down(float a, float b) { return __floats2bfloat162_rn(a, b); }
+  static __device__ __forceinline__ float2 up(type e) { return __bfloat1622float2(e); }
+};
+template <> struct TokPair<__half> {
+  using type = __half2;
+  static __device__ __forceinline__ type down(float a, float b) { return __floats2half2_rn(a, b); }
+  static __device__ __forceinline__ float2 up(type e) { return __half22float2(e); }
+};
+
 template <class T>
 __device__ __forceinline__ void tok_unpack(const uint4 &v, float (&x)[Tok<T>::VEC]) {
   const T *p = reinterpret_cast<const T *>(&v);

@@ -48,7 +48,7 @@ using TabF16Fine = TabMath<__half, __half, 2, 1>;
 // Powers of two that the operands were multiplied by, and their inverses
 struct TabScales { float q, w, dz, iq, iw, idz; };
 
-struct TabMaps { CUtensorMap a, b, c; };                              // operands; dz, to be written
+struct TabMaps { CUtensorMap a, b, c; };                              // operands; what is written by bulk stores
 struct TabArgs {
   long long M, N;                     // rows and columns of the product
   int kblocks;                        // blocks of KB k-values
@@ -63,7 +63,9 @@ struct TabArgs {
   long long ldz; int dz_planes;
   void *out; long long ldo;           // EPI_OUT: the result, or
   float *partial; int add;            //          [splits][M][N] fp32, stored or added
+  int bulk;                           //          either way by bulk stores
   int by_q, by_w, by_dz;              // which powers the product carries
+  int a_rows;                         // rows of A that are loaded: 128, or fewer where there is one row tile and nothing to fill it with
   int b_whole;                        // MN-major B: its rows are whole blocks of 64 columns, read as one box
 };
 
@@ -157,6 +159,7 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
   const int b_cols = g.BN / CG;                                          // columns of B in this CTA
   const uint32_t b_plane = B_MN ? ATOM_BYTES : (uint32_t)b_cols * ROW_BYTES;
   const uint32_t stage_bytes = A_BYTES + NPB * (uint32_t)b_cols * ROW_BYTES;
+  const uint32_t a_plane = A_MN ? ATOM_BYTES : (uint32_t)g.a_rows * ROW_BYTES;
 
   if (warp == 0) {
     // ---------------- TMA: one box per operand, or one per 64 columns of an MN-major one.  One thread does it all: a stage takes
@@ -177,7 +180,7 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
           const uint32_t a = smem_u32(smem) + (uint32_t)at.s * stage_bytes, b = a + A_BYTES;
           // a pair's loads are all counted by the first CTA, which issues the products
           const uint32_t fb = CG == 1 ? full_bar(at.s) : in_first_cta(full_bar(at.s));
-          if (rank == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(full_bar(at.s)), "r"(CG * stage_bytes) : "memory");
+          if (rank == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(full_bar(at.s)), "r"(CG * (stage_bytes - NPA * (128 - (uint32_t)g.a_rows) * ROW_BYTES)) : "memory");
           const int k = kb * KB;
           if (A_MN) tab_load_blocks<CG>(a, &maps.a, k, (int)(m0 / 64), fb);
           else tab_load<CG>(a, &maps.a, k, (int)m0, fb);
@@ -194,7 +197,7 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
     // K-major: 128-byte rows in the 128-byte swizzle (layout 2) or 64-byte rows in the 64-byte one (layout 4), 32 bytes per 16 k-values;
     // MN-major: 64 columns x KB rows in the 128-byte swizzle, 2048 bytes per 16 k-values
     constexpr uint32_t K_SBO = KB == 64 ? 1024 : 512, K_LAYOUT = KB == 64 ? 2 : 4;
-    constexpr uint32_t a_step = A_MN ? 2048 : 32, b_step = B_MN ? 2048 : 32, a_plane = A_MN ? ATOM_BYTES : 128 * ROW_BYTES;
+    constexpr uint32_t a_step = A_MN ? 2048 : 32, b_step = B_MN ? 2048 : 32;
     const bool leader = elect_one();
     StageRing at;
     int j = 0;
@@ -326,6 +329,19 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
       // the padding of dz's last columns is written too, as zeros: the contraction over the table's rows reads whole blocks
       const int span = EPI == EPI_DZ ? (c0 >= g.ldz ? 0 : g.ldz - c0 < hc ? (int)(g.ldz - c0) : hc) : cols;
       const int rows = g.M - (m0 + q * 32) < 32 ? (int)(g.M - (m0 + q * 32)) : 32;
+      // before the buffer is written again, what was stored from it has been read; then it goes
+      auto store_ready = [&]() {
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        __syncwarp();
+      };
+      auto store_go = [&](int col, int row, int part, bool any) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0 && any) {
+          asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];" :: "l"(&maps.c), "r"(col), "r"(row), "r"(part), "r"(smem_u32(buf)) : "memory");
+          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
+      };
 #pragma unroll PARTS ? 4 : 1
       for (int x = 0; x < 128; x += 32) {
         if (x >= span) break;
@@ -375,8 +391,7 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
             for (int i = 0; i < 32; ++i) if (col + i >= g.N) v[i] = 0.f;
           }
           // planes of 32 x 32 values through shared memory (64-byte swizzle); each leaves as one bulk store, clipped at the last row
-          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-          __syncwarp();
+          store_ready();
 #pragma unroll
           for (int pl = 0; pl < 2; ++pl) {
             if (pl >= planes) break;
@@ -401,7 +416,8 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
                            :: "l"(&maps.c), "r"((int)col), "r"((int)(m0 + q * 32)), "r"(pl), "r"(smem_u32(buf + pl * 2048)) : "memory");
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
           }
-        } else {
+        } else if (!g.bulk) {
+          // row by row, whatever the rows' alignment
           __syncwarp();
 #pragma unroll
           for (int u = 0; u < 8; ++u)
@@ -409,7 +425,6 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
           __syncwarp();
           const long long col = c0 + x + lane;
           if (x + lane < cols) {
-#pragma unroll 8
             for (int r0 = 0; r0 < rows; ++r0) {
               const float val = *reinterpret_cast<float *>(buf + r0 * 128 + (((lane >> 2) ^ (r0 & 7)) << 4) + ((lane & 3) << 2)) * unscale;
               const long long row = m0 + q * 32 + r0;
@@ -419,12 +434,33 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
               } else ((Out *)g.out)[row * g.ldo + col] = Tok<Out>::down(val);
             }
           }
+        } else if (sizeof(Out) == 4 || g.partial) {
+          // 32 x 32 values as one bulk store, clipped at the matrix' edges
+          store_ready();
+#pragma unroll
+          for (int u = 0; u < 8; ++u)
+            *reinterpret_cast<float4 *>(buf + lane * 128 + ((u ^ (lane & 7)) << 4)) = make_float4(v[4 * u] * unscale, v[4 * u + 1] * unscale, v[4 * u + 2] * unscale, v[4 * u + 3] * unscale);
+          store_go((int)(c0 + x), (int)(m0 + q * 32), split, rows > 0);
+        } else {
+          // 16-bit results: 64 columns to a row of 128 bytes
+          if ((x & 32) == 0) store_ready();
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const auto e = TokPair<Elem>::down(v[8 * u + 2 * i] * unscale, v[8 * u + 2 * i + 1] * unscale);
+              w[i] = *reinterpret_cast<const uint32_t *>(&e);
+            }
+            *reinterpret_cast<uint4 *>(buf + lane * 128 + (((u + (x & 32) / 8) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+          if ((x & 32) || x + 32 >= span) store_go((int)(c0 + (x & ~32)), (int)(m0 + q * 32), 0, rows > 0);
         }
       }
       if (EPI == EPI_STATS && m < g.M) g.parts[m * g.nparts + n0 / g.BN * 2 + half] = make_float4(S == 0.f ? -1e30f : r, S, T, 0.f);
       if (!PARTS && kb0 < kb1) give_back();
     }
-    if (EPI == EPI_DZ && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");         // the stores are performed
+    if (EPI != EPI_STATS && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");         // the stores are performed
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
@@ -643,8 +679,22 @@ static bool tab_launch_as(const TabOperand &a, const TabOperand &b, const TabOpe
   if (pbg_launch_failed()) return true;
   TabMaps maps;
   g.b_whole = B_MN && tab_whole(b);
-  if (!(A_MN ? tab_encode_blocks(&maps.a, bf16, a, KB, 2) : tab_encode(&maps.a, bf16, a, KB, 128, a.planes))) return false;
+  // Rows outside of the matrix are written as zeros, at a price: a box of 7 rows and 121 of zeros takes longer than one of 128 rows (7
+  // queries, 131,072 x 2048 bf16: 127 us against 100).  A row of products depends on its own row of A alone, so what
+  // stands in the rows that are not loaded is nobody's.
+  g.a_rows = !A_MN && g.M < 128 ? (int)tok_up(g.M, 8) : 128;
+  if (!(A_MN ? tab_encode_blocks(&maps.a, bf16, a, KB, 2) : tab_encode(&maps.a, bf16, a, KB, g.a_rows, a.planes))) return false;
   if (EPI == EPI_DZ && !tab_encode(&maps.c, bf16, *c, 32, 32, 1)) return false;
+  if (EPI == EPI_OUT) {
+    // rows that begin on 16-byte boundaries; sums of several launches are added row by row
+    const bool fp32 = g.partial || sizeof(typename MATH::out) == 4;
+    const void *to = g.partial ? (const void *)g.partial : g.out;
+    const long long row = (g.partial ? g.N : g.ldo) * (fp32 ? 4 : 2);
+    g.bulk = aligned16(to) && row % 16 == 0 && !(g.partial && g.add);
+    const cuuint64_t dims[3] = {(cuuint64_t)g.N, (cuuint64_t)g.M, (cuuint64_t)g.splits}, strides[2] = {(cuuint64_t)row, (cuuint64_t)row * g.M};
+    const cuuint32_t box[3] = {fp32 ? 32u : 64u, 32, 1};
+    if (g.bulk && !encode_map(&maps.c, fp32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, to, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return false;
+  }
   if (!(g.b_whole ? tab_encode_blocks(&maps.b, bf16, b, KB, g.BN / CG / 64) : tab_encode(&maps.b, bf16, b, B_MN ? 64 : KB, B_MN ? KB : g.BN / CG, b.planes))) return false;
   const int stage = MATH::NPA * 128 * KB * 2 + MATH::NPB * (g.BN / CG) * KB * 2;
   g.stages = TAB_RING_BYTES / stage < TAB_STAGES_MAX ? TAB_RING_BYTES / stage : TAB_STAGES_MAX;
@@ -815,7 +865,7 @@ static void tab_backward(TabBackward &f) {
   constexpr int KB = MATH::NPA == 1 ? 64 : 32, KB2 = DZMATH::NPA == 1 ? 64 : 32;
   tab_prepare<T>(c, f.p, true, f.g, f.h);
   const bool partial = f.p.splits > 1 || f.p.columns < c.rows;
-  auto plan = [&](TabArgs &a, bool &pairs, long long M, long long N, int splits, int step) {
+  auto plan = [&](TabArgs &a, bool &pairs, long long M, long long N, int splits, int step) {       // step: of the columns of a single CTA's tile
     pairs = tab_pairs(M, N);
     a.M = M; a.N = N; a.splits = splits; a.sc = c.sc; a.err = c.err;
     a.BN = tab_columns((M + (pairs ? 255 : 127)) / (pairs ? 256 : 128) * splits, N, pairs ? 128 : step, pairs ? 2 : 1);
@@ -840,7 +890,7 @@ static void tab_backward(TabBackward &f) {
     f.ok = tab_launch<EPI_DZ, MATH, false, false>(c.q, w, g, pairs, c.st, &written);
     if (f.dq && f.ok) {
       TabArgs d = {};
-      plan(d, pairs, c.n, c.dim, f.p.splits, 64);
+      plan(d, pairs, c.n, c.dim, f.p.splits, 128);
       d.kblocks = (int)((cols + KB2 - 1) / KB2);
       d.by_dz = d.by_w = 1;
       d.out = f.dq; d.ldo = c.dim;
@@ -849,7 +899,7 @@ static void tab_backward(TabBackward &f) {
     }
     if (f.dt && f.ok) {
       TabArgs d = {};
-      plan(d, pairs, cols, c.dim, 1, 64);
+      plan(d, pairs, cols, c.dim, 1, 128);
       d.kblocks = (int)((c.n + KB2 - 1) / KB2);
       d.by_dz = d.by_q = 1;
       d.out = (T *)f.dt + v0 * c.dim; d.ldo = c.dim;

@@ -19,6 +19,9 @@
 // in shared memory feeds twice as many products.  Alone, a tile of 128 x 256 writes and reads 192 bytes of shared memory per cycle of
 // its products where the SM moves 128; a pair 128.
 //
+// Up to sixteen fp32 queries take no tensor cores: making planes of the table reads and writes it three times over, where fp32 products
+// on the CUDA cores keep up with one reading of it (tab_few_kernel).
+//
 // Every wait is bounded: one that runs out sets bit 2 of the error word, and the CTA stops, frees its tensor memory and returns.
 #include "pbg_tc.cuh"
 #include "pbg_tokens.cuh"
@@ -34,8 +37,10 @@ enum { EPI_STATS = 0, EPI_DZ = 1, EPI_OUT = 2 };
 #define TAB_DZ_BYTES (2ll << 30)                            // most memory for dz: beyond it the table goes in pieces
 #define TAB_PARTS_BYTES (512ll << 20)                       // and for the tiles' partial sums: beyond it the queries do
 // The tensor cores cut off what they add up instead of rounding it, a bias of half a step per addition.  Contractions of
-// fp32 operands are therefore cut into parts of this many blocks of 32 k-values (48 additions), which are added in registers.
+// fp32 operands are therefore cut into parts of this many blocks of 32 k-values (48 and 18 additions: the scores' epilogue has more to do,
+// their contractions are the shorter ones), which are added in registers.
 #define TAB_F32_PART 8
+#define TAB_F32_PART_OUT 3
 
 // Operands: their elements, the planes of A and B, the type of results
 template <class E, class O, int PA, int PB> struct TabMath { using elem = E; using out = O; static constexpr int NPA = PA, NPB = PB; };
@@ -516,6 +521,89 @@ __global__ void __launch_bounds__(128) tab_stats_kernel(const T *__restrict__ qu
   if (!known && errors) atomicOr(errors, TOK_ERR_ID);
 }
 
+// ---- a few fp32 queries ----------------------------------------------------------------------------------------
+// The queries lie in shared memory; a warp takes R rows of the table at a time, its lanes along the rows, so that a query's
+// 512 bytes serve R rows.  16 queries: 32 FMAs and 4 reads of 16 bytes per lane and 16 bytes of the table.  What bounds it: HBM, up to 8
+// queries; 7 x 65,536 x 2048: see the case table.
+#define TAB_FEW 16
+#define TAB_FEW_WARPS 16
+#define TAB_FEW_BYTES 196608
+static __host__ __device__ constexpr int few_rows(int nq) { return nq <= 8 ? 4 : 2; }
+
+template <int NQ, bool WIDE>
+__global__ void __launch_bounds__(32 * TAB_FEW_WARPS, 1)
+tab_few_kernel(const float *__restrict__ queries, long long q_stride, int n, const float *__restrict__ table, long long t_stride, long long vocab, int dim, float scale,
+               float4 *parts) {
+  constexpr int R = few_rows(NQ), C = R * NQ, V = WIDE ? 4 : 1;
+  extern __shared__ __align__(16) float few_q[];                         // [NQ][dim rounded up to 4]
+  __shared__ Soft sums[TAB_FEW_WARPS][C];
+  pdl_begin();
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, ld = (dim + 3) / 4 * 4;
+  for (int q = w; q < NQ; q += TAB_FEW_WARPS)
+    for (int i = lane; i < ld; i += 32) few_q[q * ld + i] = q < n && i < dim ? queries[q * q_stride + i] : 0.f;
+  __syncthreads();
+  const float c = scale * TOK_LOG2E;
+  Soft s{-INFINITY, 0.f, 0.f, 0.f};
+  constexpr int SHIFT = C == 32 ? 0 : C == 16 ? 1 : C == 8 ? 2 : 3;
+  const int mine = lane >> SHIFT, my_row = mine / NQ;   // the product that ends in this lane
+  for (long long v0 = ((long long)blockIdx.x * TAB_FEW_WARPS + w) * R; v0 < vocab; v0 += (long long)gridDim.x * TAB_FEW_WARPS * R) {
+    float acc[C];
+#pragma unroll
+    for (int i = 0; i < C; ++i) acc[i] = 0.f;
+    const float *row[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) row[r] = table + (v0 + r < vocab ? v0 + r : vocab - 1) * t_stride;
+#pragma unroll 2
+    for (int i = lane; i < dim / V; i += 32) {
+      float x[R][V];
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        if constexpr (WIDE) { const float4 f = __ldcs((const float4 *)row[r] + i); x[r][0] = f.x; x[r][1] = f.y; x[r][2] = f.z; x[r][3] = f.w; }
+        else x[r][0] = row[r][i];
+      }
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+        float y[V];
+        if constexpr (WIDE) { const float4 f = ((const float4 *)(few_q + q * ld))[i]; y[0] = f.x; y[1] = f.y; y[2] = f.z; y[3] = f.w; }
+        else y[0] = few_q[q * ld + i];
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int k = 0; k < V; ++k) acc[r * NQ + q] = fmaf(x[r][k], y[k], acc[r * NQ + q]);
+      }
+    }
+    // the lanes' sums, halving what a lane still holds at every step
+    int have = C;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      if (have > 1) {
+        have /= 2;
+#pragma unroll
+        for (int i = 0; i < C / 2; ++i) {
+          if (i >= have) break;
+          const float keep = lane & o ? acc[i + have] : acc[i], give = lane & o ? acc[i] : acc[i + have];
+          acc[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+        }
+      } else acc[0] += __shfl_xor_sync(0xffffffffu, acc[0], o);
+    }
+    if (v0 + my_row < vocab) {
+      const float z = acc[0];
+      if (z > s.m) { s.m = z; soft_rebase(s, soft_reference(z), c); }
+      const float y = tok_max_nan((z - s.r) * c, -1000.f), e = tok_ex2(y);
+      s.S += e;
+      s.T = fmaf(y, e, s.T);
+    }
+  }
+  if ((lane & ((1 << SHIFT) - 1)) == 0) sums[w][mine] = s;
+  __syncthreads();
+  if (threadIdx.x < n) {
+    Soft a{-INFINITY, 0.f, 0.f, 0.f};
+    for (int i = 0; i < TAB_FEW_WARPS; ++i)
+      for (int r = 0; r < R; ++r) soft_join(a, sums[i][r * NQ + threadIdx.x], c);
+    parts[(long long)threadIdx.x * gridDim.x + blockIdx.x] = make_float4(a.S == 0.f ? -1e30f : a.r * c, a.S, a.T, 0.f);
+  }
+}
+
 // ---- preparation ---------------------------------------------------------------------------------------------
 // Which rows count: those whose target is not ignore_index (any: nor outside of the table); without targets all.
 struct TabRows {
@@ -739,7 +827,7 @@ static bool tab_pairs(long long M, long long N) { return M > 128 && N > 64; }
 
 template <int EPI, class MATH, bool A_MN, bool B_MN>
 static bool tab_launch(const TabOperand &a, const TabOperand &b, TabArgs &g, bool pairs, cudaStream_t st, const TabOperand *c = nullptr) {
-  g.part = MATH::NPB == 2 ? TAB_F32_PART : 0x7fffffff;
+  g.part = MATH::NPB != 2 ? 0x7fffffff : EPI == EPI_OUT ? TAB_F32_PART_OUT : TAB_F32_PART;
   return pairs ? tab_launch_as<EPI, MATH, A_MN, B_MN, 2>(a, b, c, g, st) : tab_launch_as<EPI, MATH, A_MN, B_MN, 1>(a, b, c, g, st);
 }
 
@@ -753,8 +841,9 @@ struct TabPlace {
   long long ld, columns, ldz;         // packed rows' length; table rows per piece of dz, and its rows' length
   long long piece;                    // queries per pass of the forward
   int npl, bn, nparts, splits, dz_planes;
-  bool pairs;
+  bool pairs, few;
 };
+static bool tab_few(long long n, int dim, int dtype);
 static TabPlace tab_place(long long n, long long rows, int dim, int dtype, bool grad) {
   TabPlace p;
   p.npl = dtype == PBG_F32 ? 2 : 1;
@@ -769,7 +858,13 @@ static TabPlace tab_place(long long n, long long rows, int dim, int dtype, bool 
   p.piece = n;
   p.bn = p.nparts = p.splits = p.dz_planes = 0;
   p.pairs = tab_pairs(n, rows);
-  if (!grad) {
+  p.few = !grad && tab_few(n, dim, dtype);
+  if (p.few) {
+    const long long groups = (rows + 4 * TAB_FEW_WARPS - 1) / (4 * TAB_FEW_WARPS);
+    p.nparts = (int)(groups < pbg_sm_count() ? groups : pbg_sm_count());
+    at = p.parts = p.q;                                      // no copies
+    at += n * p.nparts * 16;
+  } else if (!grad) {
     p.bn = tab_columns((n + (p.pairs ? 255 : 127)) / (p.pairs ? 256 : 128), rows, p.pairs ? 128 : 64, p.pairs ? 2 : 1);
     p.nparts = (int)((rows + p.bn - 1) / p.bn * 2);
     long long most = TAB_PARTS_BYTES / (16ll * p.nparts) / 256 * 256;
@@ -835,10 +930,41 @@ static void tab_prepare(TabCall &c, const TabPlace &p, bool grad, const float *g
   pbg_launch(tab_pack_kernel<T>, dim3(a.q.blocks + a.w.blocks), 256, 0, c.st, a);
 }
 
+static bool tab_few(long long n, int dim, int dtype) {
+  if (dtype != PBG_F32 || n > TAB_FEW) return false;
+  long long nq = 1;
+  while (nq < n) nq *= 2;
+  return nq * tok_up(dim, 4) * 4 <= TAB_FEW_BYTES;
+}
+template <int NQ>
+static void tab_few_launch(const TabCall &c, float4 *parts, int blocks) {
+  const float *q = (const float *)c.queries, *t = (const float *)c.table;
+  const bool wide = c.dim % 4 == 0 && aligned16(t) && c.t_stride % 4 == 0;
+  auto kernel = wide ? tab_few_kernel<NQ, true> : tab_few_kernel<NQ, false>;
+  const int smem = (int)(NQ * tok_up(c.dim, 4) * 4);
+  pbg_opt_in_smem((const void *)kernel, TAB_FEW_BYTES);
+  pbg_launch(kernel, dim3(blocks), 32 * TAB_FEW_WARPS, smem, c.st, q, (long long)c.q_stride, (int)c.n, t, (long long)c.t_stride, (long long)c.rows, c.dim, c.scale, parts);
+}
+
 struct TabForward { TabCall c; TabPlace p; float *logprob, *entropy, *lse; bool ok; };
 template <class T, class MATH>
 static void tab_forward(TabForward &f) {
   TabCall &c = f.c;
+  auto finish = [&](long long n0, long long n) {
+    pbg_launch(tab_stats_kernel<T>, dim3((unsigned)n), 128, 0, c.st, (const T *)c.queries + n0 * c.q_stride, (long long)c.q_stride, (const T *)c.table, (long long)c.t_stride,
+               (long long)c.rows, c.dim, c.targets + n0, (long long)c.ignore_index, c.scale, (const float4 *)(c.ws + f.p.parts), f.p.nparts, f.logprob + n0, f.entropy + n0, f.lse + n0,
+               c.errors);
+  };
+  if (f.p.few) {
+    float4 *parts = (float4 *)(c.ws + f.p.parts);
+    if (c.n == 1) tab_few_launch<1>(c, parts, f.p.nparts);
+    else if (c.n == 2) tab_few_launch<2>(c, parts, f.p.nparts);
+    else if (c.n <= 4) tab_few_launch<4>(c, parts, f.p.nparts);
+    else if (c.n <= 8) tab_few_launch<8>(c, parts, f.p.nparts);
+    else tab_few_launch<16>(c, parts, f.p.nparts);
+    finish(0, c.n);
+    return;
+  }
   tab_prepare<T>(c, f.p, false, nullptr, nullptr);
   constexpr int KB = MATH::NPA == 1 ? 64 : 32;
   for (long long n0 = 0; n0 < c.n && f.ok; n0 += f.p.piece) {
@@ -852,8 +978,7 @@ static void tab_forward(TabForward &f) {
     g.by_q = g.by_w = 1;
     g.parts = (float4 *)(c.ws + f.p.parts); g.nparts = f.p.nparts;
     f.ok = tab_launch<EPI_STATS, MATH, false, false>(q, c.w, g, f.p.pairs, c.st);
-    pbg_launch(tab_stats_kernel<T>, dim3((unsigned)n), 128, 0, c.st, (const T *)c.queries + n0 * c.q_stride, (long long)c.q_stride, (const T *)c.table, (long long)c.t_stride,
-               (long long)c.rows, c.dim, c.targets + n0, (long long)c.ignore_index, c.scale, (const float4 *)g.parts, g.nparts, f.logprob + n0, f.entropy + n0, f.lse + n0, c.errors);
+    finish(n0, n);
   }
 }
 

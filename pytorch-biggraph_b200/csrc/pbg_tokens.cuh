@@ -66,6 +66,29 @@ __device__ __forceinline__ uint4 tok_pack(const float (&x)[Tok<T>::VEC]) {
   return v;
 }
 
+// Sums in base 2 against reference r: S = sum 2^((x - r) c), T = sum (x - r) c 2^((x - r) c).  m: the largest x; r is m, or 0 where m
+// is -inf (then S = T = 0).
+struct Soft { float m, r, S, T; };
+__device__ __forceinline__ float soft_reference(float m) { return m == -INFINITY ? 0.f : m; }
+__device__ __forceinline__ void soft_rebase(Soft &a, float r, float c) {
+  // (r is not below a.r but where nothing has been added yet; bounded, because 0 * inf has no place in S and T)
+  const float d = fminf(fmaxf((a.r - r) * c, -1e30f), 0.f), f = tok_ex2(d);
+  a.T = (a.T + d * a.S) * f;
+  a.S *= f;
+  a.r = r;
+}
+__device__ __forceinline__ void soft_join(Soft &a, Soft b, float c) {
+  a.m = fmaxf(a.m, b.m);
+  const float r = soft_reference(a.m);
+  soft_rebase(a, r, c);
+  soft_rebase(b, r, c);
+  a.S += b.S;
+  a.T += b.T;
+}
+__device__ __forceinline__ Soft soft_shfl(const Soft &a, int o) {
+  return Soft{__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.r, o), __shfl_xor_sync(0xffffffffu, a.S, o), __shfl_xor_sync(0xffffffffu, a.T, o)};
+}
+
 inline size_t tok_size(int dtype) { return dtype == PBG_F32 ? 4 : 2; }
 inline bool tok_type(int dtype) { return dtype == PBG_F32 || dtype == PBG_BF16 || dtype == PBG_F16; }
 inline bool tok_scale(float s) { return s > 0.f && s <= std::numeric_limits<float>::max(); }     // (false for NaN)

@@ -5,7 +5,11 @@
 //
 // The gradient sorts (id, i) first, so that the occurrences of an id lie next to each other in the order of i, and no sum
 // depends on the order in which anything arrives.  Sums are fp32, rounded to the output's type once.
+#include <cooperative_groups.h>
+
 #include "pbg_tokens.cuh"
+
+namespace cg = cooperative_groups;
 
 // N elements of T as one access of N * sizeof(T) bytes
 template <class T, int N> struct __align__(sizeof(T) * N) Unit { T e[N]; };
@@ -38,11 +42,14 @@ lookup_kernel(const T *__restrict__ table, long long row_stride, long long num_r
 }
 
 // ---- gradient -----------------------------------------------------------------------------------
-// The sorted list is cut into tiles of LG_TILE occurrences; a warp sums one tile over 32 units of columns.  A run of one id that
-// lies inside a tile is written out at once.  A run that reaches into the next tile is left as fp32 partial sums -- the tile's
-// first run in slot 0, its last one in slot 1 -- and the join adds a run's partials in the order of the tiles.
-#define LG_TILE 16
+// The sorted list is cut into tiles of LG_TILE occurrences; a warp sums those of one tile over 32 units of columns.  Most ids occur once
+// or twice.  A run of one id that reaches into the next tiles is summed by the warp of the tile it begins in, unless it goes on for
+// LG_LONG or more: then every tile leaves its part as fp32 sums -- that of its first run in slot 0, that of its last in slot 1 -- and
+// the join adds a run's parts in the order of the tiles.
+#define LG_TILE 8
+#define LG_LONG 64
 #define LG_JOIN_WARPS 8
+#define LG_JOIN_TILES 32
 
 struct GradArgs {
   const unsigned long long *keys;      // sorted ids, those outside of the table behind all others
@@ -52,6 +59,10 @@ struct GradArgs {
   int n, dim, part_ld, accumulate;
   float scale;
 };
+// whether the run of occurrence i goes on for LG_LONG occurrences or more behind the tile that ends at `end`
+__device__ __forceinline__ bool run_is_long(const GradArgs &a, unsigned long long key, int end) {
+  return end + LG_LONG - 1 < a.n && a.keys[end + LG_LONG - 1] == key;
+}
 
 template <class T, int N>
 __device__ __forceinline__ void grad_store(T *out, const GradArgs &a, unsigned long long row, int unit, const float (&acc)[N]) {
@@ -69,7 +80,7 @@ __device__ __forceinline__ void grad_store(T *out, const GradArgs &a, unsigned l
 }
 
 template <class T, int N>
-__global__ void __launch_bounds__(256) lookup_grad_kernel(const T *__restrict__ grad, T *__restrict__ out, GradArgs a) {
+__global__ void __launch_bounds__(256, 4) lookup_grad_kernel(const T *__restrict__ grad, T *__restrict__ out, GradArgs a) {
   pdl_begin();
   const int lane = threadIdx.x & 31, units = a.dim / N, blocks = (units + 31) / 32;
   const long long job = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -77,92 +88,250 @@ __global__ void __launch_bounds__(256) lookup_grad_kernel(const T *__restrict__ 
   const int i0 = tile * LG_TILE;
   if (i0 >= a.n) return;
   const int count = a.n - i0 < LG_TILE ? a.n - i0 : LG_TILE;
-  // lane j holds occurrence j of the tile; lanes 16 and 17 the neighbours on either side
+  const unsigned long long rows = (unsigned long long)a.num_rows;
+  // lane j holds occurrence j of the tile
   unsigned long long key = ~0ull;
   unsigned int val = 0u;
   if (lane < count) { key = a.keys[i0 + lane]; val = a.vals[i0 + lane]; }
   const unsigned long long before = i0 > 0 ? a.keys[i0 - 1] : ~0ull, after = i0 + count < a.n ? a.keys[i0 + count] : ~0ull;
+  const unsigned long long first = __shfl_sync(0xffffffffu, key, 0), last = __shfl_sync(0xffffffffu, key, count - 1);
+  // the first run, where it began before this tile: part of a long one, or another warp's
+  bool lead_long = false;
+  const bool lead = first == before && first < rows;
+  if (lead) {
+    int lo = i0 > LG_LONG + LG_TILE ? i0 - LG_LONG - LG_TILE : 0, hi = i0;        // its first occurrence, if it is not further back than that
+    const bool far = lo > 0 && a.keys[lo] == first;
+    while (lo < hi) { const int mid = (lo + hi) / 2; if (a.keys[mid] == first) hi = mid; else lo = mid + 1; }
+    lead_long = far || run_is_long(a, first, (lo / LG_TILE + 1) * LG_TILE);
+  }
+  // the last run, where it goes on behind this tile
+  const bool trail = last == after && last < rows;
+  const bool trail_long = trail && run_is_long(a, last, i0 + count);
   const bool live = unit < units;
+  auto load = [&](unsigned int v) { return reinterpret_cast<const Unit<T, N> *>(grad + (long long)v * a.grad_stride)[unit]; };
   Unit<T, N> g[LG_TILE];
 #pragma unroll
   for (int j = 0; j < LG_TILE; ++j) {
     const unsigned long long k = __shfl_sync(0xffffffffu, key, j);
     const unsigned int v = __shfl_sync(0xffffffffu, val, j);
-    if (live && k < (unsigned long long)a.num_rows) g[j] = reinterpret_cast<const Unit<T, N> *>(grad + (long long)v * a.grad_stride)[unit];
+    if (live && k < rows && !(lead && !lead_long && k == first)) g[j] = load(v);
   }
   float acc[N];
   bool opened = false;                               // the run at hand began in this tile
+  auto leave = [&](int slot) {
+    float *p = a.part + ((long long)tile * 2 + slot) * a.part_ld + unit * N;
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i] = acc[i];
+  };
+  auto add = [&](const Unit<T, N> &u) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] += Tok<T>::up(u.e[i]);
+  };
 #pragma unroll
   for (int j = 0; j < LG_TILE; ++j) {
     const unsigned long long k = __shfl_sync(0xffffffffu, key, j);
     const unsigned long long prev = j == 0 ? before : __shfl_sync(0xffffffffu, key, j > 0 ? j - 1 : 0);
-    unsigned long long next = __shfl_sync(0xffffffffu, key, j + 1);
-    if (j >= count || k >= (unsigned long long)a.num_rows) continue;                // (warp-uniform)
-    if (j == count - 1) next = after;
-    const bool head = k != prev;
-    if (head || j == 0) {
-      opened = head;
+    const unsigned long long next = __shfl_sync(0xffffffffu, key, j + 1);
+    if (j >= count || k >= rows || (lead && !lead_long && k == first)) continue;   // (the whole warp)
+    if (k != prev || j == 0) {
+      opened = k != prev;
 #pragma unroll
       for (int i = 0; i < N; ++i) acc[i] = 0.f;
     }
-    if (live) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) acc[i] += Tok<T>::up(g[j].e[i]);
-    }
-    if (k == next && j < count - 1) continue;
     if (!live) continue;
-    if (opened && k != next) grad_store<T, N>(out, a, k, unit, acc);
-    else {
-      float *p = a.part + ((long long)tile * 2 + (opened ? 1 : 0)) * a.part_ld + unit * N;
-#pragma unroll
-      for (int i = 0; i < N; ++i) p[i] = acc[i];
-    }
+    add(g[j]);
+    if (j == count - 1 ? trail : k == next) continue;
+    if (opened) grad_store<T, N>(out, a, k, unit, acc);
+    else leave(0);
   }
+  if (!trail || (lead && !lead_long && last == first)) return;
+  if (!opened || trail_long) {
+    if (live) leave(opened ? 1 : 0);
+    return;
+  }
+  for (int at = i0 + count; ; at += LG_TILE) {       // the rest of the run
+    const unsigned long long kk = lane < LG_TILE && at + lane < a.n ? a.keys[at + lane] : ~0ull;
+    const unsigned int vv = lane < LG_TILE && at + lane < a.n ? a.vals[at + lane] : 0u;
+    const int more = __popc(__ballot_sync(0xffffffffu, lane < LG_TILE && kk == last));
+#pragma unroll
+    for (int u = 0; u < LG_TILE; ++u) {
+      const unsigned int v = __shfl_sync(0xffffffffu, vv, u);
+      if (live && u < more) g[u] = load(v);
+    }
+#pragma unroll
+    for (int u = 0; u < LG_TILE; ++u) if (live && u < more) add(g[u]);
+    if (more < LG_TILE) break;
+  }
+  if (live) grad_store<T, N>(out, a, last, unit, acc);
 }
 
-// One CTA per (tile, 32 units): where the tile's last run begins in it and goes on, its partials are added up.  The run's further
-// tiles are dealt to the warps in blocks and the warps' sums added in their order.
+// A CTA looks through LG_JOIN_TILES tiles for long runs that begin in them, and adds up the parts of each over 32 units of columns:
+// the run's further tiles are dealt to the warps in blocks and the warps' sums added in their order.
 template <class T, int N>
 __global__ void __launch_bounds__(32 * LG_JOIN_WARPS) lookup_grad_join_kernel(T *__restrict__ out, GradArgs a) {
   __shared__ float sums[LG_JOIN_WARPS][32 * N];
   pdl_begin();
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, units = a.dim / N, blocks = (units + 31) / 32;
-  const int tile = (int)(blockIdx.x / blocks), unit = (int)(blockIdx.x % blocks) * 32 + lane;
-  const int last = tile * LG_TILE + LG_TILE - 1;
-  if (last + 1 >= a.n) return;
-  const unsigned long long k = a.keys[last];
-  if (k >= (unsigned long long)a.num_rows || a.keys[last + 1] != k) return;
-  if (a.keys[last - LG_TILE + 1] == k && tile > 0 && a.keys[last - LG_TILE] == k) return;      // began before this tile
-  int lo = last + 1, hi = a.n;                                                                // the run's end: first key behind it
-  while (lo < hi) { const int mid = lo + (hi - lo) / 2; if (a.keys[mid] == k) lo = mid + 1; else hi = mid; }
-  const int tiles = (lo - 1) / LG_TILE - tile;                                                // further tiles of the run
-  const int per = (tiles + LG_JOIN_WARPS - 1) / LG_JOIN_WARPS, t0 = w * per, t1 = t0 + per < tiles ? t0 + per : tiles;
+  const int group = (int)(blockIdx.x / blocks), unit = (int)(blockIdx.x % blocks) * 32 + lane;
+  bool begins = false;
+  {
+    const long long tile = (long long)group * LG_JOIN_TILES + lane, end = (tile + 1) * LG_TILE;
+    if (end < a.n) {
+      const unsigned long long k = a.keys[end - 1], next = a.keys[end], before = tile > 0 ? a.keys[end - LG_TILE - 1] : ~0ull;
+      begins = k < (unsigned long long)a.num_rows && next == k && before != k && run_is_long(a, k, (int)end);
+    }
+  }
   const bool live = unit < units;
-  float acc[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) acc[i] = 0.f;
-  if (live) {
-    if (w == 0) {
-      const float *p = a.part + ((long long)tile * 2 + 1) * a.part_ld + unit * N;
-#pragma unroll
-      for (int i = 0; i < N; ++i) acc[i] = p[i];
+  for (unsigned todo = __ballot_sync(0xffffffffu, begins); todo; todo &= todo - 1u) {        // (the same in every warp)
+    const int tile = group * LG_JOIN_TILES + __ffs(todo) - 1, end = (tile + 1) * LG_TILE;
+    const unsigned long long k = a.keys[end];
+    int lo = end + LG_LONG, hi = a.n;                                                       // the run's end: first key behind it
+    while (lo < hi) {                                                                       // (32 places looked at in every step)
+      const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+      const int same = __popc(__ballot_sync(0xffffffffu, at < hi && a.keys[at < hi ? at : lo] == k));
+      hi = same < 32 && lo + same * step < hi ? lo + same * step : hi;
+      lo = same > 0 ? lo + (same - 1) * step + 1 : lo;
+      if (same == 0) break;
     }
-#pragma unroll 4
-    for (int t = t0; t < t1; ++t) {
-      const float *p = a.part + (long long)(tile + 1 + t) * 2 * a.part_ld + unit * N;
+    const int tiles = (lo - 1) / LG_TILE - tile;                                            // further tiles of the run
+    const int per = (tiles + LG_JOIN_WARPS - 1) / LG_JOIN_WARPS, t0 = w * per, t1 = t0 + per < tiles ? t0 + per : tiles;
+    float acc[N];
 #pragma unroll
-      for (int i = 0; i < N; ++i) acc[i] += p[i];
+    for (int i = 0; i < N; ++i) acc[i] = 0.f;
+    if (live) {
+      if (w == 0) {
+        const float *p = a.part + ((long long)tile * 2 + 1) * a.part_ld + unit * N;
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] = p[i];
+      }
+#pragma unroll 8
+      for (int t = t0; t < t1; ++t) {
+        const float *p = a.part + (long long)(tile + 1 + t) * 2 * a.part_ld + unit * N;
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] += p[i];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) sums[w][lane * N + i] = acc[i];
+    __syncthreads();
+    if (w != 0 || !live) continue;
+    for (int o = 1; o < LG_JOIN_WARPS; ++o) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) acc[i] += sums[o][lane * N + i];
+    }
+    grad_store<T, N>(out, a, k, unit, acc);
+  }
+}
+
+// ---- sorting and zeros in one launch --------------------------------------------------------------------
+// Up to LS_MAX occurrences: the first cluster of eight CTAs sorts them by id (a stable radix sort, digits of up to nine bits, the list in
+// registers and shared memory), while all other CTAs write the zeros of the rows that no id names -- and of those that one
+// does, which the sums then replace.  Zeros of 131,072 x 2048 bf16 take 82 us, the sort of 16,384 ids 16.
+#define LS_CTAS 8
+#define LS_THREADS 1024
+#define LS_WARPS 32
+#define LS_BINS 512
+#define LS_MAX (LS_CTAS * LS_THREADS * 8)
+
+struct SortZero {
+  const long long *ids; long long num_rows; int n, bits; unsigned long long *keys; unsigned int *vals; int *errors;
+  uint4 *zero; long long zero_units; int zero_tail;        // 16-byte units and bytes behind them; null: nothing to write
+};
+
+template <int IPT>
+static constexpr size_t ls_smem() { return (size_t)LS_THREADS * IPT * 8 + LS_WARPS * LS_BINS * 2 + LS_CTAS * LS_BINS * 4 + LS_BINS * 4 + 64; }
+
+template <int IPT>
+__global__ void __cluster_dims__(LS_CTAS, 1, 1) __launch_bounds__(LS_THREADS) lookup_sort_zero_kernel(SortZero a) {
+  extern __shared__ __align__(16) unsigned char ls_smem_raw[];
+  const int t = threadIdx.x;
+  if (blockIdx.x >= LS_CTAS) {
+    const long long step = (long long)(gridDim.x - LS_CTAS) * LS_THREADS, first = (long long)(blockIdx.x - LS_CTAS) * LS_THREADS + t;
+    for (long long i = first; i < a.zero_units; i += step) __stcs(a.zero + i, make_uint4(0u, 0u, 0u, 0u));
+    if (first < a.zero_tail) reinterpret_cast<unsigned char *>(a.zero + a.zero_units)[first] = 0;
+    return;
+  }
+  cg::cluster_group cluster = cg::this_cluster();
+  cluster.barrier_arrive();                                              // (waited for in front of the first store to another CTA)
+  uint2 *buf = (uint2 *)ls_smem_raw;                                      // this CTA's part of the list
+  unsigned short *cnt = (unsigned short *)(buf + LS_THREADS * IPT);       // [warps][bins]
+  unsigned int *all = (unsigned int *)(cnt + LS_WARPS * LS_BINS);         // [CTAs][bins]
+  unsigned int *base = all + LS_CTAS * LS_BINS, *wsum = base + LS_BINS;
+  const int rank = (int)cluster.block_rank(), lane = t & 31, w = t >> 5;
+  const int passes = (a.bits + 8) / 9, db = (a.bits + passes - 1) / passes, bins = 1 << db;
+  const unsigned int mask = (unsigned int)bins - 1u, lt = (1u << lane) - 1u;
+  uint2 item[IPT];
+  unsigned int off[IPT];
+#pragma unroll
+  for (int i = 0; i < IPT; ++i) {
+    const int o = (rank * LS_WARPS + w) * 32 * IPT + i * 32 + lane;
+    unsigned int key = 0xffffffffu;                                       // beyond the list: behind everything
+    if (o < a.n) {
+      const long long id = a.ids[o];
+      const bool bad = id < 0 || id >= a.num_rows;
+      if (bad && a.errors) atomicOr(a.errors, TOK_ERR_ID);
+      key = (unsigned int)(bad ? a.num_rows : id);
+    }
+    item[i] = make_uint2(key, (unsigned int)o);
+  }
+  unsigned short *wc = cnt + w * LS_BINS;
+  for (int pass = 0, shift = 0; pass < passes; ++pass, shift += db) {
+    for (int i = lane; i < LS_BINS / 2; i += 32) reinterpret_cast<unsigned int *>(wc)[i] = 0u;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < IPT; ++i) {
+      const unsigned int dg = (item[i].x >> shift) & mask;
+      const unsigned int peers = __match_any_sync(0xffffffffu, dg);
+      const unsigned int before = wc[dg];
+      __syncwarp();
+      if ((peers & lt) == 0u) wc[dg] = (unsigned short)(before + __popc(peers));
+      __syncwarp();
+      off[i] = before + __popc(peers & lt);
+    }
+    __syncthreads();
+    if (pass == 0) cluster.barrier_wait();
+    if (t < bins) {
+      unsigned int run = 0u;
+#pragma unroll 8
+      for (int o = 0; o < LS_WARPS; ++o) { const unsigned int c = cnt[o * LS_BINS + t]; cnt[o * LS_BINS + t] = (unsigned short)run; run += c; }
+#pragma unroll
+      for (int o = 0; o < LS_CTAS; ++o) cluster.map_shared_rank(all, o)[rank * LS_BINS + t] = run;
+    }
+    cluster.sync();                                                       // the CTAs' counts are everywhere
+    unsigned int total = 0u, lower = 0u;
+    if (t < bins) {
+#pragma unroll
+      for (int o = 0; o < LS_CTAS; ++o) { const unsigned int v = all[o * LS_BINS + t]; total += v; lower += o < rank ? v : 0u; }
+    }
+    if (t < LS_BINS) {
+      unsigned int incl = total;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) { const unsigned int v = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += v; }
+      if (lane == 31) wsum[w] = incl;
+      base[t] = incl - total + lower;
+    }
+    __syncthreads();
+    if (t < LS_BINS) {
+      unsigned int under = 0u;
+#pragma unroll
+      for (int o = 0; o < LS_BINS / 32; ++o) under += o < w ? wsum[o] : 0u;
+      base[t] += under;
+    }
+    __syncthreads();
+    const bool last = pass == passes - 1;
+#pragma unroll
+    for (int i = 0; i < IPT; ++i) {
+      const unsigned int dg = (item[i].x >> shift) & mask, pos = base[dg] + wc[dg] + off[i];
+      if (!last) cluster.map_shared_rank(buf, pos / (LS_THREADS * IPT))[pos % (LS_THREADS * IPT)] = item[i];
+      else if (pos < (unsigned int)a.n) { a.keys[pos] = item[i].x; a.vals[pos] = item[i].y; }
+    }
+    if (!last) {
+      cluster.sync();
+#pragma unroll
+      for (int i = 0; i < IPT; ++i) item[i] = buf[(w * IPT + i) * 32 + lane];
     }
   }
-#pragma unroll
-  for (int i = 0; i < N; ++i) sums[w][lane * N + i] = acc[i];
-  __syncthreads();
-  if (w != 0 || !live) return;
-  for (int o = 1; o < LG_JOIN_WARPS; ++o) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) acc[i] += sums[o][lane * N + i];
-  }
-  grad_store<T, N>(out, a, k, unit, acc);
 }
 
 // Zeros, row by row; rows that lie one behind the other come as one row of all.
@@ -241,7 +410,7 @@ static GradPlace grad_place(int64_t n, int dim) {
   p.keys = 0;
   p.vals = p.keys + 2 * tok_up(n * 8, 256);
   p.hist = p.vals + 2 * tok_up(n * 4, 256);
-  p.part = p.hist + tok_up((int64_t)pbg_sort_hist_entries((int)n) * 4, 256);
+  p.part = p.hist + (n <= LS_MAX ? 0 : tok_up((int64_t)pbg_sort_hist_entries((int)n) * 4, 256));
   p.bytes = p.part + (n + LG_TILE - 1) / LG_TILE * 2 * grad_part_ld(dim) * 4;
   return p;
 }
@@ -255,7 +424,8 @@ template <class T, int N>
 static void lookup_grad_launch(const LookupGradCall &c) {
   const long long tiles = (c.a.n + LG_TILE - 1) / LG_TILE, blocks = (c.a.dim / N + 31) / 32;
   pbg_launch(lookup_grad_kernel<T, N>, dim3((unsigned)((tiles * blocks + 7) / 8)), 256, 0, c.st, (const T *)c.grad, (T *)c.out, c.a);
-  pbg_launch(lookup_grad_join_kernel<T, N>, dim3((unsigned)(tiles * blocks)), 32 * LG_JOIN_WARPS, 0, c.st, (T *)c.out, c.a);
+  if (c.a.n <= LG_LONG) return;                                          // no run is long
+  pbg_launch(lookup_grad_join_kernel<T, N>, dim3((unsigned)((tiles + LG_JOIN_TILES - 1) / LG_JOIN_TILES * blocks)), 32 * LG_JOIN_WARPS, 0, c.st, (T *)c.out, c.a);
 }
 template <class T>
 static void lookup_grad_type(const LookupGradCall &c) {
@@ -282,6 +452,13 @@ static void zero_type(const LookupGradCall &c) {
   else zero_launch<T, 1>(c, rows, width);
 }
 
+template <int IPT>
+static void sort_zero_launch(const SortZero &a, cudaStream_t st) {
+  pbg_opt_in_smem((const void *)lookup_sort_zero_kernel<IPT>, (int)ls_smem<IPT>());
+  const long long most = 2 * pbg_sm_count() / LS_CTAS * LS_CTAS, want = tok_up((a.zero_units + LS_THREADS * 4 - 1) / (LS_THREADS * 4), LS_CTAS);
+  pbg_launch_in_order(lookup_sort_zero_kernel<IPT>, dim3((unsigned)(LS_CTAS + (!a.zero ? 0 : want < most ? (want > LS_CTAS ? want : LS_CTAS) : most))), LS_THREADS, ls_smem<IPT>(), st, a);
+}
+
 extern "C" int pbg_embedding_lookup_grad(const void *grad, int64_t grad_stride, const int64_t *ids, int64_t n, int64_t num_rows, int32_t dim,
                                          int32_t dtype, float scale, void *out, int64_t out_stride, int32_t accumulate, void *workspace,
                                          int64_t workspace_bytes, int32_t *errors, void *stream) {
@@ -298,7 +475,9 @@ extern "C" int pbg_embedding_lookup_grad(const void *grad, int64_t grad_stride, 
   LookupGradCall c{grad, out, {}, st};
   c.a.grad_stride = grad_stride; c.a.out_stride = out_stride; c.a.num_rows = num_rows;
   c.a.n = (int)n; c.a.dim = dim; c.a.part_ld = grad_part_ld(dim); c.a.accumulate = accumulate != 0; c.a.scale = scale;
-  if (!accumulate) TOK_DISPATCH(dtype, zero_type, c);
+  const bool one_launch = n > 0 && n <= LS_MAX;
+  const bool flat = out_stride == dim && aligned16(out);
+  if (!accumulate && !(one_launch && flat)) TOK_DISPATCH(dtype, zero_type, c);
   if (n > 0) {
     SortPlan sp;
     for (int i = 0; i < 2; ++i) {
@@ -310,8 +489,18 @@ extern "C" int pbg_embedding_lookup_grad(const void *grad, int64_t grad_stride, 
     sp.result = 0;
     int bits = 1;
     while ((unsigned long long)num_rows >> bits) ++bits;
-    pbg_launch_in_order(id_keys_kernel, dim3((unsigned)((n + 255) / 256)), 256, 0, st, (const long long *)ids, (long long)num_rows, (int)n, sp.keys[0], sp.vals[0], errors);
-    pbg_sort(sp, (int)n, bits, st);
+    if (one_launch) {
+      const long long bytes = num_rows * dim * (long long)tok_size(dtype);
+      const bool zero = !accumulate && flat;
+      const SortZero a{(const long long *)ids, num_rows, (int)n, bits, sp.keys[0], sp.vals[0], errors, zero ? (uint4 *)out : nullptr, zero ? bytes / 16 : 0, zero ? (int)(bytes % 16) : 0};
+      if (n <= LS_MAX / 8) sort_zero_launch<1>(a, st);
+      else if (n <= LS_MAX / 4) sort_zero_launch<2>(a, st);
+      else if (n <= LS_MAX / 2) sort_zero_launch<4>(a, st);
+      else sort_zero_launch<8>(a, st);
+    } else {
+      pbg_launch_in_order(id_keys_kernel, dim3((unsigned)((n + 255) / 256)), 256, 0, st, (const long long *)ids, (long long)num_rows, (int)n, sp.keys[0], sp.vals[0], errors);
+      pbg_sort(sp, (int)n, bits, st);
+    }
     c.a.keys = sp.keys[sp.result];
     c.a.vals = sp.vals[sp.result];
     c.a.part = (float *)(ws + p.part);

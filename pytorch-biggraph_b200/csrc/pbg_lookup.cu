@@ -47,7 +47,7 @@ lookup_kernel(const T *__restrict__ table, long long row_stride, long long num_r
 // LG_LONG or more: then every tile leaves its part as fp32 sums -- that of its first run in slot 0, that of its last in slot 1 -- and
 // the join adds a run's parts in the order of the tiles.
 #define LG_TILE 8
-#define LG_LONG 64
+#define LG_LONG 32
 #define LG_JOIN_WARPS 8
 #define LG_JOIN_TILES 32
 
@@ -79,8 +79,14 @@ __device__ __forceinline__ void grad_store(T *out, const GradArgs &a, unsigned l
   *dst = v;
 }
 
+// how many of 64 flags, 32 to a word, are set from bit `from` of the first on
+__device__ __forceinline__ int run_of(unsigned w0, unsigned w1, int from) {
+  const unsigned gap0 = ~(w0 >> from) & (0xffffffffu >> from);
+  return gap0 ? __ffs(gap0) - 1 : ~w1 ? 32 - from + __ffs(~w1) - 1 : 64 - from;
+}
+
 template <class T, int N>
-__global__ void __launch_bounds__(256, 4) lookup_grad_kernel(const T *__restrict__ grad, T *__restrict__ out, GradArgs a) {
+__global__ void __launch_bounds__(256, 3) lookup_grad_kernel(const T *__restrict__ grad, T *__restrict__ out, GradArgs a) {
   pdl_begin();
   const int lane = threadIdx.x & 31, units = a.dim / N, blocks = (units + 31) / 32;
   const long long job = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -88,33 +94,38 @@ __global__ void __launch_bounds__(256, 4) lookup_grad_kernel(const T *__restrict
   const int i0 = tile * LG_TILE;
   if (i0 >= a.n) return;
   const int count = a.n - i0 < LG_TILE ? a.n - i0 : LG_TILE;
-  const unsigned long long rows = (unsigned long long)a.num_rows;
-  // lane j holds occurrence j of the tile
-  unsigned long long key = ~0ull;
-  unsigned int val = 0u;
-  if (lane < count) { key = a.keys[i0 + lane]; val = a.vals[i0 + lane]; }
-  const unsigned long long before = i0 > 0 ? a.keys[i0 - 1] : ~0ull, after = i0 + count < a.n ? a.keys[i0 + count] : ~0ull;
-  const unsigned long long first = __shfl_sync(0xffffffffu, key, 0), last = __shfl_sync(0xffffffffu, key, count - 1);
-  // the first run, where it began before this tile: part of a long one, or another warp's
-  bool lead_long = false;
-  const bool lead = first == before && first < rows;
-  if (lead) {
-    int lo = i0 > LG_LONG + LG_TILE ? i0 - LG_LONG - LG_TILE : 0, hi = i0;        // its first occurrence, if it is not further back than that
-    const bool far = lo > 0 && a.keys[lo] == first;
-    while (lo < hi) { const int mid = (lo + hi) / 2; if (a.keys[mid] == first) hi = mid; else lo = mid + 1; }
-    lead_long = far || run_is_long(a, first, (lo / LG_TILE + 1) * LG_TILE);
+  const unsigned rows = (unsigned)a.num_rows, all = 0xffffffffu;
+  // 64 ids from the tile's first on and 64 in front of it, all asked for at once: LG_LONG + LG_TILE of them say what is to be known
+  static_assert(LG_LONG + LG_TILE <= 64, "the ids around a tile");
+  unsigned f[2], b[2], val[2];
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    const int at = i0 + 32 * w + lane, back = i0 - 1 - 32 * w - lane;
+    f[w] = at < a.n ? (unsigned)a.keys[at] : all;
+    val[w] = at < a.n ? a.vals[at] : 0u;
+    b[w] = back >= 0 ? (unsigned)a.keys[back] : all;
   }
+  const unsigned first = __shfl_sync(all, f[0], 0), last = __shfl_sync(all, f[0], count - 1);
+  // the first run, where it began before this tile: part of a long one, or another warp's
+  const int to = run_of(__ballot_sync(all, f[0] == first), __ballot_sync(all, f[1] == first), 0);
+  const int from = run_of(__ballot_sync(all, b[0] == first), __ballot_sync(all, b[1] == first), 0);
+  const bool lead = from > 0 && first < rows;
+  const int owner_end = ((i0 - from) / LG_TILE + 1) * LG_TILE;            // of the tile it began in
+  const bool lead_long = lead && (from == 64 || i0 + to - owner_end >= LG_LONG);
   // the last run, where it goes on behind this tile
-  const bool trail = last == after && last < rows;
-  const bool trail_long = trail && run_is_long(a, last, i0 + count);
+  const int behind = run_of(__ballot_sync(all, f[0] == last), __ballot_sync(all, f[1] == last), count);
+  const bool trail = behind > 0 && last < rows, trail_long = trail && behind >= LG_LONG;
+  const unsigned up = __shfl_up_sync(all, f[0], 1), down = __shfl_down_sync(all, f[0], 1);
+  const unsigned heads = __ballot_sync(all, f[0] != (lane == 0 ? b[0] : up)), ends = __ballot_sync(all, f[0] != down);
+  unsigned used = __ballot_sync(all, lane < count && f[0] < rows);
+  if (lead && !lead_long) used &= to >= 32 ? 0u : all << to;
   const bool live = unit < units;
   auto load = [&](unsigned int v) { return reinterpret_cast<const Unit<T, N> *>(grad + (long long)v * a.grad_stride)[unit]; };
   Unit<T, N> g[LG_TILE];
 #pragma unroll
   for (int j = 0; j < LG_TILE; ++j) {
-    const unsigned long long k = __shfl_sync(0xffffffffu, key, j);
-    const unsigned int v = __shfl_sync(0xffffffffu, val, j);
-    if (live && k < rows && !(lead && !lead_long && k == first)) g[j] = load(v);
+    const unsigned int v = __shfl_sync(all, val[0], j);
+    if (live && (used >> j & 1u)) g[j] = load(v);
   }
   float acc[N];
   bool opened = false;                               // the run at hand began in this tile
@@ -129,38 +140,32 @@ __global__ void __launch_bounds__(256, 4) lookup_grad_kernel(const T *__restrict
   };
 #pragma unroll
   for (int j = 0; j < LG_TILE; ++j) {
-    const unsigned long long k = __shfl_sync(0xffffffffu, key, j);
-    const unsigned long long prev = j == 0 ? before : __shfl_sync(0xffffffffu, key, j > 0 ? j - 1 : 0);
-    const unsigned long long next = __shfl_sync(0xffffffffu, key, j + 1);
-    if (j >= count || k >= rows || (lead && !lead_long && k == first)) continue;   // (the whole warp)
-    if (k != prev || j == 0) {
-      opened = k != prev;
+    const unsigned k = __shfl_sync(all, f[0], j);
+    if (!live || !(used >> j & 1u)) continue;
+    if ((heads >> j & 1u) || j == 0) {
+      opened = heads >> j & 1u;
 #pragma unroll
       for (int i = 0; i < N; ++i) acc[i] = 0.f;
     }
-    if (!live) continue;
     add(g[j]);
-    if (j == count - 1 ? trail : k == next) continue;
+    if (!(ends >> j & 1u)) continue;
     if (opened) grad_store<T, N>(out, a, k, unit, acc);
     else leave(0);
   }
-  if (!trail || (lead && !lead_long && last == first)) return;
+  if (!trail || !(used >> (count - 1) & 1u)) return;
+  opened = to < count || !lead;
   if (!opened || trail_long) {
     if (live) leave(opened ? 1 : 0);
     return;
   }
-  for (int at = i0 + count; ; at += LG_TILE) {       // the rest of the run
-    const unsigned long long kk = lane < LG_TILE && at + lane < a.n ? a.keys[at + lane] : ~0ull;
-    const unsigned int vv = lane < LG_TILE && at + lane < a.n ? a.vals[at + lane] : 0u;
-    const int more = __popc(__ballot_sync(0xffffffffu, lane < LG_TILE && kk == last));
+  for (int at = count; at < count + behind; at += LG_TILE) {       // the rest of the run
 #pragma unroll
     for (int u = 0; u < LG_TILE; ++u) {
-      const unsigned int v = __shfl_sync(0xffffffffu, vv, u);
-      if (live && u < more) g[u] = load(v);
+      const unsigned v0 = __shfl_sync(all, val[0], (at + u) & 31), v1 = __shfl_sync(all, val[1], (at + u) & 31);
+      if (live && at + u < count + behind) g[u] = load(at + u < 32 ? v0 : v1);
     }
 #pragma unroll
-    for (int u = 0; u < LG_TILE; ++u) if (live && u < more) add(g[u]);
-    if (more < LG_TILE) break;
+    for (int u = 0; u < LG_TILE; ++u) if (live && at + u < count + behind) add(g[u]);
   }
   if (live) grad_store<T, N>(out, a, last, unit, acc);
 }

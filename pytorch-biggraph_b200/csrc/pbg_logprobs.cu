@@ -31,111 +31,327 @@ struct LogprobArgs {
   int *errors;
 };
 
-// A warp's best scores so far: lane l holds the l-th, larger ones first, equal ones by id.
-struct Best { float v; int id; };
-__device__ __forceinline__ bool best_before(float v, int id, float w, int jd) { return v > w || (v == w && id < jd); }
-// v, id: the same in every lane
-__device__ __forceinline__ void best_insert(Best &b, float v, int id, int top, int lane) {
-  const int at = __popc(__ballot_sync(0xffffffffu, best_before(b.v, b.id, v, id)));
-  if (at >= top) return;
-  const float pv = __shfl_up_sync(0xffffffffu, b.v, 1);
-  const int pi = __shfl_up_sync(0xffffffffu, b.id, 1);
-  if (lane > at) { b.v = pv; b.id = pi; }
-  if (lane == at) { b.v = v; b.id = id; }
+// The 16-byte vectors of a row.  16-bit scores are compared two at a time; the rest is fp32, two products or sums to an instruction.
+template <class T> struct Row16;
+template <> struct Row16<float> {
+  static constexpr unsigned NEG_INF = 0xff800000u;
+  float cm;
+  __device__ __forceinline__ void start(unsigned w) { cm = __uint_as_float(w); }
+  __device__ __forceinline__ void seen(unsigned w) { cm = fmaxf(cm, __uint_as_float(w)); }
+  __device__ __forceinline__ float largest() const { return cm; }
+};
+template <class T, class T2> struct Row16Half {
+  T2 m;
+  __device__ __forceinline__ void start(unsigned w) { m = *reinterpret_cast<T2 *>(&w); }
+  __device__ __forceinline__ void seen(unsigned w) { m = __hmax2(m, *reinterpret_cast<T2 *>(&w)); }
+  __device__ __forceinline__ float largest() const { const float2 f = TokPair<T>::up(m); return fmaxf(f.x, f.y); }
+};
+template <> struct Row16<__nv_bfloat16> : Row16Half<__nv_bfloat16, __nv_bfloat162> { static constexpr unsigned NEG_INF = 0xff80ff80u; };
+template <> struct Row16<__half> : Row16Half<__half, __half2> { static constexpr unsigned NEG_INF = 0xfc00fc00u; };
+
+// one word of a vector: two 16-bit scores or one fp32 score
+template <class T> __device__ __forceinline__ float2 word_up(unsigned w) { return TokPair<T>::up(*reinterpret_cast<typename TokPair<T>::type *>(&w)); }
+template <> __device__ __forceinline__ float2 word_up<float>(unsigned w) { return make_float2(__uint_as_float(w), -INFINITY); }
+
+__device__ __forceinline__ unsigned long long f32x2(float a, float b) { unsigned long long p; asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b)); return p; }
+__device__ __forceinline__ float2 f32x2_parts(unsigned long long p) { float2 f; asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p)); return f; }
+__device__ __forceinline__ unsigned long long f32x2_fma(unsigned long long a, unsigned long long b, unsigned long long c) {
+  unsigned long long d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ unsigned long long f32x2_add(unsigned long long a, unsigned long long b) {
+  unsigned long long d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
 }
 
+// What a thread gathers over its part of a row: S and T of its even and odd scores against the reference s.r, and how many scores stand in
+// front of the target's.
+template <class T>
 struct RowScan {
-  Soft s;
-  Best best;
-  unsigned rank;                         // scores in front of the target's so far
-  int top, lane, target;
-  float c, mine, above;                  // scale in base 2; the target's score; the next larger number
+  static constexpr int WORDS = 4 * LP_VECS, VEC = Tok<T>::VEC;
+  Soft s;                                // S and T: joined at the end
+  unsigned long long S2, T2;
+  unsigned rank;
+  int target;
+  float c, mine, above;                  // scale in base 2; the target's score; the next larger score
+  unsigned mine2, above2;                // (the same, twice in a word)
 
-  __device__ __forceinline__ void start(float scale, float target_score, int target_id, int top_, int lane_) {
+  __device__ __forceinline__ void start(float scale, const T *row, bool known, int target_id) {
     s = Soft{-INFINITY, 0.f, 0.f, 0.f};
-    best = Best{-INFINITY, LP_NO_ID};
-    rank = 0u; top = top_; lane = lane_; target = target_id; c = scale * TOK_LOG2E; mine = target_score;
-    above = mine == INFINITY ? __int_as_float(0x7fc00000) : nextafterf(mine, INFINITY);
+    S2 = T2 = f32x2(0.f, 0.f);
+    rank = 0u; target = target_id; c = scale * TOK_LOG2E;
+    const float nan = __int_as_float(0x7fc00000);
+    mine = known ? Tok<T>::up(row[target]) : nan;
+    above = mine == INFINITY ? nan : nextafterf(mine, INFINITY);
+    if constexpr (sizeof(T) == 2) {
+      // the next larger number of the type: the next pattern, towards zero for the negative ones
+      const unsigned short b = known ? *reinterpret_cast<const unsigned short *>(row + target) : 0x7fff;
+      const unsigned short n = mine != mine || mine == INFINITY ? 0x7fff : mine == 0.f ? 1 : mine > 0.f ? b + 1 : b - 1;
+      mine2 = b * 0x10001u;
+      above2 = n * 0x10001u;
+    }
   }
-
-  // V vectors of N elements, `live` of them there (the others hold -inf); element i of vector u has the id first + u * step + i.
-  // later: every id is larger than those of the steps before.
-  template <bool TOP, int V, int N>
-  __device__ __forceinline__ void step(const float (&x)[V * N], int first, int stride, int live, bool later) {
-    float cm = x[0];
-#pragma unroll
-    for (int q = 1; q < V * N; ++q) cm = fmaxf(cm, x[q]);
-    if (cm > s.m) { s.m = cm; soft_rebase(s, soft_reference(cm), c); }
-#pragma unroll
-    for (int u = 0; u < V; ++u) {
-      const int id0 = first + u * stride;
-      // score in front of the target: larger, or equal with a smaller id
-      const float limit = id0 + N <= target ? mine : above;
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float v = x[u * N + i];
-        const float y = tok_max_nan((v - s.r) * c, -1000.f);             // 2^-1000 is 0 in fp32 too; -inf has no place in T
-        const float e = tok_ex2(y);
-        s.S += e;
-        s.T = fmaf(y, e, s.T);
-        rank += v >= limit ? 1u : 0u;
-      }
-      if (N > 1 && u < live && id0 <= target && target < id0 + N) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) rank += x[u * N + i] == mine && id0 + i < target ? 1u : 0u;
-      }
-    }
-    if (TOP) keep<V, N>(x, first, stride, live, cm, later);
+  __device__ __forceinline__ void raise(float m) {                     // a new largest score
+    s.m = m;
+    const float r = soft_reference(m), d = fminf(fmaxf((s.r - r) * c, -1e30f), 0.f), f = tok_ex2(d);
+    const unsigned long long d2 = f32x2(d, d), f2 = f32x2(f, f), zero = f32x2(0.f, 0.f);
+    T2 = f32x2_fma(f32x2_fma(d2, S2, T2), f2, zero);
+    S2 = f32x2_fma(S2, f2, zero);
+    s.r = r;
   }
-
-  template <int V, int N>
-  __device__ __forceinline__ void keep(const float (&x)[V * N], int first, int stride, int live, float cm, bool later) {
-    const float worst = __shfl_sync(0xffffffffu, best.v, top - 1);
-    const bool full = __shfl_sync(0xffffffffu, best.id, top - 1) != LP_NO_ID;
-    // where all ids are larger than the kept ones, a score equal to the worst does not enter
-    const bool strict = full && later;
-    if (full && !__any_sync(0xffffffffu, later ? cm > worst : cm >= worst)) return;
-    float floor_v = worst;
-    if (!full) {
-      // the top-th largest of the lanes' maxima: at least `top` scores are not below it
-      const float mx = live > 0 && cm == cm ? cm : -INFINITY;
-      int at = 0;
-      for (int l = 0; l < 32; ++l) {
-        const float o = __shfl_sync(0xffffffffu, mx, l);
-        at += o > mx || (o == mx && l < lane);
+  __device__ __forceinline__ void finish() {
+    const float2 a = f32x2_parts(S2), b = f32x2_parts(T2);
+    s.S = a.x + a.y;
+    s.T = b.x + b.y;
+  }
+  // LP_VECS vectors, `live` of them there (the others hold -inf); element i of vector u has the id first + u * 32 * VEC + i
+  __device__ __forceinline__ void step(const unsigned (&raw)[WORDS], int first, int live) {
+    Row16<T> top;
+    top.start(raw[0]);
+#pragma unroll
+    for (int q = 1; q < WORDS; ++q) top.seen(raw[q]);
+    const float cm = top.largest();
+    if (cm > s.m) raise(cm);
+    const float rc = s.r * c;
+    if (fabsf(rc) < 1e38f) {
+      const unsigned long long c2 = f32x2(c, c), r2 = f32x2(-rc, -rc);
+      constexpr int PAIRS = sizeof(T) == 2 ? WORDS : WORDS / 2;
+#pragma unroll
+      for (int q = 0; q < PAIRS; ++q) {
+        const float2 x = sizeof(T) == 2 ? word_up<T>(raw[q]) : make_float2(__uint_as_float(raw[2 * q % WORDS]), __uint_as_float(raw[(2 * q + 1) % WORDS]));
+        float2 y = f32x2_parts(f32x2_fma(f32x2(x.x, x.y), c2, r2));
+        y.x = tok_max_nan(y.x, -1000.f);                               // 2^-1000 is 0 in fp32 too; -inf has no place in T
+        y.y = tok_max_nan(y.y, -1000.f);
+        const unsigned long long e2 = f32x2(tok_ex2(y.x), tok_ex2(y.y));
+        S2 = f32x2_add(S2, e2);
+        T2 = f32x2_fma(f32x2(y.x, y.y), e2, T2);
       }
-      floor_v = __shfl_sync(0xffffffffu, mx, __ffs(__ballot_sync(0xffffffffu, at == top - 1)) - 1);
+    } else {                                                             // scores near the type's ends: the reference has no place in base 2
+#pragma unroll 1
+      for (int q = 0; q < WORDS; ++q) {
+        const float2 x = word_up<T>(pick(raw, q));
+        const float y0 = tok_max_nan((x.x - s.r) * c, -1000.f), y1 = tok_max_nan((x.y - s.r) * c, -1000.f);
+        const unsigned long long e2 = f32x2(tok_ex2(y0), sizeof(T) == 2 ? tok_ex2(y1) : 0.f);
+        S2 = f32x2_add(S2, e2);
+        T2 = f32x2_fma(f32x2(y0, y1), e2, T2);
+      }
     }
-    unsigned mask = 0u;
+    // scores in front of the target's: larger ones, and equal ones with a smaller id
+    if constexpr (sizeof(T) == 2) {
+      using P = typename TokPair<T>::type;
+      unsigned zero = 0u;
+      P count = *reinterpret_cast<P *>(&zero);
 #pragma unroll
-    for (int q = 0; q < V * N; ++q) {
-      const float v = x[q] == x[q] ? x[q] : -INFINITY;
-      if (q / N < live && (strict ? v > floor_v : v >= floor_v)) mask |= 1u << q;
+      for (int u = 0; u < LP_VECS; ++u) {
+        unsigned limit = first + u * 32 * VEC + VEC <= target ? mine2 : above2;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) { unsigned w = raw[4 * u + q]; count = __hadd2(count, __hge2(*reinterpret_cast<P *>(&w), *reinterpret_cast<P *>(&limit))); }
+      }
+      const float2 f = TokPair<T>::up(count);                          // (at most 16 each)
+      rank += (unsigned)(f.x + f.y);
+    } else {
+#pragma unroll
+      for (int u = 0; u < LP_VECS; ++u) {
+        const float limit = first + u * 32 * VEC + VEC <= target ? mine : above;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) rank += __uint_as_float(raw[4 * u + q]) >= limit ? 1u : 0u;
+      }
     }
-    for (unsigned have; (have = __ballot_sync(0xffffffffu, mask != 0u)) != 0u;) {
-      const int src = __ffs(have) - 1, q = __ffs(mask) - 1;
-      float pick[V * N];
-#pragma unroll
-      for (int i = 0; i < V * N; ++i) pick[i] = x[i];
-#pragma unroll
-      for (int half = V * N / 2; half >= 1; half /= 2)
-#pragma unroll
-        for (int i = 0; i < half; ++i) pick[i] = (q & half) ? pick[i + half] : pick[i];
-      const float v = __shfl_sync(0xffffffffu, pick[0] == pick[0] ? pick[0] : -INFINITY, src);
-      const int id = __shfl_sync(0xffffffffu, first + q / N * stride + q % N, src);
-      if (lane == src) mask &= mask - 1u;
-      best_insert(best, v, id, top, lane);
+    const int at = target - first, u = at / (32 * VEC), in = at - u * 32 * VEC;
+    if (at >= 0 && u < live && in < VEC) {                               // the vector that holds the target
+#pragma unroll 1
+      for (int i = 0; i < in; ++i) {
+        const float2 x = word_up<T>(pick(raw, 4 * u + i * 4 / VEC));
+        rank += ((sizeof(T) == 2 && (i & 1)) ? x.y : x.x) == mine ? 1u : 0u;
+      }
     }
+  }
+  // raw[q] for a q that is not known to the compiler (rare paths)
+  static __device__ __forceinline__ unsigned pick(const unsigned (&raw)[WORDS], int q) {
+    unsigned w = raw[0];
+#pragma unroll
+    for (int i = 1; i < WORDS; ++i) w = i == q ? raw[i] : w;
+    return w;
+  }
+  __device__ __forceinline__ void edge(float x, int id) {                // a single element
+    if (x > s.m) raise(x);
+    const float y = tok_max_nan((x - s.r) * c, -1000.f), e = tok_ex2(y);
+    S2 = f32x2_add(S2, f32x2(e, 0.f));
+    T2 = f32x2_fma(f32x2(y, 0.f), f32x2(e, 0.f), T2);
+    rank += x > mine || (x == mine && id < target) ? 1u : 0u;
   }
 };
 
+// ---- the best scores ------------------------------------------------------------------------------------
+// Order: larger scores first, equal ones by id, NaN as -inf.  The scan leaves the largest score of every thread; the top-th largest of 64
+// groups of four threads is a threshold that at least `top` scores reach and hardly more than that pass.  The threads whose largest
+// score reaches it look through their part again, all threads helping, and what reaches it is ranked by counting.  Where too
+// much does (equal scores, mostly), those above it are taken and the first of those equal to it; where even that is too much, the best
+// are found one after the other.
+#define LP_CANDIDATES 512
+struct Best { float v; int id; };
+__device__ __forceinline__ bool best_before(Best a, Best b) { return a.v > b.v || (a.v == b.v && a.id < b.id); }
+
+// A CTA's part of a row: the elements in front of the first 16-byte boundary and behind the last whole vector (the edges; the last CTA of
+// a cluster has them, an element to a lane of its last warp), and every nct-th block of LP_WARPS steps.
+template <class T> struct RowPart {
+  static constexpr int VEC = Tok<T>::VEC;
+  const T *row;
+  int vocab, head, vecs, tail, cta, nct;
+  __device__ RowPart(const T *r, long long n, int cta_, int nct_) : row(r), vocab((int)n), cta(cta_), nct(nct_) {
+    const int off = (int)(((uintptr_t)r & 15) / sizeof(T));
+    head = off == 0 ? 0 : VEC - off < n ? VEC - off : (int)n;
+    vecs = (int)((n - head) / VEC);
+    tail = (int)((n - head) % VEC);
+  }
+  __device__ bool edges() const { return cta == nct - 1; }
+  __device__ int steps() const { return (vecs + 32 * LP_VECS - 1) / (32 * LP_VECS); }                       // of all CTAs
+  __device__ int vec(int warp, int turn, int u, int lane) const { return ((turn * nct + cta) * LP_WARPS + warp) * 32 * LP_VECS + u * 32 + lane; }
+  __device__ int turns() const { return (steps() + nct * LP_WARPS - 1) / (nct * LP_WARPS); }
+  __device__ int edge_id(int lane) const { return lane < 16 ? (lane < head ? lane : -1) : lane - 16 < tail ? vocab - tail + lane - 16 : -1; }
+  __device__ float at(int id) const { const float x = Tok<T>::up(row[id]); return x != x ? -INFINITY : x; }
+};
+
+struct TopShared {
+  float group[64];
+  float tau;
+  int count, flagged;
+  unsigned short threads[LP_THREADS];
+  Best cand[LP_CANDIDATES], list[LP_TOP_MAX], warp_best[LP_WARPS];
+  int have;
+};
+
+// cand[0 .. count) to list[0 .. have), the first `top` in order
+__device__ __forceinline__ void rank_candidates(TopShared &sh, int top) {
+  const int n = sh.count;
+  for (int i = threadIdx.x; i < n; i += LP_THREADS) {
+    const Best mine = sh.cand[i];
+    int ahead = 0;
+    for (int k = 0; k < n; ++k) ahead += best_before(sh.cand[k], mine) ? 1 : 0;
+    if (ahead < top) sh.list[ahead] = mine;
+  }
+  if (threadIdx.x == 0) sh.have = n < top ? n : top;
+  __syncthreads();
+}
+
+template <class T>
+__device__ void top_of_part(const RowPart<T> &p, float m, int top, TopShared &sh) {
+  constexpr int VEC = Tok<T>::VEC;
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  float g = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, 2));
+  if ((lane & 3) == 0) sh.group[threadIdx.x / 4] = g;
+  if (threadIdx.x == 0) { sh.count = 0; sh.flagged = 0; sh.have = 0; }
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    const float mine = sh.group[threadIdx.x];
+    int ahead = 0;
+#pragma unroll 16
+    for (int k = 0; k < 64; ++k) { const float o = sh.group[k]; ahead += o > mine || (o == mine && k < (int)threadIdx.x) ? 1 : 0; }
+    if (ahead == top - 1) sh.tau = mine;
+  }
+  __syncthreads();
+  const float tau = sh.tau;
+  auto gather = [&](bool strict) {
+    if (strict ? m > tau : m >= tau) sh.threads[atomicAdd(&sh.flagged, 1)] = (unsigned short)threadIdx.x;
+    __syncthreads();
+    const int per = p.turns() * LP_VECS, items = sh.flagged * per;
+    auto take = [&](float x, int id) {
+      if (strict ? x > tau : x >= tau) { const int k = atomicAdd(&sh.count, 1); if (k < LP_CANDIDATES) sh.cand[k] = Best{x, id}; }
+    };
+    for (int i = threadIdx.x; i < items; i += LP_THREADS) {
+      const int who = sh.threads[i / per], r = i % per, v = p.vec(who / 32, r / LP_VECS, r % LP_VECS, who % 32);
+      if (v >= p.vecs) continue;
+      float x[VEC];
+      tok_unpack<T>(reinterpret_cast<const uint4 *>(p.row + p.head)[v], x);
+      float most = x[0];
+#pragma unroll
+      for (int k = 1; k < VEC; ++k) most = fmaxf(most, x[k]);
+      if (!(strict ? most > tau : most >= tau)) continue;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) take(x[k], p.head + v * VEC + k);
+    }
+    if (p.edges() && w == LP_WARPS - 1 && p.edge_id(lane) >= 0) take(p.at(p.edge_id(lane)), p.edge_id(lane));
+    __syncthreads();
+  };
+  bool strict = tau == -INFINITY;                                        // (fewer than `top` groups with a score at all)
+  gather(strict);
+  if (sh.count > LP_CANDIDATES && !strict) {
+    __syncthreads();
+    if (threadIdx.x == 0) sh.count = sh.flagged = 0;
+    __syncthreads();
+    strict = true;
+    gather(true);
+  }
+  if (sh.count > LP_CANDIDATES) {
+    // one after the other
+    Best prev{INFINITY, -1};
+    for (int k = 0; k < top; ++k) {
+      Best best{-INFINITY, LP_NO_ID};
+      auto see = [&](float x, int id) {
+        const Best b{x != x ? -INFINITY : x, id};
+        if (best_before(prev, b) && best_before(b, best)) best = b;
+      };
+      for (int turn = 0; turn < p.turns(); ++turn)
+        for (int u = 0; u < LP_VECS; ++u) {
+          const int v = p.vec(w, turn, u, lane);
+          if (v >= p.vecs) break;
+          float x[VEC];
+          tok_unpack<T>(reinterpret_cast<const uint4 *>(p.row + p.head)[v], x);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) see(x[e], p.head + v * VEC + e);
+        }
+      if (p.edges() && w == LP_WARPS - 1 && p.edge_id(lane) >= 0) see(p.at(p.edge_id(lane)), p.edge_id(lane));
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const Best b{__shfl_xor_sync(0xffffffffu, best.v, o), __shfl_xor_sync(0xffffffffu, best.id, o)};
+        if (best_before(b, best)) best = b;
+      }
+      __syncthreads();
+      if (lane == 0) sh.warp_best[w] = best;
+      __syncthreads();
+      best = sh.warp_best[0];
+      for (int o = 1; o < LP_WARPS; ++o) if (best_before(sh.warp_best[o], best)) best = sh.warp_best[o];
+      if (best.id == LP_NO_ID) break;                                    // (the same in every thread)
+      if (threadIdx.x == 0) { sh.list[k] = best; sh.have = k + 1; }
+      prev = best;
+    }
+    __syncthreads();
+    return;
+  }
+  rank_candidates(sh, top);
+  if (!strict || sh.have >= top) return;
+  // the first of those equal to the threshold
+  if (w == 0) {
+    int have = sh.have;
+    auto more = [&](bool there, int id) {                                // a warp's look at 32 elements in the order of their ids
+      const bool hit = there && p.at(id) == tau;
+      const unsigned hits = __ballot_sync(0xffffffffu, hit);
+      const int place = have + __popc(hits & ((1u << lane) - 1u));
+      if (hit && place < top) sh.list[place] = Best{tau, id};
+      have += __popc(hits);
+    };
+    if (p.edges()) more(lane < p.head, lane);
+    const int span = LP_WARPS * 32 * LP_VECS * VEC;                      // elements of a turn
+    for (int turn = 0; turn < p.turns() && have < top; ++turn) {
+      const int first = p.head + p.vec(0, turn, 0, 0) * VEC, end = p.head + p.vecs * VEC;
+      for (int i = 0; i < span && first + i < end && have < top; i += 32) more(i + lane < span && first + i + lane < end, first + i + lane);
+    }
+    if (p.edges() && have < top) more(lane < p.tail, p.vocab - p.tail + lane);
+    if (lane == 0) sh.have = have < top ? have : top;
+  }
+  __syncthreads();
+}
+
 // A cluster of CTAs per row (a single CTA where there are rows for all SMs); the warps take steps of 32 x LP_VECS vectors in turn.
 template <class T, bool TOP>
-__global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(const T *__restrict__ logits, LogprobArgs a) {
+__global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const T *__restrict__ logits, LogprobArgs a) {
   constexpr int VEC = Tok<T>::VEC;
   struct Part { Soft s; unsigned rank; };
   __shared__ Part parts[LP_WARPS], cta_part;
-  __shared__ Best bests[LP_WARPS][LP_TOP_MAX], cta_best[LP_TOP_MAX];
+  __shared__ TopShared top_shared[1];
   cg::cluster_group cluster = cg::this_cluster();
   const int nct = (int)cluster.num_blocks(), cta = (int)cluster.block_rank();
   const long long n = blockIdx.x / nct;
@@ -148,38 +364,36 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(const T *__restric
     }
     return;
   }
-  const T *row = logits + n * a.row_stride;
   const bool known = target >= 0 && target < a.vocab;
-  // the elements in front of the first 16-byte boundary and behind the last whole vector are the row's edges
-  const int off = (int)(((uintptr_t)row & 15) / sizeof(T));
-  const int head = off == 0 ? 0 : VEC - off < a.vocab ? VEC - off : (int)a.vocab;
-  const int vecs = (int)((a.vocab - head) / VEC), tail = (int)((a.vocab - head) % VEC);
-  RowScan g;
-  g.start(a.scale, known ? Tok<T>::up(row[target]) : __int_as_float(0x7fc00000), known ? (int)target : -1, a.top, lane);
-
-  const uint4 *vec = reinterpret_cast<const uint4 *>(row + head);
-  const int steps = (vecs + 32 * LP_VECS - 1) / (32 * LP_VECS);
+  const RowPart<T> p(logits + n * a.row_stride, a.vocab, cta, nct);
+  RowScan<T> g;
+  g.start(a.scale, p.row, known, known ? (int)target : -1);
+  const uint4 *vec = reinterpret_cast<const uint4 *>(p.row + p.head);
+  const int steps = p.steps();
   for (int b = cta * LP_WARPS + w; b < steps; b += nct * LP_WARPS) {
     const int v0 = b * 32 * LP_VECS + lane;
-    const int live = v0 >= vecs ? 0 : (vecs - v0 + 31) / 32 < LP_VECS ? (vecs - v0 + 31) / 32 : LP_VECS;
-    uint4 raw[LP_VECS];
+    unsigned raw[4 * LP_VECS];
+    int live = LP_VECS;
+    if ((b + 1) * 32 * LP_VECS <= p.vecs) {
 #pragma unroll
-    for (int u = 0; u < LP_VECS; ++u) if (u < live) raw[u] = __ldcs(vec + v0 + u * 32);
-    float x[LP_VECS * VEC];
+      for (int u = 0; u < LP_VECS; ++u) {
+        const uint4 x = TOP ? vec[v0 + u * 32] : __ldcs(vec + v0 + u * 32);
+        raw[4 * u] = x.x; raw[4 * u + 1] = x.y; raw[4 * u + 2] = x.z; raw[4 * u + 3] = x.w;
+      }
+    } else {
+      live = v0 >= p.vecs ? 0 : (p.vecs - v0 + 31) / 32 < LP_VECS ? (p.vecs - v0 + 31) / 32 : LP_VECS;
 #pragma unroll
-    for (int u = 0; u < LP_VECS; ++u) {
-      float y[VEC];
-      tok_unpack<T>(raw[u], y);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) x[u * VEC + i] = u < live ? y[i] : -INFINITY;
+      for (int u = 0; u < LP_VECS; ++u) {
+        uint4 x = make_uint4(Row16<T>::NEG_INF, Row16<T>::NEG_INF, Row16<T>::NEG_INF, Row16<T>::NEG_INF);
+        if (u < live) x = vec[v0 + u * 32];
+        raw[4 * u] = x.x; raw[4 * u + 1] = x.y; raw[4 * u + 2] = x.z; raw[4 * u + 3] = x.w;
+      }
     }
-    g.step<TOP, LP_VECS, VEC>(x, head + v0 * VEC, 32 * VEC, live, true);
+    g.step(raw, p.head + v0 * VEC, live);
   }
-  if (cta == nct - 1 && w == LP_WARPS - 1 && head + tail > 0) {           // the edges: an element per lane
-    const int id = lane < 16 ? (lane < head ? lane : -1) : lane - 16 < tail ? (int)(a.vocab - tail) + lane - 16 : -1;
-    const float x[1] = {id >= 0 ? Tok<T>::up(row[id]) : -INFINITY};
-    g.step<TOP, 1, 1>(x, id >= 0 ? id : LP_NO_ID - 1, 0, id >= 0 ? 1 : 0, false);
-  }
+  if (p.edges() && w == LP_WARPS - 1 && p.edge_id(lane) >= 0) g.edge(Tok<T>::up(p.row[p.edge_id(lane)]), p.edge_id(lane));
+  g.finish();
+  const float mine_m = g.s.m;
 
   // lanes, warps, CTAs
 #pragma unroll
@@ -188,41 +402,38 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(const T *__restric
     g.rank += __shfl_xor_sync(0xffffffffu, g.rank, o);
   }
   if (lane == 0) parts[w] = Part{g.s, g.rank};
-  if (TOP) bests[w][lane] = g.best;
   __syncthreads();
   if (w == 0) {
-    for (int o = 1; o < LP_WARPS; ++o) {
-      soft_join(g.s, parts[o].s, g.c);
-      g.rank += parts[o].rank;
-      if (TOP) {
-        for (int l = 0; l < a.top; ++l) {                                // (sorted: the first that does not enter ends it)
-          const Best b = bests[o][l];
-          const float wv = __shfl_sync(0xffffffffu, g.best.v, a.top - 1);
-          const int wi = __shfl_sync(0xffffffffu, g.best.id, a.top - 1);
-          if (!best_before(b.v, b.id, wv, wi)) break;
-          best_insert(g.best, b.v, b.id, a.top, lane);
-        }
-      }
+    g.s = parts[lane % LP_WARPS].s;
+    g.rank = parts[lane % LP_WARPS].rank;
+#pragma unroll
+    for (int o = LP_WARPS / 2; o > 0; o >>= 1) {
+      soft_join(g.s, soft_shfl(g.s, o), g.c);
+      g.rank += __shfl_xor_sync(0xffffffffu, g.rank, o);
     }
-    if (nct > 1) { if (lane == 0) cta_part = Part{g.s, g.rank}; if (TOP) cta_best[lane] = g.best; }
+    if (nct > 1 && lane == 0) cta_part = Part{g.s, g.rank};
   }
+  if (TOP) top_of_part<T>(p, mine_m, a.top, top_shared[0]);
   if (nct > 1) {
     cluster.sync();
-    if (cta == 0 && w == 0) {
-      for (int o = 1; o < nct; ++o) {
-        const Part p = *cluster.map_shared_rank(&cta_part, o);
-        soft_join(g.s, p.s, g.c);
-        g.rank += p.rank;
-        if (TOP) {
-          const Best *list = cluster.map_shared_rank(cta_best, o);
-          const Best mine = list[lane];
-          for (int l = 0; l < a.top; ++l) {
-            const float v = __shfl_sync(0xffffffffu, mine.v, l), wv = __shfl_sync(0xffffffffu, g.best.v, a.top - 1);
-            const int id = __shfl_sync(0xffffffffu, mine.id, l), wi = __shfl_sync(0xffffffffu, g.best.id, a.top - 1);
-            if (!best_before(v, id, wv, wi)) break;
-            best_insert(g.best, v, id, a.top, lane);
-          }
+    if (cta == 0) {
+      if (w == 0)
+        for (int o = 1; o < nct; ++o) {
+          const Part q = *cluster.map_shared_rank(&cta_part, o);
+          soft_join(g.s, q.s, g.c);
+          g.rank += q.rank;
         }
+      if (TOP) {
+        static_assert(8 * LP_TOP_MAX <= LP_CANDIDATES, "the lists of a cluster");
+        TopShared &sh = top_shared[0];
+        if (threadIdx.x == 0) sh.count = 0;
+        __syncthreads();
+        for (int i = threadIdx.x; i < nct * a.top; i += LP_THREADS) {
+          const TopShared *of = cluster.map_shared_rank(top_shared, i / a.top);
+          if (i % a.top < of->have) sh.cand[atomicAdd(&sh.count, 1)] = of->list[i % a.top];
+        }
+        __syncthreads();
+        rank_candidates(sh, a.top);
       }
     }
     cluster.sync();                                                      // nobody leaves while its shared memory is read
@@ -238,9 +449,10 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(const T *__restric
     a.rank[n] = known ? 1 + (long long)g.rank : 0;
   }
   if (TOP && lane < a.top) {
-    const float x = Tok<T>::up(row[g.best.id < a.vocab ? g.best.id : 0]);                          // (as it is: NaN stands in the list as -inf)
+    const int id = top_shared[0].list[lane].id;
+    const float x = Tok<T>::up(p.row[id >= 0 && id < a.vocab ? id : 0]);  // (as it is: NaN stands in the list as -inf)
     a.top_logprobs[n * a.top + lane] = empty ? -INFINITY : (x - g.s.r) * a.scale - log_s;
-    a.top_ids[n * a.top + lane] = g.best.id;
+    a.top_ids[n * a.top + lane] = id;
   }
 }
 

@@ -218,6 +218,37 @@ def test_logprobs_of_rows_of_equal_scores_keep_the_order_of_ids():
             assert r.rank.tolist() == [1, vocab, vocab // 2 + 1]
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,vocab", [(2, 100_003), (2, 8192), (310, 20_000), (305, 517)])
+@pytest.mark.parametrize("kind", ["falling", "rising", "few", "none but one", "steps", "block of equals", "blocks"])
+def test_best_scores_however_they_lie(dtype, n, vocab, kind):
+    """The largest scores next to each other, far fewer scores than asked for, more equal ones than a list holds: in rows of one CTA
+    and of several."""
+    ids = torch.arange(vocab, device=DEV).double()
+    if kind == "falling":
+        x = -ids / 64
+    elif kind == "rising":
+        x = ids / 64
+    elif kind == "few":
+        x = torch.where(ids % (vocab // 5) == 3, ids / vocab, -math.inf)
+    elif kind == "none but one":
+        x = torch.where(ids == vocab - 2, 1.0, -math.inf)
+    elif kind == "steps":
+        x = (ids * 7919 % vocab * 8 / vocab).floor()
+    elif kind == "block of equals":
+        x = torch.where((ids > vocab / 3) & (ids < vocab / 2), 2.0, 1.0)
+        x[vocab // 2 + 5] = 3.0
+    else:
+        x = torch.where(ids < vocab // 2, (ids / 700).floor() % 3, 0.0) + (ids % 700 == 0)
+    x = x.to(dtype).expand(n, vocab).contiguous()
+    targets = torch.randint(0, vocab, (n,), device=DEV, generator=gen(1))
+    for top in (1, 7, 32):
+        r = T.token_logprobs(x, targets, top=top)
+        want = torch.sort(x[:1].float(), dim=1, descending=True, stable=True).indices[:, :top]
+        assert torch.equal(r.top_ids, want.expand(n, top)), (kind, top)
+    assert torch.equal(r.rank, _want(x, targets, 1.0, 1)[3])
+
+
 def test_logprobs_with_nan_infinity_and_bad_targets():
     x = torch.randn(6, 3000, device=DEV, generator=gen(2))
     x[0, 5], x[1, 7], x[2, 2999] = math.nan, math.inf, math.nan

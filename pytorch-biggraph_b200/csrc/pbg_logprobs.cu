@@ -107,7 +107,8 @@ struct RowScan {
     s.T = b.x + b.y;
   }
   // LP_VECS vectors, `live` of them there (the others hold -inf); element i of vector u has the id first + u * 32 * VEC + i
-  __device__ __forceinline__ void step(const unsigned (&raw)[WORDS], int first, int live) {
+  // their largest score
+  __device__ __forceinline__ float step(const unsigned (&raw)[WORDS], int first, int live) {
     Row16<T> top;
     top.start(raw[0]);
 #pragma unroll
@@ -167,6 +168,7 @@ struct RowScan {
         rank += ((sizeof(T) == 2 && (i & 1)) ? x.y : x.x) == mine ? 1u : 0u;
       }
     }
+    return cm;
   }
   // raw[q] for a q that is not known to the compiler (rare paths)
   static __device__ __forceinline__ unsigned pick(const unsigned (&raw)[WORDS], int q) {
@@ -185,12 +187,14 @@ struct RowScan {
 };
 
 // ---- the best scores ------------------------------------------------------------------------------------
-// Order: larger scores first, equal ones by id, NaN as -inf.  The scan leaves the largest score of every thread; the top-th largest of 64
-// groups of four threads is a threshold that at least `top` scores reach and hardly more than that pass.  The threads whose largest
-// score reaches it look through their part again, all threads helping, and what reaches it is ranked by counting.  Where too
-// much does (equal scores, mostly), those above it are taken and the first of those equal to it; where even that is too much, the best
-// are found one after the other.
+// Order: larger scores first, equal ones by id, NaN as -inf.  The scan leaves the largest score of every thread, and of each sixteenth of
+// its turns.  The top-th largest of 64 groups of four threads is a threshold that at least `top` scores reach and hardly
+// more than that pass.  The sixteenths that reach it are looked through again, all threads helping, and what reaches it is ranked by
+// counting.  Where too much does (equal scores, mostly), those above it are taken and the first of those equal to it; where even
+// that is too much, the best are found one after the other.  (A sorted list per warp, kept during the scan, took longer than the scan:
+// 211 us for 1024 x 131,072 bf16 and the best 8, where the scan takes 59.)
 #define LP_CANDIDATES 512
+#define LP_SLOTS 16
 struct Best { float v; int id; };
 __device__ __forceinline__ bool best_before(Best a, Best b) { return a.v > b.v || (a.v == b.v && a.id < b.id); }
 
@@ -218,7 +222,8 @@ struct TopShared {
   float group[64];
   float tau;
   int count, flagged;
-  unsigned short threads[LP_THREADS];
+  float slot[LP_SLOTS][LP_THREADS];       // the largest score of a thread in its `per` turns of that slot
+  unsigned short places[LP_CANDIDATES];  // slot x LP_THREADS + thread
   Best cand[LP_CANDIDATES], list[LP_TOP_MAX], warp_best[LP_WARPS];
   int have;
 };
@@ -254,16 +259,26 @@ __device__ void top_of_part(const RowPart<T> &p, float m, int top, TopShared &sh
   }
   __syncthreads();
   const float tau = sh.tau;
+  const int turns = p.turns(), per = (turns + LP_SLOTS - 1) / LP_SLOTS;
   auto gather = [&](bool strict) {
-    if (strict ? m > tau : m >= tau) sh.threads[atomicAdd(&sh.flagged, 1)] = (unsigned short)threadIdx.x;
+    for (int k = 0; k * per < turns; ++k) {
+      const float x = sh.slot[k][threadIdx.x];
+      if (strict ? x > tau : x >= tau) { const int at = atomicAdd(&sh.flagged, 1); if (at < LP_CANDIDATES) sh.places[at] = (unsigned short)(k * LP_THREADS + threadIdx.x); }
+    }
     __syncthreads();
-    const int per = p.turns() * LP_VECS, items = sh.flagged * per;
+    if (sh.flagged > LP_CANDIDATES) {                                    // too much already
+      if (threadIdx.x == 0) sh.count = LP_CANDIDATES + 1;
+      __syncthreads();
+      return;
+    }
+    const int each = per * LP_VECS, items = sh.flagged * each;
     auto take = [&](float x, int id) {
       if (strict ? x > tau : x >= tau) { const int k = atomicAdd(&sh.count, 1); if (k < LP_CANDIDATES) sh.cand[k] = Best{x, id}; }
     };
     for (int i = threadIdx.x; i < items; i += LP_THREADS) {
-      const int who = sh.threads[i / per], r = i % per, v = p.vec(who / 32, r / LP_VECS, r % LP_VECS, who % 32);
-      if (v >= p.vecs) continue;
+      const int place = sh.places[i / each], r = i % each, who = place % LP_THREADS, turn = place / LP_THREADS * per + r / LP_VECS;
+      const int v = p.vec(who / 32, turn, r % LP_VECS, who % 32);
+      if (turn >= turns || v >= p.vecs) continue;
       float x[VEC];
       tok_unpack<T>(reinterpret_cast<const uint4 *>(p.row + p.head)[v], x);
       float most = x[0];
@@ -370,7 +385,11 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const T *__rest
   g.start(a.scale, p.row, known, known ? (int)target : -1);
   const uint4 *vec = reinterpret_cast<const uint4 *>(p.row + p.head);
   const int steps = p.steps();
-  for (int b = cta * LP_WARPS + w; b < steps; b += nct * LP_WARPS) {
+  const int stride = nct * LP_WARPS, per = (p.turns() + LP_SLOTS - 1) / LP_SLOTS;
+  int slot = 0, in_slot = 0;
+  float slot_max = -INFINITY;
+  if (TOP) for (int k = 0; k < LP_SLOTS; ++k) top_shared[0].slot[k][threadIdx.x] = -INFINITY;
+  for (int b = cta * LP_WARPS + w; b < steps; b += stride) {
     const int v0 = b * 32 * LP_VECS + lane;
     unsigned raw[4 * LP_VECS];
     int live = LP_VECS;
@@ -389,7 +408,11 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const T *__rest
         raw[4 * u] = x.x; raw[4 * u + 1] = x.y; raw[4 * u + 2] = x.z; raw[4 * u + 3] = x.w;
       }
     }
-    g.step(raw, p.head + v0 * VEC, live);
+    const float cm = g.step(raw, p.head + v0 * VEC, live);
+    if (TOP) {
+      slot_max = fmaxf(slot_max, cm);
+      if (++in_slot == per || b + stride >= steps) { top_shared[0].slot[slot++][threadIdx.x] = slot_max; slot_max = -INFINITY; in_slot = 0; }
+    }
   }
   if (p.edges() && w == LP_WARPS - 1 && p.edge_id(lane) >= 0) g.edge(Tok<T>::up(p.row[p.edge_id(lane)]), p.edge_id(lane));
   g.finish();

@@ -508,6 +508,21 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_grad_kernel(const T *logi
   const int off = (int)(((uintptr_t)to & 15) / sizeof(T));
   const int head = off == 0 ? 0 : VEC - off < a.vocab ? VEC - off : (int)a.vocab;
   const int vecs = (int)((a.vocab - head) / VEC), tail = (int)((a.vocab - head) % VEC);
+  uint4 *tv = reinterpret_cast<uint4 *>(to + head);
+  const int v0 = piece * STEP + threadIdx.x;
+  // the scores are asked for first: they wait for nothing that is read below
+  uint4 raw[LP_VECS];
+  float x[ALIKE ? 1 : LP_VECS][VEC];
+  if (ALIKE) {
+    const uint4 *vec = reinterpret_cast<const uint4 *>(row + head);
+#pragma unroll
+    for (int u = 0; u < LP_VECS; ++u) if (v0 + u * LP_THREADS < vecs) raw[u] = __ldcs(vec + v0 + u * LP_THREADS);
+  } else {
+#pragma unroll
+    for (int u = 0; u < LP_VECS; ++u)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) x[ALIKE ? 0 : u][i] = v0 + u * LP_THREADS < vecs ? Tok<T>::up(row[head + (v0 + u * LP_THREADS) * VEC + i]) : 0.f;
+  }
   const long long target = a.targets[n];
   const bool known = target >= 0 && target < a.vocab && target != a.ignore_index;
   if (!known && target != a.ignore_index && piece == 0 && threadIdx.x == 0 && a.errors) atomicOr(a.errors, TOK_ERR_ID);
@@ -519,31 +534,14 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_grad_kernel(const T *logi
   r.H = a.h ? a.entropy[n] : 0.f;
   const bool none = !known || r.lse == -INFINITY;                        // padding, or a row of -inf alone: zeros
   const int t = none ? -1 : (int)target;
-  uint4 *tv = reinterpret_cast<uint4 *>(to + head);
-  const int v0 = piece * STEP + threadIdx.x;
-  float x[LP_VECS][VEC];
-  if (!none) {
-    if (ALIKE) {
-      const uint4 *vec = reinterpret_cast<const uint4 *>(row + head);
-      uint4 raw[LP_VECS];
-#pragma unroll
-      for (int u = 0; u < LP_VECS; ++u) if (v0 + u * LP_THREADS < vecs) raw[u] = __ldcs(vec + v0 + u * LP_THREADS);
-#pragma unroll
-      for (int u = 0; u < LP_VECS; ++u) tok_unpack<T>(raw[u], x[u]);
-    } else {
-#pragma unroll
-      for (int u = 0; u < LP_VECS; ++u)
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) x[u][i] = v0 + u * LP_THREADS < vecs ? Tok<T>::up(row[head + (v0 + u * LP_THREADS) * VEC + i]) : 0.f;
-    }
-  }
 #pragma unroll
   for (int u = 0; u < LP_VECS; ++u) {
     if (v0 + u * LP_THREADS >= vecs) continue;
     const int id0 = head + (v0 + u * LP_THREADS) * VEC;
+    if (ALIKE) tok_unpack<T>(raw[u], x[0]);
     float d[VEC];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) d[i] = none ? 0.f : r.at(x[u][i]);
+    for (int i = 0; i < VEC; ++i) d[i] = none ? 0.f : r.at(x[ALIKE ? 0 : u][i]);
     if (id0 <= t && t < id0 + VEC) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) if (id0 + i == t) d[i] += r.g;

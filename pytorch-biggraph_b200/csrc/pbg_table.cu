@@ -13,8 +13,8 @@
 // One persistent kernel per product, one CTA per SM, tiles of 128 x BN (BN <= 256) or, by a pair of CTAs, 256 x BN:
 //   warp 0     TMA into a ring of stages (64 k-values of one plane, or 32 of two)
 //   warp 1     issues tcgen05.mma into one of two accumulators of 256 columns
-//   warps 2-9  read the other accumulator and, two warps to every 32 rows: reduce it to (maximum, S, T) per row; or turn it into dz and
-//              write that; or write the product
+//   warps 2-9  read the other accumulator, two warps to every 32 rows: reduce it to (maximum, S, T) per row; or turn it into
+//              dz and write that; or write the product
 // A pair (cta_group::2): each CTA holds 128 rows of A and half of B's columns, the first one issues for both, and an operand byte
 // in shared memory feeds twice as many products.  Alone, a tile of 128 x 256 writes and reads 192 bytes of shared memory per cycle of
 // its products where the SM moves 128; a pair 128.
@@ -29,18 +29,23 @@
 
 enum { EPI_STATS = 0, EPI_DZ = 1, EPI_OUT = 2 };
 
-#define TAB_RING_BYTES 196608                               // stages; as many as fit
 #define TAB_STAGES_MAX 6
-#define TAB_EPI_WARPS 8
-#define TAB_THREADS (64 + 32 * TAB_EPI_WARPS)
-#define TAB_SMEM (1024 + TAB_RING_BYTES + TAB_EPI_WARPS * 4096)
 #define TAB_DZ_BYTES (2ll << 30)                            // most memory for dz: beyond it the table goes in pieces
 #define TAB_PARTS_BYTES (512ll << 20)                       // and for the tiles' partial sums: beyond it the queries do
-// The tensor cores cut off what they add up instead of rounding it, a bias of half a step per addition.  Contractions of
-// fp32 operands are therefore cut into parts of this many blocks of 32 k-values (48 and 18 additions: the scores' epilogue has more to do,
-// their contractions are the shorter ones), which are added in registers.
-#define TAB_F32_PART 8
-#define TAB_F32_PART_OUT 3
+// The tensor cores cut off what they add up instead of rounding it, a bias of half a step per addition.  Where results are fp32 the
+// contraction is therefore cut into parts, which are added in registers: blocks of k-values per part, for scores and products of fp32
+// operands (18 additions to a part), for the gradient of their scores, whose epilogue has more to do (48), and for scores of 16-bit operands (32).
+// Products of 5000 fp32 terms were 3.9e-5 off in one piece and are 5e-7 off in parts.
+#define TAB_PART_F32 3
+#define TAB_PART_F32_DZ 8
+#define TAB_PART_16 8
+
+// Eight warps share a tile's columns (two to every 32 rows), each with 4 KB of shared memory to write from; the ring of stages has the
+// rest.  (Sixteen warps with half the columns each had registers for half of what they need and were slower.)
+template <int EPI, class MATH> struct TabShape {
+  static constexpr bool PARTS = MATH::NPB == 2 || EPI == EPI_STATS;
+  static constexpr int WARPS = 8, THREADS = 64 + 32 * WARPS, SHARE = WARPS / 4, RING = 196608, SMEM = 1024 + RING + WARPS * 4096;
+};
 
 // Operands: their elements, the planes of A and B, the type of results
 template <class E, class O, int PA, int PB> struct TabMath { using elem = E; using out = O; static constexpr int NPA = PA, NPB = PB; };
@@ -106,17 +111,19 @@ __device__ __forceinline__ void tab_commit(uint32_t bar) {
   else asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" :: "r"(bar), "h"((unsigned short)3) : "memory");
 }
 template <int EPI, class MATH, bool A_MN, bool B_MN, int CG>
-__global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_constant__ TabMaps maps, TabArgs g) {
+__global__ void __launch_bounds__(TabShape<EPI, MATH>::THREADS, 1) tab_kernel(const __grid_constant__ TabMaps maps, TabArgs g) {
   using Elem = typename MATH::elem;
   using Out = typename MATH::out;
   constexpr int NPA = MATH::NPA, NPB = MATH::NPB, KB = NPA == 1 ? 64 : 32;
-  constexpr bool PARTS = NPB == 2;                                        // fp32: the contraction is added up in registers
+  using Shape = TabShape<EPI, MATH>;
+  constexpr bool PARTS = Shape::PARTS;                                    // the contraction is added up in registers
+  constexpr int HC = 256 / Shape::SHARE;                                  // most columns of a warp
   constexpr uint32_t FMT = std::is_same<Elem, __nv_bfloat16>::value ? 1u : 0u;
   constexpr uint32_t ROW_BYTES = KB * 2, ATOM_BYTES = KB * 128;          // a K-major row; 64 columns of an MN-major operand's plane
   constexpr uint32_t A_BYTES = NPA * 128 * ROW_BYTES;
   extern __shared__ unsigned char smem_raw[];
   unsigned char *smem = (unsigned char *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  unsigned char *ostage = smem + TAB_RING_BYTES;
+  unsigned char *ostage = smem + Shape::RING;
   __shared__ __align__(8) unsigned long long bars[2 * TAB_STAGES_MAX + 4];
   __shared__ uint32_t tmem_base_s;
   __shared__ volatile int failed;
@@ -129,7 +136,7 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
   auto acce_bar = [&](int a) { return bar0 + 8u * (2 * TAB_STAGES_MAX + 2 + a); };
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2 * TAB_STAGES_MAX + 2; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar0 + 8u * i));
-    for (int a = 0; a < 2; ++a) asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(acce_bar(a)), "r"(TAB_EPI_WARPS * CG));
+    for (int a = 0; a < 2; ++a) asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(acce_bar(a)), "r"(Shape::WARPS * CG));
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     failed = 0;
   }
@@ -242,7 +249,7 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
     }
   } else {
     // ---------------- epilogue
-    const int q = warp & 3, half = (warp - 2) >> 2, hc = g.BN / 2;       // 32 rows of the tile; half of its columns
+    const int q = warp & 3, share = (warp - 2) >> 2, hc = g.BN / Shape::SHARE;        // 32 rows of the tile; a share of its columns
     unsigned char *buf = ostage + (size_t)(warp - 2) * 4096;
     const uint32_t drained = CG == 1 ? 0u : in_first_cta(acce_bar(0));
     float unscale = 1.f, up = g.scale;
@@ -269,16 +276,17 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
           if (g.g) g0 = gg = g.g[m] * up;
           if (g.h) { const float h = g.h[m] * up; hh = h * TOK_LN2; gg = fmaf(h, g.entropy[m], gg); }
           hot = target - g.v0;
-        } else if (target != g.ignore_index && n0 == 0 && half == 0 && g.v0 == 0) atomicOr(g.err, TOK_ERR_ID);
+        } else if (target != g.ignore_index && n0 == 0 && share == 0 && g.v0 == 0) atomicOr(g.err, TOK_ERR_ID);
       }
-      const long long c0 = n0 + half * hc;                               // first column of this warp
+      const long long c0 = n0 + share * hc;                               // first column of this warp
       const int cols = c0 >= g.N ? 0 : g.N - c0 < hc ? (int)(g.N - c0) : hc;
-      const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * hc);
+      const bool idle = m0 + q * 32 >= g.M;                              // none of these rows exists
+      const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(share * hc);
       // The tile's values.  PARTS: all of them, added up in registers as the accumulators fill; else read by 32 columns below.
-      float sum[PARTS ? 128 : 1];
+      float sum[PARTS ? HC : 1];
+      // (the whole warp waits: one lane that does and a vote behind it take 200 cycles longer)
       auto wait_full = [&]() {
-        bool w = failed == 0;
-        if (w && lane == 0) w = mbar_wait(accf_bar(j & 1), (uint32_t)(j >> 1) & 1, g.err);
+        const bool w = mbar_wait(accf_bar(j & 1), (uint32_t)(j >> 1) & 1, g.err);
         if (!__all_sync(0xffffffffu, w)) { failed = 1; return false; }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         return true;
@@ -295,13 +303,13 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
       };
       if (PARTS) {
 #pragma unroll
-        for (int i = 0; i < 128; ++i) sum[PARTS ? i : 0] = 0.f;
+        for (int i = 0; i < HC; ++i) sum[PARTS ? i : 0] = 0.f;
         for (int p0 = kb0; p0 < kb1; p0 = kb1 - p0 < g.part ? kb1 : p0 + g.part) {
           ok = wait_full();
           if (!ok) break;
 #pragma unroll
-          for (int x = 0; x < 128; x += 32) {
-            if (x >= hc) continue;
+          for (int x = 0; x < HC; x += 32) {
+            if (x >= hc || idle) continue;
             uint32_t v[32];
             tmem_ld32(lanes + (uint32_t)(j & 1) * 256u + x, v);
 #pragma unroll
@@ -348,8 +356,8 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
         }
       };
 #pragma unroll PARTS ? 4 : 1
-      for (int x = 0; x < 128; x += 32) {
-        if (x >= span) break;
+      for (int x = 0; x < HC; x += 32) {
+        if (x >= span || idle) break;
         float v[32];
         values(x, v);
         if (EPI == EPI_STATS) {
@@ -462,7 +470,7 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
           if ((x & 32) || x + 32 >= span) store_go((int)(c0 + (x & ~32)), (int)(m0 + q * 32), 0, rows > 0);
         }
       }
-      if (EPI == EPI_STATS && m < g.M) g.parts[m * g.nparts + n0 / g.BN * 2 + half] = make_float4(S == 0.f ? -1e30f : r, S, T, 0.f);
+      if (EPI == EPI_STATS && m < g.M) g.parts[m * g.nparts + n0 / g.BN * Shape::SHARE + share] = make_float4(S == 0.f ? -1e30f : r, S, T, 0.f);
       if (!PARTS && kb0 < kb1) give_back();
     }
     if (EPI != EPI_STATS && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");         // the stores are performed
@@ -784,23 +792,24 @@ static bool tab_launch_as(const TabOperand &a, const TabOperand &b, const TabOpe
     if (g.bulk && !encode_map(&maps.c, fp32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, to, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return false;
   }
   if (!(g.b_whole ? tab_encode_blocks(&maps.b, bf16, b, KB, g.BN / CG / 64) : tab_encode(&maps.b, bf16, b, B_MN ? 64 : KB, B_MN ? KB : g.BN / CG, b.planes))) return false;
+  using Shape = TabShape<EPI, MATH>;
   const int stage = MATH::NPA * 128 * KB * 2 + MATH::NPB * (g.BN / CG) * KB * 2;
-  g.stages = TAB_RING_BYTES / stage < TAB_STAGES_MAX ? TAB_RING_BYTES / stage : TAB_STAGES_MAX;
+  g.stages = Shape::RING / stage < TAB_STAGES_MAX ? Shape::RING / stage : TAB_STAGES_MAX;
   void (*kernel)(TabMaps, TabArgs) = tab_kernel<EPI, MATH, A_MN, B_MN, CG>;
-  pbg_opt_in_smem((const void *)kernel, TAB_SMEM);
+  pbg_opt_in_smem((const void *)kernel, Shape::SMEM);
   const long long tiles = (g.M + 128 * CG - 1) / (128 * CG) * ((g.N + g.BN - 1) / g.BN) * g.splits, most = pbg_sm_count() / CG;
   const unsigned groups = (unsigned)(tiles < most ? tiles : most);
-  if (CG == 1) pbg_launch(kernel, dim3(groups), TAB_THREADS, TAB_SMEM, st, maps, g);
-  else pbg_launch_clusters(kernel, (int)groups, CG, TAB_THREADS, TAB_SMEM, st, maps, g);
+  if (CG == 1) pbg_launch(kernel, dim3(groups), Shape::THREADS, Shape::SMEM, st, maps, g);
+  else pbg_launch_clusters(kernel, (int)groups, CG, Shape::THREADS, Shape::SMEM, st, maps, g);
   return true;
 }
 
-// Tile columns, a multiple of `step`: the fewest columns for the SM with the most of them, with what a tile costs beside them.
-static int tab_columns(long long tiles_m, long long N, int step, int cg) {
+// Tile columns, 128 or 256: the fewest columns for the SM with the most of them, with what a tile costs beside them.
+static int tab_columns(long long tiles_m, long long N, int cg) {
   const long long groups = pbg_sm_count() / cg > 0 ? pbg_sm_count() / cg : 1;
   int best = 256;
   long long cost = -1;
-  for (int bn = 256; bn >= step; bn -= step) {
+  for (int bn = 256; bn >= 128; bn -= 128) {
     const long long tiles = tiles_m * ((N + bn - 1) / bn), c = (tiles + groups - 1) / groups * (bn + 16);
     if (cost < 0 || c < cost) { cost = c; best = bn; }
   }
@@ -827,7 +836,7 @@ static bool tab_pairs(long long M, long long N) { return M > 128 && N > 64; }
 
 template <int EPI, class MATH, bool A_MN, bool B_MN>
 static bool tab_launch(const TabOperand &a, const TabOperand &b, TabArgs &g, bool pairs, cudaStream_t st, const TabOperand *c = nullptr) {
-  g.part = MATH::NPB != 2 ? 0x7fffffff : EPI == EPI_OUT ? TAB_F32_PART_OUT : TAB_F32_PART;
+  g.part = MATH::NPB == 2 ? (EPI == EPI_DZ ? TAB_PART_F32_DZ : TAB_PART_F32) : EPI == EPI_STATS ? TAB_PART_16 : 0x7fffffff;
   return pairs ? tab_launch_as<EPI, MATH, A_MN, B_MN, 2>(a, b, c, g, st) : tab_launch_as<EPI, MATH, A_MN, B_MN, 1>(a, b, c, g, st);
 }
 
@@ -865,8 +874,8 @@ static TabPlace tab_place(long long n, long long rows, int dim, int dtype, bool 
     at = p.parts = p.q;                                      // no copies
     at += n * p.nparts * 16;
   } else if (!grad) {
-    p.bn = tab_columns((n + (p.pairs ? 255 : 127)) / (p.pairs ? 256 : 128), rows, p.pairs ? 128 : 64, p.pairs ? 2 : 1);
-    p.nparts = (int)((rows + p.bn - 1) / p.bn * 2);
+    p.bn = tab_columns((n + (p.pairs ? 255 : 127)) / (p.pairs ? 256 : 128), rows, p.pairs ? 2 : 1);
+    p.nparts = (int)((rows + p.bn - 1) / p.bn * TabShape<EPI_STATS, TabF32>::SHARE);
     long long most = TAB_PARTS_BYTES / (16ll * p.nparts) / 256 * 256;
     if (most < 256) most = 256;
     if (p.piece > most) p.piece = most;
@@ -990,10 +999,10 @@ static void tab_backward(TabBackward &f) {
   constexpr int KB = MATH::NPA == 1 ? 64 : 32, KB2 = DZMATH::NPA == 1 ? 64 : 32;
   tab_prepare<T>(c, f.p, true, f.g, f.h);
   const bool partial = f.p.splits > 1 || f.p.columns < c.rows;
-  auto plan = [&](TabArgs &a, bool &pairs, long long M, long long N, int splits, int step) {       // step: of the columns of a single CTA's tile
+  auto plan = [&](TabArgs &a, bool &pairs, long long M, long long N, int splits) {
     pairs = tab_pairs(M, N);
     a.M = M; a.N = N; a.splits = splits; a.sc = c.sc; a.err = c.err;
-    a.BN = tab_columns((M + (pairs ? 255 : 127)) / (pairs ? 256 : 128) * splits, N, pairs ? 128 : step, pairs ? 2 : 1);
+    a.BN = tab_columns((M + (pairs ? 255 : 127)) / (pairs ? 256 : 128) * splits, N, pairs ? 2 : 1);
   };
   for (long long v0 = 0; v0 < c.rows && f.ok; v0 += f.p.columns) {
     const long long cols = c.rows - v0 < f.p.columns ? c.rows - v0 : f.p.columns;
@@ -1002,7 +1011,7 @@ static void tab_backward(TabBackward &f) {
     w.rows = cols;
     TabArgs g = {};
     bool pairs;
-    plan(g, pairs, c.n, cols, 1, 64);
+    plan(g, pairs, c.n, cols, 1);
     g.kblocks = (int)((c.dim + KB - 1) / KB);
     g.m_first = 1; g.scale = c.scale;
     g.by_q = g.by_w = 1;
@@ -1015,7 +1024,7 @@ static void tab_backward(TabBackward &f) {
     f.ok = tab_launch<EPI_DZ, MATH, false, false>(c.q, w, g, pairs, c.st, &written);
     if (f.dq && f.ok) {
       TabArgs d = {};
-      plan(d, pairs, c.n, c.dim, f.p.splits, 128);
+      plan(d, pairs, c.n, c.dim, f.p.splits);
       d.kblocks = (int)((cols + KB2 - 1) / KB2);
       d.by_dz = d.by_w = 1;
       d.out = f.dq; d.ldo = c.dim;
@@ -1024,7 +1033,7 @@ static void tab_backward(TabBackward &f) {
     }
     if (f.dt && f.ok) {
       TabArgs d = {};
-      plan(d, pairs, cols, c.dim, 1, 128);
+      plan(d, pairs, cols, c.dim, 1);
       d.kblocks = (int)((c.n + KB2 - 1) / KB2);
       d.by_dz = d.by_q = 1;
       d.out = (T *)f.dt + v0 * c.dim; d.ldo = c.dim;

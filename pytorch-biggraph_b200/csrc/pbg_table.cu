@@ -34,18 +34,21 @@ enum { EPI_STATS = 0, EPI_DZ = 1, EPI_OUT = 2 };
 #define TAB_PARTS_BYTES (512ll << 20)                       // and for the tiles' partial sums: beyond it the queries do
 // The tensor cores cut off what they add up instead of rounding it, a bias of half a step per addition.  Where results are fp32 the
 // contraction is therefore cut into parts, which are added in registers: blocks of k-values per part, for scores and products of fp32
-// operands (18 additions to a part), for the gradient of their scores, whose epilogue has more to do (48), and for scores of 16-bit operands (32).
-// Products of 5000 fp32 terms were 3.9e-5 off in one piece and are 5e-7 off in parts.
+// operands (18 additions to a part), for the gradient of their scores, whose epilogue has more to do (48), and for scores of 16-bit operands
+// (32) of more than TAB_WHOLE elements.  Products of 5000 fp32 terms were 3.9e-5 off in one piece and are 5e-7 off in parts.  Scores of
+// 2048 16-bit terms are 8e-7 off in one piece and 2e-7 in parts; the registers that the parts take cost 7 queries x
+// 131,072 x 2048 bf16 12 of 102 us, so that these are left whole.
 #define TAB_PART_F32 3
 #define TAB_PART_F32_DZ 8
 #define TAB_PART_16 8
+#define TAB_WHOLE 2048
 
 // Eight warps share a tile's columns (two to every 32 rows), each with 4 KB of shared memory to write from; the ring of stages has the
 // rest.  (Sixteen warps with half the columns each had registers for half of what they need and were slower.)
-template <int EPI, class MATH> struct TabShape {
-  static constexpr bool PARTS = MATH::NPB == 2 || EPI == EPI_STATS;
-  static constexpr int WARPS = 8, THREADS = 64 + 32 * WARPS, SHARE = WARPS / 4, RING = 196608, SMEM = 1024 + RING + WARPS * 4096;
-};
+#define TAB_EPI_WARPS 8
+#define TAB_THREADS (64 + 32 * TAB_EPI_WARPS)
+#define TAB_RING_BYTES 196608
+#define TAB_SMEM (1024 + TAB_RING_BYTES + TAB_EPI_WARPS * 4096)
 
 // Operands: their elements, the planes of A and B, the type of results
 template <class E, class O, int PA, int PB> struct TabMath { using elem = E; using out = O; static constexpr int NPA = PA, NPB = PB; };
@@ -110,20 +113,17 @@ __device__ __forceinline__ void tab_commit(uint32_t bar) {
   if (CG == 1) mma_commit(bar);
   else asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" :: "r"(bar), "h"((unsigned short)3) : "memory");
 }
-template <int EPI, class MATH, bool A_MN, bool B_MN, int CG>
-__global__ void __launch_bounds__(TabShape<EPI, MATH>::THREADS, 1) tab_kernel(const __grid_constant__ TabMaps maps, TabArgs g) {
+template <int EPI, class MATH, bool A_MN, bool B_MN, int CG, bool PARTS>        // PARTS: the contraction is added up in registers
+__global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_constant__ TabMaps maps, TabArgs g) {
   using Elem = typename MATH::elem;
   using Out = typename MATH::out;
   constexpr int NPA = MATH::NPA, NPB = MATH::NPB, KB = NPA == 1 ? 64 : 32;
-  using Shape = TabShape<EPI, MATH>;
-  constexpr bool PARTS = Shape::PARTS;                                    // the contraction is added up in registers
-  constexpr int HC = 256 / Shape::SHARE;                                  // most columns of a warp
   constexpr uint32_t FMT = std::is_same<Elem, __nv_bfloat16>::value ? 1u : 0u;
   constexpr uint32_t ROW_BYTES = KB * 2, ATOM_BYTES = KB * 128;          // a K-major row; 64 columns of an MN-major operand's plane
   constexpr uint32_t A_BYTES = NPA * 128 * ROW_BYTES;
   extern __shared__ unsigned char smem_raw[];
   unsigned char *smem = (unsigned char *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  unsigned char *ostage = smem + Shape::RING;
+  unsigned char *ostage = smem + TAB_RING_BYTES;
   __shared__ __align__(8) unsigned long long bars[2 * TAB_STAGES_MAX + 4];
   __shared__ uint32_t tmem_base_s;
   __shared__ volatile int failed;
@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(TabShape<EPI, MATH>::THREADS, 1) tab_kernel(co
   auto acce_bar = [&](int a) { return bar0 + 8u * (2 * TAB_STAGES_MAX + 2 + a); };
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2 * TAB_STAGES_MAX + 2; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar0 + 8u * i));
-    for (int a = 0; a < 2; ++a) asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(acce_bar(a)), "r"(Shape::WARPS * CG));
+    for (int a = 0; a < 2; ++a) asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(acce_bar(a)), "r"(TAB_EPI_WARPS * CG));
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     failed = 0;
   }
@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(TabShape<EPI, MATH>::THREADS, 1) tab_kernel(co
     }
   } else {
     // ---------------- epilogue
-    const int q = warp & 3, share = (warp - 2) >> 2, hc = g.BN / Shape::SHARE;        // 32 rows of the tile; a share of its columns
+    const int q = warp & 3, half = (warp - 2) >> 2, hc = g.BN / 2;       // 32 rows of the tile; half of its columns
     unsigned char *buf = ostage + (size_t)(warp - 2) * 4096;
     const uint32_t drained = CG == 1 ? 0u : in_first_cta(acce_bar(0));
     float unscale = 1.f, up = g.scale;
@@ -276,14 +276,14 @@ __global__ void __launch_bounds__(TabShape<EPI, MATH>::THREADS, 1) tab_kernel(co
           if (g.g) g0 = gg = g.g[m] * up;
           if (g.h) { const float h = g.h[m] * up; hh = h * TOK_LN2; gg = fmaf(h, g.entropy[m], gg); }
           hot = target - g.v0;
-        } else if (target != g.ignore_index && n0 == 0 && share == 0 && g.v0 == 0) atomicOr(g.err, TOK_ERR_ID);
+        } else if (target != g.ignore_index && n0 == 0 && half == 0 && g.v0 == 0) atomicOr(g.err, TOK_ERR_ID);
       }
-      const long long c0 = n0 + share * hc;                               // first column of this warp
+      const long long c0 = n0 + half * hc;                               // first column of this warp
       const int cols = c0 >= g.N ? 0 : g.N - c0 < hc ? (int)(g.N - c0) : hc;
       const bool idle = m0 + q * 32 >= g.M;                              // none of these rows exists
-      const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(share * hc);
+      const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * hc);
       // The tile's values.  PARTS: all of them, added up in registers as the accumulators fill; else read by 32 columns below.
-      float sum[PARTS ? HC : 1];
+      float sum[PARTS ? 128 : 1];
       // (the whole warp waits: one lane that does and a vote behind it take 200 cycles longer)
       auto wait_full = [&]() {
         const bool w = mbar_wait(accf_bar(j & 1), (uint32_t)(j >> 1) & 1, g.err);
@@ -303,12 +303,12 @@ __global__ void __launch_bounds__(TabShape<EPI, MATH>::THREADS, 1) tab_kernel(co
       };
       if (PARTS) {
 #pragma unroll
-        for (int i = 0; i < HC; ++i) sum[PARTS ? i : 0] = 0.f;
+        for (int i = 0; i < 128; ++i) sum[PARTS ? i : 0] = 0.f;
         for (int p0 = kb0; p0 < kb1; p0 = kb1 - p0 < g.part ? kb1 : p0 + g.part) {
           ok = wait_full();
           if (!ok) break;
 #pragma unroll
-          for (int x = 0; x < HC; x += 32) {
+          for (int x = 0; x < 128; x += 32) {
             if (x >= hc || idle) continue;
             uint32_t v[32];
             tmem_ld32(lanes + (uint32_t)(j & 1) * 256u + x, v);
@@ -355,8 +355,8 @@ __global__ void __launch_bounds__(TabShape<EPI, MATH>::THREADS, 1) tab_kernel(co
           asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         }
       };
-#pragma unroll PARTS ? 4 : 1
-      for (int x = 0; x < HC; x += 32) {
+#pragma unroll(PARTS ? 4 : 1)
+      for (int x = 0; x < 128; x += 32) {
         if (x >= span || idle) break;
         float v[32];
         values(x, v);
@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(TabShape<EPI, MATH>::THREADS, 1) tab_kernel(co
           if ((x & 32) || x + 32 >= span) store_go((int)(c0 + (x & ~32)), (int)(m0 + q * 32), 0, rows > 0);
         }
       }
-      if (EPI == EPI_STATS && m < g.M) g.parts[m * g.nparts + n0 / g.BN * Shape::SHARE + share] = make_float4(S == 0.f ? -1e30f : r, S, T, 0.f);
+      if (EPI == EPI_STATS && m < g.M) g.parts[m * g.nparts + n0 / g.BN * 2 + half] = make_float4(S == 0.f ? -1e30f : r, S, T, 0.f);
       if (!PARTS && kb0 < kb1) give_back();
     }
     if (EPI != EPI_STATS && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");         // the stores are performed
@@ -768,7 +768,7 @@ static bool tab_encode_blocks(CUtensorMap *tm, bool bf16, const TabOperand &o, i
 }
 static bool tab_whole(const TabOperand &o) { return o.inner % 64 == 0 || o.ld >= tok_up(o.inner, 64); }
 
-template <int EPI, class MATH, bool A_MN, bool B_MN, int CG>
+template <int EPI, class MATH, bool A_MN, bool B_MN, int CG, bool PARTS>
 static bool tab_launch_as(const TabOperand &a, const TabOperand &b, const TabOperand *c, TabArgs &g, cudaStream_t st) {
   constexpr int KB = MATH::NPA == 1 ? 64 : 32;
   constexpr bool bf16 = std::is_same<typename MATH::elem, __nv_bfloat16>::value;
@@ -792,15 +792,14 @@ static bool tab_launch_as(const TabOperand &a, const TabOperand &b, const TabOpe
     if (g.bulk && !encode_map(&maps.c, fp32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, to, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return false;
   }
   if (!(g.b_whole ? tab_encode_blocks(&maps.b, bf16, b, KB, g.BN / CG / 64) : tab_encode(&maps.b, bf16, b, B_MN ? 64 : KB, B_MN ? KB : g.BN / CG, b.planes))) return false;
-  using Shape = TabShape<EPI, MATH>;
   const int stage = MATH::NPA * 128 * KB * 2 + MATH::NPB * (g.BN / CG) * KB * 2;
-  g.stages = Shape::RING / stage < TAB_STAGES_MAX ? Shape::RING / stage : TAB_STAGES_MAX;
-  void (*kernel)(TabMaps, TabArgs) = tab_kernel<EPI, MATH, A_MN, B_MN, CG>;
-  pbg_opt_in_smem((const void *)kernel, Shape::SMEM);
+  g.stages = TAB_RING_BYTES / stage < TAB_STAGES_MAX ? TAB_RING_BYTES / stage : TAB_STAGES_MAX;
+  void (*kernel)(TabMaps, TabArgs) = tab_kernel<EPI, MATH, A_MN, B_MN, CG, PARTS>;
+  pbg_opt_in_smem((const void *)kernel, TAB_SMEM);
   const long long tiles = (g.M + 128 * CG - 1) / (128 * CG) * ((g.N + g.BN - 1) / g.BN) * g.splits, most = pbg_sm_count() / CG;
   const unsigned groups = (unsigned)(tiles < most ? tiles : most);
-  if (CG == 1) pbg_launch(kernel, dim3(groups), Shape::THREADS, Shape::SMEM, st, maps, g);
-  else pbg_launch_clusters(kernel, (int)groups, CG, Shape::THREADS, Shape::SMEM, st, maps, g);
+  if (CG == 1) pbg_launch(kernel, dim3(groups), TAB_THREADS, TAB_SMEM, st, maps, g);
+  else pbg_launch_clusters(kernel, (int)groups, CG, TAB_THREADS, TAB_SMEM, st, maps, g);
   return true;
 }
 
@@ -836,8 +835,16 @@ static bool tab_pairs(long long M, long long N) { return M > 128 && N > 64; }
 
 template <int EPI, class MATH, bool A_MN, bool B_MN>
 static bool tab_launch(const TabOperand &a, const TabOperand &b, TabArgs &g, bool pairs, cudaStream_t st, const TabOperand *c = nullptr) {
-  g.part = MATH::NPB == 2 ? (EPI == EPI_DZ ? TAB_PART_F32_DZ : TAB_PART_F32) : EPI == EPI_STATS ? TAB_PART_16 : 0x7fffffff;
-  return pairs ? tab_launch_as<EPI, MATH, A_MN, B_MN, 2>(a, b, c, g, st) : tab_launch_as<EPI, MATH, A_MN, B_MN, 1>(a, b, c, g, st);
+  g.part = MATH::NPB == 2 ? (EPI == EPI_DZ ? TAB_PART_F32_DZ : TAB_PART_F32) : TAB_PART_16;
+  auto as = [&](auto parts) {
+    return pairs ? tab_launch_as<EPI, MATH, A_MN, B_MN, 2, decltype(parts)::value>(a, b, c, g, st) : tab_launch_as<EPI, MATH, A_MN, B_MN, 1, decltype(parts)::value>(a, b, c, g, st);
+  };
+  if constexpr (MATH::NPB == 2) return as(std::true_type());
+  else {
+    if constexpr (EPI == EPI_STATS) if (g.kblocks > TAB_WHOLE / 64) return as(std::true_type());
+    g.part = 0x7fffffff;
+    return as(std::false_type());
+  }
 }
 
 // TMA reads rows where they lie if they start on 16-byte boundaries
@@ -875,7 +882,7 @@ static TabPlace tab_place(long long n, long long rows, int dim, int dtype, bool 
     at += n * p.nparts * 16;
   } else if (!grad) {
     p.bn = tab_columns((n + (p.pairs ? 255 : 127)) / (p.pairs ? 256 : 128), rows, p.pairs ? 2 : 1);
-    p.nparts = (int)((rows + p.bn - 1) / p.bn * TabShape<EPI_STATS, TabF32>::SHARE);
+    p.nparts = (int)((rows + p.bn - 1) / p.bn * 2);
     long long most = TAB_PARTS_BYTES / (16ll * p.nparts) / 256 * 256;
     if (most < 256) most = 256;
     if (p.piece > most) p.piece = most;

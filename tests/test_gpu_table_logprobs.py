@@ -69,7 +69,7 @@ def check_forward(q, t, targets, scale, ignore=()):
     return r
 
 
-SHAPES = [(1, 1, 1), (1, 300, 8), (3, 64, 64), (5, 65, 33), (127, 255, 40), (129, 257, 72), (7, 20_011, 400), (200, 1000, 1), (64, 3000, 520), (300, 5000, 100), (1000, 14_951, 400)]
+SHAPES = [(1, 1, 1), (1, 300, 8), (3, 64, 64), (5, 65, 33), (127, 255, 40), (129, 257, 72), (7, 20_011, 400), (200, 1000, 1), (64, 3000, 520), (300, 5000, 100), (1000, 14_951, 400), (5, 700, 2112), (300, 900, 4096)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)

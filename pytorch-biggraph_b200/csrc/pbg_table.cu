@@ -33,12 +33,13 @@ enum { EPI_STATS = 0, EPI_DZ = 1, EPI_OUT = 2 };
 #define TAB_DZ_BYTES (2ll << 30)                            // most memory for dz: beyond it the table goes in pieces
 #define TAB_PARTS_BYTES (512ll << 20)                       // and for the tiles' partial sums: beyond it the queries do
 // The tensor cores cut off what they add up instead of rounding it, a bias of half a step per addition.  Where results are fp32 the
-// contraction is therefore cut into parts, which are added in registers: blocks of k-values per part, for scores and products of fp32
-// operands (18 additions to a part), for the gradient of their scores, whose epilogue has more to do (48), and for scores of 16-bit operands
-// (32) of more than TAB_WHOLE elements.  Products of 5000 fp32 terms were 3.9e-5 off in one piece and are 5e-7 off in parts.  Scores of
+// contraction is therefore cut into parts, which are added in registers: blocks of k-values per part, for scores of fp32 operands (36
+// additions to a part; with 18 the epilogue could not keep up), for products with their gradient (18), for that gradient, whose
+// epilogue has more to do (48), and for scores of 16-bit operands (32) of more than TAB_WHOLE elements.  Products of 5000 fp32 terms were 3.9e-5 off in one piece and are 5e-7 off in parts.  Scores of
 // 2048 16-bit terms are 8e-7 off in one piece and 2e-7 in parts; the registers that the parts take cost 7 queries x
 // 131,072 x 2048 bf16 12 of 102 us, so that these are left whole.
-#define TAB_PART_F32 3
+#define TAB_PART_F32 6
+#define TAB_PART_F32_OUT 3
 #define TAB_PART_F32_DZ 8
 #define TAB_PART_16 8
 #define TAB_WHOLE 2048
@@ -835,7 +836,7 @@ static bool tab_pairs(long long M, long long N) { return M > 128 && N > 64; }
 
 template <int EPI, class MATH, bool A_MN, bool B_MN>
 static bool tab_launch(const TabOperand &a, const TabOperand &b, TabArgs &g, bool pairs, cudaStream_t st, const TabOperand *c = nullptr) {
-  g.part = MATH::NPB == 2 ? (EPI == EPI_DZ ? TAB_PART_F32_DZ : TAB_PART_F32) : TAB_PART_16;
+  g.part = MATH::NPB == 2 ? (EPI == EPI_DZ ? TAB_PART_F32_DZ : EPI == EPI_OUT ? TAB_PART_F32_OUT : TAB_PART_F32) : TAB_PART_16;
   auto as = [&](auto parts) {
     return pairs ? tab_launch_as<EPI, MATH, A_MN, B_MN, 2, decltype(parts)::value>(a, b, c, g, st) : tab_launch_as<EPI, MATH, A_MN, B_MN, 1, decltype(parts)::value>(a, b, c, g, st);
   };

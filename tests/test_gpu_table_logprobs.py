@@ -233,3 +233,81 @@ def test_refusals_and_nothing_to_do():
     targets[2] = 10
     r = T.table_logprobs(q, t, targets, errors=errors)
     assert r.logprob[2].isnan() and r.lse.isfinite().all() and errors.item() == 1
+
+
+@pytest.mark.parametrize("dtype,n,rows", [(torch.bfloat16, 70_001, 16_500), (torch.float32, 30_000, 18_100)])
+def test_more_queries_than_the_workspace_holds_at_once(dtype, n, rows):
+    """The gradient of the scores is kept for pieces of the table, the parts of dQ added up from piece to piece; a sample of the rows of
+    both gradients is checked, and the sums over all of them."""
+    q, t, targets = inputs(n, rows, 16, dtype, 7)
+    r = T.table_logprobs(q, t, targets)
+    g = torch.randn(n, device=DEV, generator=gen(1))
+    dq, dt = T.table_logprobs_grad(q, t, targets, r.lse, None, g)
+    some = torch.arange(0, n, 997, device=DEV)
+    z, E = scores(q[some], t, 1.0)
+    w = -g[some].double()[:, None] * (z - r.lse[some].double()[:, None]).exp()
+    w[torch.arange(len(some), device=DEV), targets[some]] += g[some].double()
+    step = half_step(dtype) if dtype != torch.float32 else 2 ** -22
+    size = (w.abs() + 2 * g[some].double().abs()[:, None] * (z - r.lse[some].double()[:, None]).exp()) @ t.double().abs()
+    tol = size * (step + 2 * E.max() + 2e-5 + rows * 2 ** -23) + (w @ t.double()).abs() * half_step(dtype)
+    assert ((dq[some].double() - w @ t.double()).abs() <= tol).all()
+    # <dt, x> for a vector x is sum_n <dz_n, t x^T ...>: the table's gradient summed over its rows is sum_n (sum_v dz_nv) q_n, and sum_v dz_nv = 0
+    total, each = dt.double().sum(0), (g.double().abs()[:, None] * q.double().abs()).sum(0)
+    assert (total.abs() <= 2 * each * (step + half_step(dtype) + 2e-5)).all()
+    pick = torch.arange(0, rows, 501, device=DEV)
+    want, size = torch.zeros(len(pick), 16, dtype=torch.float64, device=DEV), torch.zeros(len(pick), 16, dtype=torch.float64, device=DEV)
+    for part in torch.arange(n, device=DEV).split(4096):
+        zz = q[part].double() @ t[pick].double().T
+        p = (zz - r.lse[part].double()[:, None]).exp()
+        hot = (targets[part][:, None] == pick[None, :]).double()
+        want += (g[part].double()[:, None] * (hot - p)).T @ q[part].double()
+        size += (g[part].double().abs()[:, None] * (hot + p)).T @ q[part].double().abs()
+    assert ((dt[pick].double() - want).abs() <= size * (step + 2 * E.max() + 2e-5 + n * 2 ** -23) + want.abs() * half_step(dtype)).all()
+
+
+def test_more_partial_sums_than_the_workspace_holds_at_once():
+    """The forward pass in pieces of the queries."""
+    n, rows = 150_000, 70_000
+    q, t, targets = inputs(n, rows, 8, torch.float16, 3)
+    r = T.table_logprobs(q, t, targets)
+    some = torch.cat((torch.arange(0, n, 2999, device=DEV), torch.tensor([n - 1], device=DEV)))
+    z, E = scores(q[some], t, 1.0)
+    logprob, ent, lse = want_forward(z, targets[some])
+    assert ((r.lse[some].double() - lse).abs() <= E + 2e-5 * (1 + lse.abs())).all()
+    assert ((r.logprob[some].double() - logprob).abs() <= 2 * (E + 2e-5 * (1 + lse.abs())) + 2e-5 * logprob.abs()).all()
+    assert ((r.entropy[some].double() - ent).abs() <= 80 * E + 2e-5 * (1 + ent + math.log(rows))).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_training_step_with_both_ends_of_a_table(dtype):
+    """Rows by id, a map, log probabilities over the same table, and the gradient of a policy loss with entropy back to the table and the map;
+    against autograd in 64 bits.  Every operator rounds to its type; the bound counts the four roundings on the way to a gradient,
+    each relative to the sums of sizes, which the 64-bit graph over absolute values gives."""
+    g = gen(11)
+    rows, dim, n = 3001, 72, 260
+    table = (torch.randn(rows, dim, device=DEV, generator=g) / 8).to(dtype)
+    mix = (torch.randn(dim, dim, device=DEV, generator=g) / 8).to(dtype)
+    ids, targets = torch.randint(0, 40, (n,), device=DEV, generator=g), torch.randint(0, rows, (n,), device=DEV, generator=g)
+    targets[::17] = -100
+    weight = torch.randn(n, device=DEV, generator=g)
+    scale = math.sqrt(dim)
+    # the step as a program makes it
+    x = T.embedding_lookup(table, ids, scale=scale)
+    h = x @ mix
+    f = T.table_logprobs(h, table, targets)
+    gain = torch.full((n,), 0.1, device=DEV)
+    dh, dtable = T.table_logprobs_grad(h, table, targets, f.lse, f.entropy, weight, gain)
+    dmix, dx = x.t() @ dh, dh @ mix.t()
+    T.embedding_lookup_grad(dx, ids, rows, scale=scale, out=dtable, accumulate=True)
+    # the same in 64 bits
+    W, M = table.double().requires_grad_(), mix.double().requires_grad_()
+    keep = targets >= 0
+    H = (W[ids] * f32(scale)) @ M
+    logp = torch.log_softmax(H @ W.T, 1)[keep]
+    loss = (weight[keep].double() * logp.gather(1, targets[keep][:, None])[:, 0]).sum() + 0.1 * torch.special.entr(logp.exp()).sum()
+    gW, gM = torch.autograd.grad(loss, (W, M))
+    for got, want in ((dtable, gW), (dmix, gM)):
+        rel = ((got.double() - want).norm() / want.norm()).item()
+        # scores of size s move p by s times the rounding of h: |h| |w| summed is below 30 here
+        assert rel < (30 + 4) * half_step(dtype) + 2e-5, rel
+

@@ -628,10 +628,33 @@ struct TabSource { const void *x; long long stride, rows; TabRows counts; int bl
 struct TabPrep {
   TabSource q, w;                                          // blocks 0: not prepared
   const float *g, *h; long long n; int gblocks;            // gblocks 0: dz is not scaled
-  float scale; int dim, planes, wide;                      // wide: rows of float4 on 16-byte boundaries
+  float scale; int dim, planes, wide;                      // wide: rows of whole 16-byte vectors on 16-byte boundaries
+  FastDiv by_units;                                        // units of a row: vectors, or elements
   unsigned *block_max; TabScales *sc;
 };
 
+// Hands the units of type U of a CTA's rows (those that do not count as zeros) to a function (row, unit, value), four in flight.
+template <class U, class F>
+__device__ __forceinline__ void tab_units(const TabPrep &a, const TabSource &s, int b, F &&f) {
+  const int units = a.dim / (int)(sizeof(U) / (a.planes ? 4 : 2));
+  const long long per = (s.rows + s.blocks - 1) / s.blocks, r0 = b * per, rows = s.rows - r0 < per ? s.rows - r0 : per;
+  const int total = rows > 0 ? (int)(rows * units) : 0;
+  for (int i0 = threadIdx.x; i0 < total; i0 += 4 * 256) {
+    U v[4];
+    long long row[4];
+    int at[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = i0 + k * 256 < total ? i0 + k * 256 : i0, r = a.by_units.div(i);
+      row[k] = r0 + r;
+      at[k] = i - r * units;
+      v[k] = U{};
+      if (s.counts(row[k])) v[k] = ((const U *)((const char *)s.x + row[k] * s.stride * (a.planes ? 4 : 2)))[at[k]];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) if (i0 + k * 256 < total) f(row[k], at[k], v[k]);
+  }
+}
 // Largest finite |x| that each CTA has seen: of the queries, of the table, of the bound of dz / scale:
 // |g| + |h| (p |log p| + p H), p |log p| <= 1 / e, H <= log rows < 22.
 __global__ void __launch_bounds__(256) tab_max_kernel(TabPrep a) {
@@ -647,14 +670,8 @@ __global__ void __launch_bounds__(256) tab_max_kernel(TabPrep a) {
   if (b < a.q.blocks + a.w.blocks) {
     const TabSource &s = b < a.q.blocks ? a.q : a.w;
     if (b >= a.q.blocks) b -= a.q.blocks;
-    for (long long r = (long long)b * 8 + w; r < s.rows; r += s.blocks * 8) {
-      if (!s.counts(r)) continue;
-      const float *x = (const float *)s.x + r * s.stride;
-      if (a.wide) {
-#pragma unroll 4
-        for (int i = lane; i < a.dim / 4; i += 32) { const float4 v = ((const float4 *)x)[i]; see(v.x); see(v.y); see(v.z); see(v.w); }
-      } else for (int i = lane; i < a.dim; i += 32) see(x[i]);
-    }
+    if (a.wide) tab_units<float4>(a, s, b, [&](long long, int, const float4 &v) { see(v.x); see(v.y); see(v.z); see(v.w); });
+    else tab_units<float>(a, s, b, [&](long long, int, float v) { see(v); });
   } else {
     b -= a.q.blocks + a.w.blocks;
     for (long long i = (long long)b * 256 + threadIdx.x; i < a.n; i += a.gblocks * 256)
@@ -704,37 +721,22 @@ __global__ void __launch_bounds__(256) tab_pack_kernel(TabPrep a) {
   const TabSource &s = of_q ? a.q : a.w;
   const int b = of_q ? blockIdx.x : blockIdx.x - a.q.blocks;
   const float up = of_q ? up_q : up_w;
-  for (long long r = (long long)b * 8 + w; r < s.rows; r += s.blocks * 8) {
-    const bool keep = s.counts(r);
-    const T *x = (const T *)s.x + r * s.stride;
-    if (sizeof(T) == 4) {
-      auto split = [&](float v, __half &b0, __half &b1) {
-        b0 = __float2half_rn(v * up);
-        b1 = __hisinf(b0) || __hisnan(b0) ? __float2half_rn(0.f) : __float2half_rn(v * up - __half2float(b0));
-      };
-      __half *p0 = (__half *)s.to + r * s.ld, *p1 = p0 + s.plane;
-      if (a.wide) {
-#pragma unroll 4
-        for (int i = lane; i < a.dim / 4; i += 32) {
-          const float4 v = keep ? ((const float4 *)x)[i] : make_float4(0.f, 0.f, 0.f, 0.f);
-          __align__(8) __half h0[4], h1[4];
-          split(v.x, h0[0], h1[0]); split(v.y, h0[1], h1[1]); split(v.z, h0[2], h1[2]); split(v.w, h0[3], h1[3]);
-          ((uint2 *)p0)[i] = *(uint2 *)h0;
-          ((uint2 *)p1)[i] = *(uint2 *)h1;
-        }
-      } else for (int i = lane; i < a.dim; i += 32) {
-        __half h0, h1;
-        split(keep ? (float)Tok<T>::up(x[i]) : 0.f, h0, h1);
-        p0[i] = h0;
-        p1[i] = h1;
-      }
-    } else {
-      T *to = (T *)s.to + r * s.ld;
-      if (a.wide) {
-#pragma unroll 4
-        for (int i = lane; i < a.dim / 8; i += 32) ((uint4 *)to)[i] = keep ? ((const uint4 *)x)[i] : make_uint4(0u, 0u, 0u, 0u);
-      } else for (int i = lane; i < a.dim; i += 32) to[i] = keep ? x[i] : Tok<T>::down(0.f);
-    }
+  if constexpr (sizeof(T) == 4) {
+    auto split = [&](float v, __half &b0, __half &b1) {
+      b0 = __float2half_rn(v * up);
+      b1 = __hisinf(b0) || __hisnan(b0) ? __float2half_rn(0.f) : __float2half_rn(v * up - __half2float(b0));
+    };
+    __half *p0 = (__half *)s.to, *p1 = p0 + s.plane;
+    if (a.wide) tab_units<float4>(a, s, b, [&](long long r, int i, const float4 &v) {
+      __align__(8) __half h0[4], h1[4];
+      split(v.x, h0[0], h1[0]); split(v.y, h0[1], h1[1]); split(v.z, h0[2], h1[2]); split(v.w, h0[3], h1[3]);
+      ((uint2 *)(p0 + r * s.ld))[i] = *(uint2 *)h0;
+      ((uint2 *)(p1 + r * s.ld))[i] = *(uint2 *)h1;
+    });
+    else tab_units<float>(a, s, b, [&](long long r, int i, float v) { split(v, p0[r * s.ld + i], p1[r * s.ld + i]); });
+  } else {
+    if (a.wide) tab_units<uint4>(a, s, b, [&](long long r, int i, const uint4 &v) { ((uint4 *)((T *)s.to + r * s.ld))[i] = v; });
+    else tab_units<unsigned short>(a, s, b, [&](long long r, int i, unsigned short v) { ((unsigned short *)s.to)[r * s.ld + i] = v; });
   }
 }
 // The parts of a split contraction, added in their order.
@@ -852,7 +854,7 @@ static bool tab_launch(const TabOperand &a, const TabOperand &b, TabArgs &g, boo
 static bool tab_packed(const void *p, long long stride, int dim, int dtype) { return dtype == PBG_F32 || !aligned16(p) || stride % 8 != 0 || stride < dim; }
 
 // What the workspace holds.  Its size is asked for without addresses, so it has room for packed operands wherever they may be needed.
-#define TAB_MAX_BLOCKS 1024                                  // of a preparing kernel
+#define TAB_MAX_BLOCKS 2048                                  // of a preparing kernel
 struct TabPlace {
   int64_t scales, block_max, q, w, parts, dz, partial, bytes;
   long long ld, columns, ldz;         // packed rows' length; table rows per piece of dz, and its rows' length
@@ -938,7 +940,8 @@ static void tab_prepare(TabCall &c, const TabPlace &p, bool grad, const float *g
     o = TabOperand{s.to, rows, c.dim, p.ld, s.plane, p.npl};
   };
   if (pack_q) source(a.q, c.q, c.queries, c.q_stride, c.n, p.q, 296);
-  if (pack_w) source(a.w, c.w, c.table, c.t_stride, c.rows, p.w, 592);
+  if (pack_w) source(a.w, c.w, c.table, c.t_stride, c.rows, p.w, 1184);
+  a.by_units = FastDiv(a.wide ? c.dim / V : c.dim);
   if (planes || dz) {
     TabPrep m = a;
     if (!planes) m.q.blocks = m.w.blocks = 0;

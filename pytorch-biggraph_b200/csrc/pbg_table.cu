@@ -806,13 +806,14 @@ static bool tab_launch_as(const TabOperand &a, const TabOperand &b, const TabOpe
   return true;
 }
 
-// Tile columns, 128 or 256: the fewest columns for the SM with the most of them, with what a tile costs beside them.
+// Tile columns, 128 or 256: the fewest columns for the SM with the most of them, with what a tile costs beside them -- a pair's, whose loads
+// are no longer hidden behind its products when these are half as many, more than one of few queries, which waits for HBM either way.
 static int tab_columns(long long tiles_m, long long N, int cg) {
   const long long groups = pbg_sm_count() / cg > 0 ? pbg_sm_count() / cg : 1;
   int best = 256;
   long long cost = -1;
   for (int bn = 256; bn >= 128; bn -= 128) {
-    const long long tiles = tiles_m * ((N + bn - 1) / bn), c = (tiles + groups - 1) / groups * (bn + 16);
+    const long long tiles = tiles_m * ((N + bn - 1) / bn), c = (tiles + groups - 1) / groups * (bn + (cg == 2 ? 64 : 16));
     if (cost < 0 || c < cost) { cost = c; best = bn; }
   }
   return best;

@@ -55,15 +55,13 @@ struct GradArgs {
   const unsigned long long *keys;      // sorted ids, those outside of the table behind all others
   const unsigned int *vals;
   float *part;                         // [tiles][2][dim rounded up to 4]
+  const unsigned int *named;           // a bit per row: some id names it
   long long grad_stride, out_stride, num_rows;
   int n, dim, part_ld, accumulate;
+  int sum_ctas, zero_words;            // CTAs that sum; words of `named` to each of those that write zeros
+  FastDiv by_units;
   float scale;
 };
-// whether the run of occurrence i goes on for LG_LONG occurrences or more behind the tile that ends at `end`
-__device__ __forceinline__ bool run_is_long(const GradArgs &a, unsigned long long key, int end) {
-  return end + LG_LONG - 1 < a.n && a.keys[end + LG_LONG - 1] == key;
-}
-
 template <class T, int N>
 __device__ __forceinline__ void grad_store(T *out, const GradArgs &a, unsigned long long row, int unit, const float (&acc)[N]) {
   Unit<T, N> *dst = reinterpret_cast<Unit<T, N> *>(out + (long long)row * a.out_stride) + unit;
@@ -85,9 +83,28 @@ __device__ __forceinline__ int run_of(unsigned w0, unsigned w1, int from) {
   return gap0 ? __ffs(gap0) - 1 : ~w1 ? 32 - from + __ffs(~w1) - 1 : 64 - from;
 }
 
+// Zeros into the rows that no id names; a CTA takes zero_words x 32 rows.
+template <class T, int N>
+__device__ __forceinline__ void lookup_zeros(T *out, const GradArgs &a, long long cta) {
+  Unit<T, N> z;
+#pragma unroll
+  for (int i = 0; i < N; ++i) z.e[i] = Tok<T>::down(0.f);
+  const int units = a.dim / N;
+  const long long r0 = cta * a.zero_words * 32, rows = a.num_rows - r0 < a.zero_words * 32 ? a.num_rows - r0 : a.zero_words * 32;
+  const int total = (int)(rows * units);
+  for (int i = threadIdx.x; i < total; i += 256) {
+    const int r = a.by_units.div(i);
+    const long long row = r0 + r;
+    if (a.named[row >> 5] >> (row & 31) & 1u) continue;
+    reinterpret_cast<Unit<T, N> *>(out + row * a.out_stride)[i - r * units] = z;
+  }
+}
+
+// The first sum_ctas CTAs sum, the others write the zeros: sums wait for one thing after the other, and the zeros fill the time.
 template <class T, int N>
 __global__ void __launch_bounds__(256, 3) lookup_grad_kernel(const T *__restrict__ grad, T *__restrict__ out, GradArgs a) {
   pdl_begin();
+  if (blockIdx.x >= (unsigned)a.sum_ctas) { lookup_zeros<T, N>(out, a, (long long)blockIdx.x - a.sum_ctas); return; }
   const int lane = threadIdx.x & 31, units = a.dim / N, blocks = (units + 31) / 32;
   const long long job = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int tile = (int)(job / blocks), unit = (int)(job - (long long)tile * blocks) * 32 + lane;
@@ -170,50 +187,55 @@ __global__ void __launch_bounds__(256, 3) lookup_grad_kernel(const T *__restrict
   if (live) grad_store<T, N>(out, a, last, unit, acc);
 }
 
-// A CTA looks through LG_JOIN_TILES tiles for long runs that begin in them, and adds up the parts of each over 32 units of columns:
-// the run's further tiles are dealt to the warps in blocks and the warps' sums added in their order.
+// A CTA looks through LG_JOIN_TILES tiles for long runs that begin in them, and adds up the parts of each over 32 units of columns: the
+// warps take every LG_JOIN_WARPS-th of the run's further tiles, eight parts in flight with the ids that say whether the run reaches them,
+// and the warps' sums are added in their order.
 template <class T, int N>
 __global__ void __launch_bounds__(32 * LG_JOIN_WARPS) lookup_grad_join_kernel(T *__restrict__ out, GradArgs a) {
   __shared__ float sums[LG_JOIN_WARPS][32 * N];
   pdl_begin();
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, units = a.dim / N, blocks = (units + 31) / 32;
   const int group = (int)(blockIdx.x / blocks), unit = (int)(blockIdx.x % blocks) * 32 + lane;
-  bool begins = false;
-  {
-    const long long tile = (long long)group * LG_JOIN_TILES + lane, end = (tile + 1) * LG_TILE;
-    if (end < a.n) {
-      const unsigned long long k = a.keys[end - 1], next = a.keys[end], before = tile > 0 ? a.keys[end - LG_TILE - 1] : ~0ull;
-      begins = k < (unsigned long long)a.num_rows && next == k && before != k && run_is_long(a, k, (int)end);
-    }
+  const long long mine = (long long)group * LG_JOIN_TILES + lane, end = (mine + 1) * LG_TILE, far = end + LG_LONG - 1;
+  unsigned long long key = ~0ull, before = ~0ull, behind = ~0ull;
+  if (far < a.n) {
+    key = a.keys[end - 1];
+    behind = a.keys[far];                                                // the list is sorted: all between are the same id as well
+    if (mine > 0) before = a.keys[end - LG_TILE - 1];
   }
+  const bool begins = key < (unsigned long long)a.num_rows && behind == key && before != key;
   const bool live = unit < units;
   for (unsigned todo = __ballot_sync(0xffffffffu, begins); todo; todo &= todo - 1u) {        // (the same in every warp)
-    const int tile = group * LG_JOIN_TILES + __ffs(todo) - 1, end = (tile + 1) * LG_TILE;
-    const unsigned long long k = a.keys[end];
-    int lo = end + LG_LONG, hi = a.n;                                                       // the run's end: first key behind it
-    while (lo < hi) {                                                                       // (32 places looked at in every step)
-      const int step = (hi - lo + 31) / 32, at = lo + lane * step;
-      const int same = __popc(__ballot_sync(0xffffffffu, at < hi && a.keys[at < hi ? at : lo] == k));
-      hi = same < 32 && lo + same * step < hi ? lo + same * step : hi;
-      lo = same > 0 ? lo + (same - 1) * step + 1 : lo;
-      if (same == 0) break;
-    }
-    const int tiles = (lo - 1) / LG_TILE - tile;                                            // further tiles of the run
-    const int per = (tiles + LG_JOIN_WARPS - 1) / LG_JOIN_WARPS, t0 = w * per, t1 = t0 + per < tiles ? t0 + per : tiles;
+    const int src = __ffs(todo) - 1;
+    const long long tile = (long long)group * LG_JOIN_TILES + src;
+    const unsigned long long k = __shfl_sync(0xffffffffu, key, src);
     float acc[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) acc[i] = 0.f;
-    if (live) {
-      if (w == 0) {
-        const float *p = a.part + ((long long)tile * 2 + 1) * a.part_ld + unit * N;
+    if (w == 0 && live) {
+      const float *p = a.part + (tile * 2 + 1) * a.part_ld + unit * N;
 #pragma unroll
-        for (int i = 0; i < N; ++i) acc[i] = p[i];
+      for (int i = 0; i < N; ++i) acc[i] = p[i];
+    }
+    bool on = true;
+    for (long long t0 = tile + 1 + w; on; t0 += 8 * LG_JOIN_WARPS) {
+      float part[8][N];
+      bool in[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const long long t = t0 + u * LG_JOIN_WARPS;
+        in[u] = t * LG_TILE < a.n && a.keys[t * LG_TILE < a.n ? t * LG_TILE : 0] == k;
+        const float *p = a.part + (t * LG_TILE < a.n ? t : 0) * 2 * a.part_ld + unit * N;
+#pragma unroll
+        for (int i = 0; i < N; ++i) part[u][i] = live ? p[i] : 0.f;
       }
-#pragma unroll 8
-      for (int t = t0; t < t1; ++t) {
-        const float *p = a.part + (long long)(tile + 1 + t) * 2 * a.part_ld + unit * N;
 #pragma unroll
-        for (int i = 0; i < N; ++i) acc[i] += p[i];
+      for (int u = 0; u < 8; ++u) {
+        on = on && in[u];
+        if (on) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) acc[i] += part[u][i];
+        }
       }
     }
     __syncthreads();
@@ -229,36 +251,32 @@ __global__ void __launch_bounds__(32 * LG_JOIN_WARPS) lookup_grad_join_kernel(T 
   }
 }
 
-// ---- sorting and zeros in one launch --------------------------------------------------------------------
-// Up to LS_MAX occurrences: the first cluster of eight CTAs sorts them by id (a stable radix sort, digits of up to nine bits, the list in
-// registers and shared memory), while all other CTAs write the zeros of the rows that no id names -- and of those that one
-// does, which the sums then replace.  Zeros of 131,072 x 2048 bf16 take 82 us, the sort of 16,384 ids 16.
+// ---- sorting ------------------------------------------------------------------------------------------------
+// Up to LS_MAX occurrences: one cluster of eight CTAs sorts them by id (a stable radix sort, digits of up to nine bits, the list in
+// registers and shared memory) and notes which rows are named.  16,384 ids: 12 us.
 #define LS_CTAS 8
 #define LS_THREADS 1024
 #define LS_WARPS 32
 #define LS_BINS 512
 #define LS_MAX (LS_CTAS * LS_THREADS * 8)
 
-struct SortZero {
+struct SortIds {
   const long long *ids; long long num_rows; int n, bits; unsigned long long *keys; unsigned int *vals; int *errors;
-  uint4 *zero; long long zero_units; int zero_tail;        // 16-byte units and bytes behind them; null: nothing to write
+  unsigned int *named;                                     // null: not asked for
 };
 
 template <int IPT>
 static constexpr size_t ls_smem() { return (size_t)LS_THREADS * IPT * 8 + LS_WARPS * LS_BINS * 2 + LS_CTAS * LS_BINS * 4 + LS_BINS * 4 + 64; }
 
 template <int IPT>
-__global__ void __cluster_dims__(LS_CTAS, 1, 1) __launch_bounds__(LS_THREADS) lookup_sort_zero_kernel(SortZero a) {
+__global__ void __cluster_dims__(LS_CTAS, 1, 1) __launch_bounds__(LS_THREADS) lookup_sort_kernel(SortIds a) {
   extern __shared__ __align__(16) unsigned char ls_smem_raw[];
-  const int t = threadIdx.x;
-  if (blockIdx.x >= LS_CTAS) {
-    const long long step = (long long)(gridDim.x - LS_CTAS) * LS_THREADS, first = (long long)(blockIdx.x - LS_CTAS) * LS_THREADS + t;
-    for (long long i = first; i < a.zero_units; i += step) __stcs(a.zero + i, make_uint4(0u, 0u, 0u, 0u));
-    if (first < a.zero_tail) reinterpret_cast<unsigned char *>(a.zero + a.zero_units)[first] = 0;
-    return;
-  }
   cg::cluster_group cluster = cg::this_cluster();
-  cluster.barrier_arrive();                                              // (waited for in front of the first store to another CTA)
+  const int t = threadIdx.x;
+  pdl_begin();
+  if (a.named) for (long long i = (long long)cluster.block_rank() * LS_THREADS + t; i < (a.num_rows + 31) / 32; i += LS_CTAS * LS_THREADS) a.named[i] = 0u;
+  __threadfence();
+  cluster.sync();                                                        // no row is named yet, and every CTA of the cluster runs
   uint2 *buf = (uint2 *)ls_smem_raw;                                      // this CTA's part of the list
   unsigned short *cnt = (unsigned short *)(buf + LS_THREADS * IPT);       // [warps][bins]
   unsigned int *all = (unsigned int *)(cnt + LS_WARPS * LS_BINS);         // [CTAs][bins]
@@ -277,6 +295,7 @@ __global__ void __cluster_dims__(LS_CTAS, 1, 1) __launch_bounds__(LS_THREADS) lo
       const bool bad = id < 0 || id >= a.num_rows;
       if (bad && a.errors) atomicOr(a.errors, TOK_ERR_ID);
       key = (unsigned int)(bad ? a.num_rows : id);
+      if (a.named && !bad) atomicOr(a.named + (key >> 5), 1u << (key & 31));
     }
     item[i] = make_uint2(key, (unsigned int)o);
   }
@@ -295,7 +314,6 @@ __global__ void __cluster_dims__(LS_CTAS, 1, 1) __launch_bounds__(LS_THREADS) lo
       off[i] = before + __popc(peers & lt);
     }
     __syncthreads();
-    if (pass == 0) cluster.barrier_wait();
     if (t < bins) {
       unsigned int run = 0u;
 #pragma unroll 8
@@ -339,26 +357,15 @@ __global__ void __cluster_dims__(LS_CTAS, 1, 1) __launch_bounds__(LS_THREADS) lo
   }
 }
 
-// Zeros, row by row; rows that lie one behind the other come as one row of all.
-template <class T, int N>
-__global__ void __launch_bounds__(256) lookup_zero_kernel(T *__restrict__ out, long long stride, long long rows, long long units) {
-  Unit<T, N> z;
-#pragma unroll
-  for (int i = 0; i < N; ++i) z.e[i] = Tok<T>::down(0.f);
-  for (long long r = blockIdx.y; r < rows; r += gridDim.y) {
-    Unit<T, N> *dst = reinterpret_cast<Unit<T, N> *>(out + r * stride);
-    for (long long u = (long long)blockIdx.x * 256 + threadIdx.x; u < units; u += (long long)gridDim.x * 256) dst[u] = z;
-  }
-}
-
 // What is sorted: (id, occurrence), ids outside of the table as num_rows.
 __global__ void __launch_bounds__(256) id_keys_kernel(const long long *__restrict__ ids, long long num_rows, int n, unsigned long long *__restrict__ keys,
-                                                      unsigned int *__restrict__ vals, int *errors) {
+                                                      unsigned int *__restrict__ vals, int *errors, unsigned int *named) {
   const int i = blockIdx.x * 256 + threadIdx.x;
   if (i >= n) return;
   const long long id = ids[i];
   const bool bad = id < 0 || id >= num_rows;
   if (bad && errors) atomicOr(errors, TOK_ERR_ID);
+  if (named && !bad) atomicOr(named + (id >> 5), 1u << (id & 31));
   keys[i] = (unsigned long long)(bad ? num_rows : id);
   vals[i] = (unsigned int)i;
 }
@@ -409,28 +416,35 @@ extern "C" int pbg_embedding_lookup(const void *table, int64_t row_stride, int64
 }
 
 static int grad_part_ld(int dim) { return (dim + 3) / 4 * 4; }
-struct GradPlace { int64_t keys, vals, hist, part, bytes; };          // two of keys and of vals
-static GradPlace grad_place(int64_t n, int dim) {
+struct GradPlace { int64_t keys, vals, named, hist, part, bytes; };          // two of keys and of vals
+static GradPlace grad_place(int64_t n, int64_t num_rows, int dim) {
   GradPlace p;
   p.keys = 0;
   p.vals = p.keys + 2 * tok_up(n * 8, 256);
-  p.hist = p.vals + 2 * tok_up(n * 4, 256);
+  p.named = p.vals + 2 * tok_up(n * 4, 256);
+  p.hist = p.named + tok_up((num_rows + 31) / 32 * 4, 256);
   p.part = p.hist + (n <= LS_MAX ? 0 : tok_up((int64_t)pbg_sort_hist_entries((int)n) * 4, 256));
   p.bytes = p.part + (n + LG_TILE - 1) / LG_TILE * 2 * grad_part_ld(dim) * 4;
   return p;
 }
 extern "C" int64_t pbg_embedding_lookup_grad_workspace(int64_t n, int64_t num_rows, int32_t dim) {
   if (n <= 0 || num_rows <= 0 || dim <= 0 || n > (1ll << 30)) return 0;
-  return grad_place(n, dim).bytes;
+  return grad_place(n, num_rows, dim).bytes;
 }
 
 struct LookupGradCall { const void *grad; void *out; GradArgs a; cudaStream_t st; };
 template <class T, int N>
 static void lookup_grad_launch(const LookupGradCall &c) {
-  const long long tiles = (c.a.n + LG_TILE - 1) / LG_TILE, blocks = (c.a.dim / N + 31) / 32;
-  pbg_launch(lookup_grad_kernel<T, N>, dim3((unsigned)((tiles * blocks + 7) / 8)), 256, 0, c.st, (const T *)c.grad, (T *)c.out, c.a);
-  if (c.a.n <= LG_LONG) return;                                          // no run is long
-  pbg_launch(lookup_grad_join_kernel<T, N>, dim3((unsigned)((tiles + LG_JOIN_TILES - 1) / LG_JOIN_TILES * blocks)), 32 * LG_JOIN_WARPS, 0, c.st, (T *)c.out, c.a);
+  const long long tiles = (c.a.n + LG_TILE - 1) / LG_TILE, units = c.a.dim / N, blocks = (units + 31) / 32;
+  GradArgs a = c.a;
+  a.sum_ctas = (int)((tiles * blocks + 7) / 8);
+  a.by_units = FastDiv((int)units);
+  const long long words = 65536 / (32ll * c.a.dim * (long long)sizeof(T));                   // some 64 KB to a CTA
+  a.zero_words = (int)(words < 1 ? 1 : words);
+  const long long zero_ctas = a.accumulate ? 0 : ((a.num_rows + 31) / 32 + a.zero_words - 1) / a.zero_words;
+  pbg_launch(lookup_grad_kernel<T, N>, dim3((unsigned)(a.sum_ctas + zero_ctas)), 256, 0, c.st, (const T *)c.grad, (T *)c.out, a);
+  if (a.n <= LG_LONG) return;                                            // no run is long
+  pbg_launch(lookup_grad_join_kernel<T, N>, dim3((unsigned)((tiles + LG_JOIN_TILES - 1) / LG_JOIN_TILES * blocks)), 32 * LG_JOIN_WARPS, 0, c.st, (T *)c.out, a);
 }
 template <class T>
 static void lookup_grad_type(const LookupGradCall &c) {
@@ -441,27 +455,10 @@ static void lookup_grad_type(const LookupGradCall &c) {
   else if (V == 8 && fits(2)) lookup_grad_launch<T, 2>(c);
   else lookup_grad_launch<T, 1>(c);
 }
-template <class T, int N>
-static void zero_launch(const LookupGradCall &c, long long rows, long long width) {
-  const long long units = width / N;
-  const long long gx = (units + 255) / 256, want = 148 * 8;
-  const dim3 grid((unsigned)(gx < want ? gx : want), (unsigned)(rows < 65535 ? rows : 65535));
-  pbg_launch_in_order(lookup_zero_kernel<T, N>, grid, 256, 0, c.st, (T *)c.out, c.a.out_stride, rows, units);
-}
-template <class T>
-static void zero_type(const LookupGradCall &c) {
-  constexpr int V = Tok<T>::VEC;
-  const bool flat = c.a.out_stride == c.a.dim;
-  const long long rows = flat ? 1 : c.a.num_rows, width = flat ? c.a.num_rows * c.a.dim : c.a.dim;
-  if (aligned16(c.out) && width % V == 0 && (flat || c.a.out_stride % V == 0)) zero_launch<T, V>(c, rows, width);
-  else zero_launch<T, 1>(c, rows, width);
-}
-
 template <int IPT>
-static void sort_zero_launch(const SortZero &a, cudaStream_t st) {
-  pbg_opt_in_smem((const void *)lookup_sort_zero_kernel<IPT>, (int)ls_smem<IPT>());
-  const long long most = 2 * pbg_sm_count() / LS_CTAS * LS_CTAS, want = tok_up((a.zero_units + LS_THREADS * 4 - 1) / (LS_THREADS * 4), LS_CTAS);
-  pbg_launch_in_order(lookup_sort_zero_kernel<IPT>, dim3((unsigned)(LS_CTAS + (!a.zero ? 0 : want < most ? (want > LS_CTAS ? want : LS_CTAS) : most))), LS_THREADS, ls_smem<IPT>(), st, a);
+static void sort_launch(const SortIds &a, cudaStream_t st) {
+  pbg_opt_in_smem((const void *)lookup_sort_kernel<IPT>, (int)ls_smem<IPT>());
+  pbg_launch(lookup_sort_kernel<IPT>, dim3(LS_CTAS), LS_THREADS, ls_smem<IPT>(), st, a);
 }
 
 extern "C" int pbg_embedding_lookup_grad(const void *grad, int64_t grad_stride, const int64_t *ids, int64_t n, int64_t num_rows, int32_t dim,
@@ -471,7 +468,7 @@ extern "C" int pbg_embedding_lookup_grad(const void *grad, int64_t grad_stride, 
   if (num_rows == 0) return n == 0 ? PBG_OK : PBG_ERR_BAD_ARGUMENT;
   if (!out || (n > 0 && (!grad || !ids || !workspace))) return PBG_ERR_BAD_ARGUMENT;
   if (n > (1ll << 30) || num_rows > 0x7fffffffll - 1 || dim > 65536) return PBG_ERR_TOO_LARGE;
-  const GradPlace p = n > 0 ? grad_place(n, dim) : GradPlace{};
+  const GradPlace p = n > 0 ? grad_place(n, num_rows, dim) : GradPlace{};
   if (workspace_bytes < p.bytes || ((uintptr_t)workspace & 255)) return PBG_ERR_BAD_ARGUMENT;
   if ((n + LG_TILE - 1) / LG_TILE * (((long long)dim + 31) / 32) > 0x7fffffffll) return PBG_ERR_TOO_LARGE;
   pbg_launch_error() = cudaSuccess;
@@ -480,10 +477,12 @@ extern "C" int pbg_embedding_lookup_grad(const void *grad, int64_t grad_stride, 
   LookupGradCall c{grad, out, {}, st};
   c.a.grad_stride = grad_stride; c.a.out_stride = out_stride; c.a.num_rows = num_rows;
   c.a.n = (int)n; c.a.dim = dim; c.a.part_ld = grad_part_ld(dim); c.a.accumulate = accumulate != 0; c.a.scale = scale;
-  const bool one_launch = n > 0 && n <= LS_MAX;
-  const bool flat = out_stride == dim && aligned16(out);
-  if (!accumulate && !(one_launch && flat)) TOK_DISPATCH(dtype, zero_type, c);
-  if (n > 0) {
+  if (n == 0) {
+    if (!accumulate) {
+      const size_t e = tok_size(dtype);
+      if (cudaMemset2DAsync(out, (size_t)out_stride * e, 0, (size_t)dim * e, (size_t)num_rows, st) != cudaSuccess) pbg_note_launch();
+    }
+  } else {
     SortPlan sp;
     for (int i = 0; i < 2; ++i) {
       sp.keys[i] = (unsigned long long *)(ws + p.keys + i * tok_up(n * 8, 256));
@@ -492,20 +491,21 @@ extern "C" int pbg_embedding_lookup_grad(const void *grad, int64_t grad_stride, 
     sp.hist = (unsigned int *)(ws + p.hist);
     sp.max_n = (int)n;
     sp.result = 0;
+    unsigned int *named = accumulate ? nullptr : (unsigned int *)(ws + p.named);
     int bits = 1;
     while ((unsigned long long)num_rows >> bits) ++bits;
-    if (one_launch) {
-      const long long bytes = num_rows * dim * (long long)tok_size(dtype);
-      const bool zero = !accumulate && flat;
-      const SortZero a{(const long long *)ids, num_rows, (int)n, bits, sp.keys[0], sp.vals[0], errors, zero ? (uint4 *)out : nullptr, zero ? bytes / 16 : 0, zero ? (int)(bytes % 16) : 0};
-      if (n <= LS_MAX / 8) sort_zero_launch<1>(a, st);
-      else if (n <= LS_MAX / 4) sort_zero_launch<2>(a, st);
-      else if (n <= LS_MAX / 2) sort_zero_launch<4>(a, st);
-      else sort_zero_launch<8>(a, st);
+    if (n <= LS_MAX) {
+      const SortIds a{(const long long *)ids, num_rows, (int)n, bits, sp.keys[0], sp.vals[0], errors, named};
+      if (n <= LS_MAX / 8) sort_launch<1>(a, st);
+      else if (n <= LS_MAX / 4) sort_launch<2>(a, st);
+      else if (n <= LS_MAX / 2) sort_launch<4>(a, st);
+      else sort_launch<8>(a, st);
     } else {
-      pbg_launch_in_order(id_keys_kernel, dim3((unsigned)((n + 255) / 256)), 256, 0, st, (const long long *)ids, (long long)num_rows, (int)n, sp.keys[0], sp.vals[0], errors);
+      if (named && cudaMemsetAsync(named, 0, (size_t)(num_rows + 31) / 32 * 4, st) != cudaSuccess) pbg_note_launch();
+      pbg_launch_in_order(id_keys_kernel, dim3((unsigned)((n + 255) / 256)), 256, 0, st, (const long long *)ids, (long long)num_rows, (int)n, sp.keys[0], sp.vals[0], errors, named);
       pbg_sort(sp, (int)n, bits, st);
     }
+    c.a.named = named;
     c.a.keys = sp.keys[sp.result];
     c.a.vals = sp.vals[sp.result];
     c.a.part = (float *)(ws + p.part);

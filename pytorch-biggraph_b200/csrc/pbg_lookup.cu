@@ -83,20 +83,19 @@ __device__ __forceinline__ int run_of(unsigned w0, unsigned w1, int from) {
   return gap0 ? __ffs(gap0) - 1 : ~w1 ? 32 - from + __ffs(~w1) - 1 : 64 - from;
 }
 
-// Zeros into the rows that no id names; a CTA takes zero_words x 32 rows.
+// Zeros into the zero_words x 32 rows from r0 on that no id names.
 template <class T, int N>
-__device__ __forceinline__ void lookup_zeros(T *out, const GradArgs &a, long long cta) {
+__device__ __forceinline__ void lookup_zeros(T *out, const GradArgs &a, long long r0, const unsigned *named) {
   Unit<T, N> z;
 #pragma unroll
   for (int i = 0; i < N; ++i) z.e[i] = Tok<T>::down(0.f);
   const int units = a.dim / N;
-  const long long r0 = cta * a.zero_words * 32, rows = a.num_rows - r0 < a.zero_words * 32 ? a.num_rows - r0 : a.zero_words * 32;
+  const long long rows = a.num_rows - r0 < a.zero_words * 32 ? a.num_rows - r0 : a.zero_words * 32;
   const int total = (int)(rows * units);
   for (int i = threadIdx.x; i < total; i += 256) {
     const int r = a.by_units.div(i);
-    const long long row = r0 + r;
-    if (a.named[row >> 5] >> (row & 31) & 1u) continue;
-    reinterpret_cast<Unit<T, N> *>(out + row * a.out_stride)[i - r * units] = z;
+    if (named[r >> 5] >> (r & 31) & 1u) continue;
+    reinterpret_cast<Unit<T, N> *>(out + (r0 + r) * a.out_stride)[i - r * units] = z;
   }
 }
 
@@ -104,7 +103,11 @@ __device__ __forceinline__ void lookup_zeros(T *out, const GradArgs &a, long lon
 template <class T, int N>
 __global__ void __launch_bounds__(256, 3) lookup_grad_kernel(const T *__restrict__ grad, T *__restrict__ out, GradArgs a) {
   pdl_begin();
-  if (blockIdx.x >= (unsigned)a.sum_ctas) { lookup_zeros<T, N>(out, a, (long long)blockIdx.x - a.sum_ctas); return; }
+  if (blockIdx.x >= (unsigned)a.sum_ctas) {
+    const long long word = ((long long)blockIdx.x - a.sum_ctas) * a.zero_words;
+    lookup_zeros<T, N>(out, a, word * 32, a.named + word);
+    return;
+  }
   const int lane = threadIdx.x & 31, units = a.dim / N, blocks = (units + 31) / 32;
   const long long job = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int tile = (int)(job / blocks), unit = (int)(job - (long long)tile * blocks) * 32 + lane;
@@ -248,6 +251,86 @@ __global__ void __launch_bounds__(32 * LG_JOIN_WARPS) lookup_grad_join_kernel(T 
       for (int i = 0; i < N; ++i) acc[i] += sums[o][lane * N + i];
     }
     grad_store<T, N>(out, a, k, unit, acc);
+  }
+}
+
+// ---- a short list -------------------------------------------------------------------------------------------
+// Up to LS_SMALL occurrences in one launch: a CTA per occurrence looks through the list, leaves if its id stands further in front, and else
+// sums the rows of all occurrences of the id; the CTAs behind them write the zeros of the rows that the list does not name.  The warps
+// of a CTA take blocks of 32 units, and where there are fewer blocks than warps, parts of the occurrences, added in their order.
+#define LS_SMALL 512
+#define LS_SMALL_WORDS 1024             // most words of named rows of a CTA that writes zeros
+
+template <class T, int N>
+__global__ void __launch_bounds__(256, 3) lookup_grad_small_kernel(const T *__restrict__ grad, const long long *__restrict__ ids, T *__restrict__ out, GradArgs a, int *errors) {
+  __shared__ union { float sums[8][32 * N]; unsigned named[LS_SMALL_WORDS]; } sh;
+  __shared__ unsigned short list[LS_SMALL];
+  __shared__ int counts[8];
+  pdl_begin();
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  if (blockIdx.x >= (unsigned)a.n) {
+    const long long cta = (long long)blockIdx.x - a.n, r0 = cta * a.zero_words * 32;
+    for (int i = threadIdx.x; i < a.zero_words; i += 256) sh.named[i] = 0u;
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.n; i += 256) {
+      const long long r = ids[i] - r0;
+      if (r >= 0 && r < a.zero_words * 32ll) atomicOr(&sh.named[r >> 5], 1u << (r & 31));
+    }
+    __syncthreads();
+    lookup_zeros<T, N>(out, a, r0, sh.named);
+    return;
+  }
+  const int me = blockIdx.x;
+  const long long id = ids[me];
+  if (id < 0 || id >= a.num_rows) {
+    if (threadIdx.x == 0 && errors) atomicOr(errors, TOK_ERR_ID);
+    return;
+  }
+  // thread t looks at occurrences 2 t and 2 t + 1: the matches of the whole list lie in the order of the threads
+  static_assert(LS_SMALL == 512, "two occurrences to a thread");
+  const int i0 = 2 * threadIdx.x;
+  const bool m0 = i0 < a.n && ids[i0] == id, m1 = i0 + 1 < a.n && ids[i0 + 1] == id;
+  if (__syncthreads_or((m0 && i0 < me) || (m1 && i0 + 1 < me))) return;
+  const unsigned b0 = __ballot_sync(0xffffffffu, m0), b1 = __ballot_sync(0xffffffffu, m1);
+  if (lane == 0) counts[w] = __popc(b0) + __popc(b1);
+  __syncthreads();
+  int at = 0, total = 0;
+  for (int k = 0; k < 8; ++k) { at += k < w ? counts[k] : 0; total += counts[k]; }
+  const unsigned lt = (1u << lane) - 1u;
+  at += __popc(b0 & lt) + __popc(b1 & lt);
+  if (m0) list[at++] = (unsigned short)i0;
+  if (m1) list[at] = (unsigned short)(i0 + 1);
+  __syncthreads();
+  const int units = a.dim / N, blocks = (units + 31) / 32;
+  const int parts = blocks > 4 ? 1 : blocks > 2 ? 2 : blocks > 1 ? 4 : 8;      // warps to a block
+  const int part = w % parts, per = (total + parts - 1) / parts, lo = part * per, hi = lo + per < total ? lo + per : total;
+  for (int b = w / parts; b < (parts > 1 ? 8 / parts : blocks); b += 8 / parts) {                // (with several parts, once)
+    const int unit = b * 32 + lane;
+    const bool live = unit < units;
+    float acc[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = 0.f;
+    for (int k = lo; live && k < hi; k += 8) {
+      Unit<T, N> g[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) if (k + u < hi) g[u] = reinterpret_cast<const Unit<T, N> *>(grad + (long long)list[k + u] * a.grad_stride)[unit];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        if (k + u >= hi) break;
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] += Tok<T>::up(g[u].e[i]);
+      }
+    }
+    if (parts > 1) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) sh.sums[w][lane * N + i] = acc[i];
+      __syncthreads();
+      if (part == 0)
+        for (int o = 1; o < parts; ++o)
+#pragma unroll
+          for (int i = 0; i < N; ++i) acc[i] += sh.sums[w + o][lane * N + i];
+    }
+    if (part == 0 && live) grad_store<T, N>(out, a, (unsigned long long)id, unit, acc);
   }
 }
 
@@ -418,7 +501,8 @@ extern "C" int pbg_embedding_lookup(const void *table, int64_t row_stride, int64
 static int grad_part_ld(int dim) { return (dim + 3) / 4 * 4; }
 struct GradPlace { int64_t keys, vals, named, hist, part, bytes; };          // two of keys and of vals
 static GradPlace grad_place(int64_t n, int64_t num_rows, int dim) {
-  GradPlace p;
+  GradPlace p = {};
+  if (n <= LS_SMALL) return p;                                           // nothing is sorted
   p.keys = 0;
   p.vals = p.keys + 2 * tok_up(n * 8, 256);
   p.named = p.vals + 2 * tok_up(n * 4, 256);
@@ -432,7 +516,7 @@ extern "C" int64_t pbg_embedding_lookup_grad_workspace(int64_t n, int64_t num_ro
   return grad_place(n, num_rows, dim).bytes;
 }
 
-struct LookupGradCall { const void *grad; void *out; GradArgs a; cudaStream_t st; };
+struct LookupGradCall { const void *grad; const long long *ids; void *out; GradArgs a; int *errors; cudaStream_t st; };
 template <class T, int N>
 static void lookup_grad_launch(const LookupGradCall &c) {
   const long long tiles = (c.a.n + LG_TILE - 1) / LG_TILE, units = c.a.dim / N, blocks = (units + 31) / 32;
@@ -440,10 +524,13 @@ static void lookup_grad_launch(const LookupGradCall &c) {
   a.sum_ctas = (int)((tiles * blocks + 7) / 8);
   a.by_units = FastDiv((int)units);
   const long long words = 65536 / (32ll * c.a.dim * (long long)sizeof(T));                   // some 64 KB to a CTA
-  a.zero_words = (int)(words < 1 ? 1 : words);
+  a.zero_words = (int)(words < 1 ? 1 : words < LS_SMALL_WORDS ? words : LS_SMALL_WORDS);
   const long long zero_ctas = a.accumulate ? 0 : ((a.num_rows + 31) / 32 + a.zero_words - 1) / a.zero_words;
+  if (a.n <= LS_SMALL) {
+    pbg_launch(lookup_grad_small_kernel<T, N>, dim3((unsigned)(a.n + zero_ctas)), 256, 0, c.st, (const T *)c.grad, c.ids, (T *)c.out, a, c.errors);
+    return;
+  }
   pbg_launch(lookup_grad_kernel<T, N>, dim3((unsigned)(a.sum_ctas + zero_ctas)), 256, 0, c.st, (const T *)c.grad, (T *)c.out, a);
-  if (a.n <= LG_LONG) return;                                            // no run is long
   pbg_launch(lookup_grad_join_kernel<T, N>, dim3((unsigned)((tiles + LG_JOIN_TILES - 1) / LG_JOIN_TILES * blocks)), 32 * LG_JOIN_WARPS, 0, c.st, (T *)c.out, a);
 }
 template <class T>
@@ -466,15 +553,15 @@ extern "C" int pbg_embedding_lookup_grad(const void *grad, int64_t grad_stride, 
                                          int64_t workspace_bytes, int32_t *errors, void *stream) {
   if (n < 0 || num_rows < 0 || dim <= 0 || !tok_type(dtype) || grad_stride < 0 || out_stride < dim || scale != scale) return PBG_ERR_BAD_ARGUMENT;
   if (num_rows == 0) return n == 0 ? PBG_OK : PBG_ERR_BAD_ARGUMENT;
-  if (!out || (n > 0 && (!grad || !ids || !workspace))) return PBG_ERR_BAD_ARGUMENT;
+  if (!out || (n > 0 && (!grad || !ids))) return PBG_ERR_BAD_ARGUMENT;
   if (n > (1ll << 30) || num_rows > 0x7fffffffll - 1 || dim > 65536) return PBG_ERR_TOO_LARGE;
   const GradPlace p = n > 0 ? grad_place(n, num_rows, dim) : GradPlace{};
-  if (workspace_bytes < p.bytes || ((uintptr_t)workspace & 255)) return PBG_ERR_BAD_ARGUMENT;
+  if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes || ((uintptr_t)workspace & 255))) return PBG_ERR_BAD_ARGUMENT;
   if ((n + LG_TILE - 1) / LG_TILE * (((long long)dim + 31) / 32) > 0x7fffffffll) return PBG_ERR_TOO_LARGE;
   pbg_launch_error() = cudaSuccess;
   unsigned char *ws = (unsigned char *)workspace;
   cudaStream_t st = (cudaStream_t)stream;
-  LookupGradCall c{grad, out, {}, st};
+  LookupGradCall c{grad, (const long long *)ids, out, {}, errors, st};
   c.a.grad_stride = grad_stride; c.a.out_stride = out_stride; c.a.num_rows = num_rows;
   c.a.n = (int)n; c.a.dim = dim; c.a.part_ld = grad_part_ld(dim); c.a.accumulate = accumulate != 0; c.a.scale = scale;
   if (n == 0) {
@@ -482,6 +569,8 @@ extern "C" int pbg_embedding_lookup_grad(const void *grad, int64_t grad_stride, 
       const size_t e = tok_size(dtype);
       if (cudaMemset2DAsync(out, (size_t)out_stride * e, 0, (size_t)dim * e, (size_t)num_rows, st) != cudaSuccess) pbg_note_launch();
     }
+  } else if (n <= LS_SMALL) {
+    TOK_DISPATCH(dtype, lookup_grad_type, c);
   } else {
     SortPlan sp;
     for (int i = 0; i < 2; ++i) {

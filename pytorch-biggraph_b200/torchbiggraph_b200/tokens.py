@@ -147,7 +147,7 @@ def _workspace(name, device, *sizes):
     else:
         with torch.cuda.device(device.index):
             size = fn(*sizes)
-    return torch.empty(size, dtype=torch.uint8, device=device), size
+    return torch.empty(size, dtype=torch.uint8, device=device) if size else None, size
 
 
 def check_errors(errors: torch.Tensor) -> None:
@@ -169,7 +169,7 @@ def embedding_lookup(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1
     (rows, dim), n = table.shape, flat.shape[0]
     if rows == 0 and n > 0:
         raise ValueError("table has no rows")
-    out = torch.empty((n, dim), dtype=table.dtype, device=device)
+    out = table.new_empty((n, dim))
     _call("pbg_embedding_lookup", device, table.data_ptr(), _row_stride(table), rows, dim, code, flat.data_ptr(), n, _scale(scale, False),
           out.data_ptr(), _error_word(errors, device))
     return out if ids.dim() == 1 else out.view(*ids.shape, dim)
@@ -194,7 +194,7 @@ def embedding_lookup_grad(grad: torch.Tensor, ids: torch.Tensor, num_rows: int, 
     if accumulate and out is None:
         raise ValueError("accumulate=True adds to `out`, which is missing")
     if out is None:
-        out = torch.empty((num_rows, dim), dtype=grad.dtype, device=device)
+        out = grad.new_empty((num_rows, dim))
     else:
         _matrix("out", out, grad.dtype, device)
         if tuple(out.shape) != (num_rows, dim):
@@ -205,7 +205,7 @@ def embedding_lookup_grad(grad: torch.Tensor, ids: torch.Tensor, num_rows: int, 
             raise ValueError("out and grad share memory")
     ws, size = _workspace("pbg_embedding_lookup_grad_workspace", device, n, num_rows, dim)
     _call("pbg_embedding_lookup_grad", device, grad.data_ptr(), _row_stride(grad), flat.data_ptr(), n, num_rows, dim, code, _scale(scale, False),
-          out.data_ptr(), _row_stride(out), int(bool(accumulate)), ws.data_ptr(), size, _error_word(errors, device))
+          out.data_ptr(), _row_stride(out), int(bool(accumulate)), _ptr(ws), size, _error_word(errors, device))
     return out
 
 
@@ -309,7 +309,7 @@ def table_logprobs(queries: torch.Tensor, table: torch.Tensor, targets: torch.Te
     r = TableLogprobs(*torch.empty((3, n), dtype=torch.float32, device=device).unbind(0))
     ws, size = _workspace("pbg_table_logprobs_workspace", device, n, rows, dim, code, 0)
     _call("pbg_table_logprobs", device, queries.data_ptr(), _row_stride(queries), n, table.data_ptr(), _row_stride(table), rows, dim, code, targets.data_ptr(),
-          int(ignore_index), _scale(scale, True), r.logprob.data_ptr(), r.entropy.data_ptr(), r.lse.data_ptr(), ws.data_ptr(), size, _error_word(errors, device))
+          int(ignore_index), _scale(scale, True), r.logprob.data_ptr(), r.entropy.data_ptr(), r.lse.data_ptr(), _ptr(ws), size, _error_word(errors, device))
     return r
 
 
@@ -327,5 +327,5 @@ def table_logprobs_grad(queries: torch.Tensor, table: torch.Tensor, targets: tor
     ws, size = _workspace("pbg_table_logprobs_workspace", device, n, rows, dim, code, 1)
     _call("pbg_table_logprobs_grad", device, queries.data_ptr(), _row_stride(queries), n, table.data_ptr(), _row_stride(table), rows, dim, code, targets.data_ptr(),
           int(ignore_index), _scale(scale, True), lse.data_ptr(), _ptr(entropy), _ptr(grad_logprob), _ptr(grad_entropy), dq.data_ptr(), dt.data_ptr(),
-          ws.data_ptr(), size, _error_word(errors, device))
+          _ptr(ws), size, _error_word(errors, device))
     return dq, dt

@@ -5,6 +5,10 @@
 //
 // The gradient sorts (id, i) first, so that the occurrences of an id lie next to each other in the order of i, and no sum
 // depends on the order in which anything arrives.  Sums are fp32, rounded to the output's type once.
+//
+// Measured: 16,384 rows of 1024 fp32 13 us (134 MB, part of it from L2), five rows 2 us; gradients of 16,384 x 2048 bf16 into 131,072 rows
+// 137 us (604 MB; sort 15, sums and zeros 105 at 64 % of DRAM's peak, join 14), of 10,000 x 400 fp32 into 14,951 rows 27 us, three launches
+// of a few dependent steps each.
 #include <cooperative_groups.h>
 
 #include "pbg_tokens.cuh"
@@ -14,7 +18,7 @@ namespace cg = cooperative_groups;
 // N elements of T as one access of N * sizeof(T) bytes
 template <class T, int N> struct __align__(sizeof(T) * N) Unit { T e[N]; };
 
-// A group of G threads moves a row, U units per thread in flight.
+// A group of G threads moves a row, U units per thread in flight.  Bound by HBM where rows are many, else by two loads in a row.
 template <class T, int N, int U>
 __global__ void __launch_bounds__(256)
 lookup_kernel(const T *__restrict__ table, long long row_stride, long long num_rows, int dim, int G, const long long *__restrict__ ids, long long n,
@@ -99,7 +103,8 @@ __device__ __forceinline__ void lookup_zeros(T *out, const GradArgs &a, long lon
   }
 }
 
-// The first sum_ctas CTAs sum, the others write the zeros: sums wait for one thing after the other, and the zeros fill the time.
+// The first sum_ctas CTAs sum, the others write the zeros: sums wait for one thing after the other, and the zeros fill the time.  (Zeros
+// beside the sort and sums over them: 166 us for the 16,384 x 2048 bf16 above.)
 template <class T, int N>
 __global__ void __launch_bounds__(256, 3) lookup_grad_kernel(const T *__restrict__ grad, T *__restrict__ out, GradArgs a) {
   pdl_begin();
@@ -336,7 +341,8 @@ __global__ void __launch_bounds__(256, 3) lookup_grad_small_kernel(const T *__re
 
 // ---- sorting ------------------------------------------------------------------------------------------------
 // Up to LS_MAX occurrences: one cluster of eight CTAs sorts them by id (a stable radix sort, digits of up to nine bits, the list in
-// registers and shared memory) and notes which rows are named.  16,384 ids: 12 us.
+// registers and shared memory) and notes which rows are named.  16,384 ids: 15 us, a chain of barriers; the launches of the sort for longer
+// lists, seven for two passes, took 57 us.
 #define LS_CTAS 8
 #define LS_THREADS 1024
 #define LS_WARPS 32

@@ -19,13 +19,20 @@
 // in shared memory feeds twice as many products.  Alone, a tile of 128 x 256 writes and reads 192 bytes of shared memory per cycle of
 // its products where the SM moves 128; a pair 128.
 //
+// What the loop waits for was found by leaving out the loads, then the products: a stage of four products (512 cycles) took 890 with loads
+// alone, whatever its bytes, because of a cluster-wide acquire in front of every stage and of loads issued from several lanes.
+// 4096 x 16,384 x 2048 bf16 (ncu): dz 179 us, dQ 189, dW 176 with the tensor pipe active 84, 77 (the last round of tiles is half empty) and
+// 86 % of the time; 4099 x 65,536 x 2048, all three 2.29 to 2.63 ms (1.25 to 1.44 PFLOP/s) as the power allows.  fp32, 5000 x 14,951 x 400: 180,
+// 172 and 180 us.  7 queries x 131,072 x 2048 bf16: 89 us, 74 % of DRAM's peak.
+//
 // Up to sixteen fp32 queries take no tensor cores: making planes of the table reads and writes it three times over, where fp32 products
 // on the CUDA cores keep up with one reading of it (tab_few_kernel).
 //
 // Every wait is bounded: one that runs out sets bit 2 of the error word, and the CTA stops, frees its tensor memory and returns.
+#include <type_traits>
+
 #include "pbg_tc.cuh"
 #include "pbg_tokens.cuh"
-#include <type_traits>
 
 enum { EPI_STATS = 0, EPI_DZ = 1, EPI_OUT = 2 };
 
@@ -532,8 +539,8 @@ __global__ void __launch_bounds__(128) tab_stats_kernel(const T *__restrict__ qu
 
 // ---- a few fp32 queries ----------------------------------------------------------------------------------------
 // The queries lie in shared memory; a warp takes R rows of the table at a time, its lanes along the rows, so that a query's
-// 512 bytes serve R rows.  16 queries: 32 FMAs and 4 reads of 16 bytes per lane and 16 bytes of the table.  What bounds it: HBM, up to 8
-// queries; 7 x 65,536 x 2048: see the case table.
+// 512 bytes serve R rows.  HBM bounds it up to 8 queries (65,536 x 2048: one 85 us, seven 110, where planes took 431), then the reads
+// of the queries (sixteen 161 us).
 #define TAB_FEW 16
 #define TAB_FEW_WARPS 16
 #define TAB_FEW_BYTES 196608

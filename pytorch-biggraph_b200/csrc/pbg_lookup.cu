@@ -570,13 +570,8 @@ extern "C" int pbg_embedding_lookup_grad(const void *grad, int64_t grad_stride, 
   LookupGradCall c{grad, (const long long *)ids, out, {}, errors, st};
   c.a.grad_stride = grad_stride; c.a.out_stride = out_stride; c.a.num_rows = num_rows;
   c.a.n = (int)n; c.a.dim = dim; c.a.part_ld = grad_part_ld(dim); c.a.accumulate = accumulate != 0; c.a.scale = scale;
-  if (n == 0) {
-    if (!accumulate) {
-      const size_t e = tok_size(dtype);
-      if (cudaMemset2DAsync(out, (size_t)out_stride * e, 0, (size_t)dim * e, (size_t)num_rows, st) != cudaSuccess) pbg_note_launch();
-    }
-  } else if (n <= LS_SMALL) {
-    TOK_DISPATCH(dtype, lookup_grad_type, c);
+  if (n <= LS_SMALL) {
+    if (n > 0 || !accumulate) TOK_DISPATCH(dtype, lookup_grad_type, c);
   } else {
     SortPlan sp;
     for (int i = 0; i < 2; ++i) {

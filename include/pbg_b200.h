@@ -297,7 +297,7 @@ int pbg_sub_bucket(pbg_context *ctx, const int64_t *lhs_in, const int64_t *rhs_i
  * irrelevant); two calls in flight need two of them.  All pointers are device memory; row strides are in elements, the elements of
  * a row lie next to each other.  Types are pbg_dtype; sums, statistics and softmax sums are fp32, results are rounded once.
  * errors: device int32 word or NULL; bit 1 is set by an id or target outside of its range, bit 2 where a bounded
- * wait ran out.  Sizes: dim 1 to 65536, ids and rows below 2^31.
+ * wait ran out.  Sizes: dim 1 to 65536, ids and rows below 2^31.  scale: finite for the lookups, 1e-20 to 1e20 for the log probabilities.
  * A target equal to ignore_index marks a row of padding: it is not read, its outputs are 0 (top_ids -1), its gradients 0. ---- */
 typedef enum { PBG_F32 = 0, PBG_BF16 = 1, PBG_F16 = 2 } pbg_dtype;
 
@@ -335,8 +335,9 @@ int pbg_token_logprobs_grad(const void *logits, int64_t row_stride, int64_t n, i
 
 /* The same statistics with z = scale * queries . table^T, which is never stored: queries [n, dim], table [rows, dim], targets rows of the
  * table.  16-bit operands are multiplied as they are; fp32 ones as two fp16 planes each (22 bits), at fp32's accuracy
- * for elements down to 2^-17 of the largest, and an absolute one of 2^-39 of it below.  workspace: of
- * pbg_table_logprobs_workspace(n, rows, dim, dtype, 0) bytes. */
+ * for elements down to 2^-17 of the largest, and an absolute one of 2^-39 of it below.  NaN, or an infinity, among a
+ * query's scores makes its entropy NaN, NaN or +inf its other results too; no other query's results change.
+ * workspace: of pbg_table_logprobs_workspace(n, rows, dim, dtype, 0) bytes. */
 int64_t pbg_table_logprobs_workspace(int64_t n, int64_t rows, int32_t dim, int32_t dtype, int32_t grad);
 int pbg_table_logprobs(const void *queries, int64_t q_stride, int64_t n, const void *table, int64_t t_stride, int64_t rows,
                        int32_t dim, int32_t dtype, const int64_t *targets, int64_t ignore_index, float scale,

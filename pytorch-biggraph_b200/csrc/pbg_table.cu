@@ -692,10 +692,10 @@ __global__ void __launch_bounds__(256) tab_max_kernel(TabPrep a) {
     a.block_max[blockIdx.x] = top;
   }
 }
-// 2^k that brings a number below 2^top, -100 <= k <= 100
+// 2^k that brings a number below 2^top, |k| <= 126: 2^-k is a normal number too, and the smallest normal one comes out at 1
 __device__ __forceinline__ float tab_power(unsigned bits, int top, float &inverse) {
   int k = bits ? top - ((int)(bits >> 23) - 126) : 0;
-  k = k < -100 ? -100 : k > 100 ? 100 : k;
+  k = k < -126 ? -126 : k > 126 ? 126 : k;
   inverse = __uint_as_float((unsigned)(127 - k) << 23);
   return __uint_as_float((unsigned)(127 + k) << 23);
 }

@@ -5,7 +5,6 @@
 // synchronises, and a bad id is skipped and reported through the caller's error word.
 #pragma once
 #include <cuda_fp16.h>
-#include <limits>
 
 #include "pbg_common.cuh"
 
@@ -90,7 +89,7 @@ __device__ __forceinline__ Soft soft_shfl(const Soft &a, int o) {
 
 inline size_t tok_size(int dtype) { return dtype == PBG_F32 ? 4 : 2; }
 inline bool tok_type(int dtype) { return dtype == PBG_F32 || dtype == PBG_BF16 || dtype == PBG_F16; }
-inline bool tok_scale(float s) { return s > 0.f && s <= std::numeric_limits<float>::max(); }     // (false for NaN)
+inline bool tok_scale(float s) { return s >= 1e-20f && s <= 1e20f; }    // (false for NaN; beyond, products of powers of two would leave fp32)
 inline bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 // CALL<element type>(...) by the run-time type

@@ -91,8 +91,8 @@ def _ids(ids, device):
 
 def _scale(scale, positive):
     scale = float(scale)
-    if not math.isfinite(scale) or (positive and not 0.0 < scale < 3.4e38):
-        raise ValueError(f"scale must be {'positive and ' if positive else ''}finite")
+    if not math.isfinite(scale) or (positive and not 1e-20 <= scale <= 1e20):
+        raise ValueError("scale must lie between 1e-20 and 1e20" if positive else "scale must be finite")
     return scale
 
 
@@ -303,7 +303,8 @@ def table_logprobs(queries: torch.Tensor, table: torch.Tensor, targets: torch.Te
     """Log probabilities of rows `targets` [n] of the table under softmax(scale * queries . table^T), with the entropies and logs of the
     sums; the n x rows scores are never stored.  What token_logprobs(queries @ table.T, targets) gives, at the accuracy of
     float32 sums over the operands as they are (float32 operands are multiplied at 22 bits and more).  Queries
-    whose target is ignore_index are padding: 0."""
+    whose target is ignore_index are padding: 0.  NaN, or +inf, among a query's scores makes its results NaN
+    (-inf its entropy), no other query's."""
     code, n, rows, dim, targets = _queries_and_table(queries, table, targets)
     device = queries.device
     r = TableLogprobs(*torch.empty((3, n), dtype=torch.float32, device=device).unbind(0))

@@ -158,6 +158,29 @@ def test_float32_operands_of_any_size():
     assert (zero.entropy - math.log(900)).abs().max() < 1e-5
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [7, 100, 300])
+def test_nan_and_infinity_stay_in_their_query(dtype, n):
+    q, t, targets = inputs(n, 1700, 72, dtype, n)
+    q[[2, 4, n - 1], [3, 0, 71]] = 0.5
+    clean = T.table_logprobs(q, t, targets)
+    q[2, 3], q[4, 0], q[n - 1, 71] = math.nan, math.inf, -math.inf
+    bad = torch.zeros(n, dtype=torch.bool, device=DEV)
+    bad[[2, 4, n - 1]] = True
+    for a, b in zip(T.table_logprobs(q, t, targets), clean):
+        assert a[bad].isnan().all() and torch.equal(a[~bad], b[~bad])
+
+
+@pytest.mark.parametrize("scale,a,b", [(1e-20, 1.0, 1.0), (1e-20, 1e10, 1e10), (1e20, 1e-20, 1.0), (1.0, 1e-36, 1e36), (1.0, 1e36, 1e-36), (1e20, 1e-35, 1e15)])
+@pytest.mark.parametrize("n", [7, 300])
+def test_scales_and_float32_operands_at_the_ends_of_their_range(n, scale, a, b):
+    q, t, targets = inputs(n, 500, 64, torch.float32, n + 1)
+    q, t = q * a, t * b
+    r = check_forward(q, t, targets, scale)
+    g = torch.ones(n, device=DEV)
+    check_grad(q, t, targets, f32(scale), g, None, r, T.table_logprobs_grad(q, t, targets, r.lse, None, g, scale=scale))
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_small_gradients_do_not_vanish(dtype):
     """Most of dz = 2e-5 p lies below the smallest half-precision number, the scaled dz does not."""

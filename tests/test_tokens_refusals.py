@@ -132,3 +132,17 @@ def test_table_grad_arguments(change, status):
     a = dict(TABLE, lse=P, entropy=P, g=P, h=P, dq=P, dt=P, ws=P, size=L.pbg_table_logprobs_workspace(4, 100, 8, 1, 1))
     a.update(change)
     assert L.pbg_table_logprobs_grad(*a.values(), None, None) == status
+
+
+@pytest.mark.parametrize("scale", [1.1e20, 3.4e38, 0.9e-20, 1e-45])
+def test_scales_out_of_range(scale):
+    """In base 2, or times the powers of two of the operands, such a scale can be infinite or lose its bits."""
+    L = _lib.lib()
+    a = dict(logits=P, stride=100, n=4, vocab=100, dtype=0, targets=P, ignore=-100, scale=scale)
+    assert L.pbg_token_logprobs(*a.values(), 0, P, P, P, P, None, None, None, None) == BAD
+    assert L.pbg_token_logprobs_grad(*a.values(), P, P, P, P, P, 100, None, None) == BAD
+    a = dict(TABLE, scale=scale)
+    assert L.pbg_table_logprobs(*a.values(), P, P, P, P, L.pbg_table_logprobs_workspace(4, 100, 8, 1, 0), None, None) == BAD
+    assert L.pbg_table_logprobs_grad(*a.values(), P, P, P, P, P, P, P, L.pbg_table_logprobs_workspace(4, 100, 8, 1, 1), None, None) == BAD
+    with pytest.raises(ValueError, match="scale"):
+        T.tokens._scale(scale, True)

@@ -758,7 +758,7 @@ __global__ void __launch_bounds__(256) tab_join_kernel(const float *__restrict__
 }
 
 // ---- host --------------------------------------------------------------------------------------------------
-struct TabOperand { const void *base; long long rows, inner, ld, plane; int planes; };   // [planes][rows][ld], 16-bit elements
+struct TabOperand { const void *base; long long rows, inner, ld, plane; int planes; bool room; };   // [planes][rows][ld], 16-bit elements; ours: room for whole blocks of 64
 
 static bool tab_encode(CUtensorMap *tm, bool bf16, const TabOperand &o, int box_inner, int box_rows, int box_planes) {
   const cuuint64_t dims[3] = {(cuuint64_t)o.inner, (cuuint64_t)o.rows, (cuuint64_t)o.planes};
@@ -770,13 +770,14 @@ static bool tab_encode(CUtensorMap *tm, bool bf16, const TabOperand &o, int box_
 
 // The same for an MN-major operand whose rows (with the room behind them) are whole blocks of 64 columns: the blocks are a dimension
 // of their own, so that `blocks` of them are one box.  A box costs its issue; what lies beyond `inner` belongs to columns that are clipped.
+// (The caller's rows have no such room, however far apart they lie: behind the last one the memory may end.)
 static bool tab_encode_blocks(CUtensorMap *tm, bool bf16, const TabOperand &o, int box_rows, int blocks) {
   const cuuint64_t dims[4] = {64, (cuuint64_t)o.rows, (cuuint64_t)o.planes, (cuuint64_t)((o.inner + 63) / 64)};
   const cuuint64_t strides[3] = {(cuuint64_t)o.ld * 2, (cuuint64_t)(o.planes > 1 ? o.plane : o.ld * 8) * 2, 128};
   const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, (cuuint32_t)o.planes, (cuuint32_t)blocks};
   return encode_map(tm, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, o.base, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
-static bool tab_whole(const TabOperand &o) { return o.inner % 64 == 0 || o.ld >= tok_up(o.inner, 64); }
+static bool tab_whole(const TabOperand &o) { return o.inner % 64 == 0 || o.room; }
 
 template <int EPI, class MATH, bool A_MN, bool B_MN, int CG, bool PARTS>
 static bool tab_launch_as(const TabOperand &a, const TabOperand &b, const TabOperand *c, TabArgs &g, cudaStream_t st) {
@@ -929,8 +930,8 @@ static void tab_prepare(TabCall &c, const TabPlace &p, bool grad, const float *g
   const bool planes = c.dtype == PBG_F32, dz = grad && c.dtype != PBG_BF16;
   c.sc = planes || dz ? (TabScales *)(c.ws + p.scales) : nullptr;
   c.err = c.errors ? c.errors : (int *)(c.ws + p.scales + 128);          // (nobody reads the latter)
-  c.q = TabOperand{c.queries, c.n, c.dim, c.q_stride, 0, 1};
-  c.w = TabOperand{c.table, c.rows, c.dim, c.t_stride, 0, 1};
+  c.q = TabOperand{c.queries, c.n, c.dim, c.q_stride, 0, 1, false};
+  c.w = TabOperand{c.table, c.rows, c.dim, c.t_stride, 0, 1, false};
   const bool pack_q = grad || tab_packed(c.queries, c.q_stride, c.dim, c.dtype), pack_w = tab_packed(c.table, c.t_stride, c.dim, c.dtype);
   if (!pack_q && !pack_w) return;
   constexpr int V = sizeof(T) == 4 ? 4 : 8;
@@ -945,7 +946,7 @@ static void tab_prepare(TabCall &c, const TabPlace &p, bool grad, const float *g
     s.x = x; s.stride = stride; s.rows = rows; s.to = c.ws + at; s.ld = p.ld; s.plane = rows * p.ld;
     s.blocks = tab_blocks(rows, most);
     if (!aligned16(x) || stride % V != 0) a.wide = 0;
-    o = TabOperand{s.to, rows, c.dim, p.ld, s.plane, p.npl};
+    o = TabOperand{s.to, rows, c.dim, p.ld, s.plane, p.npl, true};
   };
   if (pack_q) source(a.q, c.q, c.queries, c.q_stride, c.n, p.q, 296);
   if (pack_w) source(a.w, c.w, c.table, c.t_stride, c.rows, p.w, 1184);
@@ -1037,7 +1038,7 @@ static void tab_backward(TabBackward &f) {
     g.targets = c.targets; g.ignore_index = c.ignore_index; g.vocab = c.rows; g.v0 = v0;
     g.lse = f.lse; g.entropy = f.entropy; g.g = f.g; g.h = f.h;
     g.ldz = f.p.ldz; g.dz_planes = f.p.dz_planes;
-    const TabOperand dz{c.ws + f.p.dz, c.n, cols, f.p.ldz, c.n * f.p.ldz, f.p.dz_planes};
+    const TabOperand dz{c.ws + f.p.dz, c.n, cols, f.p.ldz, c.n * f.p.ldz, f.p.dz_planes, true};
     TabOperand written = dz;
     written.inner = f.p.ldz;
     f.ok = tab_launch<EPI_DZ, MATH, false, false>(c.q, w, g, pairs, c.st, &written);
@@ -1070,8 +1071,8 @@ static int tab_check(const TabCall &c, int64_t bytes, bool grad) {
   if (c.dim > 65536 || c.n > (1ll << 30) || c.rows > 0x7fffffffll - 65536) return PBG_ERR_TOO_LARGE;
   if (c.n == 0) return PBG_OK;
   if (!c.queries || !c.table || !c.targets || !c.ws || ((uintptr_t)c.ws & 255) || bytes < tab_place(c.n, c.rows, c.dim, c.dtype, grad).bytes) return PBG_ERR_BAD_ARGUMENT;
-  // rows that TMA reads where they lie are less than 2^40 bytes apart
-  if (c.q_stride >= (1ll << 38) || c.t_stride >= (1ll << 38)) return PBG_ERR_TOO_LARGE;
+  // rows that TMA reads where they lie: eight of them, a plane's stride, are less than 2^40 bytes
+  if (c.q_stride >= (1ll << 36) || c.t_stride >= (1ll << 36)) return PBG_ERR_TOO_LARGE;
   return PBG_OK;
 }
 

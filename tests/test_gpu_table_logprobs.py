@@ -147,6 +147,16 @@ def test_strides(dtype, width, first):
     check_grad(same, t, targets, 1.0, g, None, r2, T.table_logprobs_grad(same, t, targets, r2.lse, None, g))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_the_last_columns_of_wider_rows(dtype):
+    """Rows that end where the memory does, in operands read where they lie."""
+    q, t, targets = inputs(200, 700, 80, dtype, 80)
+    q, t = q[:, 40:], t[:, 40:]
+    r = check_forward(q, t, targets, 1.0)
+    g = torch.ones(200, device=DEV)
+    check_grad(q, t, targets, 1.0, g, None, r, T.table_logprobs_grad(q, t, targets, r.lse, None, g))
+
+
 def test_float32_operands_of_any_size():
     """Both planes are scaled by the largest element: tables of tiny and of large numbers come out as accurately."""
     q, t, targets = inputs(40, 900, 96, torch.float32, 5)

@@ -297,7 +297,9 @@ int pbg_sub_bucket(pbg_context *ctx, const int64_t *lhs_in, const int64_t *rhs_i
  * irrelevant); two calls in flight need two of them.  All pointers are device memory; row strides are in elements, the elements of
  * a row lie next to each other.  Types are pbg_dtype; sums, statistics and softmax sums are fp32, results are rounded once.
  * errors: device int32 word or NULL; bit 1 is set by an id or target outside of its range, bit 2 where a bounded
- * wait ran out.  Sizes: dim 1 to 65536, ids and rows below 2^31.  scale: finite for the lookups, 1e-20 to 1e20 for the log probabilities.
+ * wait ran out.  scale: finite for the lookups, 1e-20 to 1e20 for the log probabilities.
+ * Sizes: dim 1 to 65536; ids, rows of scores and table rows below 2^31 (less 65536 for a row's scores and for the rows that
+ * table_logprobs scores), ids of a gradient and queries up to 2^30; PBG_ERR_TOO_LARGE beyond.
  * A target equal to ignore_index marks a row of padding: it is not read, its outputs are 0 (top_ids -1), its gradients 0. ---- */
 typedef enum { PBG_F32 = 0, PBG_BF16 = 1, PBG_F16 = 2 } pbg_dtype;
 
@@ -347,6 +349,7 @@ int pbg_table_logprobs(const void *queries, int64_t q_stride, int64_t n, const v
 /* Gradients of sum(grad_logprob * logprob + grad_entropy * entropy) with respect to the queries [n, dim] and the table [rows, dim],
  * rows one behind the other, of their type; either may be NULL (not wanted).  lse, entropy: of the forward call.  The scores are
  * computed again; their gradient is rounded to the operands' type (fp32: two fp16 planes) for the two products.
+ * NaN or an infinity in the table makes grad_queries NaN, padding's rows too; one in a query that counts makes its row and grad_table NaN.
  * workspace: of pbg_table_logprobs_workspace(n, rows, dim, dtype, 1) bytes, at most about 2 GiB beside copies of the operands. */
 int pbg_table_logprobs_grad(const void *queries, int64_t q_stride, int64_t n, const void *table, int64_t t_stride, int64_t rows,
                             int32_t dim, int32_t dtype, const int64_t *targets, int64_t ignore_index, float scale,

@@ -583,7 +583,7 @@ extern "C" int pbg_token_logprobs(const void *logits, int64_t row_stride, int64_
   if (n < 0 || vocab <= 0 || row_stride < 0 || !tok_type(dtype) || !tok_scale(scale) || top < 0 || top > vocab) return PBG_ERR_BAD_ARGUMENT;
   if (n == 0) return PBG_OK;
   if (!logits || !targets || !logprob || !entropy || !lse || !rank || (top > 0 && (!top_logprobs || !top_ids))) return PBG_ERR_BAD_ARGUMENT;
-  if (top > LP_TOP_MAX || n > 0x0fffffffll || vocab > 0x7fffffffll - 65536) return PBG_ERR_TOO_LARGE;
+  if (top > LP_TOP_MAX || n > 0x7fffffffll || vocab > 0x7fffffffll - 65536) return PBG_ERR_TOO_LARGE;
   pbg_launch_error() = cudaSuccess;
   const LogprobCall c{logits, n, LogprobArgs{row_stride, vocab, (const long long *)targets, ignore_index, scale, top, logprob, entropy, lse,
                                              (long long *)rank, top_logprobs, (long long *)top_ids, errors}, (cudaStream_t)stream};

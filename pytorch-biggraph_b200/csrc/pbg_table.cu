@@ -45,11 +45,14 @@ enum { EPI_STATS = 0, EPI_DZ = 1, EPI_OUT = 2 };
 // epilogue has more to do (48), and for scores of 16-bit operands (32) of more than TAB_WHOLE elements.  Products of 5000 fp32 terms were 3.9e-5 off in one piece and are 5e-7 off in parts.  Scores of
 // 2048 16-bit terms are 8e-7 off in one piece and 2e-7 in parts; the registers that the parts take cost 7 queries x
 // 131,072 x 2048 bf16 12 of 102 us, so that these are left whole.
+// 16-bit gradients are cut up too where half a step per addition comes near the result's own: 2^21 terms of one sign in one piece
+// were 1 % off; a part of TAB_PART_LONG blocks is 2^-13 off at most.
 #define TAB_PART_F32 6
 #define TAB_PART_F32_OUT 3
 #define TAB_PART_F32_DZ 8
 #define TAB_PART_16 8
 #define TAB_WHOLE 2048
+#define TAB_PART_LONG 512
 
 // Eight warps share a tile's columns (two to every 32 rows), each with 4 KB of shared memory to write from; the ring of stages has the
 // rest.  (Sixteen warps with half the columns each had registers for half of what they need and were slower.)
@@ -854,6 +857,11 @@ static bool tab_launch(const TabOperand &a, const TabOperand &b, TabArgs &g, boo
   if constexpr (MATH::NPB == 2) return as(std::true_type());
   else {
     if constexpr (EPI == EPI_STATS) if (g.kblocks > TAB_WHOLE / 64) return as(std::true_type());
+    if constexpr (EPI == EPI_OUT && !(A_MN && MATH::NPA == 2))            // (two planes and the contraction over queries: 128 of them at most)
+      if (g.kblocks > TAB_PART_LONG) {
+        g.part = TAB_PART_LONG;
+        return as(std::true_type());
+      }
     g.part = 0x7fffffff;
     return as(std::false_type());
   }

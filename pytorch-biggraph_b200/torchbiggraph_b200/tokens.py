@@ -319,7 +319,8 @@ def table_logprobs_grad(queries: torch.Tensor, table: torch.Tensor, targets: tor
                         ignore_index: int = IGNORE_INDEX, errors: Optional[torch.Tensor] = None):
     """Gradients (of the queries, of the table) of sum(grad_logprob * logprob + grad_entropy * entropy), from the lse and the entropy that
     table_logprobs returned (the entropy only where grad_entropy is given).  Queries that are padding, and those whose
-    target is out of range, get zeros and add nothing to the table's gradient, whatever they hold."""
+    target is out of range, get zeros and add nothing to the table's gradient, whatever they hold -- unless the table holds NaN or
+    infinities, which reach all gradients of the queries."""
     code, n, rows, dim, targets = _queries_and_table(queries, table, targets)
     device = queries.device
     lse, entropy, grad_logprob, grad_entropy = _row_grads(n, device, lse, entropy, grad_logprob, grad_entropy)

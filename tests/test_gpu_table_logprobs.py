@@ -268,6 +268,32 @@ def test_refusals_and_nothing_to_do():
     assert r.logprob[2].isnan() and r.lse.isfinite().all() and errors.item() == 1
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [8, 200])
+def test_long_sums_of_one_sign(dtype, dim):
+    """2^20 equal terms: what every addition cut off would add up.  dz and the result are rounded by half a step each; parts of 32,768 16-bit
+    terms are 2^-13 off at most, 2^14 parts of float32 terms added in float32 2^-11 (half a step each), 32 parts 2^-20."""
+    n = (1 << 20) + 3
+    g = torch.full((n,), 2.0 ** -8, device=DEV)
+    q, t, targets = torch.ones(n, dim, device=DEV, dtype=dtype), torch.zeros(3, dim, device=DEV, dtype=dtype), torch.zeros(n, dtype=torch.long, device=DEV)
+    r = T.table_logprobs(q, t, targets)
+    assert (r.lse - math.log(3)).abs().max() < 1e-6
+    dt = T.table_logprobs_grad(q, t, targets, r.lse, None, g)[1].double()
+    want = torch.tensor([2 / 3, -1 / 3, -1 / 3], dtype=torch.float64, device=DEV)[:, None] * n * 2.0 ** -8
+    assert ((dt / want - 1).abs() <= (2 * half_step(dtype) + 2 ** -13 + 2 ** -20 if dtype != torch.float32 else 2 ** -11)).all()
+    # the same over the table's rows: all of them alike but the target
+    t = torch.ones(n, dim, device=DEV, dtype=dtype)
+    t[0] = 0
+    q, targets, g = torch.zeros(140, dim, device=DEV, dtype=dtype), torch.zeros(140, dtype=torch.long, device=DEV), torch.ones(140, device=DEV)
+    r = T.table_logprobs(q, t, targets)
+    dq = T.table_logprobs_grad(q, t, targets, r.lse, None, g)[0].double()
+    # (p = 1 / n out of an exponential of the rounded lse, off by 2^-23 * 14 and two more roundings; scaled dz have all of their bits)
+    err = 2 * half_step(dtype) + 2 ** -13 + 2 ** -20 if dtype != torch.float32 else 2 ** -11
+    if dtype == torch.float16:
+        err += 2 ** -38 * n                                 # one scale for all of dz: half a step of the smallest numbers, 2^-25 of 2^-13
+    assert ((dq / (-(n - 1) / n) - 1).abs() <= err + 16 * 2 ** -23).all()
+
+
 @pytest.mark.parametrize("dtype,n,rows", [(torch.bfloat16, 70_001, 16_500), (torch.float32, 30_000, 18_100)])
 def test_more_queries_than_the_workspace_holds_at_once(dtype, n, rows):
     """The gradient of the scores is kept for pieces of the table, the parts of dQ added up from piece to piece; a sample of the rows of

@@ -7,7 +7,7 @@
 //
 // Forward: a row is read once.  Gradient: one read, one write.  HBM bounds both; the forward pass comes near the issue slots too (16-bit
 // scores at 6.5 TB/s are 11.6 to an SM and cycle, which issues 128 lanes of instructions: 11 for each score, of which the pass takes
-// some seven).  4099 x 131,072 bf16 with the best 8: 224 us, 4.8 TB/s, 62 % of the issue slots; its gradient 315 us, 6.8 TB/s; four rows
+// some seven).  4099 x 131,072 bf16 with the best 8: 212 us, 5.1 TB/s, 62 % of the issue slots; its gradient 315 us, 6.8 TB/s; four rows
 // with the best 20, eight CTAs to a row: 14 us.
 #include <cooperative_groups.h>
 
@@ -15,8 +15,7 @@
 
 namespace cg = cooperative_groups;
 
-#define LP_THREADS 256
-#define LP_WARPS (LP_THREADS / 32)
+#define LP_THREADS 256                   // of the gradient
 #define LP_TOP_MAX 32
 #define LP_VECS 4                        // 16-byte vectors per thread and step
 #define LP_NO_ID 0x7fffffff
@@ -191,7 +190,7 @@ struct RowScan {
 
 // ---- the best scores ------------------------------------------------------------------------------------
 // Order: larger scores first, equal ones by id, NaN as -inf.  The scan leaves the largest score of every thread, and of each sixteenth of
-// its turns.  The top-th largest of 64 groups of four threads is a threshold that at least `top` scores reach and hardly
+// its turns.  The top-th largest of 64 groups of threads is a threshold that at least `top` scores reach and hardly
 // more than that pass.  The sixteenths that reach it are looked through again, all threads helping, and what reaches it is ranked by
 // counting.  Where too much does (equal scores, mostly), those above it are taken and the first of those equal to it; where even
 // that is too much, the best are found one after the other.  (A sorted list per warp, kept during the scan, took longer than the scan:
@@ -202,8 +201,8 @@ struct Best { float v; int id; };
 __device__ __forceinline__ bool best_before(Best a, Best b) { return a.v > b.v || (a.v == b.v && a.id < b.id); }
 
 // A CTA's part of a row: the elements in front of the first 16-byte boundary and behind the last whole vector (the edges; the last CTA of
-// a cluster has them, an element to a lane of its last warp), and every nct-th block of LP_WARPS steps.
-template <class T> struct RowPart {
+// a cluster has them, an element to a lane of its last warp), and every nct-th block of W steps (W: its warps).
+template <class T, int W> struct RowPart {
   static constexpr int VEC = Tok<T>::VEC;
   const T *row;
   int vocab, head, vecs, tail, cta, nct;
@@ -215,26 +214,27 @@ template <class T> struct RowPart {
   }
   __device__ bool edges() const { return cta == nct - 1; }
   __device__ int steps() const { return (vecs + 32 * LP_VECS - 1) / (32 * LP_VECS); }                       // of all CTAs
-  __device__ int vec(int warp, int turn, int u, int lane) const { return ((turn * nct + cta) * LP_WARPS + warp) * 32 * LP_VECS + u * 32 + lane; }
-  __device__ int turns() const { return (steps() + nct * LP_WARPS - 1) / (nct * LP_WARPS); }
+  __device__ int vec(int warp, int turn, int u, int lane) const { return ((turn * nct + cta) * W + warp) * 32 * LP_VECS + u * 32 + lane; }
+  __device__ int turns() const { return (steps() + nct * W - 1) / (nct * W); }
   __device__ int edge_id(int lane) const { return lane < 16 ? (lane < head ? lane : -1) : lane - 16 < tail ? vocab - tail + lane - 16 : -1; }
   __device__ float at(int id) const { const float x = Tok<T>::up(row[id]); return x != x ? -INFINITY : x; }
 };
 
-struct TopShared {
+template <int W> struct TopShared {
   float group[64];
   float tau;
   int count, flagged;
-  float slot[LP_SLOTS][LP_THREADS];       // the largest score of a thread in its `per` turns of that slot
-  unsigned short places[LP_CANDIDATES];  // slot x LP_THREADS + thread
-  Best cand[LP_CANDIDATES], list[LP_TOP_MAX], warp_best[LP_WARPS];
+  float slot[LP_SLOTS][32 * W];           // the largest score of a thread in its `per` turns of that slot
+  unsigned short places[LP_CANDIDATES];  // slot x threads + thread
+  Best cand[LP_CANDIDATES], list[LP_TOP_MAX], warp_best[W];
   int have;
 };
 
 // cand[0 .. count) to list[0 .. have), the first `top` in order
-__device__ __forceinline__ void rank_candidates(TopShared &sh, int top) {
+template <int W>
+__device__ __forceinline__ void rank_candidates(TopShared<W> &sh, int top) {
   const int n = sh.count;
-  for (int i = threadIdx.x; i < n; i += LP_THREADS) {
+  for (int i = threadIdx.x; i < n; i += 32 * W) {
     const Best mine = sh.cand[i];
     int ahead = 0;
     for (int k = 0; k < n; ++k) ahead += best_before(sh.cand[k], mine) ? 1 : 0;
@@ -244,13 +244,13 @@ __device__ __forceinline__ void rank_candidates(TopShared &sh, int top) {
   __syncthreads();
 }
 
-template <class T>
-__device__ void top_of_part(const RowPart<T> &p, float m, int top, TopShared &sh) {
+template <class T, int W>
+__device__ void top_of_part(const RowPart<T, W> &p, float m, int top, TopShared<W> &sh) {
   constexpr int VEC = Tok<T>::VEC;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   float g = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-  g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, 2));
-  if ((lane & 3) == 0) sh.group[threadIdx.x / 4] = g;
+  if (W == 8) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, 2));
+  if (lane % (W / 2) == 0) sh.group[threadIdx.x / (W / 2)] = g;
   if (threadIdx.x == 0) { sh.count = 0; sh.flagged = 0; sh.have = 0; }
   __syncthreads();
   if (threadIdx.x < 64) {
@@ -266,7 +266,7 @@ __device__ void top_of_part(const RowPart<T> &p, float m, int top, TopShared &sh
   auto gather = [&](bool strict) {
     for (int k = 0; k * per < turns; ++k) {
       const float x = sh.slot[k][threadIdx.x];
-      if (strict ? x > tau : x >= tau) { const int at = atomicAdd(&sh.flagged, 1); if (at < LP_CANDIDATES) sh.places[at] = (unsigned short)(k * LP_THREADS + threadIdx.x); }
+      if (strict ? x > tau : x >= tau) { const int at = atomicAdd(&sh.flagged, 1); if (at < LP_CANDIDATES) sh.places[at] = (unsigned short)(k * (32 * W) + threadIdx.x); }
     }
     __syncthreads();
     if (sh.flagged > LP_CANDIDATES) {                                    // too much already
@@ -278,8 +278,8 @@ __device__ void top_of_part(const RowPart<T> &p, float m, int top, TopShared &sh
     auto take = [&](float x, int id) {
       if (strict ? x > tau : x >= tau) { const int k = atomicAdd(&sh.count, 1); if (k < LP_CANDIDATES) sh.cand[k] = Best{x, id}; }
     };
-    for (int i = threadIdx.x; i < items; i += LP_THREADS) {
-      const int place = sh.places[i / each], r = i % each, who = place % LP_THREADS, turn = place / LP_THREADS * per + r / LP_VECS;
+    for (int i = threadIdx.x; i < items; i += 32 * W) {
+      const int place = sh.places[i / each], r = i % each, who = place % (32 * W), turn = place / (32 * W) * per + r / LP_VECS;
       const int v = p.vec(who / 32, turn, r % LP_VECS, who % 32);
       if (turn >= turns || v >= p.vecs) continue;
       float x[VEC];
@@ -291,7 +291,7 @@ __device__ void top_of_part(const RowPart<T> &p, float m, int top, TopShared &sh
 #pragma unroll
       for (int k = 0; k < VEC; ++k) take(x[k], p.head + v * VEC + k);
     }
-    if (p.edges() && w == LP_WARPS - 1 && p.edge_id(lane) >= 0) take(p.at(p.edge_id(lane)), p.edge_id(lane));
+    if (p.edges() && w == W - 1 && p.edge_id(lane) >= 0) take(p.at(p.edge_id(lane)), p.edge_id(lane));
     __syncthreads();
   };
   bool strict = tau == -INFINITY;                                        // (fewer than `top` groups with a score at all)
@@ -321,7 +321,7 @@ __device__ void top_of_part(const RowPart<T> &p, float m, int top, TopShared &sh
 #pragma unroll
           for (int e = 0; e < VEC; ++e) see(x[e], p.head + v * VEC + e);
         }
-      if (p.edges() && w == LP_WARPS - 1 && p.edge_id(lane) >= 0) see(p.at(p.edge_id(lane)), p.edge_id(lane));
+      if (p.edges() && w == W - 1 && p.edge_id(lane) >= 0) see(p.at(p.edge_id(lane)), p.edge_id(lane));
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
         const Best b{__shfl_xor_sync(0xffffffffu, best.v, o), __shfl_xor_sync(0xffffffffu, best.id, o)};
@@ -331,7 +331,7 @@ __device__ void top_of_part(const RowPart<T> &p, float m, int top, TopShared &sh
       if (lane == 0) sh.warp_best[w] = best;
       __syncthreads();
       best = sh.warp_best[0];
-      for (int o = 1; o < LP_WARPS; ++o) if (best_before(sh.warp_best[o], best)) best = sh.warp_best[o];
+      for (int o = 1; o < W; ++o) if (best_before(sh.warp_best[o], best)) best = sh.warp_best[o];
       if (best.id == LP_NO_ID) break;                                    // (the same in every thread)
       if (threadIdx.x == 0) { sh.list[k] = best; sh.have = k + 1; }
       prev = best;
@@ -352,7 +352,7 @@ __device__ void top_of_part(const RowPart<T> &p, float m, int top, TopShared &sh
       have += __popc(hits);
     };
     if (p.edges()) more(lane < p.head, lane);
-    const int span = LP_WARPS * 32 * LP_VECS * VEC;                      // elements of a turn
+    const int span = W * 32 * LP_VECS * VEC;                             // elements of a turn
     for (int turn = 0; turn < p.turns() && have < top; ++turn) {
       const int first = p.head + p.vec(0, turn, 0, 0) * VEC, end = p.head + p.vecs * VEC;
       for (int i = 0; i < span && first + i < end && have < top; i += 32) more(i + lane < span && first + i + lane < end, first + i + lane);
@@ -363,15 +363,15 @@ __device__ void top_of_part(const RowPart<T> &p, float m, int top, TopShared &sh
   __syncthreads();
 }
 
-// A cluster of CTAs per row (a single CTA where there are rows for all SMs); the warps take steps of 32 x LP_VECS vectors in turn.
-template <class T, bool TOP>
-__global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const T *__restrict__ logits, LogprobArgs a) {
+// A CTA of W warps per row, or a cluster of them where there are fewer rows than SMs could hold; the warps take steps of 32 x LP_VECS vectors in turn.
+template <class T, bool TOP, int W>
+__global__ void __launch_bounds__(32 * W, 32 / W) logprobs_kernel(const T *__restrict__ logits, LogprobArgs a) {
   constexpr int VEC = Tok<T>::VEC;
   struct Part { Soft s; unsigned rank; };
-  __shared__ Part parts[LP_WARPS], cta_part;
-  __shared__ TopShared top_shared[1];
+  __shared__ Part parts[W], cta_part;
+  __shared__ TopShared<W> top_shared[1];
   cg::cluster_group cluster = cg::this_cluster();
-  const int nct = (int)cluster.num_blocks(), cta = (int)cluster.block_rank();
+  const int nct = W == 8 ? (int)cluster.num_blocks() : 1, cta = W == 8 ? (int)cluster.block_rank() : 0;
   const long long n = blockIdx.x / nct;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const long long target = a.targets[n];
@@ -383,16 +383,16 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const T *__rest
     return;
   }
   const bool known = target >= 0 && target < a.vocab;
-  const RowPart<T> p(logits + n * a.row_stride, a.vocab, cta, nct);
+  const RowPart<T, W> p(logits + n * a.row_stride, a.vocab, cta, nct);
   RowScan<T> g;
   g.start(a.scale, p.row, known, known ? (int)target : -1);
   const uint4 *vec = reinterpret_cast<const uint4 *>(p.row + p.head);
   const int steps = p.steps();
-  const int stride = nct * LP_WARPS, per = (p.turns() + LP_SLOTS - 1) / LP_SLOTS;
+  const int stride = nct * W, per = (p.turns() + LP_SLOTS - 1) / LP_SLOTS;
   int slot = 0, in_slot = 0;
   float slot_max = -INFINITY;
   if (TOP) for (int k = 0; k < LP_SLOTS; ++k) top_shared[0].slot[k][threadIdx.x] = -INFINITY;
-  for (int b = cta * LP_WARPS + w; b < steps; b += stride) {
+  for (int b = cta * W + w; b < steps; b += stride) {
     const int v0 = b * 32 * LP_VECS + lane;
     unsigned raw[4 * LP_VECS];
     int live = LP_VECS;
@@ -417,7 +417,7 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const T *__rest
       if (++in_slot == per || b + stride >= steps) { top_shared[0].slot[slot++][threadIdx.x] = slot_max; slot_max = -INFINITY; in_slot = 0; }
     }
   }
-  if (p.edges() && w == LP_WARPS - 1 && p.edge_id(lane) >= 0) g.edge(Tok<T>::up(p.row[p.edge_id(lane)]), p.edge_id(lane));
+  if (p.edges() && w == W - 1 && p.edge_id(lane) >= 0) g.edge(Tok<T>::up(p.row[p.edge_id(lane)]), p.edge_id(lane));
   g.finish();
   const float mine_m = g.s.m;
 
@@ -430,16 +430,16 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const T *__rest
   if (lane == 0) parts[w] = Part{g.s, g.rank};
   __syncthreads();
   if (w == 0) {
-    g.s = parts[lane % LP_WARPS].s;
-    g.rank = parts[lane % LP_WARPS].rank;
+    g.s = parts[lane % W].s;
+    g.rank = parts[lane % W].rank;
 #pragma unroll
-    for (int o = LP_WARPS / 2; o > 0; o >>= 1) {
+    for (int o = W / 2; o > 0; o >>= 1) {
       soft_join(g.s, soft_shfl(g.s, o), g.c);
       g.rank += __shfl_xor_sync(0xffffffffu, g.rank, o);
     }
     if (nct > 1 && lane == 0) cta_part = Part{g.s, g.rank};
   }
-  if (TOP) top_of_part<T>(p, mine_m, a.top, top_shared[0]);
+  if (TOP) top_of_part<T, W>(p, mine_m, a.top, top_shared[0]);
   if (nct > 1) {
     cluster.sync();
     if (cta == 0) {
@@ -451,11 +451,11 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const T *__rest
         }
       if (TOP) {
         static_assert(8 * LP_TOP_MAX <= LP_CANDIDATES, "the lists of a cluster");
-        TopShared &sh = top_shared[0];
+        TopShared<W> &sh = top_shared[0];
         if (threadIdx.x == 0) sh.count = 0;
         __syncthreads();
-        for (int i = threadIdx.x; i < nct * a.top; i += LP_THREADS) {
-          const TopShared *of = cluster.map_shared_rank(top_shared, i / a.top);
+        for (int i = threadIdx.x; i < nct * a.top; i += 32 * W) {
+          const TopShared<W> *of = cluster.map_shared_rank(top_shared, i / a.top);
           if (i % a.top < of->have) sh.cand[atomicAdd(&sh.count, 1)] = of->list[i % a.top];
         }
         __syncthreads();
@@ -565,11 +565,19 @@ static void logprobs_type(const LogprobCall &c) {
   // A row is split over a cluster only as far as SMs would stand idle and every warp still has a step.
   const long long steps = c.a.vocab / (32 * LP_VECS * Tok<T>::VEC);
   int nct = 1;
-  while (nct < 8 && c.n * nct < 2 * pbg_sm_count() && 2 * nct * LP_WARPS <= steps) nct *= 2;
-  void (*kernel)(const T *, LogprobArgs) = c.a.top > 0 ? logprobs_kernel<T, true> : logprobs_kernel<T, false>;
+  const int sms = pbg_sm_count();
+  while (nct < 8 && c.n * nct < 2 * sms && 2 * nct * 8 <= steps) nct *= 2;
+  // Four warps to a CTA once there are more rows than CTAs of eight warps at a time: twice as many rows are under way, and one row's joins
+  // and best scores, all waiting, are hidden behind others' scans (4096 x 14,951 bf16 with the best 8: 65 and 49 us; 592 rows of 50,257:
+  // 20 and 21, 700: 25 and 24; two warps gain nothing on 300 scores and lose on 4096).  Not where a second turn of them would be half
+  // empty, unless the rows are short (1500 x 131,072 fp32: 129 and 149).
+  const bool half_empty = c.n > 8ll * sms && c.n <= 12ll * sms && (c.a.top == 0 || c.a.vocab * (long long)sizeof(T) > 128 * 1024);
+  const bool eight = c.n <= 4ll * sms || half_empty;
+  void (*kernel)(const T *, LogprobArgs) = eight ? (c.a.top > 0 ? logprobs_kernel<T, true, 8> : logprobs_kernel<T, false, 8>)
+                                                 : (c.a.top > 0 ? logprobs_kernel<T, true, 4> : logprobs_kernel<T, false, 4>);
   if (pbg_launch_failed()) return;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(c.n * nct)); cfg.blockDim = dim3(LP_THREADS); cfg.stream = c.st;
+  cfg.gridDim = dim3((unsigned)(c.n * nct)); cfg.blockDim = dim3(eight ? 256 : 128); cfg.stream = c.st;
   cudaLaunchAttribute at;
   at.id = cudaLaunchAttributeClusterDimension;
   at.val.clusterDim.x = nct; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;

@@ -310,7 +310,7 @@ int pbg_embedding_lookup(const void *table, int64_t row_stride, int64_t num_rows
 /* Gradient of the table: out[v] = scale * sum of grad[i] over the i with ids[i] == v, in the order of i (sorted by id:
  * the same bits every time); rows without an id get 0.  accumulate = 1: the sums are added to out, whose other rows
  * are left alone.  An id outside [0, num_rows) is skipped.  out [num_rows, dim], of grad's type.
- * Up to 512 ids need no workspace (its size is 0, the pointer may be NULL). */
+ * Up to 1536 ids need no workspace (its size is 0, the pointer may be NULL). */
 int64_t pbg_embedding_lookup_grad_workspace(int64_t n, int64_t num_rows, int32_t dim);
 int pbg_embedding_lookup_grad(const void *grad, int64_t grad_stride, const int64_t *ids, int64_t n, int64_t num_rows,
                               int32_t dim, int32_t dtype, float scale, void *out, int64_t out_stride, int32_t accumulate,

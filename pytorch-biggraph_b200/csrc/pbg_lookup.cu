@@ -260,17 +260,19 @@ __global__ void __launch_bounds__(32 * LG_JOIN_WARPS) lookup_grad_join_kernel(T 
 }
 
 // ---- a short list -------------------------------------------------------------------------------------------
-// Up to LS_SMALL occurrences in one launch: a CTA per occurrence looks through the list, leaves if its id stands further in front, and else
-// sums the rows of all occurrences of the id; the CTAs behind them write the zeros of the rows that the list does not name.  The warps
-// of a CTA take blocks of 32 units, and where there are fewer blocks than warps, parts of the occurrences, added in their order.
-#define LS_SMALL 512
+// Up to LS_SMALL occurrences in one launch: a CTA per occurrence looks through the list for the others of its id, and the CTAs of an id's
+// first occurrences share out the blocks of 32 units of its row, a CTA to a block where there are as many; the CTAs behind them write the
+// zeros of the rows that the list does not name.  The warps of a CTA take blocks, and where it has fewer blocks than warps, parts of the
+// occurrences, added in their order.  fp32, against sorting: 512 ids into 12,574 x 516 8 us and
+// 14, 1398 11 and 17; all of one id 8 and 16, 15 and 18.
+#define LS_SMALL 1536
 #define LS_SMALL_WORDS 1024             // most words of named rows of a CTA that writes zeros
 
-template <class T, int N>
+template <class T, int N, int PER>
 __global__ void __launch_bounds__(256, 3) lookup_grad_small_kernel(const T *__restrict__ grad, const long long *__restrict__ ids, T *__restrict__ out, GradArgs a, int *errors) {
   __shared__ union { float sums[8][32 * N]; unsigned named[LS_SMALL_WORDS]; } sh;
-  __shared__ unsigned short list[LS_SMALL];
-  __shared__ int counts[8];
+  __shared__ unsigned short list[256 * PER];
+  __shared__ int counts[8], place;
   pdl_begin();
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   if (blockIdx.x >= (unsigned)a.n) {
@@ -291,25 +293,34 @@ __global__ void __launch_bounds__(256, 3) lookup_grad_small_kernel(const T *__re
     if (threadIdx.x == 0 && errors) atomicOr(errors, TOK_ERR_ID);
     return;
   }
-  // thread t looks at occurrences 2 t and 2 t + 1: the matches of the whole list lie in the order of the threads
-  static_assert(LS_SMALL == 512, "two occurrences to a thread");
-  const int i0 = 2 * threadIdx.x;
-  const bool m0 = i0 < a.n && ids[i0] == id, m1 = i0 + 1 < a.n && ids[i0 + 1] == id;
-  if (__syncthreads_or((m0 && i0 < me) || (m1 && i0 + 1 < me))) return;
-  const unsigned b0 = __ballot_sync(0xffffffffu, m0), b1 = __ballot_sync(0xffffffffu, m1);
-  if (lane == 0) counts[w] = __popc(b0) + __popc(b1);
+  // thread t looks at occurrences PER t to PER t + PER - 1: the matches of the whole list lie in the order of the threads
+  const int i0 = PER * threadIdx.x;
+  unsigned match = 0u;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) match |= i0 + k < a.n && ids[i0 + k] == id ? 1u << k : 0u;
+  const int mine = __popc(match);
+  int at = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, at, o); if (lane >= o) at += v; }
+  if (lane == 31) counts[w] = at;
+  at -= mine;
   __syncthreads();
-  int at = 0, total = 0;
+  int total = 0;
   for (int k = 0; k < 8; ++k) { at += k < w ? counts[k] : 0; total += counts[k]; }
-  const unsigned lt = (1u << lane) - 1u;
-  at += __popc(b0 & lt) + __popc(b1 & lt);
-  if (m0) list[at++] = (unsigned short)i0;
-  if (m1) list[at] = (unsigned short)(i0 + 1);
+  for (unsigned m = match; m; m &= m - 1u) {
+    const int i = i0 + __ffs(m) - 1;
+    if (i == me) place = at;
+    list[at++] = (unsigned short)i;
+  }
   __syncthreads();
   const int units = a.dim / N, blocks = (units + 31) / 32;
-  const int parts = blocks > 4 ? 1 : blocks > 2 ? 2 : blocks > 1 ? 4 : 8;      // warps to a block
+  const int share = total < blocks ? total : blocks;                     // CTAs of this id that have blocks: place, place + share, ..
+  if (place >= share) return;
+  const int own = (blocks - place + share - 1) / share;
+  const int parts = own > 4 ? 1 : own > 2 ? 2 : own > 1 ? 4 : 8;         // warps to a block
   const int part = w % parts, per = (total + parts - 1) / parts, lo = part * per, hi = lo + per < total ? lo + per : total;
-  for (int b = w / parts; b < (parts > 1 ? 8 / parts : blocks); b += 8 / parts) {                // (with several parts, once)
+  for (int o = w / parts; o < (parts > 1 ? 8 / parts : own); o += 8 / parts) {                   // (with several parts, once)
+    const int b = place + o * share;
     const int unit = b * 32 + lane;
     const bool live = unit < units;
     float acc[N];
@@ -533,7 +544,8 @@ static void lookup_grad_launch(const LookupGradCall &c) {
   a.zero_words = (int)(words < 1 ? 1 : words < LS_SMALL_WORDS ? words : LS_SMALL_WORDS);
   const long long zero_ctas = a.accumulate ? 0 : ((a.num_rows + 31) / 32 + a.zero_words - 1) / a.zero_words;
   if (a.n <= LS_SMALL) {
-    pbg_launch(lookup_grad_small_kernel<T, N>, dim3((unsigned)(a.n + zero_ctas)), 256, 0, c.st, (const T *)c.grad, c.ids, (T *)c.out, a, c.errors);
+    auto kernel = a.n <= 512 ? lookup_grad_small_kernel<T, N, 2> : lookup_grad_small_kernel<T, N, LS_SMALL / 256>;
+    pbg_launch(kernel, dim3((unsigned)(a.n + zero_ctas)), 256, 0, c.st, (const T *)c.grad, c.ids, (T *)c.out, a, c.errors);
     return;
   }
   pbg_launch(lookup_grad_kernel<T, N>, dim3((unsigned)(a.sum_ctas + zero_ctas)), 256, 0, c.st, (const T *)c.grad, (T *)c.out, a);

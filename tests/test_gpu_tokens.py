@@ -92,7 +92,8 @@ def _grad_want(grad, ids, rows, scale):
 @pytest.mark.parametrize("n,rows,dim,kind", [(1, 1, 1, "any"), (1, 500, 33, "any"), (16, 4, 8, "any"), (17, 4, 8, "one"), (33, 3, 100, "few"), (1000, 7, 400, "few"),
                                              (4096, 3000, 130, "any"), (5000, 2000, 1, "one"), (2500, 100_003, 24, "few"), (20_001, 4000, 64, "any"),
                                              (300_000, 1000, 4, "any"), (263_000, 70_000, 8, "one"), (512, 700, 2048, "few"), (511, 3, 200, "any"),
-                                             (513, 40, 96, "few"), (300, 9000, 1, "any"), (512, 1, 516, "one")])
+                                             (513, 40, 96, "few"), (300, 9000, 1, "any"), (512, 1, 516, "one"), (1536, 700, 516, "few"), (1536, 9, 33, "one"),
+                                             (1537, 700, 130, "few"), (900, 5, 2048, "any"), (1535, 20_000, 1026, "any"), (9, 2, 1024, "one")])
 def test_lookup_grad(dtype, n, rows, dim, kind):
     g = gen(n + dim)
     ids = torch.randint(0, rows, (n,), device=DEV, generator=g)

@@ -30,10 +30,10 @@ def _calls(lib, name):
     if name == "lookup":
         return lambda: lib.pbg_embedding_lookup(p(x), D, rows, D, 0, p(ids), n, 1.0, p(out), p(errors), None), 1
     if name.startswith("lookup_grad"):
-        m = {"lookup_grad_none": 0, "lookup_grad_short": 512, "lookup_grad": 513, "lookup_grad_long": 70_000}[name]
+        m = {"lookup_grad_none": 0, "lookup_grad_short": 1536, "lookup_grad": 1537, "lookup_grad_long": 70_000}[name]
         g, size = F.dev((m + 1, 4), np.float32), lib.pbg_embedding_lookup_grad_workspace(m, rows, 4)
         ws = F.dev(size + 256, np.uint8)
-        return lambda: lib.pbg_embedding_lookup_grad(p(g), 4, p(ids), m, rows, 4, 0, 1.0, p(out), 4, 0, p(ws), size, p(errors), None), {0: 1, 512: 1, 513: 3, 70_000: 6}[m]
+        return lambda: lib.pbg_embedding_lookup_grad(p(g), 4, p(ids), m, rows, 4, 0, 1.0, p(out), 4, 0, p(ws), size, p(errors), None), {0: 1, 1536: 1, 1537: 3, 70_000: 6}[m]
     logits, rank, best = F.dev((n, 100), np.float32), F.dev(n, np.int64), F.dev((n, 8), np.int64)
     if name == "logprobs":
         return lambda: lib.pbg_token_logprobs(p(logits), 100, n, 100, 0, p(ids), -100, 1.0, 8, p(f), p(f), p(f), p(rank), p(best), p(best), p(errors), None), 1

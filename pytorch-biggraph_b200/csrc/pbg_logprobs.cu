@@ -7,7 +7,7 @@
 //
 // Forward: a row is read once.  Gradient: one read, one write.  HBM bounds both; the forward pass comes near the issue slots too (16-bit
 // scores at 6.5 TB/s are 11.6 to an SM and cycle, which issues 128 lanes of instructions: 11 for each score, of which the pass takes
-// some seven).  4099 x 131,072 bf16 with the best 8: 212 us, 5.1 TB/s, 62 % of the issue slots; its gradient 315 us, 6.8 TB/s; four rows
+// some seven).  4099 x 131,072 bf16 with the best 8: 218 us, 4.9 TB/s, 60 % of the issue slots; its gradient 315 us, 6.8 TB/s; four rows
 // with the best 20, eight CTAs to a row: 14 us.
 #include <cooperative_groups.h>
 

@@ -117,29 +117,18 @@ struct RowScan {
     for (int q = 1; q < WORDS; ++q) top.seen(raw[q]);
     const float cm = top.largest();
     if (cm > s.m) raise(cm);
-    const float rc = s.r * c;
-    if (fabsf(rc) < 1e38f) {
-      const unsigned long long c2 = f32x2(c, c), r2 = f32x2(-rc, -rc);
-      constexpr int PAIRS = sizeof(T) == 2 ? WORDS : WORDS / 2;
+    // (x - r) c, not x c - r c: the rounding of r c would be a factor of all sums, 2^64 where every score is -1e9
+    const unsigned long long c2 = f32x2(c, c), r2 = f32x2(-s.r, -s.r), zero = f32x2(0.f, 0.f);
+    constexpr int PAIRS = sizeof(T) == 2 ? WORDS : WORDS / 2;
 #pragma unroll
-      for (int q = 0; q < PAIRS; ++q) {
-        const float2 x = sizeof(T) == 2 ? word_up<T>(raw[q]) : make_float2(__uint_as_float(raw[2 * q % WORDS]), __uint_as_float(raw[(2 * q + 1) % WORDS]));
-        float2 y = f32x2_parts(f32x2_fma(f32x2(x.x, x.y), c2, r2));
-        y.x = tok_max_nan(y.x, -1000.f);                               // 2^-1000 is 0 in fp32 too; -inf has no place in T
-        y.y = tok_max_nan(y.y, -1000.f);
-        const unsigned long long e2 = f32x2(tok_ex2(y.x), tok_ex2(y.y));
-        S2 = f32x2_add(S2, e2);
-        T2 = f32x2_fma(f32x2(y.x, y.y), e2, T2);
-      }
-    } else {                                                             // scores near the type's ends: the reference has no place in base 2
-#pragma unroll 1
-      for (int q = 0; q < WORDS; ++q) {
-        const float2 x = word_up<T>(pick(raw, q));
-        const float y0 = tok_max_nan((x.x - s.r) * c, -1000.f), y1 = tok_max_nan((x.y - s.r) * c, -1000.f);
-        const unsigned long long e2 = f32x2(tok_ex2(y0), sizeof(T) == 2 ? tok_ex2(y1) : 0.f);
-        S2 = f32x2_add(S2, e2);
-        T2 = f32x2_fma(f32x2(y0, y1), e2, T2);
-      }
+    for (int q = 0; q < PAIRS; ++q) {
+      const float2 x = sizeof(T) == 2 ? word_up<T>(raw[q]) : make_float2(__uint_as_float(raw[2 * q % WORDS]), __uint_as_float(raw[(2 * q + 1) % WORDS]));
+      float2 y = f32x2_parts(f32x2_fma(f32x2_add(f32x2(x.x, x.y), r2), c2, zero));
+      y.x = tok_max_nan(y.x, -1000.f);                                   // 2^-1000 is 0 in fp32 too; -inf has no place in T
+      y.y = tok_max_nan(y.y, -1000.f);
+      const unsigned long long e2 = f32x2(tok_ex2(y.x), tok_ex2(y.y));
+      S2 = f32x2_add(S2, e2);
+      T2 = f32x2_fma(f32x2(y.x, y.y), e2, T2);
     }
     // scores in front of the target's: larger ones, and equal ones with a smaller id
     if constexpr (sizeof(T) == 2) {

@@ -210,6 +210,33 @@ def test_logprobs(dtype, kind, n, vocab, pad, top):
         assert r.top_ids is None and r.top_logprobs is None
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("base", [-1e30, -1e9, -65_000.0, -300.0, 3e4, 1e6, 1e30])
+@pytest.mark.parametrize("n,vocab", [(3, 11), (2, 30_000), (700, 2051)])
+def test_logprobs_far_from_zero(dtype, base, n, vocab):
+    """Rows that a mask of -1e9 leaves nothing of, and others around a large number: the differences of the scores are exact, and so the
+    log probabilities, which do not pass through lse, are as good as those around zero: 2e-5 of 1 + their size."""
+    if dtype == torch.float16 and abs(base) > 65_504:
+        base = math.copysign(6e4, base)
+    x = torch.full((n, vocab), base, device=DEV).to(dtype)
+    step = x[0, 0].float().abs().item() * torch.finfo(dtype).eps               # the next numbers of the type, where they are near
+    if step < 64:
+        x = (x.float() + torch.randint(-3, 4, (n, vocab), device=DEV, generator=gen(9)) * step).to(dtype)
+    targets = torch.randint(0, vocab, (n,), device=DEV, generator=gen(3))
+    r = T.token_logprobs(x, targets, top=4)
+    z = x.double() - x.double().amax(1, keepdim=True)
+    lse = torch.logsumexp(z, 1)
+    logprob = z.gather(1, targets[:, None])[:, 0] - lse
+    assert ((r.logprob.double() - logprob).abs() <= 2e-5 * (1 + logprob.abs())).all()
+    p = torch.softmax(z, 1)
+    ent = torch.special.entr(p).sum(1)
+    assert ((r.entropy.double() - ent).abs() <= 2e-5 * (1 + ent + math.log(vocab))).all()
+    best = z.gather(1, r.top_ids) - lse[:, None]
+    assert ((r.top_logprobs.double() - best).abs() <= 2e-5 * (1 + best.abs())).all()
+    top = x.double().amax(1)
+    assert ((r.lse.double() - top - lse).abs() <= 2e-5 * (1 + lse.abs()) + 2 ** -23 * top.abs()).all()
+
+
 def test_logprobs_of_rows_of_equal_scores_keep_the_order_of_ids():
     for vocab in (64, 5000, 131_073):
         for value in (0.0, -3.0, -math.inf):

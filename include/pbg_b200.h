@@ -329,6 +329,8 @@ int pbg_token_logprobs(const void *logits, int64_t row_stride, int64_t n, int64_
 
 /* d(sum of grad_logprob * logprob + grad_entropy * entropy) / d(logits), from the lse and entropy of the forward call:
  *   out_v = scale * (grad_logprob * ([v == t] - p_v) - grad_entropy * p_v * (log p_v + entropy))
+ * p_v = e^(z_v - lse) is off by half a step of lse, relatively (4e-6 for an lse of 64); a row with an lse below -1e6, of which a mask
+ * has left nothing, gets zeros.
  * Either gradient may be NULL (zero); entropy is read where grad_entropy is given.  out may be logits itself (with its row stride). */
 int pbg_token_logprobs_grad(const void *logits, int64_t row_stride, int64_t n, int64_t vocab, int32_t dtype,
                             const int64_t *targets, int64_t ignore_index, float scale, const float *lse, const float *entropy,

@@ -524,7 +524,8 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_grad_kernel(const T *logi
   r.g = a.g ? a.g[n] * a.scale : 0.f;
   r.h = a.h ? a.h[n] * a.scale : 0.f;
   r.H = a.h ? a.entropy[n] : 0.f;
-  const bool none = !known || r.lse == -INFINITY;                        // padding, or a row of -inf alone: zeros
+  // zeros for padding, and where a mask left nothing: -inf alone, or scores around -1e9, whose lse in fp32 says nothing about p
+  const bool none = !known || r.lse < -1e6f;
   const int t = none ? -1 : (int)target;
 #pragma unroll
   for (int u = 0; u < LP_VECS; ++u) {

@@ -257,7 +257,8 @@ def token_logprobs_grad(logits: torch.Tensor, targets: torch.Tensor, lse: torch.
                         ignore_index: int = IGNORE_INDEX, out: Optional[torch.Tensor] = None, errors: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Gradient with respect to the logits of sum(grad_logprob * logprob + grad_entropy * entropy), from the lse and the entropy that
     token_logprobs returned (the entropy only where grad_entropy is given).  `out` may be `logits` itself: the gradient then takes the scores'
-    place.  Rows of padding, rows whose target is out of range and rows of -inf alone get zeros."""
+    place.  Rows of padding, rows whose target is out of range and rows of which a mask has left nothing (an lse of -inf, or below -1e6)
+    get zeros.  Probabilities are e^(z - lse): off by half a step of lse, relatively."""
     code, device = _matrix("logits", logits), logits.device
     n, vocab = logits.shape
     targets = _vector("targets", targets, torch.long, n, device)

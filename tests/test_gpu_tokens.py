@@ -339,6 +339,38 @@ def test_logprobs_grad(dtype, kind, n, vocab, pad, out):
         close(T.token_logprobs_grad(x, targets, f.lse, f.entropy, None, h, scale=1.3), want, 1.0, half_step(dtype) * want.abs() + 2e-5 * size, floor)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("mask", [-math.inf, -1e9, -3e38])
+def test_a_mask_that_leaves_nothing_gives_no_gradient(dtype, mask):
+    x = torch.randn(3, 2051, device=DEV, generator=gen(4)).to(dtype)
+    x[1] = mask
+    x[2, 5:] = mask
+    targets = torch.tensor([7, 8, 2], device=DEV)
+    g, h = torch.ones(3, device=DEV), torch.ones(3, device=DEV)
+    r = T.token_logprobs(x, targets)
+    got = T.token_logprobs_grad(x, targets, r.lse, r.entropy, g, h)
+    assert (got[1] == 0).all() and (got[2, 5:] == 0).all() and got.isfinite().all()
+    assert r.logprob[1] == -math.inf if mask == -math.inf else abs(r.logprob[1].item() + math.log(2051)) < 2e-4
+    p = torch.softmax(x.double(), 1)
+    H = torch.special.entr(p).sum(1, keepdim=True)
+    for row in (0, 2):
+        want = -p[row] - (-torch.special.entr(p[row]) + p[row] * H[row])
+        want[targets[row]] += 1
+        assert ((got[row].double() - want).abs() <= half_step(dtype) * want.abs() + 2e-4 * p[row] + 1e-6 * (1 if dtype == torch.float32 else 0)).all()
+
+
+@pytest.mark.parametrize("n,kind", [(7, "one"), (600, "half"), (1536, "one"), (1537, "half"), (70_000, "half")])
+def test_ids_of_padding_that_are_most_of_the_list(n, kind):
+    """One id far more often than the others: the list is summed in parts, in the same order every time."""
+    ids = torch.randint(0, 5000, (n,), device=DEV, generator=gen(n))
+    ids[torch.rand(n, device=DEV, generator=gen(1)) < (2.0 if kind == "one" else 0.5)] = 17
+    grad = torch.randn(n, 1026, device=DEV, generator=gen(2))
+    want, size = _grad_want(grad, ids, 5000, 1.0)
+    got = T.embedding_lookup_grad(grad, ids, 5000)
+    close(got, want, 1.0, 2 ** -24 * want.abs() + (n + 4) * 2 ** -24 * size, floor=1e-37)
+    assert torch.equal(got, T.embedding_lookup_grad(grad, ids, 5000))
+
+
 def test_logprobs_gradient_is_the_slope():
     """Central differences of the 64-bit definition with step e: off by e^2 / 6 of a third derivative below 2, and by what fp32 makes
     of the gradient itself."""

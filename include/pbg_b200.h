@@ -341,6 +341,7 @@ int pbg_token_logprobs_grad(const void *logits, int64_t row_stride, int64_t n, i
  * table.  16-bit operands are multiplied as they are; fp32 ones as two fp16 planes each (22 bits), at fp32's accuracy
  * for elements down to 2^-17 of the largest, and an absolute one of 2^-39 of it below.  NaN, or an infinity, among a
  * query's scores makes its entropy NaN, NaN or +inf its other results too; no other query's results change.
+ * Scores are fp32 sums: beyond 1e7 in size nothing is left of their differences, and results may be NaN.
  * workspace: of pbg_table_logprobs_workspace(n, rows, dim, dtype, 0) bytes. */
 int64_t pbg_table_logprobs_workspace(int64_t n, int64_t rows, int32_t dim, int32_t dtype, int32_t grad);
 int pbg_table_logprobs(const void *queries, int64_t q_stride, int64_t n, const void *table, int64_t t_stride, int64_t rows,

@@ -55,20 +55,24 @@ EDGES_PER_STEP_CAP = 269_507
 # DRAM bytes per trained edge of each kernel class come from the ncu summaries under profiles/: the file
 # of a (workload, precision) pair carries one line
 #   traffic_per_edge_bytes: gather=... score=... grad=... update=... csrc_sha256=<digest>
-# where the digest is csrc_digest() of the kernel sources the capture ran.  A summary whose digest is
+# where the digest is csrc_digest() of the training step's kernel sources that the capture ran.  A summary whose digest is
 # not that of the sources in the tree describes other kernels: its figures are then not used.
 PROFILE_FILES = {("c3", "bf16x6"): "kernels_c3_bf16x6.md"}
 
 
 def csrc_digest():
-    """sha256 over the CUDA sources of the library (names and contents, sorted by name)."""
+    """sha256 over the CUDA sources of the training step and its evaluation (names and contents, sorted by name).  The
+    token operators, which are pbg_tokens.cuh and what includes it, run in neither."""
     import glob
     import hashlib
     h = hashlib.sha256()
     for path in sorted(glob.glob(os.path.join(ROOT, "pytorch-biggraph_b200", "csrc", "*.cu*"))):
-        h.update(os.path.basename(path).encode())
         with open(path, "rb") as f:
-            h.update(f.read())
+            text = f.read()
+        if os.path.basename(path) == "pbg_tokens.cuh" or b'#include "pbg_tokens.cuh"' in text:
+            continue
+        h.update(os.path.basename(path).encode())
+        h.update(text)
     return h.hexdigest()[:16]
 
 

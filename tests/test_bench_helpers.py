@@ -51,14 +51,18 @@ def test_committed_summary_is_used_only_for_its_own_sources():
         assert per_class["gather"] + per_class["score"] + per_class["grad"] + per_class["update"] > b.algorithmic(b.WORKLOADS["c3"])["bytes"]
 
 
-def test_sources_of_the_token_operators_leave_the_capture_as_it_is():
-    """They run in no training step: with them or without, the summary of the step's kernels describes the tree's."""
+def test_sources_of_the_token_operators_leave_the_digest_as_it_is(tmp_path):
+    """They run in no training step: with them or without, a summary of the step's kernels describes the tree's."""
     b = _bench()
-    csrc = os.path.join(ROOT, "pytorch-biggraph_b200", "csrc")
-    users = {n for n in os.listdir(csrc) if '#include "pbg_tokens.cuh"' in open(os.path.join(csrc, n)).read()}
-    assert users == {"pbg_lookup.cu", "pbg_logprobs.cu", "pbg_table.cu"}
-    per_class, source = b.ncu_traffic_per_edge("c3", "bf16x6")
-    assert per_class is not None, source
+    digest = b.csrc_digest()
+    csrc = tmp_path / "pytorch-biggraph_b200" / "csrc"
+    shutil.copytree(os.path.join(ROOT, "pytorch-biggraph_b200", "csrc"), csrc)
+    for name in ("pbg_lookup.cu", "pbg_logprobs.cu", "pbg_table.cu", "pbg_tokens.cuh"):
+        (csrc / name).unlink()
+    b.ROOT = str(tmp_path)
+    assert b.csrc_digest() == digest
+    (csrc / "pbg_update.cu").write_text((csrc / "pbg_update.cu").read_text() + "\n")
+    assert b.csrc_digest() != digest
 
 
 def test_algorithmic_figures_of_the_headline_workload():

@@ -3,7 +3,8 @@
 They stand on either side of what this package trains: a table of embeddings, and answers that are rows of a table.  The
 reference has no counterpart (it gathers with F.embedding and takes its losses over sampled negatives).  As everywhere
 here the arithmetic runs in libpbg_b200.so and gradients are functions of their own: nothing is recorded for autograd, and a tensor
-that requires a gradient is refused while gradients are being recorded -- detach it, or call under torch.no_grad().
+that requires a gradient is refused while gradients are being recorded -- detach it, or call under torch.no_grad() -- as is one
+that carries a forward-mode tangent.
 
 All calls are queued on PyTorch's current stream of the tensors' device and return at once; workspaces come from PyTorch's allocator.
 No call synchronises, so all of them can be captured into a CUDA graph.  Ids and targets are int64.  One outside of its range
@@ -15,6 +16,7 @@ import math
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -43,6 +45,8 @@ def _matrix(name, t, dtype=None, device=None):
     """The pbg_dtype of a matrix whose rows can be read."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor")
+    if t.requires_grad or forward_ad._current_level >= 0:
+        _no_grad(name, t)
     if not t.is_cuda:
         raise RuntimeError(f"{name} is on {t.device}: the token operators work on CUDA tensors only (no CPU fallback)")
     if device is not None and t.device != device:
@@ -57,14 +61,14 @@ def _matrix(name, t, dtype=None, device=None):
         raise ValueError(f"{name} has rows without elements")
     if width > 1 and t.stride(1) != 1:
         raise ValueError(f"the elements of a row of {name} must lie next to each other")
-    if t.requires_grad:
-        _no_grad(name)
     return code
 
 
-def _no_grad(name):
-    if torch.is_grad_enabled():
+def _no_grad(name, t):
+    if t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{name} requires a gradient, which the token operators do not record: detach it or call under torch.no_grad()")
+    if forward_ad.unpack_dual(t).tangent is not None:
+        raise RuntimeError(f"{name} carries a forward-mode tangent, which the token operators do not propagate: take its primal")
 
 
 def _vector(name, t, dtype, n, device):
@@ -74,8 +78,8 @@ def _vector(name, t, dtype, n, device):
         raise ValueError(f"{name} is on {t.device}, not on {device}")
     if t.dim() != 1 or t.shape[0] != n:
         raise ValueError(f"{name} must have one dimension of {n} elements")
-    if t.requires_grad:
-        _no_grad(name)
+    if t.requires_grad or forward_ad._current_level >= 0:
+        _no_grad(name, t)
     return t if t.is_contiguous() else t.contiguous()
 
 

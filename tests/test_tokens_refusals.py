@@ -18,6 +18,22 @@ def test_python_refuses_cpu_tensors():
             call()
 
 
+def test_python_refuses_forward_mode_tangents():
+    """A tangent would be lost without a word: refused, of matrices and of vectors, and only where there is one."""
+    from torch.autograd import forward_ad
+    x, ids, f = torch.zeros(3, 4), torch.zeros(3, dtype=torch.long), torch.zeros(3)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: T.embedding_lookup(dual, ids), lambda: T.embedding_lookup_grad(dual, ids, 5), lambda: T.token_logprobs(dual, ids),
+                     lambda: T.token_logprobs_grad(dual, ids, f, None, f), lambda: T.table_logprobs(dual, x, ids), lambda: T.table_logprobs_grad(dual, x, ids, f, None, f),
+                     lambda: T.tokens._vector("lse", forward_ad.make_dual(f, torch.ones(3)), torch.float32, 3, f.device)):
+            with pytest.raises(RuntimeError, match="tangent"):
+                call()
+        assert T.tokens._vector("lse", f, torch.float32, 3, f.device) is f
+        with pytest.raises(RuntimeError, match="CUDA"):
+            T.embedding_lookup(x, ids)
+
+
 @pytest.mark.parametrize("change,status", [
     (dict(table=None), BAD), (dict(ids=None), BAD), (dict(out=None), BAD), (dict(dim=0), BAD), (dict(dim=65_537), LARGE), (dict(rows=-1), BAD), (dict(rows=0), BAD),
     (dict(rows=2 ** 31), LARGE), (dict(n=-1), BAD), (dict(n=2 ** 31), LARGE), (dict(dtype=3), BAD), (dict(dtype=-1), BAD), (dict(stride=-4), BAD), (dict(scale=float("nan")), BAD)])

@@ -4,7 +4,7 @@ They stand on either side of what this package trains: a table of embeddings, an
 reference has no counterpart (it gathers with F.embedding and takes its losses over sampled negatives).  As everywhere
 here the arithmetic runs in libpbg_b200.so and gradients are functions of their own: nothing is recorded for autograd, and a tensor
 that requires a gradient is refused while gradients are being recorded -- detach it, or call under torch.no_grad() -- as is one
-that carries a forward-mode tangent.
+that carries a forward-mode tangent.  A tensor given as `out` counts as modified: what autograd has saved of it is not used any more.
 
 All calls are queued on PyTorch's current stream of the tensors' device and return at once; workspaces come from PyTorch's allocator.
 No call synchronises, so all of them can be captured into a CUDA graph.  Ids and targets are int64.  One outside of its range
@@ -207,6 +207,7 @@ def embedding_lookup_grad(grad: torch.Tensor, ids: torch.Tensor, num_rows: int, 
             raise ValueError("the rows of out overlap")
         if _overlap(out, grad):
             raise ValueError("out and grad share memory")
+        torch.autograd.graph.increment_version(out)
     ws, size = _workspace("pbg_embedding_lookup_grad_workspace", device, n, num_rows, dim)
     _call("pbg_embedding_lookup_grad", device, grad.data_ptr(), _row_stride(grad), flat.data_ptr(), n, num_rows, dim, code, _scale(scale, False),
           out.data_ptr(), _row_stride(out), int(bool(accumulate)), _ptr(ws), size, _error_word(errors, device))
@@ -279,6 +280,7 @@ def token_logprobs_grad(logits: torch.Tensor, targets: torch.Tensor, lse: torch.
             raise ValueError("the rows of out overlap")
         if _overlap(out, logits) and (out.data_ptr() != logits.data_ptr() or _row_stride(out) != _row_stride(logits)):
             raise ValueError("out shares memory with logits without being them")
+        torch.autograd.graph.increment_version(out)
     _call("pbg_token_logprobs_grad", device, logits.data_ptr(), _row_stride(logits), n, vocab, code, targets.data_ptr(), int(ignore_index),
           _scale(scale, True), lse.data_ptr(), _ptr(entropy), _ptr(grad_logprob), _ptr(grad_entropy), out.data_ptr(), _row_stride(out),
           _error_word(errors, device))

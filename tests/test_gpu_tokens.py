@@ -425,6 +425,22 @@ def test_on_a_side_stream_and_in_a_graph():
         assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
+def test_what_is_written_to_counts_as_modified():
+    """What autograd has saved for a backward pass is refused there once a call has written over it."""
+    x, ids = torch.randn(4, 8, device=DEV), torch.arange(4, device=DEV)
+    w = torch.ones(8, device=DEV, requires_grad=True)
+    loss = (x * w).sum()
+    r = T.token_logprobs(x, ids)
+    T.token_logprobs_grad(x, ids, r.lse, None, torch.ones(4, device=DEV), out=x)
+    with pytest.raises(RuntimeError, match="modified"):
+        loss.backward()
+    for accumulate in (False, True):
+        loss = (x * w).sum()
+        T.embedding_lookup_grad(torch.ones(4, 8, device=DEV), ids, 4, out=x, accumulate=accumulate)
+        with pytest.raises(RuntimeError, match="modified"):
+            loss.backward()
+
+
 def test_offsets_beyond_32_bits():
     rows, dim = 2_200_000, 1024                      # 2.25e9 elements
     table = torch.empty(rows, dim, dtype=torch.bfloat16, device=DEV)

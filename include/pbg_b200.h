@@ -297,7 +297,7 @@ int pbg_sub_bucket(pbg_context *ctx, const int64_t *lhs_in, const int64_t *rhs_i
  * irrelevant); two calls in flight need two of them.  All pointers are device memory; row strides are in elements, the elements of
  * a row lie next to each other.  Types are pbg_dtype; sums, statistics and softmax sums are fp32, results are rounded once.
  * errors: device int32 word or NULL; bit 1 is set by an id or target outside of its range, bit 2 where a bounded
- * wait ran out.  scale: finite for the lookups, 1e-20 to 1e20 for the log probabilities.
+ * wait ran out (results that depend on it are NaN, with or without the word).  scale: finite for the lookups, 1e-20 to 1e20 for the log probabilities.
  * Sizes: dim 1 to 65536; ids, rows of scores and table rows below 2^31 (less 65536 for a row's scores and for the rows that
  * table_logprobs scores), ids of a gradient and queries up to 2^30; PBG_ERR_TOO_LARGE beyond.
  * A target equal to ignore_index marks a row of padding: it is not read, its outputs are 0 (top_ids -1), its gradients 0. ---- */
@@ -348,6 +348,10 @@ int pbg_table_logprobs(const void *queries, int64_t q_stride, int64_t n, const v
                        int32_t dim, int32_t dtype, const int64_t *targets, int64_t ignore_index, float scale,
                        float *logprob, float *entropy, float *lse, void *workspace, int64_t workspace_bytes,
                        int32_t *errors, void *stream);
+
+/* How often a wait inside the kernels of table_logprobs and its gradient asks before it gives up, for calls from here on; returns what
+ * it was.  Negative: the usual 4,000,000.  0 gives up at once, which shows what a call leaves then. */
+int32_t pbg_table_logprobs_wait_limit(int32_t limit);
 
 /* Gradients of sum(grad_logprob * logprob + grad_entropy * entropy) with respect to the queries [n, dim] and the table [rows, dim],
  * rows one behind the other, of their type; either may be NULL (not wanted).  lse, entropy: of the forward call.  The scores are

@@ -28,7 +28,10 @@
 // Up to sixteen fp32 queries take no tensor cores: making planes of the table reads and writes it three times over, where fp32 products
 // on the CUDA cores keep up with one reading of it (tab_few_kernel).
 //
-// Every wait is bounded: one that runs out sets bit 2 of the error word, and the CTA stops, frees its tensor memory and returns.
+// Every wait is bounded: one that runs out sets bit 2 of the error word, the CTA's products stop, and whatever it had still to
+// write is NaN -- partial sums, dz or results, so that all results that depend on them are NaN too; then it frees its tensor memory
+// and returns.
+#include <atomic>
 #include <type_traits>
 
 #include "pbg_tc.cuh"
@@ -91,6 +94,7 @@ struct TabArgs {
   int by_q, by_w, by_dz;              // which powers the product carries
   int a_rows;                         // rows of A that are loaded: 128, or fewer where there is one row tile and nothing to fill it with
   int b_whole;                        // MN-major B: its rows are whole blocks of 64 columns, read as one box
+  int wait_limit;                     // how often a wait asks before it gives up
 };
 
 __device__ __forceinline__ uint32_t cta_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
@@ -123,6 +127,16 @@ template <int CG>
 __device__ __forceinline__ void tab_commit(uint32_t bar) {
   if (CG == 1) mma_commit(bar);
   else asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" :: "r"(bar), "h"((unsigned short)3) : "memory");
+}
+__device__ __forceinline__ bool tab_wait(uint32_t bar, uint32_t parity, const TabArgs &g) {
+  for (int it = 0; it < g.wait_limit; ++it) {
+    uint32_t ok;
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    if (ok) return true;
+  }
+  atomicOr(g.err, TOK_ERR_TIMEOUT);
+  return false;
 }
 template <int EPI, class MATH, bool A_MN, bool B_MN, int CG, bool PARTS>        // PARTS: the contraction is added up in registers
 __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_constant__ TabMaps maps, TabArgs g) {
@@ -198,7 +212,7 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
         n0 += rank * b_cols;
         ok = failed == 0;
         for (int kb = kb0; kb < kb1 && ok; ++kb, at.next(g.stages)) {
-          ok = mbar_wait(empty_bar(at.s), at.parity ^ 1u, g.err);
+          ok = tab_wait(empty_bar(at.s), at.parity ^ 1u, g);
           if (!ok) { failed = 1; break; }
           const uint32_t a = smem_u32(smem) + (uint32_t)at.s * stage_bytes, b = a + A_BYTES;
           // a pair's loads are all counted by the first CTA, which issues the products
@@ -232,12 +246,12 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
       for (int p0 = kb0, p1; p0 < kb1 && ok; p0 = p1, ++j) {
         const int ab = j & 1;
         p1 = kb1 - p0 < g.part ? kb1 : p0 + g.part;
-        ok = failed == 0 && mbar_wait(acce_bar(ab), (uint32_t)((j >> 1) & 1) ^ 1u, g.err);
+        ok = failed == 0 && tab_wait(acce_bar(ab), (uint32_t)((j >> 1) & 1) ^ 1u, g);
         if (!__all_sync(0xffffffffu, ok)) { failed = 1; ok = false; break; }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t acc = tmem + (uint32_t)ab * 256u;
         for (int kb = p0; kb < p1; ++kb, at.next(g.stages)) {
-          ok = mbar_wait(full_bar(at.s), at.parity, g.err);
+          ok = tab_wait(full_bar(at.s), at.parity, g);
           if (!__all_sync(0xffffffffu, ok)) { failed = 1; ok = false; break; }
           const uint32_t a = smem_u32(smem) + (uint32_t)at.s * stage_bytes, b = a + A_BYTES;
           const uint64_t da = A_MN ? smem_desc(a, NPA * ATOM_BYTES, 1024, 2) : smem_desc(a, 0, K_SBO, K_LAYOUT);
@@ -271,8 +285,8 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
     const float to2 = g.scale * unscale * TOK_LOG2E;                      // from an accumulator to a score in base 2
     const int planes = NPB == 2 ? 2 : g.dz_planes;
     int j = 0;
-    bool ok = true;
-    for (long long t = first; t < ntiles && ok; t += step) {
+    bool lost = false;                                                   // a wait has run out: this warp waits no more, and what is left is NaN
+    for (long long t = first; t < ntiles; t += step) {
       long long m0, n0;
       int split, kb0, kb1;
       tile(t, m0, n0, split, kb0, kb1);
@@ -297,10 +311,9 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
       float sum[PARTS ? 128 : 1];
       // (the whole warp waits: one lane that does and a vote behind it take 200 cycles longer)
       auto wait_full = [&]() {
-        const bool w = mbar_wait(accf_bar(j & 1), (uint32_t)(j >> 1) & 1, g.err);
-        if (!__all_sync(0xffffffffu, w)) { failed = 1; return false; }
+        const bool w = tab_wait(accf_bar(j & 1), (uint32_t)(j >> 1) & 1, g);
+        if (!__all_sync(0xffffffffu, w)) { failed = 1; lost = true; return; }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        return true;
       };
       // (one arrival per warp, and no release beyond the tensor memory's: a release to the cluster waits for every store made so far)
       auto give_back = [&]() {
@@ -315,9 +328,9 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
       if (PARTS) {
 #pragma unroll
         for (int i = 0; i < 128; ++i) sum[PARTS ? i : 0] = 0.f;
-        for (int p0 = kb0; p0 < kb1; p0 = kb1 - p0 < g.part ? kb1 : p0 + g.part) {
-          ok = wait_full();
-          if (!ok) break;
+        for (int p0 = kb0; p0 < kb1 && !lost; p0 = kb1 - p0 < g.part ? kb1 : p0 + g.part) {
+          wait_full();
+          if (lost) break;
 #pragma unroll
           for (int x = 0; x < 128; x += 32) {
             if (x >= hc || idle) continue;
@@ -328,14 +341,13 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
           }
           give_back();
         }
-        if (!ok) break;
-      } else if (kb0 < kb1) {
-        ok = wait_full();
-        if (!ok) break;
-      }
+      } else if (kb0 < kb1 && !lost) wait_full();
       // 32 columns of the tile (a split without k-values holds zeros)
       auto values = [&](int x, float (&v)[32]) {
-        if (PARTS) {
+        if (lost) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = __int_as_float(0x7fc00000);
+        } else if (PARTS) {
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] = sum[PARTS ? x + i : 0];
         } else if (kb0 < kb1) {
@@ -482,7 +494,7 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
         }
       }
       if (EPI == EPI_STATS && m < g.M) g.parts[m * g.nparts + n0 / g.BN * 2 + half] = make_float4(S == 0.f ? -1e30f : r, S, T, 0.f);
-      if (!PARTS && kb0 < kb1) give_back();
+      if (!PARTS && kb0 < kb1 && !lost) give_back();
     }
     if (EPI != EPI_STATS && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");         // the stores are performed
   }
@@ -761,6 +773,9 @@ __global__ void __launch_bounds__(256) tab_join_kernel(const float *__restrict__
 }
 
 // ---- host --------------------------------------------------------------------------------------------------
+static std::atomic<int> tab_wait_limit{TC_WAIT_LIMIT};
+extern "C" int32_t pbg_table_logprobs_wait_limit(int32_t limit) { return tab_wait_limit.exchange(limit < 0 ? TC_WAIT_LIMIT : limit); }
+
 struct TabOperand { const void *base; long long rows, inner, ld, plane; int planes; bool room; };   // [planes][rows][ld], 16-bit elements; ours: room for whole blocks of 64
 
 static bool tab_encode(CUtensorMap *tm, bool bf16, const TabOperand &o, int box_inner, int box_rows, int box_planes) {
@@ -788,6 +803,7 @@ static bool tab_launch_as(const TabOperand &a, const TabOperand &b, const TabOpe
   constexpr bool bf16 = std::is_same<typename MATH::elem, __nv_bfloat16>::value;
   if (pbg_launch_failed()) return true;
   TabMaps maps;
+  g.wait_limit = tab_wait_limit.load();
   g.b_whole = B_MN && tab_whole(b);
   // Rows outside of the matrix are written as zeros, at a price: a box of 7 rows and 121 of zeros takes longer than one of 128 rows (7
   // queries, 131,072 x 2048 bf16: 127 us against 100).  A row of products depends on its own row of A alone, so what

@@ -9,7 +9,8 @@ that carries a forward-mode tangent.  A tensor given as `out` counts as modified
 All calls are queued on PyTorch's current stream of the tensors' device and return at once; workspaces come from PyTorch's allocator.
 No call synchronises, so all of them can be captured into a CUDA graph.  Ids and targets are int64.  One outside of its range
 cannot raise: its row of the result is NaN (its part of a gradient is left out), and bit 1 is set in `errors`, an
-int32 tensor of one element, where one is given (`check_errors` reads it and raises).
+int32 tensor of one element, where one is given (`check_errors` reads it and raises).  Results of a kernel whose bounded
+wait ran out are NaN, and bit 2 is set.
 
 Types: float32, bfloat16, float16; sums and statistics are float32 and results rounded once."""
 import math

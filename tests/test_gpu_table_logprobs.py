@@ -370,3 +370,30 @@ def test_a_training_step_with_both_ends_of_a_table(dtype):
         # scores of size s move p by s times the rounding of h: |h| |w| summed is below 30 here
         assert rel < (30 + 4) * half_step(dtype) + 2e-5, rel
 
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,rows,dim", [(40, 300, 64), (300, 1000, 100), (200, 3000, 2112)])
+def test_a_wait_that_runs_out_leaves_nan(dtype, n, rows, dim):
+    """With a limit of 0 every wait of the kernels runs out at once: nothing is loaded or multiplied.  Then no result is left as the memory was, with
+    or without an error word, and the next call is as good as the one before."""
+    q, t, targets = inputs(n, rows, dim, dtype, 3)
+    g = torch.ones(n, device=DEV)
+    want = T.table_logprobs(q, t, targets)
+    want_grad = T.table_logprobs_grad(q, t, targets, want.lse, want.entropy, g, g)
+    errors = torch.zeros(1, dtype=torch.int32, device=DEV)
+    before = T.tokens._lib.lib().pbg_table_logprobs_wait_limit(0)
+    try:
+        for word in (None, errors):
+            r = T.table_logprobs(q, t, targets, errors=word)
+            assert all(x.isnan().all() for x in r)
+            dq, dt = T.table_logprobs_grad(q, t, targets, want.lse, want.entropy, g, g, errors=word)
+            assert dq.isnan().all() and dt.isnan().all()
+        assert errors.item() == 2
+        with pytest.raises(T.tokens._lib.PbgError):
+            T.check_errors(errors)
+    finally:
+        T.tokens._lib.lib().pbg_table_logprobs_wait_limit(before)
+    r = T.table_logprobs(q, t, targets, errors=errors)
+    assert all(torch.equal(a, b) for a, b in zip(r, want))
+    assert all(torch.equal(a, b) for a, b in zip(T.table_logprobs_grad(q, t, targets, want.lse, want.entropy, g, g, errors=errors), want_grad)) and errors.item() == 0

@@ -88,7 +88,7 @@ struct TabArgs {
   const long long *targets; long long ignore_index, vocab, v0;         // EPI_DZ; v0: the table's row of column 0
   const float *lse, *entropy, *g, *h;
   long long ldz; int dz_planes;
-  void *out; long long ldo;           // EPI_OUT: the result, or
+  void *out; long long ldo;           // EPI_DZ: dz; EPI_OUT: the result, or
   float *partial; int add;            //          [splits][M][N] fp32, stored or added
   int bulk;                           //          either way by bulk stores
   int by_q, by_w, by_dz;              // which powers the product carries
@@ -285,8 +285,9 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
     const float to2 = g.scale * unscale * TOK_LOG2E;                      // from an accumulator to a score in base 2
     const int planes = NPB == 2 ? 2 : g.dz_planes;
     int j = 0;
-    bool lost = false;                                                   // a wait has run out: this warp waits no more, and what is left is NaN
-    for (long long t = first; t < ntiles; t += step) {
+    bool ok = true;
+    long long t = first;
+    for (; t < ntiles; t += step) {
       long long m0, n0;
       int split, kb0, kb1;
       tile(t, m0, n0, split, kb0, kb1);
@@ -312,8 +313,9 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
       // (the whole warp waits: one lane that does and a vote behind it take 200 cycles longer)
       auto wait_full = [&]() {
         const bool w = tab_wait(accf_bar(j & 1), (uint32_t)(j >> 1) & 1, g);
-        if (!__all_sync(0xffffffffu, w)) { failed = 1; lost = true; return; }
+        if (!__all_sync(0xffffffffu, w)) { failed = 1; return false; }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        return true;
       };
       // (one arrival per warp, and no release beyond the tensor memory's: a release to the cluster waits for every store made so far)
       auto give_back = [&]() {
@@ -328,9 +330,9 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
       if (PARTS) {
 #pragma unroll
         for (int i = 0; i < 128; ++i) sum[PARTS ? i : 0] = 0.f;
-        for (int p0 = kb0; p0 < kb1 && !lost; p0 = kb1 - p0 < g.part ? kb1 : p0 + g.part) {
-          wait_full();
-          if (lost) break;
+        for (int p0 = kb0; p0 < kb1; p0 = kb1 - p0 < g.part ? kb1 : p0 + g.part) {
+          ok = wait_full();
+          if (!ok) break;
 #pragma unroll
           for (int x = 0; x < 128; x += 32) {
             if (x >= hc || idle) continue;
@@ -341,13 +343,14 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
           }
           give_back();
         }
-      } else if (kb0 < kb1 && !lost) wait_full();
+        if (!ok) break;
+      } else if (kb0 < kb1) {
+        ok = wait_full();
+        if (!ok) break;
+      }
       // 32 columns of the tile (a split without k-values holds zeros)
       auto values = [&](int x, float (&v)[32]) {
-        if (lost) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = __int_as_float(0x7fc00000);
-        } else if (PARTS) {
+        if (PARTS) {
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] = sum[PARTS ? x + i : 0];
         } else if (kb0 < kb1) {
@@ -494,7 +497,22 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
         }
       }
       if (EPI == EPI_STATS && m < g.M) g.parts[m * g.nparts + n0 / g.BN * 2 + half] = make_float4(S == 0.f ? -1e30f : r, S, T, 0.f);
-      if (!PARTS && kb0 < kb1 && !lost) give_back();
+      if (!PARTS && kb0 < kb1) give_back();
+    }
+    // a wait has run out: what this warp had still to write
+    if (!ok) for (; t < ntiles; t += step) {
+      long long m0, n0;
+      int split, kb0, kb1;
+      tile(t, m0, n0, split, kb0, kb1);
+      const long long m = m0 + q * 32 + lane, c0 = n0 + half * hc, c1 = c0 + hc < g.N ? c0 + hc : g.N;
+      const float nan = __int_as_float(0x7fc00000);
+      if (m >= g.M) continue;
+      if (EPI == EPI_STATS) g.parts[m * g.nparts + n0 / g.BN * 2 + half] = make_float4(0.f, nan, nan, 0.f);
+      else for (long long c = c0; c < c1; ++c) {
+        if (EPI == EPI_DZ) for (int pl = 0; pl < planes; ++pl) ((Elem *)g.out)[(pl * g.M + m) * g.ldz + c] = Tok<Elem>::down(nan);
+        else if (g.partial) g.partial[((long long)split * g.M + m) * g.N + c] = nan;
+        else ((Out *)g.out)[m * g.ldo + c] = Tok<Out>::down(nan);
+      }
     }
     if (EPI != EPI_STATS && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");         // the stores are performed
   }
@@ -1061,7 +1079,7 @@ static void tab_backward(TabBackward &f) {
     g.by_q = g.by_w = 1;
     g.targets = c.targets; g.ignore_index = c.ignore_index; g.vocab = c.rows; g.v0 = v0;
     g.lse = f.lse; g.entropy = f.entropy; g.g = f.g; g.h = f.h;
-    g.ldz = f.p.ldz; g.dz_planes = f.p.dz_planes;
+    g.ldz = f.p.ldz; g.dz_planes = f.p.dz_planes; g.out = c.ws + f.p.dz;
     const TabOperand dz{c.ws + f.p.dz, c.n, cols, f.p.ldz, c.n * f.p.ldz, f.p.dz_planes, true};
     TabOperand written = dz;
     written.inner = f.p.ldz;

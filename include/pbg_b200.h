@@ -296,8 +296,8 @@ int pbg_sub_bucket(pbg_context *ctx, const int64_t *lhs_in, const int64_t *rhs_i
  * outputs is `workspace`, device memory of the size its *_workspace function gives (256-byte aligned, contents
  * irrelevant); two calls in flight need two of them.  All pointers are device memory; row strides are in elements, the elements of
  * a row lie next to each other.  Types are pbg_dtype; sums, statistics and softmax sums are fp32, results are rounded once.
- * errors: device int32 word or NULL; bit 1 is set by an id or target outside of its range, bit 2 where a bounded
- * wait ran out (results that depend on it are NaN, with or without the word).  scale: finite for the lookups, 1e-20 to 1e20 for the log probabilities.
+ * errors: device int32 word or NULL; 1 is set by an id or target outside of its range, 4 by an lse that a gradient can do
+ * nothing with (token_logprobs_grad), 2 where a bounded wait ran out (results that depend on it are NaN, with or without the word).  scale: finite for the lookups, 1e-20 to 1e20 for the log probabilities.
  * Sizes: dim 1 to 65536; ids, rows of scores and table rows below 2^31 (less 65536 for a row's scores and for the rows that
  * table_logprobs scores), ids of a gradient and queries up to 2^30; PBG_ERR_TOO_LARGE beyond.
  * A target equal to ignore_index marks a row of padding: it is not read, its outputs are 0 (top_ids -1), its gradients 0. ---- */
@@ -326,16 +326,26 @@ int pbg_embedding_lookup_grad(const void *grad, int64_t grad_stride, const int64
 int pbg_token_logprobs(const void *logits, int64_t row_stride, int64_t n, int64_t vocab, int32_t dtype,
                        const int64_t *targets, int64_t ignore_index, float scale, int32_t top, float *logprob,
                        float *entropy, float *lse, int64_t *rank, float *top_logprobs, int64_t *top_ids, int32_t *errors, void *stream);
+/* The same with lse_rest [n] (or NULL): what float32 cannot hold of lse, for a gradient that is exact wherever the scores lie. */
+int pbg_token_logprobs_wide(const void *logits, int64_t row_stride, int64_t n, int64_t vocab, int32_t dtype,
+                            const int64_t *targets, int64_t ignore_index, float scale, int32_t top, float *logprob,
+                            float *entropy, float *lse, float *lse_rest, int64_t *rank, float *top_logprobs, int64_t *top_ids,
+                            int32_t *errors, void *stream);
 
 /* d(sum of grad_logprob * logprob + grad_entropy * entropy) / d(logits), from the lse and entropy of the forward call:
  *   out_v = scale * (grad_logprob * ([v == t] - p_v) - grad_entropy * p_v * (log p_v + entropy))
- * p_v = e^(z_v - lse) is off by half a step of lse, relatively (4e-6 for an lse of 64); a row with an lse below -1e6, of which a mask
- * has left nothing, gets zeros.
+ * p_v = e^(z_v - lse - lse_rest).  Without lse_rest p is off by half a step of lse, relatively (4e-6 for an lse of 64, 2e-3 for 65,000),
+ * and where lse is finite and beyond 1e6 in size it cannot be had: such a row sets 4 in errors and gets zeros below -1e6 (a mask of
+ * -1e9 has left nothing) and NaN above 1e6.  With or without it, a row with an lse of -inf gets zeros and one of +inf NaN and the 4.
  * Either gradient may be NULL (zero); entropy is read where grad_entropy is given.  out may be logits itself (with its row stride). */
 int pbg_token_logprobs_grad(const void *logits, int64_t row_stride, int64_t n, int64_t vocab, int32_t dtype,
                             const int64_t *targets, int64_t ignore_index, float scale, const float *lse, const float *entropy,
                             const float *grad_logprob, const float *grad_entropy, void *out, int64_t out_stride,
                             int32_t *errors, void *stream);
+int pbg_token_logprobs_grad_wide(const void *logits, int64_t row_stride, int64_t n, int64_t vocab, int32_t dtype,
+                                 const int64_t *targets, int64_t ignore_index, float scale, const float *lse, const float *lse_rest,
+                                 const float *entropy, const float *grad_logprob, const float *grad_entropy, void *out, int64_t out_stride,
+                                 int32_t *errors, void *stream);
 
 /* The same statistics with z = scale * queries . table^T, which is never stored: queries [n, dim], table [rows, dim], targets rows of the
  * table.  16-bit operands are multiplied as they are; fp32 ones as two fp16 planes each (22 bits), at fp32's accuracy

@@ -4,6 +4,8 @@
 //   lse = m + log S     log p_t = (z_t - m) - log S     H = log S - T / S
 // T is never positive, so H is a sum of two numbers of one sign: no cancellation where the distribution is sharp.  The
 // exponentials run in base 2, against the largest element so far (each thread its own; the sums are rebased where they join).
+// Far from zero an fp32 lse says little about p = e^(z - lse) (half a step of it is 0.03 at 1e6), so that what it leaves of m + log S is
+// handed on beside it.
 //
 // Forward: a row is read once.  Gradient: one read, one write.  HBM bounds both; the forward pass comes near the issue slots too (16-bit
 // scores at 6.5 TB/s are 11.6 to an SM and cycle, which issues 128 lanes of instructions: 11 for each score, of which the pass takes
@@ -26,7 +28,7 @@ struct LogprobArgs {
   long long ignore_index;
   float scale;
   int top;
-  float *logprob, *entropy, *lse;
+  float *logprob, *entropy, *lse, *lse_rest;      // lse_rest: null where it is not asked for
   long long *rank;
   float *top_logprobs;
   long long *top_ids;
@@ -366,7 +368,7 @@ __global__ void __launch_bounds__(32 * W, 32 / W) logprobs_kernel(const T *__res
   const long long target = a.targets[n];
   if (target == a.ignore_index) {                                      // (the whole cluster)
     if (cta == 0 && w == 0) {
-      if (lane == 0) { a.logprob[n] = 0.f; a.entropy[n] = 0.f; a.lse[n] = 0.f; a.rank[n] = 0; }
+      if (lane == 0) { a.logprob[n] = 0.f; a.entropy[n] = 0.f; a.lse[n] = 0.f; a.rank[n] = 0; if (a.lse_rest) a.lse_rest[n] = 0.f; }
       if (TOP && lane < a.top) { a.top_logprobs[n * a.top + lane] = 0.f; a.top_ids[n * a.top + lane] = -1; }
     }
     return;
@@ -459,6 +461,7 @@ __global__ void __launch_bounds__(32 * W, 32 / W) logprobs_kernel(const T *__res
   if (lane == 0) {
     if (!known && a.errors) atomicOr(a.errors, TOK_ERR_ID);
     a.lse[n] = lse;
+    if (a.lse_rest) a.lse_rest[n] = empty ? 0.f : fmaf(g.s.r, a.scale, -lse) + log_s;
     a.entropy[n] = empty ? 0.f : log_s - g.s.T * TOK_LN2 / g.s.S;
     a.logprob[n] = known && empty ? -INFINITY : (g.mine - g.s.r) * a.scale - log_s;
     a.rank[n] = known ? 1 + (long long)g.rank : 0;
@@ -478,13 +481,13 @@ struct LogprobGradArgs {
   const long long *targets;
   long long ignore_index;
   float scale;
-  const float *lse, *entropy, *g, *h;
+  const float *lse, *lse_rest, *entropy, *g, *h;
   int *errors;
 };
 struct RowGrad {
-  float scale, lse, g, h, H;             // g, h times the scale
+  float scale, lse, rest, g, h, H;       // g, h times the scale
   __device__ __forceinline__ float at(float x) const {
-    const float logp = fmaf(x, scale, -lse), p = tok_ex2(logp * TOK_LOG2E);
+    const float logp = fmaf(x, scale, -lse) - rest, p = tok_ex2(logp * TOK_LOG2E);
     return p > 0.f || p != p ? -p * fmaf(h, logp + H, g) : 0.f;         // (p = 0: log p may be -inf)
   }
 };
@@ -517,15 +520,23 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_grad_kernel(const T *logi
   }
   const long long target = a.targets[n];
   const bool known = target >= 0 && target < a.vocab && target != a.ignore_index;
-  if (!known && target != a.ignore_index && piece == 0 && threadIdx.x == 0 && a.errors) atomicOr(a.errors, TOK_ERR_ID);
   RowGrad r;
   r.scale = a.scale;
   r.lse = a.lse[n];
+  r.rest = a.lse_rest ? a.lse_rest[n] : 0.f;
+  // an lse that is too far from zero for p, and nothing beside it
+  const bool far = known && (r.lse == INFINITY || (!a.lse_rest && fabsf(r.lse) > 1e6f && r.lse != -INFINITY));
+  if (piece == 0 && threadIdx.x == 0 && a.errors) {
+    const int bad = (known || target == a.ignore_index ? 0 : TOK_ERR_ID) | (far ? TOK_ERR_LSE : 0);
+    if (bad) atomicOr(a.errors, bad);
+  }
   r.g = a.g ? a.g[n] * a.scale : 0.f;
   r.h = a.h ? a.h[n] * a.scale : 0.f;
   r.H = a.h ? a.entropy[n] : 0.f;
-  // zeros for padding, and where a mask left nothing: -inf alone, or scores around -1e9, whose lse in fp32 says nothing about p
-  const bool none = !known || r.lse < -1e6f;
+  // zeros for padding and where a mask left nothing: -inf alone, or -1e9 and the like below an lse that has nothing beside it (masks push
+  // down; above 1e6 nothing explains the row, and it becomes NaN)
+  const bool none = !known || r.lse == -INFINITY || (far && r.lse < 0.f);
+  if (far && r.lse > 0.f) r.lse = __int_as_float(0x7fc00000);
   const int t = none ? -1 : (int)target;
 #pragma unroll
   for (int u = 0; u < LP_VECS; ++u) {
@@ -575,18 +586,24 @@ static void logprobs_type(const LogprobCall &c) {
   pbg_note_launch(cudaLaunchKernelEx(&cfg, kernel, (const T *)c.logits, c.a));
 }
 
-extern "C" int pbg_token_logprobs(const void *logits, int64_t row_stride, int64_t n, int64_t vocab, int32_t dtype, const int64_t *targets,
-                                  int64_t ignore_index, float scale, int32_t top, float *logprob, float *entropy, float *lse, int64_t *rank,
-                                  float *top_logprobs, int64_t *top_ids, int32_t *errors, void *stream) {
+extern "C" int pbg_token_logprobs_wide(const void *logits, int64_t row_stride, int64_t n, int64_t vocab, int32_t dtype, const int64_t *targets,
+                                       int64_t ignore_index, float scale, int32_t top, float *logprob, float *entropy, float *lse, float *lse_rest,
+                                       int64_t *rank, float *top_logprobs, int64_t *top_ids, int32_t *errors, void *stream) {
   if (n < 0 || vocab <= 0 || row_stride < 0 || !tok_type(dtype) || !tok_scale(scale) || top < 0 || top > vocab) return PBG_ERR_BAD_ARGUMENT;
   if (n == 0) return PBG_OK;
   if (!logits || !targets || !logprob || !entropy || !lse || !rank || (top > 0 && (!top_logprobs || !top_ids))) return PBG_ERR_BAD_ARGUMENT;
   if (top > LP_TOP_MAX || n > 0x7fffffffll || vocab > 0x7fffffffll - 65536) return PBG_ERR_TOO_LARGE;
   pbg_launch_error() = cudaSuccess;
-  const LogprobCall c{logits, n, LogprobArgs{row_stride, vocab, (const long long *)targets, ignore_index, scale, top, logprob, entropy, lse,
+  const LogprobCall c{logits, n, LogprobArgs{row_stride, vocab, (const long long *)targets, ignore_index, scale, top, logprob, entropy, lse, lse_rest,
                                              (long long *)rank, top_logprobs, (long long *)top_ids, errors}, (cudaStream_t)stream};
   TOK_DISPATCH(dtype, logprobs_type, c);
   return tok_status();
+}
+extern "C" int pbg_token_logprobs(const void *logits, int64_t row_stride, int64_t n, int64_t vocab, int32_t dtype, const int64_t *targets,
+                                  int64_t ignore_index, float scale, int32_t top, float *logprob, float *entropy, float *lse, int64_t *rank,
+                                  float *top_logprobs, int64_t *top_ids, int32_t *errors, void *stream) {
+  return pbg_token_logprobs_wide(logits, row_stride, n, vocab, dtype, targets, ignore_index, scale, top, logprob, entropy, lse, nullptr, rank, top_logprobs, top_ids,
+                                 errors, stream);
 }
 
 struct LogprobGradCall { const void *logits; void *out; long long n; LogprobGradArgs a; cudaStream_t st; };
@@ -599,16 +616,22 @@ static void logprobs_grad_type(const LogprobGradCall &c) {
   pbg_launch_in_order(kernel, dim3((unsigned)(c.n * pieces)), LP_THREADS, 0, c.st, (const T *)c.logits, (T *)c.out, c.a, (int)pieces);
 }
 
-extern "C" int pbg_token_logprobs_grad(const void *logits, int64_t row_stride, int64_t n, int64_t vocab, int32_t dtype, const int64_t *targets,
-                                       int64_t ignore_index, float scale, const float *lse, const float *entropy, const float *grad_logprob,
-                                       const float *grad_entropy, void *out, int64_t out_stride, int32_t *errors, void *stream) {
+extern "C" int pbg_token_logprobs_grad_wide(const void *logits, int64_t row_stride, int64_t n, int64_t vocab, int32_t dtype, const int64_t *targets,
+                                            int64_t ignore_index, float scale, const float *lse, const float *lse_rest, const float *entropy,
+                                            const float *grad_logprob, const float *grad_entropy, void *out, int64_t out_stride, int32_t *errors, void *stream) {
   if (n < 0 || vocab <= 0 || row_stride < 0 || out_stride < vocab || !tok_type(dtype) || !tok_scale(scale)) return PBG_ERR_BAD_ARGUMENT;
   if (n == 0) return PBG_OK;
   if (!logits || !targets || !lse || !out || (grad_entropy && !entropy)) return PBG_ERR_BAD_ARGUMENT;
   if (vocab > 0x7fffffffll - 65536 || n > 0x7fffffffll || n * ((vocab + 4095) / 4096) > 0x7fffffffll) return PBG_ERR_TOO_LARGE;
   pbg_launch_error() = cudaSuccess;
-  const LogprobGradCall c{logits, out, n, LogprobGradArgs{row_stride, out_stride, vocab, (const long long *)targets, ignore_index, scale, lse, entropy,
+  const LogprobGradCall c{logits, out, n, LogprobGradArgs{row_stride, out_stride, vocab, (const long long *)targets, ignore_index, scale, lse, lse_rest, entropy,
                                                           grad_logprob, grad_entropy, errors}, (cudaStream_t)stream};
   TOK_DISPATCH(dtype, logprobs_grad_type, c);
   return tok_status();
+}
+extern "C" int pbg_token_logprobs_grad(const void *logits, int64_t row_stride, int64_t n, int64_t vocab, int32_t dtype, const int64_t *targets,
+                                       int64_t ignore_index, float scale, const float *lse, const float *entropy, const float *grad_logprob,
+                                       const float *grad_entropy, void *out, int64_t out_stride, int32_t *errors, void *stream) {
+  return pbg_token_logprobs_grad_wide(logits, row_stride, n, vocab, dtype, targets, ignore_index, scale, lse, nullptr, entropy, grad_logprob, grad_entropy, out,
+                                      out_stride, errors, stream);
 }

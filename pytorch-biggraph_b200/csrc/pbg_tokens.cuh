@@ -12,6 +12,7 @@
 #define TOK_LN2 0.6931471805599453f
 #define TOK_ERR_ID 1                       // bits of the caller's error word
 #define TOK_ERR_TIMEOUT 2
+#define TOK_ERR_LSE 4
 
 // ex2 takes z to 2^z within 2 ulp, results below 2^-126 to 0.
 __device__ __forceinline__ float tok_ex2(float z) { float e; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z)); return e; }

@@ -85,6 +85,9 @@ SYMBOLS = [
     ("pbg_embedding_lookup_grad", C.c_int, [_P, C.c_int64, _P, C.c_int64, C.c_int64, C.c_int32, C.c_int32, C.c_float, _P, C.c_int64,
                                             C.c_int32, _P, C.c_int64, _P, _P]),
     ("pbg_token_logprobs", C.c_int, [_P, C.c_int64, C.c_int64, C.c_int64, C.c_int32, _P, C.c_int64, C.c_float, C.c_int32] + [_P] * 8),
+    ("pbg_token_logprobs_wide", C.c_int, [_P, C.c_int64, C.c_int64, C.c_int64, C.c_int32, _P, C.c_int64, C.c_float, C.c_int32] + [_P] * 9),
+    ("pbg_token_logprobs_grad_wide", C.c_int, [_P, C.c_int64, C.c_int64, C.c_int64, C.c_int32, _P, C.c_int64, C.c_float, _P, _P, _P, _P, _P, _P,
+                                               C.c_int64, _P, _P]),
     ("pbg_token_logprobs_grad", C.c_int, [_P, C.c_int64, C.c_int64, C.c_int64, C.c_int32, _P, C.c_int64, C.c_float, _P, _P, _P, _P, _P,
                                           C.c_int64, _P, _P]),
     ("pbg_table_logprobs_workspace", C.c_int64, [C.c_int64, C.c_int64, C.c_int32, C.c_int32, C.c_int32]),

@@ -8,9 +8,9 @@ that carries a forward-mode tangent.  A tensor given as `out` counts as modified
 
 All calls are queued on PyTorch's current stream of the tensors' device and return at once; workspaces come from PyTorch's allocator.
 No call synchronises, so all of them can be captured into a CUDA graph.  Ids and targets are int64.  One outside of its range
-cannot raise: its row of the result is NaN (its part of a gradient is left out), and bit 1 is set in `errors`, an
-int32 tensor of one element, where one is given (`check_errors` reads it and raises).  Results of a kernel whose bounded
-wait ran out are NaN, and bit 2 is set.
+cannot raise: a looked-up row and a log probability of it are NaN and a rank of it 0 (a row's lse and entropy, which do not depend on the
+target, are as they are), its part of a gradient is left out, and 1 is set in `errors`, an int32 tensor of one element, where
+one is given (`check_errors` reads it and raises).  Results of a kernel whose bounded wait ran out are NaN, and 2 is set.
 
 Types: float32, bfloat16, float16; sums and statistics are float32 and results rounded once."""
 import math
@@ -25,15 +25,20 @@ IGNORE_INDEX = -100
 MAX_TOP = 32
 
 
-class TokenLogprobs(NamedTuple):
-    """Per row: log probability of the target, entropy, log of the sum of exponentials (float32), rank of the target (1 = best; 0
-    for padding); with top > 0 the best log probabilities [n, top] and their ids."""
+class _TokenLogprobs(NamedTuple):
     logprob: torch.Tensor
     entropy: torch.Tensor
     lse: torch.Tensor
     rank: torch.Tensor
     top_logprobs: Optional[torch.Tensor]
     top_ids: Optional[torch.Tensor]
+
+
+class TokenLogprobs(_TokenLogprobs):
+    """Per row: log probability of the target, entropy, log of the sum of exponentials (float32), rank of the target (1 = best; 0
+    for padding); with top > 0 the best log probabilities [n, top] and their ids.  Beside these six stands the attribute lse_rest: what float32
+    cannot hold of lse, for token_logprobs_grad."""
+    lse_rest: Optional[torch.Tensor] = None
 
 
 # A call is tens of microseconds of host work or it is not: the checks below ask each tensor for as little as they can.
@@ -164,6 +169,8 @@ def check_errors(errors: torch.Tensor) -> None:
         raise _lib.PbgError(_lib.PBG_ERR_TIMEOUT, "a bounded device-side wait ran out")
     if found & 1:
         raise IndexError("an id or target lies outside of its range")
+    if found & 4:
+        raise ValueError("the lse of a row lies beyond 1e6: the gradient needs the lse_rest of the forward call")
 
 
 def embedding_lookup(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, errors: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -229,14 +236,16 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, scale: float 
     top = int(top)
     if not 0 <= top <= min(MAX_TOP, vocab):
         raise ValueError(f"top must lie between 0 and {min(MAX_TOP, vocab)}")
-    logprob, entropy, lse = torch.empty((3, n), dtype=torch.float32, device=device).unbind(0)
+    logprob, entropy, lse, lse_rest = torch.empty((4, n), dtype=torch.float32, device=device).unbind(0)
     rank = torch.empty(n, dtype=torch.long, device=device)
     best = torch.empty((n, top), dtype=torch.float32, device=device) if top else None
     best_ids = torch.empty((n, top), dtype=torch.long, device=device) if top else None
-    _call("pbg_token_logprobs", device, logits.data_ptr(), _row_stride(logits), n, vocab, code, targets.data_ptr(), int(ignore_index),
-          _scale(scale, True), top, logprob.data_ptr(), entropy.data_ptr(), lse.data_ptr(), rank.data_ptr(), _ptr(best), _ptr(best_ids),
-          _error_word(errors, device))
-    return TokenLogprobs(logprob, entropy, lse, rank, best, best_ids)
+    _call("pbg_token_logprobs_wide", device, logits.data_ptr(), _row_stride(logits), n, vocab, code, targets.data_ptr(), int(ignore_index),
+          _scale(scale, True), top, logprob.data_ptr(), entropy.data_ptr(), lse.data_ptr(), lse_rest.data_ptr(), rank.data_ptr(), _ptr(best),
+          _ptr(best_ids), _error_word(errors, device))
+    result = TokenLogprobs(logprob, entropy, lse, rank, best, best_ids)
+    result.lse_rest = lse_rest
+    return result
 
 
 def _row_grads(n, device, lse, entropy, grad_logprob, grad_entropy):
@@ -260,15 +269,21 @@ def _ptr(t):
 
 def token_logprobs_grad(logits: torch.Tensor, targets: torch.Tensor, lse: torch.Tensor, entropy: Optional[torch.Tensor],
                         grad_logprob: Optional[torch.Tensor], grad_entropy: Optional[torch.Tensor] = None, *, scale: float = 1.0,
-                        ignore_index: int = IGNORE_INDEX, out: Optional[torch.Tensor] = None, errors: Optional[torch.Tensor] = None) -> torch.Tensor:
+                        ignore_index: int = IGNORE_INDEX, out: Optional[torch.Tensor] = None, errors: Optional[torch.Tensor] = None,
+                        lse_rest: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Gradient with respect to the logits of sum(grad_logprob * logprob + grad_entropy * entropy), from the lse and the entropy that
     token_logprobs returned (the entropy only where grad_entropy is given).  `out` may be `logits` itself: the gradient then takes the scores'
-    place.  Rows of padding, rows whose target is out of range and rows of which a mask has left nothing (an lse of -inf, or below -1e6)
-    get zeros.  Probabilities are e^(z - lse): off by half a step of lse, relatively."""
+    place.  Rows of padding, rows whose target is out of range and rows of -inf alone (an lse of -inf) get zeros.
+
+    Probabilities are e^(z - lse - lse_rest).  With the lse_rest of the forward call they are exact wherever the scores lie; without it they
+    are off by half a step of lse, relatively (4e-6 for an lse of 64, 2e-3 for 65,000), and cannot be had where lse is beyond 1e6: such
+    a row sets 4 in `errors` and gets zeros below -1e6 (a mask of -1e9 that has left nothing) and NaN above 1e6."""
     code, device = _matrix("logits", logits), logits.device
     n, vocab = logits.shape
     targets = _vector("targets", targets, torch.long, n, device)
     lse, entropy, grad_logprob, grad_entropy = _row_grads(n, device, lse, entropy, grad_logprob, grad_entropy)
+    if lse_rest is not None:
+        lse_rest = _vector("lse_rest", lse_rest, torch.float32, n, device)
     if out is None:
         # rows as far apart as those of the scores, so that both lie alike against 16 bytes
         stride = max(_row_stride(logits), vocab)
@@ -282,8 +297,8 @@ def token_logprobs_grad(logits: torch.Tensor, targets: torch.Tensor, lse: torch.
         if _overlap(out, logits) and (out.data_ptr() != logits.data_ptr() or _row_stride(out) != _row_stride(logits)):
             raise ValueError("out shares memory with logits without being them")
         torch.autograd.graph.increment_version(out)
-    _call("pbg_token_logprobs_grad", device, logits.data_ptr(), _row_stride(logits), n, vocab, code, targets.data_ptr(), int(ignore_index),
-          _scale(scale, True), lse.data_ptr(), _ptr(entropy), _ptr(grad_logprob), _ptr(grad_entropy), out.data_ptr(), _row_stride(out),
+    _call("pbg_token_logprobs_grad_wide", device, logits.data_ptr(), _row_stride(logits), n, vocab, code, targets.data_ptr(), int(ignore_index),
+          _scale(scale, True), lse.data_ptr(), _ptr(lse_rest), _ptr(entropy), _ptr(grad_logprob), _ptr(grad_entropy), out.data_ptr(), _row_stride(out),
           _error_word(errors, device))
     return out
 

@@ -359,6 +359,68 @@ def test_a_mask_that_leaves_nothing_gives_no_gradient(dtype, mask):
         assert ((got[row].double() - want).abs() <= half_step(dtype) * want.abs() + 2e-4 * p[row] + 1e-6 * (1 if dtype == torch.float32 else 0)).all()
 
 
+def _exact_grad(x, targets, scale, g, h):
+    """From the scores alone, the differences to the largest one first: the gradient, and the sum of its terms' sizes."""
+    z = (x.double() - x.double().amax(1, keepdim=True)) * f32(scale)
+    logp = z - torch.logsumexp(z, 1, keepdim=True)
+    p = logp.exp()
+    hot = torch.zeros_like(p).scatter_(1, targets[:, None], 1.0)
+    plogp, H = torch.special.entr(p), torch.special.entr(p).sum(1, keepdim=True)
+    want = g.double()[:, None] * (hot - p) + h.double()[:, None] * (plogp - p * H)
+    size = g.double().abs()[:, None] * (hot + p) + h.double().abs()[:, None] * (plogp + p * H)
+    return want * f32(scale), size * f32(scale), p
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("base,scale", [(-1e30, 1.0), (-1e9, 1.0), (-1e9, 0.7), (-65_000.0, 1.0), (-300.0, 1.3), (3e4, 1.0), (1e6, 1.0), (1e6, 0.7), (1e9, 1.0), (1e30, 1.0),
+                                        (-20.0, 1e5), (20.0, 1e5), (-3.0, 1e20)])
+@pytest.mark.parametrize("n,vocab,own", [(3, 11, False), (2, 30_000, True), (150, 2051, False)])
+def test_logprobs_grad_far_from_zero(dtype, base, scale, n, vocab, own):
+    """With the rest of lse the gradient is that of the scores themselves, wherever they lie: p is off by a few roundings of log p, as around
+    zero.  Without it, p is off by half a step of lse more, and where lse is beyond 1e6 the row says so."""
+    if dtype == torch.float16 and abs(base) > 65_504:
+        base = math.copysign(6e4, base)
+    x = torch.full((n, vocab), base, device=DEV).to(dtype)
+    step = x[0, 0].float().abs().item() * torch.finfo(dtype).eps
+    if step * scale < 64:
+        x = (x.float() + torch.randint(-3, 4, (n, vocab), device=DEV, generator=gen(9)) * step).to(dtype)
+    targets = torch.randint(0, vocab, (n,), device=DEV, generator=gen(3))
+    g, h = torch.randn(n, device=DEV, generator=gen(4)) / scale, torch.randn(n, device=DEV, generator=gen(5)) / scale
+    want, size, p = _exact_grad(x, targets, scale, g, h)
+    r = T.token_logprobs(x, targets, scale=scale)
+    assert len(r) == 6 and r.lse_rest.dtype == torch.float32
+    lse = r.lse.double()
+    errors = torch.zeros(1, dtype=torch.int32, device=DEV)
+    tol, floor = half_step(dtype) * want.abs() + 2e-5 * size, torch.finfo(dtype).smallest_normal
+    to = x.clone() if own else None
+    close(T.token_logprobs_grad(to if own else x, targets, r.lse, r.entropy, g, h, scale=scale, errors=errors, lse_rest=r.lse_rest, out=to), want, 1.0, tol, floor)
+    assert errors.item() == 0
+    got = T.token_logprobs_grad(x, targets, r.lse, r.entropy, g, h, scale=scale, errors=errors)
+    if lse.abs().max() <= 1e6:
+        close(got, want, 1.0, tol + torch.expm1(2 ** -24 * 2 * lse.abs())[:, None] * size * 20, floor)   # (p log p: its own slope, below 20, more)
+        assert errors.item() == 0
+    else:
+        assert (got == 0).all() if lse.max() < 0 else got.isnan().all()
+        assert errors.item() == 4
+        with pytest.raises(ValueError, match="lse_rest"):
+            T.check_errors(errors)
+
+
+def test_rows_with_an_infinite_lse_have_no_gradient_to_give():
+    """-inf: nothing is left, zeros.  +inf, where scale times the scores leaves float32: NaN, and it is reported."""
+    x = torch.full((3, 100), -math.inf, device=DEV)
+    x[1] = 3e38
+    x[2] = torch.randn(100, device=DEV, generator=gen(1))
+    targets, g = torch.tensor([1, 2, 3], device=DEV), torch.ones(3, device=DEV)
+    r = T.token_logprobs(x, targets, scale=2.0)
+    for rest in (None, r.lse_rest):
+        errors = torch.zeros(1, dtype=torch.int32, device=DEV)
+        got = T.token_logprobs_grad(x, targets, r.lse, None, g, scale=2.0, errors=errors, lse_rest=rest)
+        assert (got[0] == 0).all() and got[1].isnan().all() and errors.item() == 4
+        want, size, _ = _exact_grad(x[2:], targets[2:], 2.0, g[2:], 0 * g[2:])
+        close(got[2:], want, 1.0, 2e-5 * size)
+
+
 @pytest.mark.parametrize("n,kind", [(7, "one"), (600, "half"), (1536, "one"), (1537, "half"), (70_000, "half")])
 def test_ids_of_padding_that_are_most_of_the_list(n, kind):
     """One id far more often than the others: the list is summed in parts, in the same order every time."""

@@ -348,8 +348,9 @@ int pbg_token_logprobs_grad_wide(const void *logits, int64_t row_stride, int64_t
                                  int32_t *errors, void *stream);
 
 /* The same statistics with z = scale * queries . table^T, which is never stored: queries [n, dim], table [rows, dim], targets rows of the
- * table.  16-bit operands are multiplied as they are; fp32 ones as two fp16 planes each (22 bits), at fp32's accuracy
- * for elements down to 2^-17 of the largest, and an absolute one of 2^-39 of it below.  NaN, or an infinity, among a
+ * table.  16-bit operands are multiplied as they are; fp32 ones as two fp16 planes each, at fp32's accuracy for elements down to
+ * 2^-17 of the largest of the same row, and an absolute one of 2^-39 of that below: neither a query nor a row of the table takes
+ * anything from another one.  (Up to sixteen fp32 queries: in fp32 throughout.)  NaN, or an infinity, among a
  * query's scores makes its entropy NaN, NaN or +inf its other results too; no other query's results change.
  * Scores are fp32 sums: beyond 1e7 in size nothing is left of their differences, and results may be NaN.
  * workspace: of pbg_table_logprobs_workspace(n, rows, dim, dtype, 0) bytes. */

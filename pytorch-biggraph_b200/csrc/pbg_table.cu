@@ -9,6 +9,8 @@
 //   fp32         every operand as two fp16 planes, x 2^k = b0 + b1 (22 bits; k from the largest finite element, so that the
 //                planes of everything down to 2^-17 of it are whole), and the three products b1 b0 + b0 b1 + b0 b0: the
 //                dropped b1 b1 is 2^-22 of a product, the size of fp32 rounding.  Half the work of three bf16 planes.
+//                Forward: k for each query and each row of the table, whose powers leave the scores as factors of a row and of a
+//                column.  One k for a whole matrix would let one large row take the bits of all others.
 //
 // One persistent kernel per product, one CTA per SM, tiles of 128 x BN (BN <= 256) or, by a pair of CTAs, 256 x BN:
 //   warp 0     TMA into a ring of stages (64 k-values of one plane, or 32 of two)
@@ -82,6 +84,7 @@ struct TabArgs {
   int BN, splits, m_first;            // tile columns; parts of the contraction; the tiles of one column go to neighbouring CTAs
   int stages, part;                   // stages of the ring; k-blocks added up in tensor memory at a time
   float scale;
+  const float *row_f, *col_f;         // EPI_STATS of fp32: what takes a product to a score in base 2, by row and by column
   const TabScales *sc;                // null: all 1
   int *err;
   float4 *parts; int nparts;          // EPI_STATS: [M][nparts] (reference in base 2, S, T)
@@ -308,6 +311,15 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
       const int cols = c0 >= g.N ? 0 : g.N - c0 < hc ? (int)(g.N - c0) : hc;
       const bool idle = m0 + q * 32 >= g.M;                              // none of these rows exists
       const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * hc);
+      // the columns' factors, for all rows of the warp
+      constexpr bool SCALED = EPI == EPI_STATS && NPB == 2;
+      float row_f = 0.f;
+      if (SCALED) {
+        __syncwarp();
+        if (4 * lane < hc) reinterpret_cast<float4 *>(buf)[lane] = reinterpret_cast<const float4 *>(g.col_f + c0)[lane];
+        if (m < g.M) row_f = g.row_f[m];
+        __syncwarp();
+      }
       // The tile's values.  PARTS: all of them, added up in registers as the accumulators fill; else read by 32 columns below.
       float sum[PARTS ? 128 : 1];
       // (the whole warp waits: one lane that does and a vote behind it take 200 cycles longer)
@@ -387,28 +399,36 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
         float v[32];
         values(x, v);
         if (EPI == EPI_STATS) {
+          const float c = SCALED ? 1.f : to2;
+          if (SCALED) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              const float4 f = reinterpret_cast<const float4 *>(buf)[(x + i) / 4];
+              v[i] *= row_f * f.x; v[i + 1] *= row_f * f.y; v[i + 2] *= row_f * f.z; v[i + 3] *= row_f * f.w;
+            }
+          }
           float cm = -INFINITY;
           const bool whole = cols - x >= 32;                               // (else columns that do not exist are left out)
 #pragma unroll
           for (int i = 0; i < 32; ++i) if (whole || i < cols - x) cm = fmaxf(cm, v[i]);
           if (cm > mx) {
             mx = cm;
-            const float d = fminf(fmaxf(r - cm * to2, -1e30f), 0.f), f = tok_ex2(d);
+            const float d = fminf(fmaxf(r - cm * c, -1e30f), 0.f), f = tok_ex2(d);
             T = (T + d * S) * f;
             S *= f;
-            r = cm * to2;
+            r = cm * c;
           }
           if (whole) {
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
-              const float y = fmaf(v[i], to2, -r), e = tok_ex2(y);
+              const float y = fmaf(v[i], c, -r), e = tok_ex2(y);
               S += e;
               T = fmaf(y, e, T);
             }
           } else {
 #pragma unroll
             for (int i = 0; i < 32; ++i) if (i < cols - x) {
-              const float y = fmaf(v[i], to2, -r), e = tok_ex2(y);
+              const float y = fmaf(v[i], c, -r), e = tok_ex2(y);
               S += e;
               T = fmaf(y, e, T);
             }
@@ -732,6 +752,10 @@ __device__ __forceinline__ float tab_power(unsigned bits, int top, float &invers
   inverse = __uint_as_float((unsigned)(127 - k) << 23);
   return __uint_as_float((unsigned)(127 + k) << 23);
 }
+__device__ __forceinline__ void tab_split(float v, __half &b0, __half &b1) {
+  b0 = __float2half_rn(v);
+  b1 = __hisinf(b0) || __hisnan(b0) ? __float2half_rn(0.f) : __float2half_rn(v - __half2float(b0));
+}
 // fp32 to two fp16 planes; 16-bit elements as they are (rows that TMA cannot read where they lie, and the gradient's queries).
 // Rows that do not count become zeros: whatever stands in padding, a product with its zero gradient is zero.
 template <class T>
@@ -762,10 +786,7 @@ __global__ void __launch_bounds__(256) tab_pack_kernel(TabPrep a) {
   const int b = of_q ? blockIdx.x : blockIdx.x - a.q.blocks;
   const float up = of_q ? up_q : up_w;
   if constexpr (sizeof(T) == 4) {
-    auto split = [&](float v, __half &b0, __half &b1) {
-      b0 = __float2half_rn(v * up);
-      b1 = __hisinf(b0) || __hisnan(b0) ? __float2half_rn(0.f) : __float2half_rn(v * up - __half2float(b0));
-    };
+    auto split = [&](float v, __half &b0, __half &b1) { tab_split(v * up, b0, b1); };
     __half *p0 = (__half *)s.to, *p1 = p0 + s.plane;
     if (a.wide) tab_units<float4>(a, s, b, [&](long long r, int i, const float4 &v) {
       __align__(8) __half h0[4], h1[4];
@@ -777,6 +798,64 @@ __global__ void __launch_bounds__(256) tab_pack_kernel(TabPrep a) {
   } else {
     if (a.wide) tab_units<uint4>(a, s, b, [&](long long r, int i, const uint4 &v) { ((uint4 *)((T *)s.to + r * s.ld))[i] = v; });
     else tab_units<unsigned short>(a, s, b, [&](long long r, int i, unsigned short v) { ((unsigned short *)s.to)[r * s.ld + i] = v; });
+  }
+}
+// Rows of fp32 to two fp16 planes, each times the power of two that brings its own largest finite element below 2^14; `factors` takes what
+// undoes it, times `factor`.  `group` threads to a row (up to the whole CTA), which stays in registers up to 8 units to a thread and is read
+// again from there on.  Rows that do not count become zeros.
+template <class U>
+__global__ void __launch_bounds__(256) tab_rows_kernel(TabSource s, int dim, int group, float factor, float *factors) {
+  __shared__ unsigned tops[8];
+  pdl_begin();
+  constexpr int V = sizeof(U) / 4;
+  const int sub = threadIdx.x % group, units = dim / V;
+  const long long per = 256 / group;
+  __half *p0 = (__half *)s.to, *p1 = p0 + s.plane;
+  for (long long r0 = blockIdx.x * per; r0 < s.rows; r0 += gridDim.x * per) {
+    const long long r = r0 + threadIdx.x / group;
+    const bool there = r < s.rows, counts = there && s.counts(r);
+    const U *row = (const U *)((const float *)s.x + r * s.stride);
+    U v[8];
+    auto load = [&](int i0) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) { v[k] = U{}; if (counts && i0 + k * group < units) v[k] = row[i0 + k * group]; }
+    };
+    unsigned top = 0u;
+    for (int i0 = sub; i0 < units; i0 += 8 * group) {
+      load(i0);
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const unsigned bits = __float_as_uint(reinterpret_cast<const float *>(&v[k])[e]) & 0x7fffffffu;
+          if (bits < 0x7f800000u) top = max(top, bits);
+        }
+    }
+    for (int o = group < 32 ? group / 2 : 16; o > 0; o /= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (group > 32) {
+      const int w = threadIdx.x / 32, warps = group / 32;
+      if (threadIdx.x % 32 == 0) tops[w] = top;
+      __syncthreads();
+      for (int k = w / warps * warps; k < (w / warps + 1) * warps; ++k) top = max(top, tops[k]);
+      __syncthreads();
+    }
+    float inverse;
+    const float up = tab_power(top, 14, inverse);
+    if (there && sub == 0) factors[r] = inverse * factor;
+    for (int i0 = sub; i0 < units; i0 += 8 * group) {
+      if (units > 8 * group) load(i0);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (!there || i0 + k * group >= units) continue;
+        __align__(8) __half h0[V], h1[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) tab_split(reinterpret_cast<const float *>(&v[k])[e] * up, h0[e], h1[e]);
+        if (V == 4) {
+          reinterpret_cast<uint2 *>(p0 + r * s.ld)[i0 + k * group] = *reinterpret_cast<uint2 *>(h0);
+          reinterpret_cast<uint2 *>(p1 + r * s.ld)[i0 + k * group] = *reinterpret_cast<uint2 *>(h1);
+        } else { p0[r * s.ld + i0 + k * group] = h0[0]; p1[r * s.ld + i0 + k * group] = h1[0]; }
+      }
+    }
   }
 }
 // The parts of a split contraction, added in their order.
@@ -907,7 +986,7 @@ static bool tab_packed(const void *p, long long stride, int dim, int dtype) { re
 // What the workspace holds.  Its size is asked for without addresses, so it has room for packed operands wherever they may be needed.
 #define TAB_MAX_BLOCKS 2048                                  // of a preparing kernel
 struct TabPlace {
-  int64_t scales, block_max, q, w, parts, dz, partial, bytes;
+  int64_t scales, block_max, q, w, row_f, col_f, parts, dz, partial, bytes;
   long long ld, columns, ldz;         // packed rows' length; table rows per piece of dz, and its rows' length
   long long piece;                    // queries per pass of the forward
   int npl, bn, nparts, splits, dz_planes;
@@ -923,6 +1002,9 @@ static TabPlace tab_place(long long n, long long rows, int dim, int dtype, bool 
   p.q = p.block_max + TAB_MAX_BLOCKS * 4;
   p.w = p.q + tok_up(n * p.ld * 2 * p.npl, 256);
   int64_t at = p.w + tok_up(rows * p.ld * 2 * p.npl, 256);
+  p.row_f = at;
+  p.col_f = p.row_f + tok_up(n * 4, 256);
+  if (!grad && dtype == PBG_F32) at = p.col_f + tok_up(rows, 256) * 4;      // (whole tiles of columns are read)
   p.parts = p.dz = p.partial = at;
   p.columns = p.ldz = 0;
   p.piece = n;
@@ -1001,6 +1083,25 @@ static void tab_prepare(TabCall &c, const TabPlace &p, bool grad, const float *g
   pbg_launch(tab_pack_kernel<T>, dim3(a.q.blocks + a.w.blocks), 256, 0, c.st, a);
 }
 
+// The same for the forward pass of fp32 operands.  (The factors carry half of the scale's power each: their product is one of a score.)
+static void tab_prepare_rows(TabCall &c, const TabPlace &p) {
+  c.sc = nullptr;
+  c.err = c.errors ? c.errors : (int *)(c.ws + p.scales + 128);
+  const float to2 = c.scale * TOK_LOG2E, half = ldexpf(1.f, ilogbf(to2) / 2);
+  auto rows = [&](TabOperand &o, const void *x, long long stride, long long rows, int64_t at, float factor, int64_t factors, const TabRows &counts) {
+    const bool wide = c.dim % 4 == 0 && stride % 4 == 0 && aligned16(x);
+    const int units = wide ? c.dim / 4 : c.dim;
+    int group = 1;
+    while (group < 256 && group * 8 < units) group *= 2;
+    TabSource s = {x, stride, rows, counts, 0, c.ws + at, p.ld, rows * p.ld};
+    const long long ctas = (rows + 256 / group - 1) / (256 / group), most = 8 * pbg_sm_count();
+    pbg_launch(wide ? tab_rows_kernel<float4> : tab_rows_kernel<float>, dim3((unsigned)(ctas < most ? ctas : most)), 256, 0, c.st, s, c.dim, group, factor, (float *)(c.ws + factors));
+    o = TabOperand{s.to, rows, c.dim, p.ld, s.plane, 2, true};
+  };
+  rows(c.q, c.queries, c.q_stride, c.n, p.q, half, p.row_f, TabRows{c.targets, c.ignore_index, c.rows, 1});
+  rows(c.w, c.table, c.t_stride, c.rows, p.w, to2 / half, p.col_f, TabRows{nullptr, 0, 0, 1});
+}
+
 static bool tab_few(long long n, int dim, int dtype) {
   if (dtype != PBG_F32 || n > TAB_FEW) return false;
   long long nq = 1;
@@ -1036,7 +1137,8 @@ static void tab_forward(TabForward &f) {
     finish(0, c.n);
     return;
   }
-  tab_prepare<T>(c, f.p, false, nullptr, nullptr);
+  if (MATH::NPB == 2) tab_prepare_rows(c, f.p);
+  else tab_prepare<T>(c, f.p, false, nullptr, nullptr);
   constexpr int KB = MATH::NPA == 1 ? 64 : 32;
   for (long long n0 = 0; n0 < c.n && f.ok; n0 += f.p.piece) {
     const long long n = c.n - n0 < f.p.piece ? c.n - n0 : f.p.piece;
@@ -1046,7 +1148,7 @@ static void tab_forward(TabForward &f) {
     TabArgs g = {};
     g.M = n; g.N = c.rows; g.kblocks = (int)((c.dim + KB - 1) / KB);
     g.BN = f.p.bn; g.splits = 1; g.m_first = 1; g.scale = c.scale; g.sc = c.sc; g.err = c.err;
-    g.by_q = g.by_w = 1;
+    g.row_f = (const float *)(c.ws + f.p.row_f) + n0; g.col_f = (const float *)(c.ws + f.p.col_f);
     g.parts = (float4 *)(c.ws + f.p.parts); g.nparts = f.p.nparts;
     f.ok = tab_launch<EPI_STATS, MATH, false, false>(q, c.w, g, f.p.pairs, c.st);
     finish(n0, n);

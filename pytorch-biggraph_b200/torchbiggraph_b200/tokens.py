@@ -325,8 +325,8 @@ def table_logprobs(queries: torch.Tensor, table: torch.Tensor, targets: torch.Te
                    errors: Optional[torch.Tensor] = None) -> TableLogprobs:
     """Log probabilities of rows `targets` [n] of the table under softmax(scale * queries . table^T), with the entropies and logs of the
     sums; the n x rows scores are never stored.  What token_logprobs(queries @ table.T, targets) gives, at the accuracy of
-    float32 sums over the operands as they are (float32 operands are multiplied at 22 bits and more).  Queries
-    whose target is ignore_index are padding: 0.  NaN, or +inf, among a query's scores makes its results NaN
+    float32 sums over the operands as they are (float32 operands are multiplied at 22 bits and more where they reach 2^-17 of the largest
+    element of their own row; what other rows hold does not matter).  Queries whose target is ignore_index are padding: 0.  NaN, or +inf, among a query's scores makes its results NaN
     (-inf its entropy), no other query's.  Scores are float32 sums: of differences between scores beyond 1e7 nothing is left."""
     code, n, rows, dim, targets = _queries_and_table(queries, table, targets)
     device = queries.device

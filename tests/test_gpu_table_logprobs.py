@@ -397,3 +397,46 @@ def test_a_wait_that_runs_out_leaves_nan(dtype, n, rows, dim):
     r = T.table_logprobs(q, t, targets, errors=errors)
     assert all(torch.equal(a, b) for a, b in zip(r, want))
     assert all(torch.equal(a, b) for a, b in zip(T.table_logprobs_grad(q, t, targets, want.lse, want.entropy, g, g, errors=errors), want_grad)) and errors.item() == 0
+
+
+def uneven(n, dim, big, rows=2000):
+    """Inputs among which one query and one row of the table are far larger than the rest (the row where no query looks), one of each far smaller; the
+    bound E on the others' scores is that of the others."""
+    q, t, targets = inputs(n, rows, dim, torch.float32, n + dim)
+    q[:, 0] = q[:, 0].abs() + 0.1
+    t[7] = 0
+    t[7, 0] = -big
+    t[11] /= big
+    targets[(targets == 7) | (targets == 11)] = 12
+    q[5] /= big
+    z, E = scores(q, torch.cat((t[:7], t[8:])), 1.0)
+    q[3] *= big
+    keep = torch.arange(n, device=DEV) != 3
+    return q, t, targets, keep, torch.cat((z[:, :7], -big * q[:, :1].double(), z[:, 7:]), 1)[keep], E[keep]
+
+
+@pytest.mark.parametrize("big", [1e4, 1e8, 1e12, 1e30])
+@pytest.mark.parametrize("n,dim", [(16, 72), (17, 72), (17, 400), (140, 33), (1000, 400), (20, 2501), (20, 2052), (20, 9004)])
+def test_a_large_row_takes_nothing_from_the_others(n, dim, big):
+    """Forward, fp32: what a query gets depends neither on another query's size nor on that of a row it has no score for."""
+    q, t, targets, keep, z, E = uneven(n, dim, big)
+    r = T.table_logprobs(q, t, targets)
+    logprob, ent, lse = want_forward(z, targets[keep])
+    tol = E + 2e-5 * (1 + lse.abs())
+    assert ((r.lse[keep].double() - lse).abs() <= tol).all()
+    assert ((r.logprob[keep].double() - logprob).abs() <= 2 * tol + 2e-5 * logprob.abs()).all()
+    assert ((r.entropy[keep].double() - ent).abs() <= 80 * E + 2e-5 * (1 + ent + math.log(len(t)))).all()
+
+
+def test_float32_queries_in_pieces():
+    """More partial sums than the workspace holds at once: every piece takes its own rows' powers of two."""
+    n, rows = 150_000, 70_000
+    q, t, targets = inputs(n, rows, 8, torch.float32, 3)
+    q *= torch.exp(torch.arange(n, device=DEV) % 9 - 4.0)[:, None]
+    r = T.table_logprobs(q, t, targets, scale=0.5)
+    some = torch.cat((torch.arange(0, n, 2999, device=DEV), torch.tensor([n - 1], device=DEV)))
+    z, E = scores(q[some], t, 0.5)
+    logprob, ent, lse = want_forward(z, targets[some])
+    assert ((r.lse[some].double() - lse).abs() <= E + 2e-5 * (1 + lse.abs())).all()
+    assert ((r.logprob[some].double() - logprob).abs() <= 2 * (E + 2e-5 * (1 + lse.abs())) + 2e-5 * logprob.abs()).all()
+    assert ((r.entropy[some].double() - ent).abs() <= 80 * E + 2e-5 * (1 + ent + math.log(rows))).all()

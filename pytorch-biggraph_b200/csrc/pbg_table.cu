@@ -6,11 +6,13 @@
 // All products run on the tensor cores (tcgen05, kind::f16) with fp32 accumulators in tensor memory:
 //   bf16, fp16   the tensors themselves are the operands, read by TMA where they lie; dz is rounded to the operands' type (that of
 //                fp16 scaled by a power of two so that it cannot leave the type's range: its bound is known from g and h)
-//   fp32         every operand as two fp16 planes, x 2^k = b0 + b1 (22 bits; k from the largest finite element, so that the
-//                planes of everything down to 2^-17 of it are whole), and the three products b1 b0 + b0 b1 + b0 b0: the
-//                dropped b1 b1 is 2^-22 of a product, the size of fp32 rounding.  Half the work of three bf16 planes.
-//                Forward: k for each query and each row of the table, whose powers leave the scores as factors of a row and of a
-//                column.  One k for a whole matrix would let one large row take the bits of all others.
+//   fp32         scores: every operand as two fp16 planes, x 2^k = b0 + b1 (22 bits; k from the largest finite element of its row, so
+//                that the planes of everything down to 2^-17 of it are whole), and the three products b1 b0 + b0 b1 + b0 b0: the dropped
+//                b1 b1 is 2^-22 of a product, the size of fp32 rounding.  The powers leave the scores as factors of a row and of a column;
+//                one k for a whole matrix would let one large row take the bits of all others.
+//                Products with dz: three bf16 planes (24 bits) and six products.  Their sums run over the table's rows or over the
+//                queries, whose powers are no factors of them, and dz spans more binades than fp16 has: bf16 has fp32's range, so that
+//                elements, rows of dz with a small g and columns that no query comes near keep their bits down to 2^-150 of the largest.
 //
 // One persistent kernel per product, one CTA per SM, tiles of 128 x BN (BN <= 256) or, by a pair of CTAs, 256 x BN:
 //   warp 0     TMA into a ring of stages (64 k-values of one plane, or 32 of two)
@@ -33,6 +35,7 @@
 // Every wait is bounded: one that runs out sets bit 2 of the error word, the CTA's products stop, and whatever it had still to
 // write is NaN -- partial sums, dz or results, so that all results that depend on them are NaN too; then it frees its tensor memory
 // and returns.
+#include <algorithm>
 #include <atomic>
 #include <type_traits>
 
@@ -46,14 +49,14 @@ enum { EPI_STATS = 0, EPI_DZ = 1, EPI_OUT = 2 };
 #define TAB_PARTS_BYTES (512ll << 20)                       // and for the tiles' partial sums: beyond it the queries do
 // The tensor cores cut off what they add up instead of rounding it, a bias of half a step per addition.  Where results are fp32 the
 // contraction is therefore cut into parts, which are added in registers: blocks of k-values per part, for scores of fp32 operands (36
-// additions to a part; with 18 the epilogue could not keep up), for products with their gradient (18), for that gradient, whose
-// epilogue has more to do (48), and for scores of 16-bit operands (32) of more than TAB_WHOLE elements.  Products of 5000 fp32 terms were 3.9e-5 off in one piece and are 5e-7 off in parts.  Scores of
-// 2048 16-bit terms are 8e-7 off in one piece and 2e-7 in parts; the registers that the parts take cost 7 queries x
-// 131,072 x 2048 bf16 12 of 102 us, so that these are left whole.
+// additions to a part in the forward pass, where with 18 the epilogue could not keep up, 48 in the gradient), for the products with
+// their gradient (24), and for scores of 16-bit operands (32) of more than TAB_WHOLE elements.  Products of 5000 fp32 terms were 3.9e-5
+// off in one piece and are 5e-7 off in parts.  Scores of 2048 16-bit terms are 8e-7 off in one piece and 2e-7 in parts; the registers that
+// the parts take cost 7 queries x 131,072 x 2048 bf16 12 of 102 us, so that these are left whole.
 // 16-bit gradients are cut up too where half a step per addition comes near the result's own: 2^21 terms of one sign in one piece
 // were 1 % off; a part of TAB_PART_LONG blocks is 2^-13 off at most.
 #define TAB_PART_F32 6
-#define TAB_PART_F32_OUT 3
+#define TAB_PART_F32_OUT 2
 #define TAB_PART_F32_DZ 8
 #define TAB_PART_16 8
 #define TAB_WHOLE 2048
@@ -63,18 +66,23 @@ enum { EPI_STATS = 0, EPI_DZ = 1, EPI_OUT = 2 };
 // rest.  (Sixteen warps with half the columns each had registers for half of what they need and were slower.)
 #define TAB_EPI_WARPS 8
 #define TAB_THREADS (64 + 32 * TAB_EPI_WARPS)
-#define TAB_RING_BYTES 196608
-#define TAB_SMEM (1024 + TAB_RING_BYTES + TAB_EPI_WARPS * 4096)
+#define TAB_SMEM 230400
+// (three planes of dz take 6, and the factors of 128 columns stand behind them)
+template <int EPI, class MATH> struct TabSmem {
+  static constexpr int OUT = EPI == EPI_DZ && MATH::NPB == 2 ? 6144 + 512 : 4096, RING = TAB_SMEM - 1024 - TAB_EPI_WARPS * OUT;
+};
 
 // Operands: their elements, the planes of A and B, the type of results
-template <class E, class O, int PA, int PB> struct TabMath { using elem = E; using out = O; static constexpr int NPA = PA, NPB = PB; };
+template <class E, class O, int PA, int PB, class DZ = E> struct TabMath { using elem = E; using out = O; using dz = DZ; static constexpr int NPA = PA, NPB = PB; };
 using TabBf16 = TabMath<__nv_bfloat16, __nv_bfloat16, 1, 1>;
 using TabF16 = TabMath<__half, __half, 1, 1>;
-using TabF32 = TabMath<__half, float, 2, 2>;
+using TabF32 = TabMath<__half, float, 2, 2, __nv_bfloat16>;               // scores, whose dz has three bf16 planes
+using TabF32Out = TabMath<__nv_bfloat16, float, 3, 3>;
 using TabBf16Fine = TabMath<__nv_bfloat16, __nv_bfloat16, 2, 1>;          // dz in two planes
 using TabF16Fine = TabMath<__half, __half, 2, 1>;
 
-// Powers of two that the operands were multiplied by, and their inverses
+// Powers of two that the operands were multiplied by, and their inverses: fp32 operands and their dz, to below 2^40 (products of two and
+// sums of 2^31 of them stay in fp32); dz of fp16 operands, to below 2^14
 struct TabScales { float q, w, dz, iq, iw, idz; };
 
 struct TabMaps { CUtensorMap a, b, c; };                              // operands; what is written by bulk stores
@@ -84,7 +92,7 @@ struct TabArgs {
   int BN, splits, m_first;            // tile columns; parts of the contraction; the tiles of one column go to neighbouring CTAs
   int stages, part;                   // stages of the ring; k-blocks added up in tensor memory at a time
   float scale;
-  const float *row_f, *col_f;         // EPI_STATS of fp32: what takes a product to a score in base 2, by row and by column
+  const float *row_f, *col_f;         // scores of fp32 operands: what takes a product to a score in base 2, by row and by column
   const TabScales *sc;                // null: all 1
   int *err;
   float4 *parts; int nparts;          // EPI_STATS: [M][nparts] (reference in base 2, S, T)
@@ -94,7 +102,7 @@ struct TabArgs {
   void *out; long long ldo;           // EPI_DZ: dz; EPI_OUT: the result, or
   float *partial; int add;            //          [splits][M][N] fp32, stored or added
   int bulk;                           //          either way by bulk stores
-  int by_q, by_w, by_dz;              // which powers the product carries
+  int by_q;                           // EPI_OUT: the other operand is the queries
   int a_rows;                         // rows of A that are loaded: 128, or fewer where there is one row tile and nothing to fill it with
   int b_whole;                        // MN-major B: its rows are whole blocks of 64 columns, read as one box
   int wait_limit;                     // how often a wait asks before it gives up
@@ -145,13 +153,14 @@ template <int EPI, class MATH, bool A_MN, bool B_MN, int CG, bool PARTS>        
 __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_constant__ TabMaps maps, TabArgs g) {
   using Elem = typename MATH::elem;
   using Out = typename MATH::out;
+  using Dz = typename MATH::dz;
   constexpr int NPA = MATH::NPA, NPB = MATH::NPB, KB = NPA == 1 ? 64 : 32;
   constexpr uint32_t FMT = std::is_same<Elem, __nv_bfloat16>::value ? 1u : 0u;
   constexpr uint32_t ROW_BYTES = KB * 2, ATOM_BYTES = KB * 128;          // a K-major row; 64 columns of an MN-major operand's plane
   constexpr uint32_t A_BYTES = NPA * 128 * ROW_BYTES;
   extern __shared__ unsigned char smem_raw[];
   unsigned char *smem = (unsigned char *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  unsigned char *ostage = smem + TAB_RING_BYTES;
+  unsigned char *ostage = smem + TabSmem<EPI, MATH>::RING;
   __shared__ __align__(8) unsigned long long bars[2 * TAB_STAGES_MAX + 4];
   __shared__ uint32_t tmem_base_s;
   __shared__ volatile int failed;
@@ -231,7 +240,7 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
       }
     }
   } else if (warp == 1) {
-    // ---------------- products.  D fp32; both operands of one type; planes (a, b): b1 b0, b0 b1, b0 b0
+    // ---------------- products.  D fp32; both operands of one type; the smallest planes' products first, (0, 0) last
     const uint32_t idesc = (1u << 4) | (FMT << 7) | (FMT << 10) | ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16) |
                            ((uint32_t)(g.BN >> 3) << 17) | ((uint32_t)(128 * CG >> 4) << 24);
     // K-major: 128-byte rows in the 128-byte swizzle (layout 2) or 64-byte rows in the 64-byte one (layout 4), 32 bytes per 16 k-values;
@@ -263,10 +272,15 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
           if (leader) {
 #pragma unroll
             for (int k = 0; k < KB / 16; ++k) {
-              const bool more = k > 0 || kb > p0;
-              if (NPA == 2) tab_mma<CG>(acc, desc_at(da, a_plane + k * a_step), desc_at(db, k * b_step), idesc, more);
-              if (NPB == 2) tab_mma<CG>(acc, desc_at(da, k * a_step), desc_at(db, b_plane + k * b_step), idesc, true);
-              tab_mma<CG>(acc, desc_at(da, k * a_step), desc_at(db, k * b_step), idesc, NPA == 2 || more);
+              bool more = k > 0 || kb > p0;
+#pragma unroll
+              for (int sum = (NPA > NPB ? NPA : NPB) - 1; sum >= 0; --sum)
+#pragma unroll
+                for (int pa = sum; pa >= 0; --pa) {
+                  if (pa >= NPA || sum - pa >= NPB) continue;
+                  tab_mma<CG>(acc, desc_at(da, pa * a_plane + k * a_step), desc_at(db, (sum - pa) * b_plane + k * b_step), idesc, more);
+                  more = true;
+                }
             }
             tab_commit<CG>(empty_bar(at.s));
           }
@@ -278,15 +292,20 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
   } else {
     // ---------------- epilogue
     const int q = warp & 3, half = (warp - 2) >> 2, hc = g.BN / 2;       // 32 rows of the tile; half of its columns
-    unsigned char *buf = ostage + (size_t)(warp - 2) * 4096;
+    unsigned char *buf = ostage + (size_t)(warp - 2) * TabSmem<EPI, MATH>::OUT;
     const uint32_t drained = CG == 1 ? 0u : in_first_cta(acce_bar(0));
-    float unscale = 1.f, up = g.scale;
+    // what a result is multiplied by (two factors where one could leave fp32), and a score's way to base 2
+    float unscale = 1.f, unscale2 = 1.f, up = 1.f;
+    const float to2 = g.scale * TOK_LOG2E;
     if (g.sc) {
-      unscale = (g.by_q ? g.sc->iq : 1.f) * (g.by_w ? g.sc->iw : 1.f) * (g.by_dz ? g.sc->idz : 1.f);
-      up *= g.sc->dz;
+      up = g.sc->dz;
+      const float iop = g.by_q ? g.sc->iq : g.sc->iw;
+      unscale = NPB == 3 ? fminf(iop, g.sc->idz) : iop * g.sc->idz;      // (the smaller one first)
+      unscale2 = fmaxf(iop, g.sc->idz);
     }
-    const float to2 = g.scale * unscale * TOK_LOG2E;                      // from an accumulator to a score in base 2
-    const int planes = NPB == 2 ? 2 : g.dz_planes;
+    auto result = [&](float v) { return NPB == 3 ? v * unscale * unscale2 : v * unscale; };
+    constexpr int MOST_PLANES = NPB == 2 ? 3 : 2;
+    const int planes = NPB == 2 ? 3 : g.dz_planes;
     int j = 0;
     bool ok = true;
     long long t = first;
@@ -302,8 +321,8 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
         const long long target = g.targets[m];
         if (target >= 0 && target < g.vocab && target != g.ignore_index) {
           lse = g.lse[m] * TOK_LOG2E;
-          if (g.g) g0 = gg = g.g[m] * up;
-          if (g.h) { const float h = g.h[m] * up; hh = h * TOK_LN2; gg = fmaf(h, g.entropy[m], gg); }
+          if (g.g) g0 = gg = g.g[m] * g.scale * up;
+          if (g.h) { const float h = g.h[m] * g.scale * up; hh = h * TOK_LN2; gg = fmaf(h, g.entropy[m], gg); }
           hot = target - g.v0;
         } else if (target != g.ignore_index && n0 == 0 && half == 0 && g.v0 == 0) atomicOr(g.err, TOK_ERR_ID);
       }
@@ -312,11 +331,12 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
       const bool idle = m0 + q * 32 >= g.M;                              // none of these rows exists
       const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * hc);
       // the columns' factors, for all rows of the warp
-      constexpr bool SCALED = EPI == EPI_STATS && NPB == 2;
+      constexpr bool SCALED = EPI != EPI_OUT && NPB == 2;
+      float4 *cols_f = reinterpret_cast<float4 *>(buf + (EPI == EPI_DZ ? 6144 : 0));
       float row_f = 0.f;
       if (SCALED) {
         __syncwarp();
-        if (4 * lane < hc) reinterpret_cast<float4 *>(buf)[lane] = reinterpret_cast<const float4 *>(g.col_f + c0)[lane];
+        if (4 * lane < hc) cols_f[lane] = reinterpret_cast<const float4 *>(g.col_f + c0)[lane];
         if (m < g.M) row_f = g.row_f[m];
         __syncwarp();
       }
@@ -398,15 +418,15 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
         if (x >= span || idle) break;
         float v[32];
         values(x, v);
-        if (EPI == EPI_STATS) {
-          const float c = SCALED ? 1.f : to2;
-          if (SCALED) {
+        const float c = SCALED ? 1.f : to2;                              // from here to a score in base 2
+        if (SCALED) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              const float4 f = reinterpret_cast<const float4 *>(buf)[(x + i) / 4];
-              v[i] *= row_f * f.x; v[i + 1] *= row_f * f.y; v[i + 2] *= row_f * f.z; v[i + 3] *= row_f * f.w;
-            }
+          for (int i = 0; i < 32; i += 4) {
+            const float4 f = cols_f[(x + i) / 4];
+            v[i] *= row_f * f.x; v[i + 1] *= row_f * f.y; v[i + 2] *= row_f * f.z; v[i + 3] *= row_f * f.w;
           }
+        }
+        if (EPI == EPI_STATS) {
           float cm = -INFINITY;
           const bool whole = cols - x >= 32;                               // (else columns that do not exist are left out)
 #pragma unroll
@@ -421,14 +441,14 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
           if (whole) {
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
-              const float y = fmaf(v[i], c, -r), e = tok_ex2(y);
+              const float y = tok_max_nan(fmaf(v[i], c, -r), -1000.f), e = tok_ex2(y);
               S += e;
               T = fmaf(y, e, T);
             }
           } else {
 #pragma unroll
             for (int i = 0; i < 32; ++i) if (i < cols - x) {
-              const float y = fmaf(v[i], c, -r), e = tok_ex2(y);
+              const float y = tok_max_nan(fmaf(v[i], c, -r), -1000.f), e = tok_ex2(y);
               S += e;
               T = fmaf(y, e, T);
             }
@@ -438,7 +458,9 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
           // a row that does not count is a query of zeros: its score is 0, and with lse = gg = hh = 0 so is its dz
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
-            const float y = fmaf(v[i], to2, -lse), p = tok_ex2(y);       // log p and p, in base 2
+            // log p and p, in base 2.  p is 0 for a score of -inf, and never above 1, however little the score and lse share where both are large
+            // (a query of 1e12 with a gradient of 0 adds 0 to the table's)
+            const float y = tok_min_nan(tok_max_nan(fmaf(v[i], c, -lse), -1000.f), 0.f), p = tok_ex2(y);
             v[i] = -p * fmaf(hh, y, gg);
           }
           if (__any_sync(0xffffffffu, hot >= col && hot < col + 32)) {
@@ -452,7 +474,7 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
           // planes of 32 x 32 values through shared memory (64-byte swizzle); each leaves as one bulk store, clipped at the last row
           store_ready();
 #pragma unroll
-          for (int pl = 0; pl < 2; ++pl) {
+          for (int pl = 0; pl < MOST_PLANES; ++pl) {
             if (pl >= planes) break;
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
@@ -460,8 +482,8 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 float &a = v[8 * u + 2 * i], &b = v[8 * u + 2 * i + 1];
-                const typename TokPair<Elem>::type e = TokPair<Elem>::down(a, b);
-                if (pl == 0) { const float2 f = TokPair<Elem>::up(e); a -= f.x; b -= f.y; }          // what the second plane holds
+                const typename TokPair<Dz>::type e = TokPair<Dz>::down(a, b);
+                if (pl < MOST_PLANES - 1) { const float2 f = TokPair<Dz>::up(e); a -= f.x; b -= f.y; }      // what the next plane holds
                 w[i] = *reinterpret_cast<const uint32_t *>(&e);
               }
               *reinterpret_cast<uint4 *>(buf + pl * 2048 + lane * 64 + ((u ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -485,7 +507,7 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
           const long long col = c0 + x + lane;
           if (x + lane < cols) {
             for (int r0 = 0; r0 < rows; ++r0) {
-              const float val = *reinterpret_cast<float *>(buf + r0 * 128 + (((lane >> 2) ^ (r0 & 7)) << 4) + ((lane & 3) << 2)) * unscale;
+              const float val = result(*reinterpret_cast<float *>(buf + r0 * 128 + (((lane >> 2) ^ (r0 & 7)) << 4) + ((lane & 3) << 2)));
               const long long row = m0 + q * 32 + r0;
               if (g.partial) {
                 float *to = g.partial + ((long long)split * g.M + row) * g.N + col;
@@ -498,7 +520,7 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
           store_ready();
 #pragma unroll
           for (int u = 0; u < 8; ++u)
-            *reinterpret_cast<float4 *>(buf + lane * 128 + ((u ^ (lane & 7)) << 4)) = make_float4(v[4 * u] * unscale, v[4 * u + 1] * unscale, v[4 * u + 2] * unscale, v[4 * u + 3] * unscale);
+            *reinterpret_cast<float4 *>(buf + lane * 128 + ((u ^ (lane & 7)) << 4)) = make_float4(result(v[4 * u]), result(v[4 * u + 1]), result(v[4 * u + 2]), result(v[4 * u + 3]));
           store_go((int)(c0 + x), (int)(m0 + q * 32), split, rows > 0);
         } else {
           // 16-bit results: 64 columns to a row of 128 bytes
@@ -508,7 +530,7 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
             uint32_t w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const auto e = TokPair<Elem>::down(v[8 * u + 2 * i] * unscale, v[8 * u + 2 * i + 1] * unscale);
+              const auto e = TokPair<Elem>::down(result(v[8 * u + 2 * i]), result(v[8 * u + 2 * i + 1]));
               w[i] = *reinterpret_cast<const uint32_t *>(&e);
             }
             *reinterpret_cast<uint4 *>(buf + lane * 128 + (((u + (x & 32) / 8) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -529,7 +551,7 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
       if (m >= g.M) continue;
       if (EPI == EPI_STATS) g.parts[m * g.nparts + n0 / g.BN * 2 + half] = make_float4(0.f, nan, nan, 0.f);
       else for (long long c = c0; c < c1; ++c) {
-        if (EPI == EPI_DZ) for (int pl = 0; pl < planes; ++pl) ((Elem *)g.out)[(pl * g.M + m) * g.ldz + c] = Tok<Elem>::down(nan);
+        if (EPI == EPI_DZ) for (int pl = 0; pl < planes; ++pl) ((Dz *)g.out)[(pl * g.M + m) * g.ldz + c] = Tok<Dz>::down(nan);
         else if (g.partial) g.partial[((long long)split * g.M + m) * g.N + c] = nan;
         else ((Out *)g.out)[m * g.ldo + c] = Tok<Out>::down(nan);
       }
@@ -690,7 +712,8 @@ struct TabPrep {
   const float *g, *h; long long n; int gblocks;            // gblocks 0: dz is not scaled
   float scale; int dim, planes, wide;                      // wide: rows of whole 16-byte vectors on 16-byte boundaries
   FastDiv by_units;                                        // units of a row: vectors, or elements
-  unsigned *block_max; TabScales *sc;
+  unsigned *block_max; int max_q, max_w;                   // the largest elements of parts of the queries, of the table, and of dz's bound
+  TabScales *sc;
 };
 
 // Hands the units of type U of a CTA's rows (those that do not count as zeros) to a function (row, unit, value), four in flight.
@@ -715,35 +738,31 @@ __device__ __forceinline__ void tab_units(const TabPrep &a, const TabSource &s, 
     for (int k = 0; k < 4; ++k) if (i0 + k * 256 < total) f(row[k], at[k], v[k]);
   }
 }
-// Largest finite |x| that each CTA has seen: of the queries, of the table, of the bound of dz / scale:
-// |g| + |h| (p |log p| + p H), p |log p| <= 1 / e, H <= log rows < 22.
-__global__ void __launch_bounds__(256) tab_max_kernel(TabPrep a) {
-  __shared__ unsigned tops[8];
-  pdl_begin();
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  int b = blockIdx.x;
+// The bound of dz / scale: |g| + |h| (p |log p| + p H), p |log p| <= 1 / e, H <= log rows < 22.  The largest finite one of a CTA's queries,
+// bit by bit (of a thread).
+__device__ __forceinline__ unsigned tab_dz_bound(const float *g, const float *h, const TabRows &counts, long long n, int b, int blocks) {
   unsigned top = 0u;
-  auto see = [&](float v) {
-    const unsigned bits = __float_as_uint(v) & 0x7fffffffu;
-    if (bits < 0x7f800000u && bits > top) top = bits;
-  };
-  if (b < a.q.blocks + a.w.blocks) {
-    const TabSource &s = b < a.q.blocks ? a.q : a.w;
-    if (b >= a.q.blocks) b -= a.q.blocks;
-    if (a.wide) tab_units<float4>(a, s, b, [&](long long, int, const float4 &v) { see(v.x); see(v.y); see(v.z); see(v.w); });
-    else tab_units<float>(a, s, b, [&](long long, int, float v) { see(v); });
-  } else {
-    b -= a.q.blocks + a.w.blocks;
-    for (long long i = (long long)b * 256 + threadIdx.x; i < a.n; i += a.gblocks * 256)
-      if (a.q.counts(i)) see((a.g ? fabsf(a.g[i]) : 0.f) + (a.h ? 23.f * fabsf(a.h[i]) : 0.f));
+  for (long long i = (long long)b * 256 + threadIdx.x; i < n; i += blocks * 256) {
+    if (!counts(i)) continue;
+    const unsigned bits = __float_as_uint((g ? fabsf(g[i]) : 0.f) + (h ? 23.f * fabsf(h[i]) : 0.f));
+    if (bits < 0x7f800000u) top = max(top, bits);
   }
+  return top;
+}
+// The largest of a CTA's threads' numbers to block_max[blockIdx.x].
+__device__ __forceinline__ void tab_leave_max(unsigned top, unsigned *block_max) {
+  __shared__ unsigned tops[8];
   top = __reduce_max_sync(0xffffffffu, top);
-  if (lane == 0) tops[w] = top;
+  if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = top;
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int i = 1; i < 8; ++i) top = max(top, tops[i]);
-    a.block_max[blockIdx.x] = top;
+    block_max[blockIdx.x] = top;
   }
+}
+__global__ void __launch_bounds__(256) tab_max_kernel(TabPrep a) {
+  pdl_begin();
+  tab_leave_max(tab_dz_bound(a.g, a.h, a.q.counts, a.n, blockIdx.x, a.gblocks), a.block_max);
 }
 // 2^k that brings a number below 2^top, |k| <= 126: 2^-k is a normal number too, and the smallest normal one comes out at 1
 __device__ __forceinline__ float tab_power(unsigned bits, int top, float &inverse) {
@@ -752,11 +771,17 @@ __device__ __forceinline__ float tab_power(unsigned bits, int top, float &invers
   inverse = __uint_as_float((unsigned)(127 - k) << 23);
   return __uint_as_float((unsigned)(127 + k) << 23);
 }
+__device__ __forceinline__ void tab_split3(float v, __nv_bfloat16 &b0, __nv_bfloat16 &b1, __nv_bfloat16 &b2) {
+  b0 = __float2bfloat16_rn(v);
+  const float r = __hisinf(b0) || __hisnan(b0) ? 0.f : v - __bfloat162float(b0);
+  b1 = __float2bfloat16_rn(r);
+  b2 = __float2bfloat16_rn(r - __bfloat162float(b1));
+}
 __device__ __forceinline__ void tab_split(float v, __half &b0, __half &b1) {
   b0 = __float2half_rn(v);
   b1 = __hisinf(b0) || __hisnan(b0) ? __float2half_rn(0.f) : __float2half_rn(v - __half2float(b0));
 }
-// fp32 to two fp16 planes; 16-bit elements as they are (rows that TMA cannot read where they lie, and the gradient's queries).
+// fp32 to three bf16 planes; 16-bit elements as they are (rows that TMA cannot read where they lie, and the gradient's queries).
 // Rows that do not count become zeros: whatever stands in padding, a product with its zero gradient is zero.
 template <class T>
 __global__ void __launch_bounds__(256) tab_pack_kernel(TabPrep a) {
@@ -765,7 +790,7 @@ __global__ void __launch_bounds__(256) tab_pack_kernel(TabPrep a) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   float up_q = 1.f, up_w = 1.f;
   if (a.sc) {
-    const int nq = a.planes ? a.q.blocks : 0, nw = a.planes ? a.w.blocks : 0;
+    const int nq = a.max_q, nw = a.max_w;
     if (w < 3) {                                                          // a warp each: queries, table, gradients
       const int lo = w == 0 ? 0 : w == 1 ? nq : nq + nw, hi = w == 0 ? nq : w == 1 ? nq + nw : nq + nw + a.gblocks;
       unsigned top = 0u;
@@ -775,8 +800,8 @@ __global__ void __launch_bounds__(256) tab_pack_kernel(TabPrep a) {
     }
     __syncthreads();
     TabScales s = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
-    if (a.planes) { s.q = tab_power(tops[0], 14, s.iq); s.w = tab_power(tops[1], 14, s.iw); }
-    if (a.gblocks) s.dz = tab_power(__float_as_uint(fminf(__uint_as_float(tops[2]) * a.scale, 1e38f)), 14, s.idz);
+    if (a.planes) { s.q = tab_power(tops[0], 40, s.iq); s.w = tab_power(tops[1], 40, s.iw); }
+    if (a.gblocks) s.dz = tab_power(__float_as_uint(fminf(__uint_as_float(tops[2]) * a.scale, 1e38f)), a.planes ? 40 : 14, s.idz);
     up_q = s.q;
     up_w = s.w;
     if (blockIdx.x == 0 && threadIdx.x == 0) *a.sc = s;
@@ -786,32 +811,50 @@ __global__ void __launch_bounds__(256) tab_pack_kernel(TabPrep a) {
   const int b = of_q ? blockIdx.x : blockIdx.x - a.q.blocks;
   const float up = of_q ? up_q : up_w;
   if constexpr (sizeof(T) == 4) {
-    auto split = [&](float v, __half &b0, __half &b1) { tab_split(v * up, b0, b1); };
-    __half *p0 = (__half *)s.to, *p1 = p0 + s.plane;
+    __nv_bfloat16 *p0 = (__nv_bfloat16 *)s.to, *p1 = p0 + s.plane, *p2 = p1 + s.plane;
     if (a.wide) tab_units<float4>(a, s, b, [&](long long r, int i, const float4 &v) {
-      __align__(8) __half h0[4], h1[4];
-      split(v.x, h0[0], h1[0]); split(v.y, h0[1], h1[1]); split(v.z, h0[2], h1[2]); split(v.w, h0[3], h1[3]);
+      __align__(8) __nv_bfloat16 h0[4], h1[4], h2[4];
+      tab_split3(v.x * up, h0[0], h1[0], h2[0]); tab_split3(v.y * up, h0[1], h1[1], h2[1]);
+      tab_split3(v.z * up, h0[2], h1[2], h2[2]); tab_split3(v.w * up, h0[3], h1[3], h2[3]);
       ((uint2 *)(p0 + r * s.ld))[i] = *(uint2 *)h0;
       ((uint2 *)(p1 + r * s.ld))[i] = *(uint2 *)h1;
+      ((uint2 *)(p2 + r * s.ld))[i] = *(uint2 *)h2;
     });
-    else tab_units<float>(a, s, b, [&](long long r, int i, float v) { split(v, p0[r * s.ld + i], p1[r * s.ld + i]); });
+    else tab_units<float>(a, s, b, [&](long long r, int i, float v) { tab_split3(v * up, p0[r * s.ld + i], p1[r * s.ld + i], p2[r * s.ld + i]); });
   } else {
     if (a.wide) tab_units<uint4>(a, s, b, [&](long long r, int i, const uint4 &v) { ((uint4 *)((T *)s.to + r * s.ld))[i] = v; });
     else tab_units<unsigned short>(a, s, b, [&](long long r, int i, unsigned short v) { ((unsigned short *)s.to)[r * s.ld + i] = v; });
   }
 }
-// Rows of fp32 to two fp16 planes, each times the power of two that brings its own largest finite element below 2^14; `factors` takes what
-// undoes it, times `factor`.  `group` threads to a row (up to the whole CTA), which stays in registers up to 8 units to a thread and is read
-// again from there on.  Rows that do not count become zeros.
+// Rows of fp32 to two fp16 planes, each times the power of two that brings its own largest finite element below 2^14; the factors take
+// what undoes it, times fq or fw.  `group` threads to a row (up to the whole CTA), which stays in registers up to 8 units to a thread and
+// is read again from there on.  Rows that do not count become zeros.
+struct TabRowsPrep {
+  TabSource q, w;                                          // blocks 0: not prepared
+  float fq, fw, *row_f, *col_f;
+  int dim, group;
+  const float *g, *h; long long n; int gblocks;
+  unsigned *block_max;                                     // null, or for the largest element that each CTA has seen
+};
 template <class U>
-__global__ void __launch_bounds__(256) tab_rows_kernel(TabSource s, int dim, int group, float factor, float *factors) {
+__global__ void __launch_bounds__(256) tab_rows_kernel(TabRowsPrep a) {
   __shared__ unsigned tops[8];
   pdl_begin();
   constexpr int V = sizeof(U) / 4;
-  const int sub = threadIdx.x % group, units = dim / V;
+  const bool of_q = (int)blockIdx.x < a.q.blocks;
+  const int b = of_q ? blockIdx.x : blockIdx.x - a.q.blocks, group = a.group;
+  if (!of_q && b >= a.w.blocks) {
+    tab_leave_max(tab_dz_bound(a.g, a.h, a.q.counts, a.n, b - a.w.blocks, a.gblocks), a.block_max);
+    return;
+  }
+  const TabSource &s = of_q ? a.q : a.w;
+  float *factors = of_q ? a.row_f : a.col_f;
+  const float factor = of_q ? a.fq : a.fw;
+  const int sub = threadIdx.x % group, units = a.dim / V;
   const long long per = 256 / group;
+  unsigned most = 0u;
   __half *p0 = (__half *)s.to, *p1 = p0 + s.plane;
-  for (long long r0 = blockIdx.x * per; r0 < s.rows; r0 += gridDim.x * per) {
+  for (long long r0 = b * per; r0 < s.rows; r0 += s.blocks * per) {
     const long long r = r0 + threadIdx.x / group;
     const bool there = r < s.rows, counts = there && s.counts(r);
     const U *row = (const U *)((const float *)s.x + r * s.stride);
@@ -839,6 +882,7 @@ __global__ void __launch_bounds__(256) tab_rows_kernel(TabSource s, int dim, int
       for (int k = w / warps * warps; k < (w / warps + 1) * warps; ++k) top = max(top, tops[k]);
       __syncthreads();
     }
+    most = max(most, top);
     float inverse;
     const float up = tab_power(top, 14, inverse);
     if (there && sub == 0) factors[r] = inverse * factor;
@@ -857,6 +901,7 @@ __global__ void __launch_bounds__(256) tab_rows_kernel(TabSource s, int dim, int
       }
     }
   }
+  if (a.block_max) tab_leave_max(most, a.block_max);
 }
 // The parts of a split contraction, added in their order.
 template <class T>
@@ -907,7 +952,8 @@ static bool tab_launch_as(const TabOperand &a, const TabOperand &b, const TabOpe
   // stands in the rows that are not loaded is nobody's.
   g.a_rows = !A_MN && g.M < 128 ? (int)tok_up(g.M, 8) : 128;
   if (!(A_MN ? tab_encode_blocks(&maps.a, bf16, a, KB, 2) : tab_encode(&maps.a, bf16, a, KB, g.a_rows, a.planes))) return false;
-  if (EPI == EPI_DZ && !tab_encode(&maps.c, bf16, *c, 32, 32, 1)) return false;
+  constexpr bool dz_bf16 = std::is_same<typename MATH::dz, __nv_bfloat16>::value;
+  if (EPI == EPI_DZ && !tab_encode(&maps.c, dz_bf16, *c, 32, 32, 1)) return false;
   if (EPI == EPI_OUT) {
     // rows that begin on 16-byte boundaries; sums of several launches are added row by row
     const bool fp32 = g.partial || sizeof(typename MATH::out) == 4;
@@ -920,7 +966,7 @@ static bool tab_launch_as(const TabOperand &a, const TabOperand &b, const TabOpe
   }
   if (!(g.b_whole ? tab_encode_blocks(&maps.b, bf16, b, KB, g.BN / CG / 64) : tab_encode(&maps.b, bf16, b, B_MN ? 64 : KB, B_MN ? KB : g.BN / CG, b.planes))) return false;
   const int stage = MATH::NPA * 128 * KB * 2 + MATH::NPB * (g.BN / CG) * KB * 2;
-  g.stages = TAB_RING_BYTES / stage < TAB_STAGES_MAX ? TAB_RING_BYTES / stage : TAB_STAGES_MAX;
+  g.stages = std::min(int(TabSmem<EPI, MATH>::RING) / stage, TAB_STAGES_MAX);
   void (*kernel)(TabMaps, TabArgs) = tab_kernel<EPI, MATH, A_MN, B_MN, CG, PARTS>;
   pbg_opt_in_smem((const void *)kernel, TAB_SMEM);
   const long long tiles = (g.M + 128 * CG - 1) / (128 * CG) * ((g.N + g.BN - 1) / g.BN) * g.splits, most = pbg_sm_count() / CG;
@@ -963,11 +1009,11 @@ static bool tab_pairs(long long M, long long N) { return M > 128 && N > 64; }
 
 template <int EPI, class MATH, bool A_MN, bool B_MN>
 static bool tab_launch(const TabOperand &a, const TabOperand &b, TabArgs &g, bool pairs, cudaStream_t st, const TabOperand *c = nullptr) {
-  g.part = MATH::NPB == 2 ? (EPI == EPI_DZ ? TAB_PART_F32_DZ : EPI == EPI_OUT ? TAB_PART_F32_OUT : TAB_PART_F32) : TAB_PART_16;
+  g.part = MATH::NPB == 1 ? TAB_PART_16 : EPI == EPI_DZ ? TAB_PART_F32_DZ : EPI == EPI_OUT ? TAB_PART_F32_OUT : TAB_PART_F32;
   auto as = [&](auto parts) {
     return pairs ? tab_launch_as<EPI, MATH, A_MN, B_MN, 2, decltype(parts)::value>(a, b, c, g, st) : tab_launch_as<EPI, MATH, A_MN, B_MN, 1, decltype(parts)::value>(a, b, c, g, st);
   };
-  if constexpr (MATH::NPB == 2) return as(std::true_type());
+  if constexpr (MATH::NPB > 1) return as(std::true_type());
   else {
     if constexpr (EPI == EPI_STATS) if (g.kblocks > TAB_WHOLE / 64) return as(std::true_type());
     if constexpr (EPI == EPI_OUT && !(A_MN && MATH::NPA == 2))            // (two planes and the contraction over queries: 128 of them at most)
@@ -986,7 +1032,7 @@ static bool tab_packed(const void *p, long long stride, int dim, int dtype) { re
 // What the workspace holds.  Its size is asked for without addresses, so it has room for packed operands wherever they may be needed.
 #define TAB_MAX_BLOCKS 2048                                  // of a preparing kernel
 struct TabPlace {
-  int64_t scales, block_max, q, w, row_f, col_f, parts, dz, partial, bytes;
+  int64_t scales, block_max, q, w, q3, w3, row_f, col_f, parts, dz, partial, bytes;                // q3, w3: bf16 planes of fp32 operands
   long long ld, columns, ldz;         // packed rows' length; table rows per piece of dz, and its rows' length
   long long piece;                    // queries per pass of the forward
   int npl, bn, nparts, splits, dz_planes;
@@ -1002,9 +1048,13 @@ static TabPlace tab_place(long long n, long long rows, int dim, int dtype, bool 
   p.q = p.block_max + TAB_MAX_BLOCKS * 4;
   p.w = p.q + tok_up(n * p.ld * 2 * p.npl, 256);
   int64_t at = p.w + tok_up(rows * p.ld * 2 * p.npl, 256);
-  p.row_f = at;
-  p.col_f = p.row_f + tok_up(n * 4, 256);
-  if (!grad && dtype == PBG_F32) at = p.col_f + tok_up(rows, 256) * 4;      // (whole tiles of columns are read)
+  p.row_f = p.col_f = p.q3 = p.w3 = at;
+  if (dtype == PBG_F32) {
+    p.col_f = p.row_f + tok_up(n * 4, 256);
+    p.q3 = p.col_f + tok_up(rows, 256) * 4;                                 // (whole tiles of columns are read)
+    p.w3 = p.q3 + (grad ? tok_up(n * p.ld * 6, 256) : 0);
+    at = p.w3 + (grad ? tok_up(rows * p.ld * 6, 256) : 0);
+  }
   p.parts = p.dz = p.partial = at;
   p.columns = p.ldz = 0;
   p.piece = n;
@@ -1026,14 +1076,14 @@ static TabPlace tab_place(long long n, long long rows, int dim, int dtype, bool 
   } else {
     // dz of 16-bit operands in two planes where the queries leave most of a tile's rows idle: few targets do not average the
     // rounding of dz out, and the products with more planes cost nothing that the reading of the table does not cover
-    p.dz_planes = dtype == PBG_F32 || n <= 128 ? 2 : 1;
+    p.dz_planes = dtype == PBG_F32 ? 3 : n <= 128 ? 2 : 1;
     long long most = TAB_DZ_BYTES / (2 * p.dz_planes * n) / 256 * 256;
     if (most < 256) most = 256;
     p.columns = rows < most ? rows : most;
     p.ldz = tok_up(p.columns, 64);
     at += tok_up(n * p.ldz * 2 * p.dz_planes, 256);
     p.partial = at;
-    p.splits = tab_splits(n, dim, p.columns, dtype == PBG_F32 ? 3 : p.dz_planes);
+    p.splits = tab_splits(n, dim, p.columns, dtype == PBG_F32 ? 6 : p.dz_planes);
     if (p.splits > 1 || p.columns < rows) at += tok_up((int64_t)p.splits * n * dim * 4, 256);
   }
   p.bytes = at;
@@ -1044,62 +1094,69 @@ struct TabCall {
   const void *queries; int64_t q_stride, n; const void *table; int64_t t_stride, rows; int dim, dtype;
   const long long *targets; int64_t ignore_index; float scale; unsigned char *ws; int *errors; cudaStream_t st;
   TabScales *sc; int *err;
-  TabOperand q, w;
+  TabOperand q, w, q3, w3;            // for the scores, and for the products with dz
 };
 
 static int tab_blocks(long long rows, int most) { const long long b = (rows + 7) / 8; return (int)(b < most ? b : most); }
-// Scales and operands.  For the gradient the queries are always copied: the rows that do not count have to be zeros.
+static void tab_begin(TabCall &c, const TabPlace &p) {
+  c.err = c.errors ? c.errors : (int *)(c.ws + p.scales + 128);          // (nobody reads the latter: the results say it)
+  c.sc = nullptr;
+  c.q = c.q3 = TabOperand{c.queries, c.n, c.dim, c.q_stride, 0, 1, false};
+  c.w = c.w3 = TabOperand{c.table, c.rows, c.dim, c.t_stride, 0, 1, false};
+}
+static TabRows tab_counts(const TabCall &c, bool grad) { return TabRows{c.targets, c.ignore_index, c.rows, grad ? 0 : 1}; }
+// Scales and operands, but for the scores of fp32.  For the gradient the queries are always copied: the rows that do not count have to be zeros.
 template <class T>
-static void tab_prepare(TabCall &c, const TabPlace &p, bool grad, const float *g, const float *h) {
-  const bool planes = c.dtype == PBG_F32, dz = grad && c.dtype != PBG_BF16;
-  c.sc = planes || dz ? (TabScales *)(c.ws + p.scales) : nullptr;
-  c.err = c.errors ? c.errors : (int *)(c.ws + p.scales + 128);          // (nobody reads the latter)
-  c.q = TabOperand{c.queries, c.n, c.dim, c.q_stride, 0, 1, false};
-  c.w = TabOperand{c.table, c.rows, c.dim, c.t_stride, 0, 1, false};
+static void tab_prepare(TabCall &c, const TabPlace &p, bool grad, const float *g, const float *h, int max_q, int max_w, int gblocks) {
+  constexpr bool F32 = sizeof(T) == 4;
   const bool pack_q = grad || tab_packed(c.queries, c.q_stride, c.dim, c.dtype), pack_w = tab_packed(c.table, c.t_stride, c.dim, c.dtype);
   if (!pack_q && !pack_w) return;
-  constexpr int V = sizeof(T) == 4 ? 4 : 8;
+  constexpr int V = F32 ? 4 : 8;
   TabPrep a = {};
-  a.q.counts = TabRows{c.targets, c.ignore_index, c.rows, grad ? 0 : 1};
+  a.q.counts = tab_counts(c, grad);
   a.w.counts = TabRows{nullptr, 0, 0, 1};
-  a.g = g; a.h = h; a.n = c.n; a.scale = c.scale; a.dim = c.dim; a.planes = planes; a.sc = c.sc;
-  a.gblocks = dz ? tab_blocks((c.n + 31) / 32, 64) : 0;
+  a.g = g; a.h = h; a.n = c.n; a.scale = c.scale; a.dim = c.dim; a.planes = F32; a.sc = c.sc;
+  a.gblocks = gblocks; a.max_q = max_q; a.max_w = max_w;
   a.block_max = (unsigned *)(c.ws + p.block_max);
   a.wide = c.dim % V == 0;
   auto source = [&](TabSource &s, TabOperand &o, const void *x, long long stride, long long rows, int64_t at, int most) {
     s.x = x; s.stride = stride; s.rows = rows; s.to = c.ws + at; s.ld = p.ld; s.plane = rows * p.ld;
     s.blocks = tab_blocks(rows, most);
     if (!aligned16(x) || stride % V != 0) a.wide = 0;
-    o = TabOperand{s.to, rows, c.dim, p.ld, s.plane, p.npl, true};
+    o = TabOperand{s.to, rows, c.dim, p.ld, s.plane, F32 ? 3 : 1, true};
   };
-  if (pack_q) source(a.q, c.q, c.queries, c.q_stride, c.n, p.q, 296);
-  if (pack_w) source(a.w, c.w, c.table, c.t_stride, c.rows, p.w, 1184);
+  if (pack_q) source(a.q, c.q3, c.queries, c.q_stride, c.n, F32 ? p.q3 : p.q, 296);
+  if (pack_w) source(a.w, c.w3, c.table, c.t_stride, c.rows, F32 ? p.w3 : p.w, 1184);
   a.by_units = FastDiv(a.wide ? c.dim / V : c.dim);
-  if (planes || dz) {
-    TabPrep m = a;
-    if (!planes) m.q.blocks = m.w.blocks = 0;
-    pbg_launch(tab_max_kernel, dim3(m.q.blocks + m.w.blocks + m.gblocks), 256, 0, c.st, m);
-  }
   pbg_launch(tab_pack_kernel<T>, dim3(a.q.blocks + a.w.blocks), 256, 0, c.st, a);
+  if (!F32) { c.q = c.q3; c.w = c.w3; }
 }
 
-// The same for the forward pass of fp32 operands.  (The factors carry half of the scale's power each: their product is one of a score.)
-static void tab_prepare_rows(TabCall &c, const TabPlace &p) {
-  c.sc = nullptr;
-  c.err = c.errors ? c.errors : (int *)(c.ws + p.scales + 128);
-  const float to2 = c.scale * TOK_LOG2E, half = ldexpf(1.f, ilogbf(to2) / 2);
-  auto rows = [&](TabOperand &o, const void *x, long long stride, long long rows, int64_t at, float factor, int64_t factors, const TabRows &counts) {
-    const bool wide = c.dim % 4 == 0 && stride % 4 == 0 && aligned16(x);
-    const int units = wide ? c.dim / 4 : c.dim;
-    int group = 1;
-    while (group < 256 && group * 8 < units) group *= 2;
-    TabSource s = {x, stride, rows, counts, 0, c.ws + at, p.ld, rows * p.ld};
-    const long long ctas = (rows + 256 / group - 1) / (256 / group), most = 8 * pbg_sm_count();
-    pbg_launch(wide ? tab_rows_kernel<float4> : tab_rows_kernel<float>, dim3((unsigned)(ctas < most ? ctas : most)), 256, 0, c.st, s, c.dim, group, factor, (float *)(c.ws + factors));
-    o = TabOperand{s.to, rows, c.dim, p.ld, s.plane, 2, true};
-  };
-  rows(c.q, c.queries, c.q_stride, c.n, p.q, half, p.row_f, TabRows{c.targets, c.ignore_index, c.rows, 1});
-  rows(c.w, c.table, c.t_stride, c.rows, p.w, to2 / half, p.col_f, TabRows{nullptr, 0, 0, 1});
+// The operands of fp32 scores.  (The factors carry half of the scale's power each: their product is one of a score.)
+static TabRowsPrep tab_rows_prep(TabCall &c, const TabPlace &p, bool grad) {
+  TabRowsPrep a = {};
+  const float to2 = c.scale * TOK_LOG2E;
+  a.fq = ldexpf(1.f, ilogbf(to2) / 2);
+  a.fw = to2 / a.fq;
+  a.row_f = (float *)(c.ws + p.row_f);
+  a.col_f = (float *)(c.ws + p.col_f);
+  a.dim = c.dim;
+  a.q = {c.queries, c.q_stride, c.n, tab_counts(c, grad), 0, c.ws + p.q, p.ld, c.n * p.ld};
+  a.w = {c.table, c.t_stride, c.rows, TabRows{nullptr, 0, 0, 1}, 0, c.ws + p.w, p.ld, c.rows * p.ld};
+  c.q = TabOperand{a.q.to, c.n, c.dim, p.ld, a.q.plane, 2, true};
+  c.w = TabOperand{a.w.to, c.rows, c.dim, p.ld, a.w.plane, 2, true};
+  return a;
+}
+static void tab_rows_launch(const TabCall &c, TabRowsPrep &a, bool q, bool w) {
+  auto fits = [&](const TabSource &s) { return c.dim % 4 == 0 && s.stride % 4 == 0 && aligned16(s.x); };
+  const bool wide = (!q || fits(a.q)) && (!w || fits(a.w));
+  a.group = 1;
+  while (a.group < 256 && a.group * 8 < (wide ? c.dim / 4 : c.dim)) a.group *= 2;
+  const int per = 256 / a.group;
+  auto blocks = [&](long long rows, int most) { const long long b = (rows + per - 1) / per; return (int)(b < most ? b : most); };
+  a.q.blocks = q ? blocks(a.q.rows, w ? 296 : 1184) : 0;
+  a.w.blocks = w ? blocks(a.w.rows, 1184) : 0;
+  pbg_launch(wide ? tab_rows_kernel<float4> : tab_rows_kernel<float>, dim3(a.q.blocks + a.w.blocks + a.gblocks), 256, 0, c.st, a);
 }
 
 static bool tab_few(long long n, int dim, int dtype) {
@@ -1137,8 +1194,12 @@ static void tab_forward(TabForward &f) {
     finish(0, c.n);
     return;
   }
-  if (MATH::NPB == 2) tab_prepare_rows(c, f.p);
-  else tab_prepare<T>(c, f.p, false, nullptr, nullptr);
+  tab_begin(c, f.p);
+  if (MATH::NPB == 2) {
+    TabRowsPrep a = tab_rows_prep(c, f.p, false);
+    tab_rows_launch(c, a, true, false);
+    tab_rows_launch(c, a, false, true);
+  } else tab_prepare<T>(c, f.p, false, nullptr, nullptr, 0, 0, 0);
   constexpr int KB = MATH::NPA == 1 ? 64 : 32;
   for (long long n0 = 0; n0 < c.n && f.ok; n0 += f.p.piece) {
     const long long n = c.n - n0 < f.p.piece ? c.n - n0 : f.p.piece;
@@ -1161,7 +1222,22 @@ template <class T, class MATH, class DZMATH>
 static void tab_backward(TabBackward &f) {
   TabCall &c = f.c;
   constexpr int KB = MATH::NPA == 1 ? 64 : 32, KB2 = DZMATH::NPA == 1 ? 64 : 32;
-  tab_prepare<T>(c, f.p, true, f.g, f.h);
+  tab_begin(c, f.p);
+  const bool scaled = c.dtype != PBG_BF16;                               // dz is (and fp32 operands are)
+  const int gblocks = scaled ? tab_blocks((c.n + 31) / 32, 64) : 0;
+  int max_q = 0, max_w = 0;
+  if (scaled) c.sc = (TabScales *)(c.ws + f.p.scales);
+  if (MATH::NPB == 2) {
+    TabRowsPrep a = tab_rows_prep(c, f.p, true);
+    a.g = f.g; a.h = f.h; a.n = c.n; a.gblocks = gblocks; a.block_max = (unsigned *)(c.ws + f.p.block_max);
+    tab_rows_launch(c, a, true, true);
+    max_q = a.q.blocks; max_w = a.w.blocks;
+  } else if (scaled) {
+    TabPrep a = {};
+    a.g = f.g; a.h = f.h; a.n = c.n; a.q.counts = tab_counts(c, true); a.gblocks = gblocks; a.block_max = (unsigned *)(c.ws + f.p.block_max);
+    pbg_launch(tab_max_kernel, dim3(gblocks), 256, 0, c.st, a);
+  }
+  tab_prepare<T>(c, f.p, true, f.g, f.h, max_q, max_w, gblocks);
   const bool partial = f.p.splits > 1 || f.p.columns < c.rows;
   auto plan = [&](TabArgs &a, bool &pairs, long long M, long long N, int splits) {
     pairs = tab_pairs(M, N);
@@ -1170,15 +1246,14 @@ static void tab_backward(TabBackward &f) {
   };
   for (long long v0 = 0; v0 < c.rows && f.ok; v0 += f.p.columns) {
     const long long cols = c.rows - v0 < f.p.columns ? c.rows - v0 : f.p.columns;
-    TabOperand w = c.w;
-    w.base = (const char *)w.base + v0 * w.ld * 2;
-    w.rows = cols;
+    TabOperand w = c.w, w3 = c.w3;
+    for (TabOperand *o : {&w, &w3}) { o->base = (const char *)o->base + v0 * o->ld * 2; o->rows = cols; }
     TabArgs g = {};
     bool pairs;
     plan(g, pairs, c.n, cols, 1);
     g.kblocks = (int)((c.dim + KB - 1) / KB);
     g.m_first = 1; g.scale = c.scale;
-    g.by_q = g.by_w = 1;
+    g.row_f = (const float *)(c.ws + f.p.row_f); g.col_f = (const float *)(c.ws + f.p.col_f) + v0;
     g.targets = c.targets; g.ignore_index = c.ignore_index; g.vocab = c.rows; g.v0 = v0;
     g.lse = f.lse; g.entropy = f.entropy; g.g = f.g; g.h = f.h;
     g.ldz = f.p.ldz; g.dz_planes = f.p.dz_planes; g.out = c.ws + f.p.dz;
@@ -1190,18 +1265,17 @@ static void tab_backward(TabBackward &f) {
       TabArgs d = {};
       plan(d, pairs, c.n, c.dim, f.p.splits);
       d.kblocks = (int)((cols + KB2 - 1) / KB2);
-      d.by_dz = d.by_w = 1;
       d.out = f.dq; d.ldo = c.dim;
       if (partial) { d.partial = (float *)(c.ws + f.p.partial); d.add = v0 > 0; }
-      f.ok = tab_launch<EPI_OUT, DZMATH, false, true>(dz, w, d, pairs, c.st);
+      f.ok = tab_launch<EPI_OUT, DZMATH, false, true>(dz, w3, d, pairs, c.st);
     }
     if (f.dt && f.ok) {
       TabArgs d = {};
       plan(d, pairs, cols, c.dim, 1);
       d.kblocks = (int)((c.n + KB2 - 1) / KB2);
-      d.by_dz = d.by_q = 1;
+      d.by_q = 1;
       d.out = (T *)f.dt + v0 * c.dim; d.ldo = c.dim;
-      f.ok = tab_launch<EPI_OUT, DZMATH, true, true>(dz, c.q, d, pairs, c.st);
+      f.ok = tab_launch<EPI_OUT, DZMATH, true, true>(dz, c.q3, d, pairs, c.st);
     }
   }
   if (f.dq && partial && f.ok) {
@@ -1258,7 +1332,7 @@ extern "C" int pbg_table_logprobs_grad(const void *queries, int64_t q_stride, in
   if (!lse || (grad_entropy && !entropy) || (!grad_queries && !grad_table)) return PBG_ERR_BAD_ARGUMENT;
   if (!get_encode()) return PBG_ERR_CUDA;
   f.p = tab_place(n, rows, dim, dtype, true);
-  if (dtype == PBG_F32) tab_backward<float, TabF32, TabF32>(f);
+  if (dtype == PBG_F32) tab_backward<float, TabF32, TabF32Out>(f);
   else if (dtype == PBG_BF16) {
     if (f.p.dz_planes == 2) tab_backward<__nv_bfloat16, TabBf16, TabBf16Fine>(f);
     else tab_backward<__nv_bfloat16, TabBf16, TabBf16>(f);

@@ -16,7 +16,8 @@
 
 // ex2 takes z to 2^z within 2 ulp, results below 2^-126 to 0.
 __device__ __forceinline__ float tok_ex2(float z) { float e; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z)); return e; }
-// the larger, NaN if either is one
+// the smaller, the larger; NaN if either is one
+__device__ __forceinline__ float tok_min_nan(float a, float b) { float m; asm("min.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b)); return m; }
 __device__ __forceinline__ float tok_max_nan(float a, float b) { float m; asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b)); return m; }
 
 // Element types: storage type, elements of a 16-byte vector, conversions.  Results are rounded to nearest, once.

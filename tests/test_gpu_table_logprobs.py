@@ -440,3 +440,42 @@ def test_float32_queries_in_pieces():
     assert ((r.lse[some].double() - lse).abs() <= E + 2e-5 * (1 + lse.abs())).all()
     assert ((r.logprob[some].double() - logprob).abs() <= 2 * (E + 2e-5 * (1 + lse.abs())) + 2e-5 * logprob.abs()).all()
     assert ((r.entropy[some].double() - ent).abs() <= 80 * E + 2e-5 * (1 + ent + math.log(rows))).all()
+
+
+@pytest.mark.parametrize("big", [1e4, 1e8, 1e12, 1e30])
+@pytest.mark.parametrize("n,dim", [(7, 72), (17, 400), (140, 33), (1000, 400)])
+def test_gradients_of_uneven_inputs(n, dim, big):
+    """fp32: a query of 1e30 whose gradients are zero, a row of the table where no query looks, a query with gradients of 1e-12 and a row of which every
+    query is far.  Each result against the sum of its own terms' sizes: neither what others hold nor a common bound of all dz takes bits from it."""
+    q, t, targets, _, _, _ = uneven(n, dim, big)
+    t[13] = 0
+    t[13, 0] = -400.0
+    targets[targets == 13] = 12
+    g, h = torch.randn(n, device=DEV, generator=gen(1)) / n, torch.randn(n, device=DEV, generator=gen(2)) / n
+    g[3], h[3], g[6], h[6] = 0, 0, 1e-12, 1e-12
+    r = T.table_logprobs(q, t, targets)
+    dq, dt = T.table_logprobs_grad(q, t, targets, r.lse, r.entropy, g, h)
+    keep = torch.arange(n, device=DEV) != 3
+    Q, A = q[keep].double(), t.double()
+    z = Q @ A.T
+    p = (z - r.lse[keep].double()[:, None]).exp()
+    hot = torch.zeros_like(p).scatter_(1, targets[keep][:, None], 1.0)
+    gk, hk, H = g[keep].double()[:, None], h[keep].double()[:, None], r.entropy[keep].double()[:, None]
+    plogp = torch.special.entr(p)
+    w = gk * (hot - p) + hk * (plogp - p * H)
+    size = gk.abs() * (hot + p) + hk.abs() * (plogp + p * H)
+    # each score is off by its own terms' sizes times E's factor, and lse by what that is in the mean under p
+    own = (Q.abs() @ A.abs().T) * (dim * 2 ** -23 + 3 * 2 ** -22)
+    score = own + (p * own).sum(1, keepdim=True)
+    err = size * (2 * score + 2e-5) + hk.abs() * p * score + w.abs() * 2 ** -22
+    planes = 3 * 2 ** -22
+    # an operand's largest element is brought to 2^39 or above and cut into bf16 planes, whose smallest step is 2^-133: an element is off by at
+    # most half a step, 2^-173 of the largest, beside the 2^-24 of its own size (1e-30 among 1e30 is lost)
+    least_q, least_t = (x.abs().max().item() * 2.0 ** -173 for x in (q, t))
+    want = w @ A
+    tol = err @ A.abs() + (w.abs() @ A.abs()) * (len(t) * 2 ** -23 + planes) + want.abs() * 2 ** -24 + 1e-37 + w.abs().sum(1, keepdim=True) * least_t
+    assert ((dq[keep].double() - want).abs() <= tol).all()
+    want = w.T @ Q
+    assert want[13].abs().max() > 1e-37
+    tol = err.T @ Q.abs() + (w.abs().T @ Q.abs()) * (n * 2 ** -23 + planes) + want.abs() * 2 ** -24 + 1e-37 + w.abs().sum(0)[:, None] * least_q
+    assert ((dt.double() - want).abs() <= tol).all()

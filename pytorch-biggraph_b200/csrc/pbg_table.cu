@@ -67,9 +67,10 @@ enum { EPI_STATS = 0, EPI_DZ = 1, EPI_OUT = 2 };
 #define TAB_EPI_WARPS 8
 #define TAB_THREADS (64 + 32 * TAB_EPI_WARPS)
 #define TAB_SMEM 230400
-// (three planes of dz take 6, and the factors of 128 columns stand behind them)
+// (three planes of dz take 12, and the factors of each warp's 128 columns stand behind them all)
 template <int EPI, class MATH> struct TabSmem {
-  static constexpr int OUT = EPI == EPI_DZ && MATH::NPB == 2 ? 6144 + 512 : 4096, RING = TAB_SMEM - 1024 - TAB_EPI_WARPS * OUT;
+  static constexpr bool DZ3 = EPI == EPI_DZ && MATH::NPB == 2;
+  static constexpr int OUT = DZ3 ? 12288 : 4096, RING = TAB_SMEM - 1024 - TAB_EPI_WARPS * (OUT + (DZ3 ? 512 : 0));
 };
 
 // Operands: their elements, the planes of A and B, the type of results
@@ -332,7 +333,7 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
       const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * hc);
       // the columns' factors, for all rows of the warp
       constexpr bool SCALED = EPI != EPI_OUT && NPB == 2;
-      float4 *cols_f = reinterpret_cast<float4 *>(buf + (EPI == EPI_DZ ? 6144 : 0));
+      float4 *cols_f = reinterpret_cast<float4 *>(EPI == EPI_DZ ? ostage + TAB_EPI_WARPS * TabSmem<EPI, MATH>::OUT + (warp - 2) * 512 : buf);
       float row_f = 0.f;
       if (SCALED) {
         __syncwarp();
@@ -471,8 +472,10 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
 #pragma unroll
             for (int i = 0; i < 32; ++i) if (col + i >= g.N) v[i] = 0.f;
           }
-          // planes of 32 x 32 values through shared memory (64-byte swizzle); each leaves as one bulk store, clipped at the last row
-          store_ready();
+          // planes of 32 rows through shared memory; each leaves as one bulk store, clipped at the last row (columns come in 64s)
+          constexpr bool WIDE = NPB == 2;                                // 64 columns to a store of 128-byte rows, else 32 and 64 (64-byte swizzle)
+          constexpr int PLANE = WIDE ? 4096 : 2048;
+          if (!WIDE || (x & 32) == 0) store_ready();
 #pragma unroll
           for (int pl = 0; pl < MOST_PLANES; ++pl) {
             if (pl >= planes) break;
@@ -486,15 +489,16 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
                 if (pl < MOST_PLANES - 1) { const float2 f = TokPair<Dz>::up(e); a -= f.x; b -= f.y; }      // what the next plane holds
                 w[i] = *reinterpret_cast<const uint32_t *>(&e);
               }
-              *reinterpret_cast<uint4 *>(buf + pl * 2048 + lane * 64 + ((u ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+              unsigned char *at = buf + pl * PLANE + (WIDE ? lane * 128 + (((u + (x & 32) / 8) ^ (lane & 7)) << 4) : lane * 64 + ((u ^ ((lane >> 1) & 3)) << 4));
+              *reinterpret_cast<uint4 *>(at) = make_uint4(w[0], w[1], w[2], w[3]);
             }
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
-          if (lane == 0 && rows > 0) {
+          if (lane == 0 && rows > 0 && (!WIDE || (x & 32))) {
             for (int pl = 0; pl < planes; ++pl)
               asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];"
-                           :: "l"(&maps.c), "r"((int)col), "r"((int)(m0 + q * 32)), "r"(pl), "r"(smem_u32(buf + pl * 2048)) : "memory");
+                           :: "l"(&maps.c), "r"((int)(WIDE ? col - 32 : col)), "r"((int)(m0 + q * 32)), "r"(pl), "r"(smem_u32(buf + pl * PLANE)) : "memory");
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
           }
         } else if (!g.bulk) {
@@ -953,7 +957,7 @@ static bool tab_launch_as(const TabOperand &a, const TabOperand &b, const TabOpe
   g.a_rows = !A_MN && g.M < 128 ? (int)tok_up(g.M, 8) : 128;
   if (!(A_MN ? tab_encode_blocks(&maps.a, bf16, a, KB, 2) : tab_encode(&maps.a, bf16, a, KB, g.a_rows, a.planes))) return false;
   constexpr bool dz_bf16 = std::is_same<typename MATH::dz, __nv_bfloat16>::value;
-  if (EPI == EPI_DZ && !tab_encode(&maps.c, dz_bf16, *c, 32, 32, 1)) return false;
+  if (EPI == EPI_DZ && !tab_encode(&maps.c, dz_bf16, *c, MATH::NPB == 2 ? 64 : 32, 32, 1)) return false;
   if (EPI == EPI_OUT) {
     // rows that begin on 16-byte boundaries; sums of several launches are added row by row
     const bool fp32 = g.partial || sizeof(typename MATH::out) == 4;

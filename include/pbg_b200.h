@@ -350,9 +350,10 @@ int pbg_token_logprobs_grad_wide(const void *logits, int64_t row_stride, int64_t
 /* The same statistics with z = scale * queries . table^T, which is never stored: queries [n, dim], table [rows, dim], targets rows of the
  * table.  16-bit operands are multiplied as they are; fp32 ones as two fp16 planes each, at fp32's accuracy for elements down to
  * 2^-17 of the largest of the same row, and an absolute one of 2^-39 of that below: neither a query nor a row of the table takes
- * anything from another one.  (Up to sixteen fp32 queries: in fp32 throughout.)  NaN, or an infinity, among a
- * query's scores makes its entropy NaN, NaN or +inf its other results too; no other query's results change.
- * Scores are fp32 sums: beyond 1e7 in size nothing is left of their differences, and results may be NaN.
+ * anything from another one.  (Up to sixteen fp32 queries: in fp32 throughout.)  NaN or +inf among a query's scores makes its
+ * results NaN and -inf is a probability of 0; no other query's results change.  (An infinite element of more than sixteen fp32 queries, or
+ * of a row of their table, makes NaN of its scores.)  Scores are fp32 sums: beyond 1e7 in size nothing is left of their
+ * differences.  logprob is never above 0.
  * workspace: of pbg_table_logprobs_workspace(n, rows, dim, dtype, 0) bytes. */
 int64_t pbg_table_logprobs_workspace(int64_t n, int64_t rows, int32_t dim, int32_t dtype, int32_t grad);
 int pbg_table_logprobs(const void *queries, int64_t q_stride, int64_t n, const void *table, int64_t t_stride, int64_t rows,

@@ -57,19 +57,6 @@ template <> struct Row16<__half> : Row16Half<__half, __half2> { static constexpr
 template <class T> __device__ __forceinline__ float2 word_up(unsigned w) { return TokPair<T>::up(*reinterpret_cast<typename TokPair<T>::type *>(&w)); }
 template <> __device__ __forceinline__ float2 word_up<float>(unsigned w) { return make_float2(__uint_as_float(w), -INFINITY); }
 
-__device__ __forceinline__ unsigned long long f32x2(float a, float b) { unsigned long long p; asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b)); return p; }
-__device__ __forceinline__ float2 f32x2_parts(unsigned long long p) { float2 f; asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p)); return f; }
-__device__ __forceinline__ unsigned long long f32x2_fma(unsigned long long a, unsigned long long b, unsigned long long c) {
-  unsigned long long d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ unsigned long long f32x2_add(unsigned long long a, unsigned long long b) {
-  unsigned long long d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-
 // What a thread gathers over its part of a row: S and T of its even and odd scores against the reference s.r, and how many scores stand in
 // front of the target's.
 template <class T>

@@ -96,8 +96,9 @@ struct TabArgs {
   const float *row_f, *col_f;         // scores of fp32 operands: what takes a product to a score in base 2, by row and by column
   const TabScales *sc;                // null: all 1
   int *err;
-  float4 *parts; int nparts;          // EPI_STATS: [M][nparts] (reference in base 2, S, T)
-  const long long *targets; long long ignore_index, vocab, v0;         // EPI_DZ; v0: the table's row of column 0
+  float4 *parts; int nparts;          // EPI_STATS: [M][nparts] (the members of Soft)
+  float *at_target;                   //            [M] the target's product, as it stands in S
+  const long long *targets; long long ignore_index, vocab, v0;         // v0: the table's row of column 0
   const float *lse, *entropy, *g, *h;
   long long ldz; int dz_planes;
   void *out; long long ldo;           // EPI_DZ: dz; EPI_OUT: the result, or
@@ -318,14 +319,16 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
       // what a row of dz takes, read while the products run: dz = -p (gg + hh log2 p) (+ g0 at the target)
       float lse = 0.f, g0 = 0.f, gg = 0.f, hh = 0.f;
       long long hot = -1;
-      if (EPI == EPI_DZ && m < g.M) {
+      if (EPI != EPI_OUT && m < g.M) {
         const long long target = g.targets[m];
         if (target >= 0 && target < g.vocab && target != g.ignore_index) {
-          lse = g.lse[m] * TOK_LOG2E;
-          if (g.g) g0 = gg = g.g[m] * g.scale * up;
-          if (g.h) { const float h = g.h[m] * g.scale * up; hh = h * TOK_LN2; gg = fmaf(h, g.entropy[m], gg); }
+          if (EPI == EPI_DZ) {
+            lse = g.lse[m] * TOK_LOG2E;
+            if (g.g) g0 = gg = g.g[m] * g.scale * up;
+            if (g.h) { const float h = g.h[m] * g.scale * up; hh = h * TOK_LN2; gg = fmaf(h, g.entropy[m], gg); }
+          }
           hot = target - g.v0;
-        } else if (target != g.ignore_index && n0 == 0 && half == 0 && g.v0 == 0) atomicOr(g.err, TOK_ERR_ID);
+        } else if (EPI == EPI_DZ && target != g.ignore_index && n0 == 0 && half == 0 && g.v0 == 0) atomicOr(g.err, TOK_ERR_ID);
       }
       const long long c0 = n0 + half * hc;                               // first column of this warp
       const int cols = c0 >= g.N ? 0 : g.N - c0 < hc ? (int)(g.N - c0) : hc;
@@ -397,7 +400,8 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
         }
       };
 
-      float mx = -INFINITY, r = 0.f, S = 0.f, T = 0.f;                   // EPI_STATS
+      float mx = -INFINITY, r = 0.f;                                     // EPI_STATS: largest product, reference; sums of even and odd columns
+      unsigned long long S2 = f32x2(0.f, 0.f), T2 = S2;
       // the padding of dz's last columns is written too, as zeros: the contraction over the table's rows reads whole blocks
       const int span = EPI == EPI_DZ ? (c0 >= g.ldz ? 0 : g.ldz - c0 < hc ? (int)(g.ldz - c0) : hc) : cols;
       const int rows = g.M - (m0 + q * 32) < 32 ? (int)(g.M - (m0 + q * 32)) : 32;
@@ -428,31 +432,36 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
           }
         }
         if (EPI == EPI_STATS) {
-          float cm = -INFINITY;
-          const bool whole = cols - x >= 32;                               // (else columns that do not exist are left out)
+          if (__any_sync(0xffffffffu, hot >= c0 + x && hot < c0 + x + 32)) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) if (whole || i < cols - x) cm = fmaxf(cm, v[i]);
+            for (int i = 0; i < 32; ++i) if (hot == c0 + x + i) g.at_target[m] = v[i];
+          }
+          if (cols - x < 32) {                                             // columns that do not exist
+#pragma unroll
+            for (int i = 0; i < 32; ++i) if (i >= cols - x) v[i] = -INFINITY;
+          }
+          float cm = v[0];
+#pragma unroll
+          for (int i = 1; i < 32; ++i) cm = fmaxf(cm, v[i]);
           if (cm > mx) {
             mx = cm;
-            const float d = fminf(fmaxf(r - cm * c, -1e30f), 0.f), f = tok_ex2(d);
-            T = (T + d * S) * f;
-            S *= f;
-            r = cm * c;
+            const float d = fminf(fmaxf((r - cm) * c, -1e30f), 0.f), f = tok_ex2(d);
+            const unsigned long long f2 = f32x2(f, f), zero = f32x2(0.f, 0.f);
+            T2 = f32x2_fma(f32x2_fma(f32x2(d, d), S2, T2), f2, zero);
+            S2 = f32x2_fma(S2, f2, zero);
+            r = cm;
           }
-          if (whole) {
+          // (the difference to the largest is formed first: nothing of it is lost, however large the two are)
+          const unsigned long long r2 = f32x2(-r, -r), c2 = f32x2(c, c);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const float y = tok_max_nan(fmaf(v[i], c, -r), -1000.f), e = tok_ex2(y);
-              S += e;
-              T = fmaf(y, e, T);
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) if (i < cols - x) {
-              const float y = tok_max_nan(fmaf(v[i], c, -r), -1000.f), e = tok_ex2(y);
-              S += e;
-              T = fmaf(y, e, T);
-            }
+          for (int i = 0; i < 32; i += 2) {
+            unsigned long long d2 = f32x2_add(f32x2(v[i], v[i + 1]), r2);
+            if (!SCALED) d2 = f32x2_fma(d2, c2, f32x2(0.f, 0.f));
+            const float2 d = f32x2_parts(d2);
+            const float y0 = tok_max_nan(d.x, -1000.f), y1 = tok_max_nan(d.y, -1000.f);      // (2^-1000 is 0 too, and 0 times -inf no number)
+            const unsigned long long e2 = f32x2(tok_ex2(y0), tok_ex2(y1));
+            S2 = f32x2_add(S2, e2);
+            T2 = f32x2_fma(f32x2(y0, y1), e2, T2);
           }
         } else if (EPI == EPI_DZ) {
           const long long col = c0 + x;
@@ -542,7 +551,7 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
           if ((x & 32) || x + 32 >= span) store_go((int)(c0 + (x & ~32)), (int)(m0 + q * 32), 0, rows > 0);
         }
       }
-      if (EPI == EPI_STATS && m < g.M) g.parts[m * g.nparts + n0 / g.BN * 2 + half] = make_float4(S == 0.f ? -1e30f : r, S, T, 0.f);
+      if (EPI == EPI_STATS && m < g.M) g.parts[m * g.nparts + n0 / g.BN * 2 + half] = make_float4(mx, r, f32x2_parts(S2).x + f32x2_parts(S2).y, f32x2_parts(T2).x + f32x2_parts(T2).y);
       if (!PARTS && kb0 < kb1) give_back();
     }
     // a wait has run out: what this warp had still to write
@@ -553,7 +562,7 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
       const long long m = m0 + q * 32 + lane, c0 = n0 + half * hc, c1 = c0 + hc < g.N ? c0 + hc : g.N;
       const float nan = __int_as_float(0x7fc00000);
       if (m >= g.M) continue;
-      if (EPI == EPI_STATS) g.parts[m * g.nparts + n0 / g.BN * 2 + half] = make_float4(0.f, nan, nan, 0.f);
+      if (EPI == EPI_STATS) g.parts[m * g.nparts + n0 / g.BN * 2 + half] = make_float4(0.f, 0.f, nan, nan);
       else for (long long c = c0; c < c1; ++c) {
         if (EPI == EPI_DZ) for (int pl = 0; pl < planes; ++pl) ((Dz *)g.out)[(pl * g.M + m) * g.ldz + c] = Tok<Dz>::down(nan);
         else if (g.partial) g.partial[((long long)split * g.M + m) * g.N + c] = nan;
@@ -573,12 +582,12 @@ __global__ void __launch_bounds__(TAB_THREADS, 1) tab_kernel(const __grid_consta
   }
 }
 
-// A query's partial sums to its statistics; the target's score is a dot product of its own, in fp32.
-template <class T>
-__global__ void __launch_bounds__(128) tab_stats_kernel(const T *__restrict__ queries, long long q_stride, const T *__restrict__ table, long long t_stride, long long vocab,
-                                                        int dim, const long long *__restrict__ targets, long long ignore_index, float scale,
-                                                        const float4 *__restrict__ parts, int nparts, float *logprob, float *entropy, float *lse, int *errors) {
-  __shared__ float4 sums[4];
+// A query's partial sums to its statistics; c and natural take a product to a score in base 2 and to one.  The target's score is the
+// product that S was made of: another one, as exact as it may be, could come out above lse.
+__global__ void __launch_bounds__(128) tab_stats_kernel(const long long *__restrict__ targets, long long ignore_index, long long vocab, float c, float natural,
+                                                        const float4 *__restrict__ parts, int nparts, const float *__restrict__ at_target, float *logprob, float *entropy,
+                                                        float *lse, int *errors) {
+  __shared__ Soft sums[4];
   pdl_begin();
   const long long n = blockIdx.x, target = targets[n];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
@@ -587,32 +596,20 @@ __global__ void __launch_bounds__(128) tab_stats_kernel(const T *__restrict__ qu
     return;
   }
   const bool known = target >= 0 && target < vocab;
-  float r = -1e30f, S = 0.f, A = 0.f, dot = 0.f;
-  auto join = [&](float r2, float S2, float A2) {
-    const float top = fmaxf(r, r2), d1 = r - top, d2 = r2 - top, f1 = tok_ex2(d1), f2 = tok_ex2(d2);
-    A = (A + d1 * S) * f1 + (A2 + d2 * S2) * f2;
-    S = S * f1 + S2 * f2;
-    r = top;
-  };
-  for (int i = threadIdx.x; i < nparts; i += 128) { const float4 p = parts[n * nparts + i]; join(p.x, p.y, p.z); }
-  if (known) {
-    const T *a = queries + n * q_stride, *b = table + target * t_stride;
-    for (int i = threadIdx.x; i < dim; i += 128) dot = fmaf(Tok<T>::up(a[i]), Tok<T>::up(b[i]), dot);
-  }
+  Soft s{-INFINITY, 0.f, 0.f, 0.f};
+  for (int i = threadIdx.x; i < nparts; i += 128) { const float4 p = parts[n * nparts + i]; soft_join(s, Soft{p.x, p.y, p.z, p.w}, c); }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float r2 = __shfl_xor_sync(0xffffffffu, r, o), S2 = __shfl_xor_sync(0xffffffffu, S, o), A2 = __shfl_xor_sync(0xffffffffu, A, o);
-    join(r2, S2, A2);
-    dot += __shfl_xor_sync(0xffffffffu, dot, o);
-  }
-  if (lane == 0) sums[w] = make_float4(r, S, A, dot);
+  for (int o = 16; o > 0; o >>= 1) soft_join(s, soft_shfl(s, o), c);
+  if (lane == 0) sums[w] = s;
   __syncthreads();
   if (threadIdx.x != 0) return;
-  for (int i = 1; i < 4; ++i) { join(sums[i].x, sums[i].y, sums[i].z); dot += sums[i].w; }
-  const float log_s = logf(S), l = fmaf(r, TOK_LN2, log_s);
-  lse[n] = l;
-  entropy[n] = log_s - A * TOK_LN2 / S;
-  logprob[n] = known ? dot * scale - l : __int_as_float(0x7fc00000);
+  for (int i = 1; i < 4; ++i) soft_join(s, sums[i], c);
+  const bool empty = s.m == -INFINITY && s.S == 0.f;                     // nothing but -inf
+  const float log_s = logf(s.S);
+  lse[n] = empty ? -INFINITY : fmaf(s.r, natural, log_s);
+  // (S holds the largest score's term, which is 1, and the target's)
+  entropy[n] = empty ? 0.f : tok_max_nan(log_s - s.T * TOK_LN2 / s.S, 0.f);
+  logprob[n] = !known ? __int_as_float(0x7fc00000) : empty ? -INFINITY : tok_min_nan(fmaf(at_target[n] - s.r, natural, -log_s), 0.f);
   if (!known && errors) atomicOr(errors, TOK_ERR_ID);
 }
 
@@ -628,7 +625,7 @@ static __host__ __device__ constexpr int few_rows(int nq) { return nq <= 8 ? 4 :
 template <int NQ, bool WIDE>
 __global__ void __launch_bounds__(32 * TAB_FEW_WARPS, 1)
 tab_few_kernel(const float *__restrict__ queries, long long q_stride, int n, const float *__restrict__ table, long long t_stride, long long vocab, int dim, float scale,
-               float4 *parts) {
+               const long long *__restrict__ targets, float4 *parts, float *at_target) {
   constexpr int R = few_rows(NQ), C = R * NQ, V = WIDE ? 4 : 1;
   extern __shared__ __align__(16) float few_q[];                         // [NQ][dim rounded up to 4]
   __shared__ Soft sums[TAB_FEW_WARPS][C];
@@ -641,6 +638,7 @@ tab_few_kernel(const float *__restrict__ queries, long long q_stride, int n, con
   Soft s{-INFINITY, 0.f, 0.f, 0.f};
   constexpr int SHIFT = C == 32 ? 0 : C == 16 ? 1 : C == 8 ? 2 : 3;
   const int mine = lane >> SHIFT, my_row = mine / NQ;   // the product that ends in this lane
+  const long long target = mine % NQ < n && (lane & ((1 << SHIFT) - 1)) == 0 ? targets[mine % NQ] : -1;
   for (long long v0 = ((long long)blockIdx.x * TAB_FEW_WARPS + w) * R; v0 < vocab; v0 += (long long)gridDim.x * TAB_FEW_WARPS * R) {
     float acc[C];
 #pragma unroll
@@ -683,6 +681,7 @@ tab_few_kernel(const float *__restrict__ queries, long long q_stride, int n, con
     }
     if (v0 + my_row < vocab) {
       const float z = acc[0];
+      if (v0 + my_row == target) at_target[mine % NQ] = z;
       if (z > s.m) { s.m = z; soft_rebase(s, soft_reference(z), c); }
       const float y = tok_max_nan((z - s.r) * c, -1000.f), e = tok_ex2(y);
       s.S += e;
@@ -695,7 +694,7 @@ tab_few_kernel(const float *__restrict__ queries, long long q_stride, int n, con
     Soft a{-INFINITY, 0.f, 0.f, 0.f};
     for (int i = 0; i < TAB_FEW_WARPS; ++i)
       for (int r = 0; r < R; ++r) soft_join(a, sums[i][r * NQ + threadIdx.x], c);
-    parts[(long long)threadIdx.x * gridDim.x + blockIdx.x] = make_float4(a.S == 0.f ? -1e30f : a.r * c, a.S, a.T, 0.f);
+    parts[(long long)threadIdx.x * gridDim.x + blockIdx.x] = make_float4(a.m, a.r, a.S, a.T);
   }
 }
 
@@ -1036,7 +1035,7 @@ static bool tab_packed(const void *p, long long stride, int dim, int dtype) { re
 // What the workspace holds.  Its size is asked for without addresses, so it has room for packed operands wherever they may be needed.
 #define TAB_MAX_BLOCKS 2048                                  // of a preparing kernel
 struct TabPlace {
-  int64_t scales, block_max, q, w, q3, w3, row_f, col_f, parts, dz, partial, bytes;                // q3, w3: bf16 planes of fp32 operands
+  int64_t scales, block_max, q, w, q3, w3, row_f, col_f, parts, at_target, dz, partial, bytes;                // q3, w3: bf16 planes of fp32 operands
   long long ld, columns, ldz;         // packed rows' length; table rows per piece of dz, and its rows' length
   long long piece;                    // queries per pass of the forward
   int npl, bn, nparts, splits, dz_planes;
@@ -1059,7 +1058,7 @@ static TabPlace tab_place(long long n, long long rows, int dim, int dtype, bool 
     p.w3 = p.q3 + (grad ? tok_up(n * p.ld * 6, 256) : 0);
     at = p.w3 + (grad ? tok_up(rows * p.ld * 6, 256) : 0);
   }
-  p.parts = p.dz = p.partial = at;
+  p.parts = p.at_target = p.dz = p.partial = at;
   p.columns = p.ldz = 0;
   p.piece = n;
   p.bn = p.nparts = p.splits = p.dz_planes = 0;
@@ -1069,14 +1068,16 @@ static TabPlace tab_place(long long n, long long rows, int dim, int dtype, bool 
     const long long groups = (rows + 4 * TAB_FEW_WARPS - 1) / (4 * TAB_FEW_WARPS);
     p.nparts = (int)(groups < pbg_sm_count() ? groups : pbg_sm_count());
     at = p.parts = p.q;                                      // no copies
-    at += n * p.nparts * 16;
+    p.at_target = p.parts + n * p.nparts * 16;
+    at = p.at_target + n * 4;
   } else if (!grad) {
     p.bn = tab_columns((n + (p.pairs ? 255 : 127)) / (p.pairs ? 256 : 128), rows, p.pairs ? 2 : 1);
     p.nparts = (int)((rows + p.bn - 1) / p.bn * 2);
     long long most = TAB_PARTS_BYTES / (16ll * p.nparts) / 256 * 256;
     if (most < 256) most = 256;
     if (p.piece > most) p.piece = most;
-    at += p.piece * p.nparts * 16;
+    p.at_target = at + p.piece * p.nparts * 16;
+    at = p.at_target + p.piece * 4;
   } else {
     // dz of 16-bit operands in two planes where the queries leave most of a tile's rows idle: few targets do not average the
     // rounding of dz out, and the products with more planes cost nothing that the reading of the table does not cover
@@ -1170,32 +1171,33 @@ static bool tab_few(long long n, int dim, int dtype) {
   return nq * tok_up(dim, 4) * 4 <= TAB_FEW_BYTES;
 }
 template <int NQ>
-static void tab_few_launch(const TabCall &c, float4 *parts, int blocks) {
+static void tab_few_launch(const TabCall &c, float4 *parts, int64_t at_target, int blocks) {
   const float *q = (const float *)c.queries, *t = (const float *)c.table;
   const bool wide = c.dim % 4 == 0 && aligned16(t) && c.t_stride % 4 == 0;
   auto kernel = wide ? tab_few_kernel<NQ, true> : tab_few_kernel<NQ, false>;
   const int smem = (int)(NQ * tok_up(c.dim, 4) * 4);
   pbg_opt_in_smem((const void *)kernel, TAB_FEW_BYTES);
-  pbg_launch(kernel, dim3(blocks), 32 * TAB_FEW_WARPS, smem, c.st, q, (long long)c.q_stride, (int)c.n, t, (long long)c.t_stride, (long long)c.rows, c.dim, c.scale, parts);
+  pbg_launch(kernel, dim3(blocks), 32 * TAB_FEW_WARPS, smem, c.st, q, (long long)c.q_stride, (int)c.n, t, (long long)c.t_stride, (long long)c.rows, c.dim, c.scale, c.targets, parts,
+             (float *)(c.ws + at_target));
 }
 
 struct TabForward { TabCall c; TabPlace p; float *logprob, *entropy, *lse; bool ok; };
 template <class T, class MATH>
 static void tab_forward(TabForward &f) {
   TabCall &c = f.c;
-  auto finish = [&](long long n0, long long n) {
-    pbg_launch(tab_stats_kernel<T>, dim3((unsigned)n), 128, 0, c.st, (const T *)c.queries + n0 * c.q_stride, (long long)c.q_stride, (const T *)c.table, (long long)c.t_stride,
-               (long long)c.rows, c.dim, c.targets + n0, (long long)c.ignore_index, c.scale, (const float4 *)(c.ws + f.p.parts), f.p.nparts, f.logprob + n0, f.entropy + n0, f.lse + n0,
-               c.errors);
+  auto finish = [&](long long n0, long long n, float to2, float natural) {
+    pbg_launch(tab_stats_kernel, dim3((unsigned)n), 128, 0, c.st, c.targets + n0, (long long)c.ignore_index, (long long)c.rows, to2, natural, (const float4 *)(c.ws + f.p.parts),
+               f.p.nparts, (const float *)(c.ws + f.p.at_target), f.logprob + n0, f.entropy + n0, f.lse + n0, c.errors);
   };
+  const float to2 = c.scale * TOK_LOG2E;
   if (f.p.few) {
     float4 *parts = (float4 *)(c.ws + f.p.parts);
-    if (c.n == 1) tab_few_launch<1>(c, parts, f.p.nparts);
-    else if (c.n == 2) tab_few_launch<2>(c, parts, f.p.nparts);
-    else if (c.n <= 4) tab_few_launch<4>(c, parts, f.p.nparts);
-    else if (c.n <= 8) tab_few_launch<8>(c, parts, f.p.nparts);
-    else tab_few_launch<16>(c, parts, f.p.nparts);
-    finish(0, c.n);
+    if (c.n == 1) tab_few_launch<1>(c, parts, f.p.at_target, f.p.nparts);
+    else if (c.n == 2) tab_few_launch<2>(c, parts, f.p.at_target, f.p.nparts);
+    else if (c.n <= 4) tab_few_launch<4>(c, parts, f.p.at_target, f.p.nparts);
+    else if (c.n <= 8) tab_few_launch<8>(c, parts, f.p.at_target, f.p.nparts);
+    else tab_few_launch<16>(c, parts, f.p.at_target, f.p.nparts);
+    finish(0, c.n, to2, c.scale);
     return;
   }
   tab_begin(c, f.p);
@@ -1214,9 +1216,11 @@ static void tab_forward(TabForward &f) {
     g.M = n; g.N = c.rows; g.kblocks = (int)((c.dim + KB - 1) / KB);
     g.BN = f.p.bn; g.splits = 1; g.m_first = 1; g.scale = c.scale; g.sc = c.sc; g.err = c.err;
     g.row_f = (const float *)(c.ws + f.p.row_f) + n0; g.col_f = (const float *)(c.ws + f.p.col_f);
-    g.parts = (float4 *)(c.ws + f.p.parts); g.nparts = f.p.nparts;
+    g.parts = (float4 *)(c.ws + f.p.parts); g.nparts = f.p.nparts; g.at_target = (float *)(c.ws + f.p.at_target);
+    g.targets = c.targets + n0; g.ignore_index = c.ignore_index; g.vocab = c.rows;
     f.ok = tab_launch<EPI_STATS, MATH, false, false>(q, c.w, g, f.p.pairs, c.st);
-    finish(n0, n);
+    if (MATH::NPB == 2) finish(n0, n, 1.f, TOK_LN2);
+    else finish(n0, n, to2, c.scale);
   }
 }
 

@@ -20,6 +20,20 @@ __device__ __forceinline__ float tok_ex2(float z) { float e; asm("ex2.approx.ftz
 __device__ __forceinline__ float tok_min_nan(float a, float b) { float m; asm("min.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b)); return m; }
 __device__ __forceinline__ float tok_max_nan(float a, float b) { float m; asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b)); return m; }
 
+// two fp32 numbers to an instruction
+__device__ __forceinline__ unsigned long long f32x2(float a, float b) { unsigned long long p; asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b)); return p; }
+__device__ __forceinline__ float2 f32x2_parts(unsigned long long p) { float2 f; asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p)); return f; }
+__device__ __forceinline__ unsigned long long f32x2_fma(unsigned long long a, unsigned long long b, unsigned long long c) {
+  unsigned long long d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ unsigned long long f32x2_add(unsigned long long a, unsigned long long b) {
+  unsigned long long d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 // Element types: storage type, elements of a 16-byte vector, conversions.  Results are rounded to nearest, once.
 template <class T> struct Tok;
 template <> struct Tok<float> {

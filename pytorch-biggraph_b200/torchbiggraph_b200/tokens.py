@@ -326,8 +326,10 @@ def table_logprobs(queries: torch.Tensor, table: torch.Tensor, targets: torch.Te
     """Log probabilities of rows `targets` [n] of the table under softmax(scale * queries . table^T), with the entropies and logs of the
     sums; the n x rows scores are never stored.  What token_logprobs(queries @ table.T, targets) gives, at the accuracy of
     float32 sums over the operands as they are (float32 operands are multiplied at 22 bits and more where they reach 2^-17 of the largest
-    element of their own row; what other rows hold does not matter).  Queries whose target is ignore_index are padding: 0.  NaN, or +inf, among a query's scores makes its results NaN
-    (-inf its entropy), no other query's.  Scores are float32 sums: of differences between scores beyond 1e7 nothing is left."""
+    element of their own row; what other rows hold does not matter).  Queries whose target is ignore_index
+    are padding: 0.  NaN or +inf among a query's scores makes its results NaN, -inf is a probability of 0; no other query's results change.
+    (An infinite element of more than sixteen float32 queries, or of a row of their table, makes NaN of its scores.)  Scores are float32
+    sums: of differences between scores beyond 1e7 nothing is left.  No log probability is above 0."""
     code, n, rows, dim, targets = _queries_and_table(queries, table, targets)
     device = queries.device
     r = TableLogprobs(*torch.empty((3, n), dtype=torch.float32, device=device).unbind(0))

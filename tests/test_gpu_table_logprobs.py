@@ -479,3 +479,53 @@ def test_gradients_of_uneven_inputs(n, dim, big):
     assert want[13].abs().max() > 1e-37
     tol = err.T @ Q.abs() + (w.abs().T @ Q.abs()) * (n * 2 ** -23 + planes) + want.abs() * 2 ** -24 + 1e-37 + w.abs().sum(0)[:, None] * least_q
     assert ((dt.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,rows,dim", [(5, 3000, 400), (16, 500, 2048), (100, 3000, 72), (300, 5000, 400), (700, 900, 2048), (260, 700, 4096)])
+def test_no_log_probability_above_zero(dtype, n, rows, dim):
+    """Queries that are sure of their target, whose score is large: log p is between 0 and what the others' scores allow, never on the other
+    side."""
+    g = gen(n + dim)
+    table = (torch.rand(rows, dim, device=DEV, generator=g) / math.sqrt(dim)).to(dtype)
+    targets = torch.randint(0, rows, (n,), device=DEV, generator=g)
+    for size in (30.0, 300.0, 3000.0):
+        q = (size * table[targets].float()).to(dtype)
+        r = T.table_logprobs(q, table, targets)
+        assert (r.logprob <= 0).all() and (r.entropy >= 0).all()
+        z, E = scores(q, table, 1.0)
+        logprob, _, lse = want_forward(z, targets)
+        assert ((r.logprob.double() - logprob).abs() <= 2 * E + 2e-5 * (1 + lse.abs() + logprob.abs())).all()
+
+
+@pytest.mark.parametrize("dtype,n", [(torch.float32, 3), (torch.float32, 40), (torch.bfloat16, 3), (torch.float16, 300)])
+def test_queries_whose_scores_are_all_minus_infinity(dtype, n):
+    """As a row of scores in memory: nothing is left, log probabilities of -inf and no entropy.  (Among float32 queries that are cut into planes an infinity
+    has no second part, infinity times 0: NaN.)"""
+    q, t, targets = inputs(n, 300, 8, dtype, 4)
+    t[:, 0] = 1.0
+    q[1, 0] = -math.inf
+    r, s = T.table_logprobs(q, t, targets), T.token_logprobs(q.float() @ t.float().T, targets)
+    others = torch.arange(n, device=DEV) != 1
+    assert r.lse[others].isfinite().all() and r.entropy[others].isfinite().all()
+    if dtype == torch.float32 and n > 16:
+        assert r.logprob[1].isnan() and r.lse[1].isnan() and r.entropy[1].isnan()
+    else:
+        assert r.logprob[1] == r.lse[1] == s.logprob[1] == s.lse[1] == -math.inf and r.entropy[1] == s.entropy[1] == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [3, 40, 300])
+def test_scores_far_beyond_what_float32_tells_apart(dtype, n):
+    """Nothing is left of differences between scores of 1e9; what there is is kept: the largest score has its share of p, no result is NaN and no p above
+    1."""
+    q, t, targets = inputs(n, 700, 64, dtype, 9)
+    q, t = (q.float() * 3e4 / q.float().abs().max()).to(dtype), (t.float() * 3e4 / t.float().abs().max()).to(dtype)
+    r = T.table_logprobs(q, t, targets)
+    z = q.double() @ t.double().T
+    assert z.abs().max() > 1e8
+    assert ((r.lse.double() - torch.logsumexp(z, 1)).abs() <= 1e-5 * z.abs().amax(1)).all()
+    assert (r.entropy >= 0).all() and (r.entropy <= math.log(700) + 1e-4).all() and (r.logprob <= 0).all() and r.logprob.isfinite().all()
+    g = torch.ones(n, device=DEV)
+    dq, dt = T.table_logprobs_grad(q, t, targets, r.lse, r.entropy, g, g)
+    assert not dq.isnan().any() and not dt.isnan().any()

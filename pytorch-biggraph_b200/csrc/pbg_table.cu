@@ -47,19 +47,19 @@ enum { EPI_STATS = 0, EPI_DZ = 1, EPI_OUT = 2 };
 #define TAB_STAGES_MAX 6
 #define TAB_DZ_BYTES (2ll << 30)                            // most memory for dz: beyond it the table goes in pieces
 #define TAB_PARTS_BYTES (512ll << 20)                       // and for the tiles' partial sums: beyond it the queries do
-// The tensor cores cut off what they add up instead of rounding it, a bias of half a step per addition.  Where results are fp32 the
-// contraction is therefore cut into parts, which are added in registers: blocks of k-values per part, for scores of fp32 operands (36
-// additions to a part in the forward pass, where with 18 the epilogue could not keep up, 48 in the gradient), for the products with
-// their gradient (24), and for scores of 16-bit operands (32) of more than TAB_WHOLE elements.  Products of 5000 fp32 terms were 3.9e-5
-// off in one piece and are 5e-7 off in parts.  Scores of 2048 16-bit terms are 8e-7 off in one piece and 2e-7 in parts; the registers that
-// the parts take cost 7 queries x 131,072 x 2048 bf16 12 of 102 us, so that these are left whole.
+// The tensor cores cut off what they add up instead of rounding it, a bias of half a step (2^-25 of the sum) per instruction and, of
+// products that reach below the sum's last bit, for each of its 16.  Scores and fp32 results are therefore added up in parts, which
+// are added in registers: blocks of k-values per part, 18 instructions for scores of fp32 operands, 32 for those of 16-bit operands, 24 for
+// the products with fp32 dz.  Scores of 2048 terms of one sign are 3e-7 off (fp32), 5e-7 (bf16) and 1.6e-6 (fp16, whose products are the
+// longest), in one piece 7e-7 with 36 instructions a part, 3e-6 and 7e-6; of both signs 1 to 2e-7.  The forward pass and the gradient cut the
+// scores alike, so that what is cut off is the same in z and in lse, and the p of a row add up to 1.  Both sides: with 36
+// instructions a part 4096 x 65,536 x 1024 fp32 take 7 % less time; in one piece 7 x 131,072 x 2048 bf16 take 91 us instead of 99,
+// 4099 x 65,536 x 2048 700 instead of 780.  Products of 5000 fp32 terms with dz were 3.9e-5 off in one piece.
 // 16-bit gradients are cut up too where half a step per addition comes near the result's own: 2^21 terms of one sign in one piece
 // were 1 % off; a part of TAB_PART_LONG blocks is 2^-13 off at most.
-#define TAB_PART_F32 6
+#define TAB_PART_F32 3
 #define TAB_PART_F32_OUT 2
-#define TAB_PART_F32_DZ 8
 #define TAB_PART_16 8
-#define TAB_WHOLE 2048
 #define TAB_PART_LONG 512
 
 // Eight warps share a tile's columns (two to every 32 rows), each with 4 KB of shared memory to write from; the ring of stages has the
@@ -1012,13 +1012,13 @@ static bool tab_pairs(long long M, long long N) { return M > 128 && N > 64; }
 
 template <int EPI, class MATH, bool A_MN, bool B_MN>
 static bool tab_launch(const TabOperand &a, const TabOperand &b, TabArgs &g, bool pairs, cudaStream_t st, const TabOperand *c = nullptr) {
-  g.part = MATH::NPB == 1 ? TAB_PART_16 : EPI == EPI_DZ ? TAB_PART_F32_DZ : EPI == EPI_OUT ? TAB_PART_F32_OUT : TAB_PART_F32;
+  g.part = MATH::NPB == 1 ? TAB_PART_16 : EPI == EPI_OUT ? TAB_PART_F32_OUT : TAB_PART_F32;
   auto as = [&](auto parts) {
     return pairs ? tab_launch_as<EPI, MATH, A_MN, B_MN, 2, decltype(parts)::value>(a, b, c, g, st) : tab_launch_as<EPI, MATH, A_MN, B_MN, 1, decltype(parts)::value>(a, b, c, g, st);
   };
   if constexpr (MATH::NPB > 1) return as(std::true_type());
   else {
-    if constexpr (EPI == EPI_STATS) if (g.kblocks > TAB_WHOLE / 64) return as(std::true_type());
+    if constexpr (EPI != EPI_OUT) if (g.kblocks > TAB_PART_16) return as(std::true_type());
     if constexpr (EPI == EPI_OUT && !(A_MN && MATH::NPA == 2))            // (two planes and the contraction over queries: 128 of them at most)
       if (g.kblocks > TAB_PART_LONG) {
         g.part = TAB_PART_LONG;

@@ -529,3 +529,28 @@ def test_scores_far_beyond_what_float32_tells_apart(dtype, n):
     g = torch.ones(n, device=DEV)
     dq, dt = T.table_logprobs_grad(q, t, targets, r.lse, r.entropy, g, g)
     assert not dq.isnan().any() and not dt.isnan().any()
+
+
+def lse_size(z):
+    return torch.logsumexp(z, 1).abs()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,dim", [(20, 2048), (100, 4096), (100, 16_384), (20, 65_536)])
+def test_probabilities_of_long_rows_add_up_to_one(dtype, n, dim):
+    """Scores around 50 whose terms have one sign, so that what a sum cuts off adds up.  The last column of the table is 1: the queries' gradient
+    there is the sum of dz, g (1 - sum p).  With z and lse cut alike p is off by the roundings of z and lse, 50 * 3 * 2^-24 < 1e-5, by ex2 and by
+    the sums, 2e-6; dz is rounded to 16 bits or more (two planes), the target's by 2^-17 of g."""
+    g = gen(dim)
+    q, t = torch.rand(n, dim, device=DEV, generator=g).to(dtype), torch.rand(300, dim, device=DEV, generator=g).to(dtype)
+    t[:, -1] = 1.0
+    targets = torch.randint(0, 300, (n,), device=DEV, generator=g)
+    scale = 200.0 / dim
+    r = T.table_logprobs(q, t, targets, scale=scale)
+    z, _ = scores(q, t, scale)
+    # the sums against 64 bits.  An instruction adds 16 products, each cut off at the sum's last bit as the sum itself is: 17 times 2^-25 of the sum so
+    # far, half of a part's in the mean, 32 times to a part; the parts are added in fp32 (2^-25 each, in the mean) and lse and z rounded
+    tol = lse_size(z) * (32 * 17 * 2 ** -26 + dim / 512 * 2 ** -25 + 4 * 2 ** -24) + 2e-6
+    assert ((r.lse.double() - torch.logsumexp(z, 1)).abs() <= tol).all()
+    dq, _ = T.table_logprobs_grad(q, t, targets, r.lse, None, torch.full((n,), 1.0 / scale, device=DEV), scale=scale)
+    assert dq[:, -1].abs().max() <= 1.2e-5 + 2 ** -17 + 2 ** -17 * 0.5

@@ -4,8 +4,9 @@
 //   gradient  dz = s (g ([v = t] - p) - h p (log p + H));  dQ = dz W,  dW = dz^T Q   6 N V D operations (the scores once more)
 //
 // All products run on the tensor cores (tcgen05, kind::f16) with fp32 accumulators in tensor memory:
-//   bf16, fp16   the tensors themselves are the operands, read by TMA where they lie; dz is rounded to the operands' type (that of
-//                fp16 scaled by a power of two so that it cannot leave the type's range: its bound is known from g and h)
+//   bf16, fp16   the tensors themselves are the operands, read by TMA where they lie; dz is rounded to the operands' type, or kept in two
+//                planes of it (tab_place).  That of fp16 is scaled by a power of two so that its bound, known from g and h, lies below 2^14:
+//                what is cut off below fp16's smallest step is 2^-39 of the bound, and results in fp16 end at 2^-25
 //   fp32         scores: every operand as two fp16 planes, x 2^k = b0 + b1 (22 bits; k from the largest finite element of its row, so
 //                that the planes of everything down to 2^-17 of it are whole), and the three products b1 b0 + b0 b1 + b0 b0: the dropped
 //                b1 b1 is 2^-22 of a product, the size of fp32 rounding.  The powers leave the scores as factors of a row and of a column;
@@ -1019,7 +1020,7 @@ static bool tab_launch(const TabOperand &a, const TabOperand &b, TabArgs &g, boo
   if constexpr (MATH::NPB > 1) return as(std::true_type());
   else {
     if constexpr (EPI != EPI_OUT) if (g.kblocks > TAB_PART_16) return as(std::true_type());
-    if constexpr (EPI == EPI_OUT && !(A_MN && MATH::NPA == 2))            // (two planes and the contraction over queries: 128 of them at most)
+    if constexpr (EPI == EPI_OUT)
       if (g.kblocks > TAB_PART_LONG) {
         g.part = TAB_PART_LONG;
         return as(std::true_type());
@@ -1042,7 +1043,7 @@ struct TabPlace {
   bool pairs, few;
 };
 static bool tab_few(long long n, int dim, int dtype);
-static TabPlace tab_place(long long n, long long rows, int dim, int dtype, bool grad) {
+static TabPlace tab_place(long long n, long long rows, int dim, int dtype, bool grad, bool fine = false) {
   TabPlace p;
   p.npl = dtype == PBG_F32 ? 2 : 1;
   p.ld = tok_up(dim, 64);
@@ -1079,9 +1080,11 @@ static TabPlace tab_place(long long n, long long rows, int dim, int dtype, bool 
     p.at_target = at + p.piece * p.nparts * 16;
     at = p.at_target + p.piece * 4;
   } else {
-    // dz of 16-bit operands in two planes where the queries leave most of a tile's rows idle: few targets do not average the
-    // rounding of dz out, and the products with more planes cost nothing that the reading of the table does not cover
-    p.dz_planes = dtype == PBG_F32 ? 3 : n <= 128 ? 2 : 1;
+    // dz of 16-bit operands in one plane is rounded as the results are, and these come out 2.3e-3 off (bf16; 3.8e-3 where the table's rows have
+    // much in common) instead of 1.7e-3, what their own rounding leaves.  Two planes keep 16 bits of it; they cost half as much time again
+    // (4099 x 65,536 x 2048: 2.7 and 4.2 ms; 1000 x 65,536 x 1024: 0.39 and 0.64), but nothing where the queries leave most of a tile's
+    // rows idle and the reading of the table covers the products.
+    p.dz_planes = dtype == PBG_F32 ? 3 : n <= 128 || fine ? 2 : 1;
     long long most = TAB_DZ_BYTES / (2 * p.dz_planes * n) / 256 * 256;
     if (most < 256) most = 256;
     p.columns = rows < most ? rows : most;
@@ -1292,11 +1295,11 @@ static void tab_backward(TabBackward &f) {
   }
 }
 
-static int tab_check(const TabCall &c, int64_t bytes, bool grad) {
+static int tab_check(const TabCall &c, int64_t bytes, bool grad, bool fine = false) {
   if (c.n < 0 || c.rows <= 0 || c.dim <= 0 || c.q_stride < 0 || c.t_stride < 0 || !tok_type(c.dtype) || !tok_scale(c.scale)) return PBG_ERR_BAD_ARGUMENT;
   if (c.dim > 65536 || c.n > (1ll << 30) || c.rows > 0x7fffffffll - 65536) return PBG_ERR_TOO_LARGE;
   if (c.n == 0) return PBG_OK;
-  if (!c.queries || !c.table || !c.targets || !c.ws || ((uintptr_t)c.ws & 255) || bytes < tab_place(c.n, c.rows, c.dim, c.dtype, grad).bytes) return PBG_ERR_BAD_ARGUMENT;
+  if (!c.queries || !c.table || !c.targets || !c.ws || ((uintptr_t)c.ws & 255) || bytes < tab_place(c.n, c.rows, c.dim, c.dtype, grad, fine).bytes) return PBG_ERR_BAD_ARGUMENT;
   // rows that TMA reads where they lie: eight of them, a plane's stride, are less than 2^40 bytes
   if (c.q_stride >= (1ll << 36) || c.t_stride >= (1ll << 36)) return PBG_ERR_TOO_LARGE;
   return PBG_OK;
@@ -1304,7 +1307,7 @@ static int tab_check(const TabCall &c, int64_t bytes, bool grad) {
 
 extern "C" int64_t pbg_table_logprobs_workspace(int64_t n, int64_t rows, int32_t dim, int32_t dtype, int32_t grad) {
   if (n <= 0 || rows <= 0 || dim <= 0 || !tok_type(dtype) || n > (1ll << 30) || rows > 0x7fffffffll) return 0;
-  return tab_place(n, rows, dim, dtype, grad != 0).bytes;
+  return tab_place(n, rows, dim, dtype, grad != 0, grad == 2).bytes;
 }
 
 extern "C" int pbg_table_logprobs(const void *queries, int64_t q_stride, int64_t n, const void *table, int64_t t_stride, int64_t rows, int32_t dim, int32_t dtype,
@@ -1325,12 +1328,12 @@ extern "C" int pbg_table_logprobs(const void *queries, int64_t q_stride, int64_t
   return f.ok ? status : PBG_ERR_CUDA;
 }
 
-extern "C" int pbg_table_logprobs_grad(const void *queries, int64_t q_stride, int64_t n, const void *table, int64_t t_stride, int64_t rows, int32_t dim, int32_t dtype,
-                                       const int64_t *targets, int64_t ignore_index, float scale, const float *lse, const float *entropy, const float *grad_logprob,
-                                       const float *grad_entropy, void *grad_queries, void *grad_table, void *workspace, int64_t workspace_bytes, int32_t *errors, void *stream) {
+static int tab_grad(const void *queries, int64_t q_stride, int64_t n, const void *table, int64_t t_stride, int64_t rows, int32_t dim, int32_t dtype,
+                    const int64_t *targets, int64_t ignore_index, float scale, const float *lse, const float *entropy, const float *grad_logprob,
+                    const float *grad_entropy, void *grad_queries, void *grad_table, void *workspace, int64_t workspace_bytes, int32_t *errors, void *stream, bool fine) {
   TabBackward f{{queries, q_stride, n, table, t_stride, rows, dim, dtype, (const long long *)targets, ignore_index, scale, (unsigned char *)workspace, errors, (cudaStream_t)stream},
                 {}, lse, entropy, grad_logprob, grad_entropy, grad_queries, grad_table, true};
-  const int rc = tab_check(f.c, workspace_bytes, true);
+  const int rc = tab_check(f.c, workspace_bytes, true, fine);
   if (rc != PBG_OK) return rc;
   pbg_launch_error() = cudaSuccess;
   if (n == 0) {
@@ -1339,7 +1342,7 @@ extern "C" int pbg_table_logprobs_grad(const void *queries, int64_t q_stride, in
   }
   if (!lse || (grad_entropy && !entropy) || (!grad_queries && !grad_table)) return PBG_ERR_BAD_ARGUMENT;
   if (!get_encode()) return PBG_ERR_CUDA;
-  f.p = tab_place(n, rows, dim, dtype, true);
+  f.p = tab_place(n, rows, dim, dtype, true, fine);
   if (dtype == PBG_F32) tab_backward<float, TabF32, TabF32Out>(f);
   else if (dtype == PBG_BF16) {
     if (f.p.dz_planes == 2) tab_backward<__nv_bfloat16, TabBf16, TabBf16Fine>(f);
@@ -1350,4 +1353,17 @@ extern "C" int pbg_table_logprobs_grad(const void *queries, int64_t q_stride, in
   }
   const int status = tok_status();
   return f.ok ? status : PBG_ERR_CUDA;
+}
+extern "C" int pbg_table_logprobs_grad(const void *queries, int64_t q_stride, int64_t n, const void *table, int64_t t_stride, int64_t rows, int32_t dim, int32_t dtype,
+                                       const int64_t *targets, int64_t ignore_index, float scale, const float *lse, const float *entropy, const float *grad_logprob,
+                                       const float *grad_entropy, void *grad_queries, void *grad_table, void *workspace, int64_t workspace_bytes, int32_t *errors, void *stream) {
+  return tab_grad(queries, q_stride, n, table, t_stride, rows, dim, dtype, targets, ignore_index, scale, lse, entropy, grad_logprob, grad_entropy, grad_queries, grad_table,
+                  workspace, workspace_bytes, errors, stream, false);
+}
+extern "C" int pbg_table_logprobs_grad_fine(const void *queries, int64_t q_stride, int64_t n, const void *table, int64_t t_stride, int64_t rows, int32_t dim, int32_t dtype,
+                                            const int64_t *targets, int64_t ignore_index, float scale, const float *lse, const float *entropy, const float *grad_logprob,
+                                            const float *grad_entropy, void *grad_queries, void *grad_table, void *workspace, int64_t workspace_bytes, int32_t *errors,
+                                            void *stream) {
+  return tab_grad(queries, q_stride, n, table, t_stride, rows, dim, dtype, targets, ignore_index, scale, lse, entropy, grad_logprob, grad_entropy, grad_queries, grad_table,
+                  workspace, workspace_bytes, errors, stream, true);
 }

@@ -354,7 +354,9 @@ int pbg_token_logprobs_grad_wide(const void *logits, int64_t row_stride, int64_t
  * results NaN and -inf is a probability of 0; no other query's results change.  (An infinite element of more than sixteen fp32 queries, or
  * of a row of their table, makes NaN of its scores.)  Scores are fp32 sums: beyond 1e7 in size nothing is left of their
  * differences.  logprob is never above 0.
- * workspace: of pbg_table_logprobs_workspace(n, rows, dim, dtype, 0) bytes. */
+ * workspace: of pbg_table_logprobs_workspace(n, rows, dim, dtype, 0) bytes: room for copies of the operands, (n + rows) * ld elements
+ * of the table's type (ld: dim rounded up to 64), needed or not, and for partial sums at most 512 MiB, or 64 bytes per row of the table
+ * if that is more.  Up to sixteen fp32 queries: 16 bytes for each of them and of the SMs, no copies. */
 int64_t pbg_table_logprobs_workspace(int64_t n, int64_t rows, int32_t dim, int32_t dtype, int32_t grad);
 int pbg_table_logprobs(const void *queries, int64_t q_stride, int64_t n, const void *table, int64_t t_stride, int64_t rows,
                        int32_t dim, int32_t dtype, const int64_t *targets, int64_t ignore_index, float scale,
@@ -372,7 +374,9 @@ int32_t pbg_table_logprobs_wait_limit(int32_t limit);
  * as long again, and its workspace is asked for with grad = 2).  fp32: three bf16 parts of it and of the operands; elements below 2^-150 of
  * the largest of their matrix lose bits.
  * NaN or an infinity in the table makes grad_queries NaN, padding's rows too; one in a query that counts makes its row and grad_table NaN.
- * workspace: of pbg_table_logprobs_workspace(n, rows, dim, dtype, 1) bytes, at most about 2 GiB beside copies of the operands. */
+ * workspace: of pbg_table_logprobs_workspace(n, rows, dim, dtype, 1) bytes: copies as in the forward pass (fp32: two and a half
+ * times as much), dz, at most 2 GiB or 256 columns of it, and, where the table goes in pieces or the sum over its rows in parts,
+ * partial sums of grad_queries in fp32: n * dim of them, or a multiple of that up to 512 MiB. */
 int pbg_table_logprobs_grad(const void *queries, int64_t q_stride, int64_t n, const void *table, int64_t t_stride, int64_t rows,
                             int32_t dim, int32_t dtype, const int64_t *targets, int64_t ignore_index, float scale,
                             const float *lse, const float *entropy, const float *grad_logprob, const float *grad_entropy,

@@ -48,6 +48,7 @@ enum { EPI_STATS = 0, EPI_DZ = 1, EPI_OUT = 2 };
 #define TAB_STAGES_MAX 6
 #define TAB_DZ_BYTES (2ll << 30)                            // most memory for dz: beyond it the table goes in pieces
 #define TAB_PARTS_BYTES (512ll << 20)                       // and for the tiles' partial sums: beyond it the queries do
+#define TAB_SPLIT_BYTES (512ll << 20)                       // and for the parts of dQ
 // The tensor cores cut off what they add up instead of rounding it, a bias of half a step (2^-25 of the sum) per instruction and, of
 // products that reach below the sum's last bit, for each of its 16.  Scores and fp32 results are therefore added up in parts, which
 // are added in registers: blocks of k-values per part, 18 instructions for scores of fp32 operands, 32 for those of 16-bit operands, 24 for
@@ -1001,7 +1002,7 @@ static int tab_splits(long long n, long long dim, long long K, int products) {
   const long long tiles = (n + (pairs ? 255 : 127)) / (pairs ? 256 : 128) * ((dim + 255) / 256);
   int best = 1;
   double cost = 0.;
-  for (int s = 1; s <= 64 && (s == 1 || s * 512ll <= K); ++s) {
+  for (int s = 1; s <= 64 && (s == 1 || (s * 512ll <= K && 4ll * s * n * dim <= TAB_SPLIT_BYTES)); ++s) {
     const double rounds = (double)((tiles * s + groups - 1) / groups) / s;
     const double c = rounds * ((double)K / 16 * products * 128 / 1.7) + (s > 1 ? 3000. + s * 8. * n * dim / 5000. : 0.);
     if (s == 1 || c < cost) { cost = c; best = s; }

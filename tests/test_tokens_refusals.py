@@ -162,3 +162,25 @@ def test_scales_out_of_range(scale):
     assert L.pbg_table_logprobs_grad(*a.values(), P, P, P, P, P, P, P, L.pbg_table_logprobs_workspace(4, 100, 8, 1, 1), None, None) == BAD
     with pytest.raises(ValueError, match="scale"):
         T.tokens._scale(scale, True)
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("n,rows,dim", [(1, 1, 1), (7, 131_072, 2048), (16, 65_536, 3000), (17, 65_536, 2048), (1000, 14_951, 400), (5000, 14_951, 400), (4099, 65_536, 2048),
+                                        (1 << 20, 131_072, 2048), (1 << 22, 1000, 64), (100, 20_000_000, 64), (30_000, 18_100, 16), (300, 1 << 20, 100), (2000, 500_000, 128)])
+def test_workspaces_are_as_large_as_the_header_says(dtype, n, rows, dim):
+    L = _lib.lib()
+    size, ld, some = (4 if dtype == 0 else 2), (dim + 63) // 64 * 64, 16_384                  # (some: what is rounded up, scales, maxima)
+    copies, sums = (n + rows) * ld * size + 4 * (n + rows if dtype == 0 else 0), max(512 << 20, 64 * (rows + 256))
+    forward = L.pbg_table_logprobs_workspace(n, rows, dim, dtype, 0)
+    if dtype == 0 and n <= 16:
+        assert 0 < forward <= 20 * n * 256 + some
+    else:
+        assert copies <= forward <= copies + sums + 4 * n + some
+    planes = 3 if dtype == 0 else 2
+    for grad in (1, 2):
+        got = L.pbg_table_logprobs_workspace(n, rows, dim, dtype, grad)
+        dz = max(2 << 30, 2 * planes * n * 256)
+        most = (2.5 if dtype == 0 else 1) * copies + 4 * (n + rows) + dz + max(512 << 20, 4 * n * dim) + some
+        assert copies <= got <= most, (got, most)
+        if rows * n * planes * 2 <= 1 << 30 and n * dim * 4 <= 1 << 20:                       # small ones do not ask for the limits
+            assert got <= (2.5 if dtype == 0 else 1) * copies + 4 * (n + rows) + n * (rows + 64) * planes * 2 + 64 * 4 * n * dim + some

@@ -490,7 +490,7 @@ static void lookup_launch(const LookupCall &c) {
 template <class T, int N>
 static void lookup_units(const LookupCall &c) {
   // Four units per thread hide the loads' latency where there is work for all SMs; a few rows are spread as thin as they go.
-  if (c.n * (c.dim / N) >= 148ll * 1024) lookup_launch<T, N, 4>(c);
+  if (c.n * (c.dim / N) >= 1024ll * pbg_sm_count()) lookup_launch<T, N, 4>(c);
   else lookup_launch<T, N, 1>(c);
 }
 template <class T>

@@ -521,3 +521,31 @@ def test_offsets_beyond_32_bits():
     assert r.top_ids[-1, 0] == logits[-1].float().argmax()
     d = T.token_logprobs_grad(logits, targets, r.lse, None, torch.ones(2200, device=DEV), out=logits)
     assert abs(d[-1].float().sum().item()) < 1024 * 1000 * 2 ** -9 * 1e-3 and (d[-2] == 0).all()
+
+
+@pytest.mark.parametrize("own", [False, True])
+def test_rows_of_scores_beyond_2_to_the_31_elements(own):
+    """Every result of the rows that begin, or go on, behind the 2^31st element, against the definition: a target, a score or a result taken from an offset
+    cut to 32 bits would be another row's."""
+    n, vocab = 2104, 1_024_000                                   # the 2098th row holds element 2^31
+    logits = torch.zeros(n, vocab, dtype=torch.bfloat16, device=DEV)
+    rows = [0, 2096, 2097, 2098, 2103]
+    for k, row in enumerate(rows):
+        logits[row] = torch.randn(vocab, device=DEV, generator=gen(row)) + k
+    targets = torch.full((n,), -100, device=DEV)
+    at = torch.tensor(rows, device=DEV)
+    targets[at] = torch.tensor([5, vocab - 1, 700_000, 0, 512_001], device=DEV)
+    x = logits[at].clone()
+    r = T.token_logprobs(logits, targets, top=3)
+    logprob, ent, lse, rank, best, ids = _want(x, targets[at], 1.0, 3)
+    close(r.lse[at], lse, 2e-5, 1 + lse.abs())
+    close(r.logprob[at], logprob, 2e-5, 1 + lse.abs() + logprob.abs())
+    close(r.entropy[at], ent, 2e-5, 1 + ent + math.log(vocab))
+    assert torch.equal(r.rank[at], rank) and torch.equal(r.top_ids[at], ids)
+    g = torch.randn(n, device=DEV, generator=gen(1))
+    want, size = _want_grad(x, targets[at], 1.0, r.lse[at], r.entropy[at], g[at], 0.5 * g[at])
+    got = T.token_logprobs_grad(logits, targets, r.lse, r.entropy, g, 0.5 * g, lse_rest=r.lse_rest, out=logits if own else None)
+    close(got[at], want, 1.0, half_step(torch.bfloat16) * want.abs() + 2e-5 * size + torch.expm1(2 ** -23 * lse.abs())[:, None] * size, torch.finfo(torch.bfloat16).smallest_normal)
+    between = torch.ones(n, dtype=torch.bool, device=DEV)
+    between[at] = False
+    assert not got[between].any()

@@ -563,10 +563,11 @@ static void logprobs_type(const LogprobCall &c) {
   const int sms = pbg_sm_count();
   while (nct < 8 && c.n * nct < 2 * sms && 2 * nct * 8 <= steps) nct *= 2;
   // Four warps to a CTA once there are more rows than CTAs of eight warps at a time: twice as many rows are under way, and one row's joins
-  // and best scores, all waiting, are hidden behind others' scans (4096 x 14,951 bf16 with the best 8: 65 and 49 us; 592 rows of 50,257:
-  // 20 and 21, 700: 25 and 24; two warps gain nothing on 300 scores and lose on 4096).  Not where a second turn of them would be half
-  // empty, unless the rows are short (1500 x 131,072 fp32: 129 and 149).
-  const bool half_empty = c.n > 8ll * sms && c.n <= 12ll * sms && (c.a.top == 0 || c.a.vocab * (long long)sizeof(T) > 128 * 1024);
+  // and best scores, all waiting, are hidden behind others' scans (bf16, eight warps and four: 2368 x 14,951 with the best 8 36 and 28 us,
+  // 131,072 140 and 136; two warps gain nothing on 300 scores and lose on 4096).  Not for long rows where a second turn of four-warp CTAs,
+  // eight to an SM, would be half empty: 1500 rows of 131,072 fp32 126 and 143, of 131,072 bf16 84 and 86, of 50,257 fp32 56 and 61;
+  // of 50,257 bf16 39.7 and 38.8, of 14,951 16.5 and 14.5.  128 KB is the size between these.
+  const bool half_empty = c.n > 8ll * sms && c.n <= 12ll * sms && c.a.vocab * (long long)sizeof(T) > 128 * 1024;
   const bool eight = c.n <= 4ll * sms || half_empty;
   void (*kernel)(const T *, LogprobArgs) = eight ? (c.a.top > 0 ? logprobs_kernel<T, true, 8> : logprobs_kernel<T, false, 8>)
                                                  : (c.a.top > 0 ? logprobs_kernel<T, true, 4> : logprobs_kernel<T, false, 4>);

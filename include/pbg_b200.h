@@ -369,9 +369,10 @@ int32_t pbg_table_logprobs_wait_limit(int32_t limit);
 
 /* Gradients of sum(grad_logprob * logprob + grad_entropy * entropy) with respect to the queries [n, dim] and the table [rows, dim],
  * rows one behind the other, of their type; either may be NULL (not wanted).  lse, entropy: of the forward call.  The scores are
- * computed again; their gradient is rounded to the operands' type for the two products, or, up to 128 queries and by the second form, kept in
- * two parts of it (bf16 results are 2.3e-3 off in the first case, 1.7e-3 in the second, which their own rounding is; the second form takes half
- * as long again, and its workspace is asked for with grad = 2).  fp32: three bf16 parts of it and of the operands; elements below 2^-150 of
+ * computed again; their gradient is kept in two parts of the operands' type for the two products.  The second form rounds it to that type above
+ * 128 queries: a third less time, bf16 results 2.3e-3 off instead of the 1.7e-3 of their own rounding (more where all rows of the table
+ * have much in common); its workspace is asked for with grad = 2.  Of fp16's, what lies below 2^-39 of the largest |g| + 23 |h| is
+ * cut off.  fp32: three bf16 parts of it and of the operands; elements below 2^-150 of
  * the largest of their matrix lose bits.
  * NaN or an infinity in the table makes grad_queries NaN, padding's rows too; one in a query that counts makes its row and grad_table NaN.
  * workspace: of pbg_table_logprobs_workspace(n, rows, dim, dtype, 1) bytes: copies as in the forward pass (fp32: two and a half
@@ -382,7 +383,7 @@ int pbg_table_logprobs_grad(const void *queries, int64_t q_stride, int64_t n, co
                             const float *lse, const float *entropy, const float *grad_logprob, const float *grad_entropy,
                             void *grad_queries, void *grad_table, void *workspace, int64_t workspace_bytes,
                             int32_t *errors, void *stream);
-int pbg_table_logprobs_grad_fine(const void *queries, int64_t q_stride, int64_t n, const void *table, int64_t t_stride, int64_t rows,
+int pbg_table_logprobs_grad_rounded(const void *queries, int64_t q_stride, int64_t n, const void *table, int64_t t_stride, int64_t rows,
                             int32_t dim, int32_t dtype, const int64_t *targets, int64_t ignore_index, float scale,
                             const float *lse, const float *entropy, const float *grad_logprob, const float *grad_entropy,
                             void *grad_queries, void *grad_table, void *workspace, int64_t workspace_bytes,

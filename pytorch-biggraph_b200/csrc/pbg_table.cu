@@ -4,8 +4,8 @@
 //   gradient  dz = s (g ([v = t] - p) - h p (log p + H));  dQ = dz W,  dW = dz^T Q   6 N V D operations (the scores once more)
 //
 // All products run on the tensor cores (tcgen05, kind::f16) with fp32 accumulators in tensor memory:
-//   bf16, fp16   the tensors themselves are the operands, read by TMA where they lie; dz is rounded to the operands' type, or kept in two
-//                planes of it (tab_place).  That of fp16 is scaled by a power of two so that its bound, known from g and h, lies below 2^14:
+//   bf16, fp16   the tensors themselves are the operands, read by TMA where they lie; dz is kept in two planes of the operands' type, or
+//                rounded to it (tab_place).  That of fp16 is scaled by a power of two so that its bound, known from g and h, lies below 2^14:
 //                what is cut off below fp16's smallest step is 2^-39 of the bound, and results in fp16 end at 2^-25
 //   fp32         scores: every operand as two fp16 planes, x 2^k = b0 + b1 (22 bits; k from the largest finite element of its row, so
 //                that the planes of everything down to 2^-17 of it are whole), and the three products b1 b0 + b0 b1 + b0 b0: the dropped
@@ -1044,7 +1044,7 @@ struct TabPlace {
   bool pairs, few;
 };
 static bool tab_few(long long n, int dim, int dtype);
-static TabPlace tab_place(long long n, long long rows, int dim, int dtype, bool grad, bool fine = false) {
+static TabPlace tab_place(long long n, long long rows, int dim, int dtype, bool grad, bool rounded = false) {
   TabPlace p;
   p.npl = dtype == PBG_F32 ? 2 : 1;
   p.ld = tok_up(dim, 64);
@@ -1081,11 +1081,11 @@ static TabPlace tab_place(long long n, long long rows, int dim, int dtype, bool 
     p.at_target = at + p.piece * p.nparts * 16;
     at = p.at_target + p.piece * 4;
   } else {
-    // dz of 16-bit operands in one plane is rounded as the results are, and these come out 2.3e-3 off (bf16; 3.8e-3 where the table's rows have
-    // much in common) instead of 1.7e-3, what their own rounding leaves.  Two planes keep 16 bits of it; they cost half as much time again
-    // (4099 x 65,536 x 2048: 2.7 and 4.2 ms; 1000 x 65,536 x 1024: 0.39 and 0.64), but nothing where the queries leave most of a tile's
-    // rows idle and the reading of the table covers the products.
-    p.dz_planes = dtype == PBG_F32 ? 3 : n <= 128 || fine ? 2 : 1;
+    // dz of 16-bit operands keeps 16 bits or more in two planes of their type, and results are off by their own rounding (bf16 1.7e-3).  In one
+    // plane it is rounded as they are: 2.3e-3, 3.8e-3 where the table's rows have much in common, for a third less time (4099 x 65,536 x 2048:
+    // 4.2 and 2.7 ms; 1000 x 65,536 x 1024: 0.64 and 0.39).  Where the queries leave most of a tile's rows idle the reading of the
+    // table covers the products, and one plane gains nothing.
+    p.dz_planes = dtype == PBG_F32 ? 3 : rounded && n > 128 ? 1 : 2;
     long long most = TAB_DZ_BYTES / (2 * p.dz_planes * n) / 256 * 256;
     if (most < 256) most = 256;
     p.columns = rows < most ? rows : most;
@@ -1296,11 +1296,11 @@ static void tab_backward(TabBackward &f) {
   }
 }
 
-static int tab_check(const TabCall &c, int64_t bytes, bool grad, bool fine = false) {
+static int tab_check(const TabCall &c, int64_t bytes, bool grad, bool rounded = false) {
   if (c.n < 0 || c.rows <= 0 || c.dim <= 0 || c.q_stride < 0 || c.t_stride < 0 || !tok_type(c.dtype) || !tok_scale(c.scale)) return PBG_ERR_BAD_ARGUMENT;
   if (c.dim > 65536 || c.n > (1ll << 30) || c.rows > 0x7fffffffll - 65536) return PBG_ERR_TOO_LARGE;
   if (c.n == 0) return PBG_OK;
-  if (!c.queries || !c.table || !c.targets || !c.ws || ((uintptr_t)c.ws & 255) || bytes < tab_place(c.n, c.rows, c.dim, c.dtype, grad, fine).bytes) return PBG_ERR_BAD_ARGUMENT;
+  if (!c.queries || !c.table || !c.targets || !c.ws || ((uintptr_t)c.ws & 255) || bytes < tab_place(c.n, c.rows, c.dim, c.dtype, grad, rounded).bytes) return PBG_ERR_BAD_ARGUMENT;
   // rows that TMA reads where they lie: eight of them, a plane's stride, are less than 2^40 bytes
   if (c.q_stride >= (1ll << 36) || c.t_stride >= (1ll << 36)) return PBG_ERR_TOO_LARGE;
   return PBG_OK;
@@ -1331,10 +1331,10 @@ extern "C" int pbg_table_logprobs(const void *queries, int64_t q_stride, int64_t
 
 static int tab_grad(const void *queries, int64_t q_stride, int64_t n, const void *table, int64_t t_stride, int64_t rows, int32_t dim, int32_t dtype,
                     const int64_t *targets, int64_t ignore_index, float scale, const float *lse, const float *entropy, const float *grad_logprob,
-                    const float *grad_entropy, void *grad_queries, void *grad_table, void *workspace, int64_t workspace_bytes, int32_t *errors, void *stream, bool fine) {
+                    const float *grad_entropy, void *grad_queries, void *grad_table, void *workspace, int64_t workspace_bytes, int32_t *errors, void *stream, bool rounded) {
   TabBackward f{{queries, q_stride, n, table, t_stride, rows, dim, dtype, (const long long *)targets, ignore_index, scale, (unsigned char *)workspace, errors, (cudaStream_t)stream},
                 {}, lse, entropy, grad_logprob, grad_entropy, grad_queries, grad_table, true};
-  const int rc = tab_check(f.c, workspace_bytes, true, fine);
+  const int rc = tab_check(f.c, workspace_bytes, true, rounded);
   if (rc != PBG_OK) return rc;
   pbg_launch_error() = cudaSuccess;
   if (n == 0) {
@@ -1343,7 +1343,7 @@ static int tab_grad(const void *queries, int64_t q_stride, int64_t n, const void
   }
   if (!lse || (grad_entropy && !entropy) || (!grad_queries && !grad_table)) return PBG_ERR_BAD_ARGUMENT;
   if (!get_encode()) return PBG_ERR_CUDA;
-  f.p = tab_place(n, rows, dim, dtype, true, fine);
+  f.p = tab_place(n, rows, dim, dtype, true, rounded);
   if (dtype == PBG_F32) tab_backward<float, TabF32, TabF32Out>(f);
   else if (dtype == PBG_BF16) {
     if (f.p.dz_planes == 2) tab_backward<__nv_bfloat16, TabBf16, TabBf16Fine>(f);
@@ -1361,7 +1361,7 @@ extern "C" int pbg_table_logprobs_grad(const void *queries, int64_t q_stride, in
   return tab_grad(queries, q_stride, n, table, t_stride, rows, dim, dtype, targets, ignore_index, scale, lse, entropy, grad_logprob, grad_entropy, grad_queries, grad_table,
                   workspace, workspace_bytes, errors, stream, false);
 }
-extern "C" int pbg_table_logprobs_grad_fine(const void *queries, int64_t q_stride, int64_t n, const void *table, int64_t t_stride, int64_t rows, int32_t dim, int32_t dtype,
+extern "C" int pbg_table_logprobs_grad_rounded(const void *queries, int64_t q_stride, int64_t n, const void *table, int64_t t_stride, int64_t rows, int32_t dim, int32_t dtype,
                                             const int64_t *targets, int64_t ignore_index, float scale, const float *lse, const float *entropy, const float *grad_logprob,
                                             const float *grad_entropy, void *grad_queries, void *grad_table, void *workspace, int64_t workspace_bytes, int32_t *errors,
                                             void *stream) {

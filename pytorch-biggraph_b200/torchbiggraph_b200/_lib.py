@@ -95,7 +95,7 @@ SYMBOLS = [
                                      _P, _P, _P, _P, C.c_int64, _P, _P]),
     ("pbg_table_logprobs_grad", C.c_int, [_P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64, C.c_int32, C.c_int32, _P, C.c_int64, C.c_float,
                                           _P, _P, _P, _P, _P, _P, _P, C.c_int64, _P, _P]),
-    ("pbg_table_logprobs_grad_fine", C.c_int, [_P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64, C.c_int32, C.c_int32, _P, C.c_int64, C.c_float,
+    ("pbg_table_logprobs_grad_rounded", C.c_int, [_P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64, C.c_int32, C.c_int32, _P, C.c_int64, C.c_float,
                                           _P, _P, _P, _P, _P, _P, _P, C.c_int64, _P, _P]),
     ("pbg_table_logprobs_wait_limit", C.c_int32, [C.c_int32]),
     ("pbg_launch_count", C.c_int64, [_P]),

@@ -341,22 +341,22 @@ def table_logprobs(queries: torch.Tensor, table: torch.Tensor, targets: torch.Te
 
 def table_logprobs_grad(queries: torch.Tensor, table: torch.Tensor, targets: torch.Tensor, lse: torch.Tensor, entropy: Optional[torch.Tensor],
                         grad_logprob: Optional[torch.Tensor], grad_entropy: Optional[torch.Tensor] = None, *, scale: float = 1.0,
-                        ignore_index: int = IGNORE_INDEX, errors: Optional[torch.Tensor] = None, fine: bool = False):
+                        ignore_index: int = IGNORE_INDEX, errors: Optional[torch.Tensor] = None, rounded: bool = False):
     """Gradients (of the queries, of the table) of sum(grad_logprob * logprob + grad_entropy * entropy), from the lse and the entropy that
     table_logprobs returned (the entropy only where grad_entropy is given).  Queries that are padding, and those whose
     target is out of range, get zeros and add nothing to the table's gradient, whatever they hold -- unless the table holds NaN or
     infinities, which reach all gradients of the queries.
 
-    16-bit operands: the gradient of the scores is rounded to their type before it is multiplied with the table and the queries, above 128 queries unless
-    fine=True.  bf16 results are then 2.3e-3 off instead of the 1.7e-3 of their own rounding (more where all rows of the table have much in common);
-    fine=True takes half as long again."""
+    16-bit operands: the gradient of the scores keeps 16 bits or more on its way into the two products.  rounded=True rounds it to the
+    operands' type above 128 queries, as training in 16 bits commonly does: a third less time, bf16 results 2.3e-3 off instead of the 1.7e-3
+    of their own rounding (more where all rows of the table have much in common)."""
     code, n, rows, dim, targets = _queries_and_table(queries, table, targets)
     device = queries.device
     lse, entropy, grad_logprob, grad_entropy = _row_grads(n, device, lse, entropy, grad_logprob, grad_entropy)
     dq = torch.empty((n, dim), dtype=queries.dtype, device=device)
     dt = torch.empty((rows, dim), dtype=table.dtype, device=device)
-    ws, size = _workspace("pbg_table_logprobs_workspace", device, n, rows, dim, code, 2 if fine else 1)
-    _call("pbg_table_logprobs_grad_fine" if fine else "pbg_table_logprobs_grad", device, queries.data_ptr(), _row_stride(queries), n, table.data_ptr(), _row_stride(table), rows, dim, code, targets.data_ptr(),
+    ws, size = _workspace("pbg_table_logprobs_workspace", device, n, rows, dim, code, 2 if rounded else 1)
+    _call("pbg_table_logprobs_grad_rounded" if rounded else "pbg_table_logprobs_grad", device, queries.data_ptr(), _row_stride(queries), n, table.data_ptr(), _row_stride(table), rows, dim, code, targets.data_ptr(),
           int(ignore_index), _scale(scale, True), lse.data_ptr(), _ptr(entropy), _ptr(grad_logprob), _ptr(grad_entropy), dq.data_ptr(), dt.data_ptr(),
           _ptr(ws), size, _error_word(errors, device))
     return dq, dt

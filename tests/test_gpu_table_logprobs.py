@@ -558,17 +558,17 @@ def test_probabilities_of_long_rows_add_up_to_one(dtype, n, dim):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("n,rows,dim", [(129, 700, 72), (300, 3000, 400), (40_000, 300, 16)])
-def test_fine_gradients_are_as_good_as_their_rounding(dtype, n, rows, dim):
-    """A table whose rows have much in common: what rounding takes from dz does not cancel where dz does.  With fine=True dz keeps two planes, 2^-17 of
+def test_gradients_are_as_good_as_their_rounding(dtype, n, rows, dim):
+    """A table whose rows have much in common: what rounding takes from dz does not cancel where dz does.  dz keeps two planes, 2^-17 of
     it (fp16: 2^-22 and 2^-39 of its bound), and the results are off by half a step of their own, 1.2e-3 in the mean over the numbers between two
-    powers of two (bf16), what a rounding of exact results leaves, and hardly more; without it by up to three times as much."""
+    powers of two (bf16), what a rounding of exact results leaves, and hardly more; with rounded=True by up to three times as much."""
     g = gen(n)
     t = ((1 + torch.randn(rows, dim, device=DEV, generator=g)) / math.sqrt(dim)).to(dtype)
     targets = torch.randint(0, rows, (n,), device=DEV, generator=g)
     q = torch.randn(n, dim, device=DEV, generator=g).to(dtype)
     gr = torch.randn(n, device=DEV, generator=g) / (1 if dtype == torch.float16 else n)
     r = T.table_logprobs(q, t, targets)
-    dq, dt = T.table_logprobs_grad(q, t, targets, r.lse, None, gr, fine=True)
+    dq, dt = T.table_logprobs_grad(q, t, targets, r.lse, None, gr)
     z = q.double() @ t.double().T
     w = -(z - r.lse.double()[:, None]).exp()
     w[torch.arange(n, device=DEV), targets] += 1
@@ -577,8 +577,18 @@ def test_fine_gradients_are_as_good_as_their_rounding(dtype, n, rows, dim):
         rounding = (want.to(dtype).double() - want).norm()
         assert (got.double() - want).norm() <= 1.05 * rounding + 2e-5 * want.norm()
     if dtype == torch.bfloat16:
-        d1 = T.table_logprobs_grad(q, t, targets, r.lse, None, gr)[0]
+        d1 = T.table_logprobs_grad(q, t, targets, r.lse, None, gr, rounded=True)[0]
         assert (d1.double() - w @ t.double()).norm() <= 4 * (dq.double() - w @ t.double()).norm()
     one = T.table_logprobs_grad(q[:128], t, targets[:128], r.lse[:128], None, gr[:128])
-    two = T.table_logprobs_grad(q[:128], t, targets[:128], r.lse[:128], None, gr[:128], fine=True)
+    two = T.table_logprobs_grad(q[:128], t, targets[:128], r.lse[:128], None, gr[:128], rounded=True)
     assert all(torch.equal(a, b) for a, b in zip(one, two))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,rows,dim", [(129, 257, 72), (300, 5000, 100), (1000, 14_951, 400), (40_000, 300, 16)])
+def test_rounded_gradients(dtype, n, rows, dim):
+    q, t, targets = inputs(n, rows, dim, dtype, n + rows)
+    targets[4], q[4] = -100, math.nan
+    r = T.table_logprobs(q, t, targets, scale=1.1)
+    g, h = torch.randn(n, device=DEV, generator=gen(1)) / n, torch.randn(n, device=DEV, generator=gen(2)) / n
+    check_grad(q, t, targets, 1.1, g, h, r, T.table_logprobs_grad(q, t, targets, r.lse, r.entropy, g, h, scale=1.1, rounded=True), [4])

@@ -9,8 +9,8 @@
 //
 // Forward: a row is read once.  Gradient: one read, one write.  HBM bounds both; the forward pass comes near the issue slots too (16-bit
 // scores at 6.5 TB/s are 11.6 to an SM and cycle, which issues 128 lanes of instructions: 11 for each score, of which the pass takes
-// some seven).  4099 x 131,072 bf16 with the best 8: 218 us, 4.9 TB/s, 60 % of the issue slots; its gradient 315 us, 6.8 TB/s; four rows
-// with the best 20, eight CTAs to a row: 14 us.
+// some seven).  4099 x 131,072 bf16 with the best 8, a call on other buffers each time: 227 to 240 us, 4.7 TB/s, 60 % of the issue slots; the gradient
+// of 4096 336 to 349 us, 6.3 TB/s; four rows with the best 20, eight CTAs to a row: 14 us in a graph.
 #include <cooperative_groups.h>
 
 #include "pbg_tokens.cuh"

@@ -6,9 +6,9 @@
 // The gradient sorts (id, i) first, so that the occurrences of an id lie next to each other in the order of i, and no sum
 // depends on the order in which anything arrives.  Sums are fp32, rounded to the output's type once.
 //
-// Measured: 16,384 rows of 1024 fp32 13 us (134 MB, part of it from L2), five rows 2 us; gradients of 16,384 x 2048 bf16 into 131,072 rows
-// 137 us (604 MB; sort 15, sums and zeros 105 at 64 % of DRAM's peak, join 14), of 10,000 x 400 fp32 into 14,951 rows 27 us, three launches
-// of a few dependent steps each.
+// Measured, calls on other buffers each time: 16,384 rows of 1024 fp32 19 us (134 MB, part of it from L2); gradients of 16,384 x 2048 bf16 into
+// 131,072 rows 140 us (604 MB; sort 15, sums and zeros 105 at 64 % of DRAM's peak, join 14), of 10,000 x 400 fp32 into 14,951 rows 29 us,
+// three launches of a few dependent steps each.  Five rows: 2 us in a graph.
 #include <cooperative_groups.h>
 
 #include "pbg_tokens.cuh"

@@ -16,7 +16,7 @@
 //                elements, rows of dz with a small g and columns that no query comes near keep their bits down to 2^-150 of the largest.
 //
 // One persistent kernel per product, one CTA per SM, tiles of 128 x BN (BN <= 256) or, by a pair of CTAs, 256 x BN:
-//   warp 0     TMA into a ring of stages (64 k-values of one plane, or 32 of two)
+//   warp 0     TMA into a ring of stages (64 k-values of one plane, or 32 of two or three)
 //   warp 1     issues tcgen05.mma into one of two accumulators of 256 columns
 //   warps 2-9  read the other accumulator, two warps to every 32 rows: reduce it to (maximum, S, T) per row; or turn it into
 //              dz and write that; or write the product
@@ -26,14 +26,14 @@
 //
 // What the loop waits for was found by leaving out the loads, then the products: a stage of four products (512 cycles) took 890 with loads
 // alone, whatever its bytes, because of a cluster-wide acquire in front of every stage and of loads issued from several lanes.
-// 4096 x 16,384 x 2048 bf16 (ncu): dz 179 us, dQ 189, dW 176 with the tensor pipe active 84, 77 (the last round of tiles is half empty) and
-// 86 % of the time; 4099 x 65,536 x 2048, all three 2.29 to 2.63 ms (1.25 to 1.44 PFLOP/s) as the power allows.  fp32, 5000 x 14,951 x 400: 180,
-// 172 and 180 us.  7 queries x 131,072 x 2048 bf16: 89 us, 74 % of DRAM's peak.
+// 4096 x 16,384 x 2048 bf16 (ncu): dz 227 us, dQ 354 and dW 330 with the tensor pipe active 61, 81 (the last round of tiles is half empty)
+// and 90 % of the time; 4099 x 65,536 x 2048, a call: 4.3 ms, 1.28 PFLOP/s with both planes of dz counted, as the power allows.  fp32, 5000 x
+// 14,951 x 400: dz 199 us, dQ 304, dW 331 (six products, 512 columns for 400).  7 queries x 131,072 x 2048 bf16: 98 us, 68 % of DRAM's peak.
 //
 // Up to sixteen fp32 queries take no tensor cores: making planes of the table reads and writes it three times over, where fp32 products
 // on the CUDA cores keep up with one reading of it (tab_few_kernel).
 //
-// Every wait is bounded: one that runs out sets bit 2 of the error word, the CTA's products stop, and whatever it had still to
+// Every wait is bounded: one that runs out sets 2 in the error word, the CTA's products stop, and whatever it had still to
 // write is NaN -- partial sums, dz or results, so that all results that depend on them are NaN too; then it frees its tensor memory
 // and returns.
 #include <algorithm>
@@ -616,7 +616,7 @@ __global__ void __launch_bounds__(128) tab_stats_kernel(const long long *__restr
 
 // ---- a few fp32 queries ----------------------------------------------------------------------------------------
 // The queries lie in shared memory; a warp takes R rows of the table at a time, its lanes along the rows, so that a query's
-// 512 bytes serve R rows.  HBM bounds it up to 8 queries (65,536 x 2048: one 85 us, seven 110, where planes took 431), then the reads
+// 512 bytes serve R rows.  HBM bounds it up to 8 queries (65,536 x 2048: one 85 us, seven 107; planes take 300 for 17), then the reads
 // of the queries (sixteen 161 us).
 #define TAB_FEW 16
 #define TAB_FEW_WARPS 16

@@ -297,7 +297,8 @@ int pbg_sub_bucket(pbg_context *ctx, const int64_t *lhs_in, const int64_t *rhs_i
  * irrelevant); two calls in flight need two of them.  All pointers are device memory; row strides are in elements, the elements of
  * a row lie next to each other.  Types are pbg_dtype; sums, statistics and softmax sums are fp32, results are rounded once.
  * errors: device int32 word or NULL; 1 is set by an id or target outside of its range, 4 by an lse that a gradient can do
- * nothing with (token_logprobs_grad), 2 where a bounded wait ran out (results that depend on it are NaN, with or without the word).  scale: finite for the lookups, 1e-20 to 1e20 for the log probabilities.
+ * nothing with (token_logprobs_grad), 2 where a bounded wait ran out (results that depend on it are NaN, with or without the
+ * word).  scale: finite for the lookups, 1e-20 to 1e20 for the log probabilities.
  * Sizes: dim 1 to 65536; ids, rows of scores and table rows below 2^31 (less 65536 for a row's scores and for the rows that
  * table_logprobs scores), ids of a gradient and queries up to 2^30; PBG_ERR_TOO_LARGE beyond.
  * A target equal to ignore_index marks a row of padding: it is not read, its outputs are 0 (top_ids -1), its gradients 0. ---- */
@@ -369,11 +370,11 @@ int32_t pbg_table_logprobs_wait_limit(int32_t limit);
 
 /* Gradients of sum(grad_logprob * logprob + grad_entropy * entropy) with respect to the queries [n, dim] and the table [rows, dim],
  * rows one behind the other, of their type; either may be NULL (not wanted).  lse, entropy: of the forward call.  The scores are
- * computed again; their gradient is kept in two parts of the operands' type for the two products.  The second form rounds it to that type above
- * 128 queries: a third less time, bf16 results 2.3e-3 off instead of the 1.7e-3 of their own rounding (more where all rows of the table
- * have much in common); its workspace is asked for with grad = 2.  Of fp16's, what lies below 2^-39 of the largest |g| + 23 |h| is
- * cut off.  fp32: three bf16 parts of it and of the operands; elements below 2^-150 of
- * the largest of their matrix lose bits.
+ * computed again; their gradient is kept in two parts of the operands' type for the two products.  The second form rounds it to that
+ * type above 128 queries: a third less time, bf16 results 2.3e-3 off instead of the 1.7e-3 of their own rounding (more where all rows of
+ * the table have much in common); its workspace is asked for with grad = 2.  Of fp16's, what lies below 2^-39 of the largest
+ * |g| + 23 |h| is cut off.  fp32: three bf16 parts of it and of the operands; elements below 2^-150 of the largest of their matrix
+ * lose bits.
  * NaN or an infinity in the table makes grad_queries NaN, padding's rows too; one in a query that counts makes its row and grad_table NaN.
  * workspace: of pbg_table_logprobs_workspace(n, rows, dim, dtype, 1) bytes: copies as in the forward pass (fp32: two and a half
  * times as much), dz, at most 2 GiB or 256 columns of it, and, where the table goes in pieces or the sum over its rows in parts,
@@ -384,10 +385,10 @@ int pbg_table_logprobs_grad(const void *queries, int64_t q_stride, int64_t n, co
                             void *grad_queries, void *grad_table, void *workspace, int64_t workspace_bytes,
                             int32_t *errors, void *stream);
 int pbg_table_logprobs_grad_rounded(const void *queries, int64_t q_stride, int64_t n, const void *table, int64_t t_stride, int64_t rows,
-                            int32_t dim, int32_t dtype, const int64_t *targets, int64_t ignore_index, float scale,
-                            const float *lse, const float *entropy, const float *grad_logprob, const float *grad_entropy,
-                            void *grad_queries, void *grad_table, void *workspace, int64_t workspace_bytes,
-                            int32_t *errors, void *stream);
+                                    int32_t dim, int32_t dtype, const int64_t *targets, int64_t ignore_index, float scale,
+                                    const float *lse, const float *entropy, const float *grad_logprob, const float *grad_entropy,
+                                    void *grad_queries, void *grad_table, void *workspace, int64_t workspace_bytes,
+                                    int32_t *errors, void *stream);
 
 /* Kernel launches issued by this context since creation (for launch accounting). */
 int64_t pbg_launch_count(const pbg_context *ctx);

@@ -356,7 +356,8 @@ def table_logprobs_grad(queries: torch.Tensor, table: torch.Tensor, targets: tor
     dq = torch.empty((n, dim), dtype=queries.dtype, device=device)
     dt = torch.empty((rows, dim), dtype=table.dtype, device=device)
     ws, size = _workspace("pbg_table_logprobs_workspace", device, n, rows, dim, code, 2 if rounded else 1)
-    _call("pbg_table_logprobs_grad_rounded" if rounded else "pbg_table_logprobs_grad", device, queries.data_ptr(), _row_stride(queries), n, table.data_ptr(), _row_stride(table), rows, dim, code, targets.data_ptr(),
-          int(ignore_index), _scale(scale, True), lse.data_ptr(), _ptr(entropy), _ptr(grad_logprob), _ptr(grad_entropy), dq.data_ptr(), dt.data_ptr(),
+    _call("pbg_table_logprobs_grad_rounded" if rounded else "pbg_table_logprobs_grad", device, queries.data_ptr(), _row_stride(queries), n,
+          table.data_ptr(), _row_stride(table), rows, dim, code, targets.data_ptr(), int(ignore_index), _scale(scale, True),
+          lse.data_ptr(), _ptr(entropy), _ptr(grad_logprob), _ptr(grad_entropy), dq.data_ptr(), dt.data_ptr(),
           _ptr(ws), size, _error_word(errors, device))
     return dq, dt

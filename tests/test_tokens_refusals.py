@@ -184,3 +184,45 @@ def test_workspaces_are_as_large_as_the_header_says(dtype, n, rows, dim):
         assert copies <= got <= most, (got, most)
         if rows * n * planes * 2 <= 1 << 30 and n * dim * 4 <= 1 << 20:                       # small ones do not ask for the limits
             assert got <= (2.5 if dtype == 0 else 1) * copies + 4 * (n + rows) + n * (rows + 64) * planes * 2 + 64 * 4 * n * dim + some
+
+
+@pytest.mark.parametrize("change,status", [(dict(logits=None), BAD), (dict(lse=None), BAD), (dict(vocab=0), BAD), (dict(top=33), LARGE), (dict(scale=0.0), BAD), (dict(n=2 ** 31), LARGE)])
+def test_logprobs_arguments_with_the_rest_of_lse(change, status):
+    a = dict(logits=P, stride=100, n=4, vocab=100, dtype=0, targets=P, ignore=-100, scale=1.0, top=0, logprob=P, entropy=P, lse=P, rest=P, rank=P, top_logprobs=P, top_ids=P)
+    a.update(change)
+    assert _lib.lib().pbg_token_logprobs_wide(*a.values(), None, None) == status
+
+
+@pytest.mark.parametrize("change,status", [(dict(logits=None), BAD), (dict(lse=None), BAD), (dict(entropy=None), BAD), (dict(out=None), BAD), (dict(out_stride=99), BAD),
+                                           (dict(vocab=2 ** 31, out_stride=2 ** 31), LARGE)])
+def test_logprobs_grad_arguments_with_the_rest_of_lse(change, status):
+    a = dict(logits=P, stride=100, n=4, vocab=100, dtype=0, targets=P, ignore=-100, scale=1.0, lse=P, rest=P, entropy=P, g=P, h=P, out=P, out_stride=100)
+    a.update(change)
+    assert _lib.lib().pbg_token_logprobs_grad_wide(*a.values(), None, None) == status
+
+
+@pytest.mark.parametrize("change,status", TABLE_CHANGES + [(dict(ws=None), BAD), (dict(size=255), BAD), (dict(lse=None), BAD), (dict(entropy=None), BAD), (dict(dq=None, dt=None), BAD)])
+def test_table_grad_rounded_arguments(change, status):
+    L = _lib.lib()
+    a = dict(TABLE, n=200, lse=P, entropy=P, g=P, h=P, dq=P, dt=P, ws=P, size=L.pbg_table_logprobs_workspace(200, 100, 8, 1, 2))
+    assert a["size"] < L.pbg_table_logprobs_workspace(200, 100, 8, 1, 1)
+    a.update(change)
+    assert L.pbg_table_logprobs_grad_rounded(*a.values(), None, None) == status
+
+
+def test_the_limit_of_waits_is_handed_back():
+    L = _lib.lib()
+    usual = L.pbg_table_logprobs_wait_limit(5)
+    assert usual > 1000 and L.pbg_table_logprobs_wait_limit(-1) == 5 and L.pbg_table_logprobs_wait_limit(-1) == usual
+
+
+@pytest.mark.gpu
+def test_python_refuses_a_rest_of_lse_that_does_not_fit():
+    x, ids, f = torch.zeros(6, 8, device="cuda"), torch.zeros(6, dtype=torch.long, device="cuda"), torch.zeros(6, device="cuda")
+    for bad, error in ((f.double(), TypeError), (f[:5], ValueError), (f.cpu(), ValueError), (f.view(2, 3), ValueError)):
+        with pytest.raises(error):
+            T.token_logprobs_grad(x, ids, f, None, f, lse_rest=bad)
+    # every second element of a vector, as a row that lies apart
+    r = T.token_logprobs(x + 3e7, ids)
+    apart = torch.stack((r.lse_rest, f), 1)[:, 0]
+    assert torch.equal(T.token_logprobs_grad(x + 3e7, ids, r.lse, None, f + 1, lse_rest=apart), T.token_logprobs_grad(x + 3e7, ids, r.lse, None, f + 1, lse_rest=r.lse_rest))
